@@ -6,8 +6,8 @@ Every case names an `op`:
   linear    Y = act.(W*X .+ b) .+ R, or with `grad` its gradients dX, dW, db
   grouped   the same with a weight matrix per group: column p of Y takes the
             matrix of group ids[p]; `copies` consecutive columns of Y share one
-            column of X (the `copies` experts of a token); a column whose id
-            names no group keeps R alone, or zeros
+            column of X (the `copies` experts of a token, ids being copies x
+            cols); a column whose id names no group keeps R alone, or zeros
   norm      layer norm of every column of X, or with `grad` its gradients
 
 A column is one token, one node of a graph or one sample.  Dense matrices are
@@ -163,6 +163,8 @@ def prepare(case, seed):
         if case["drop"]:
             ids[torch.rand(n, generator=g, device=DEV) < case["drop"]] = 0
         s["ids"] = ids.to(torch.int32)
+        if case["copies"] > 1:
+            s["ids"] = s["ids"].view(cols, case["copies"]).t()      # a column of ids for each column of X
     if case["bias"]:
         s["bias"] = _matrix(g, out, groups or 1, T, 0.2)
         s["bias"] = s["bias"] if groups else s["bias"][:, 0]
@@ -279,7 +281,7 @@ def _plain_linear(s, c):
 def _slots(ids, groups):
     """The columns in the order of their groups, their groups, their places in
     them, and the size of the largest group."""
-    e = ids.long() - 1
+    e = ids.t().reshape(-1).long() - 1
     e = torch.where((e >= 0) & (e < groups), e, groups)
     e, order = torch.sort(e, stable=True)
     counts = torch.bincount(e, minlength=groups + 1)
@@ -381,7 +383,7 @@ def exact(case, seed):
     W = s["W"].double() if "groups" in case else s["W"].double()[:, :, None]
     groups, copies, out = W.shape[2], case.get("copies", 1), case["out"]
     n = case["cols"] * copies
-    group = s["ids"].long() - 1 if "ids" in s else torch.zeros(n, dtype=torch.long, device=X.device)
+    group = s["ids"].t().reshape(-1).long() - 1 if "ids" in s else torch.zeros(n, dtype=torch.long, device=X.device)
     members = [torch.nonzero(group == k)[:, 0] for k in range(groups)]
     if case["grad"]:
         G = s["dY"].double() if s["Z"] is None else s["dY"].double() * _exact_slope(s["Z"].double(), case["act"])
