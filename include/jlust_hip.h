@@ -392,7 +392,9 @@ enum jlust_fn_kind {
     JLUST_FN_SQRT = 4,      /* sqrt(v)                  */
     JLUST_FN_EXP = 5,       /* exp(v)                   */
     JLUST_FN_LOG = 6,       /* log(v)                   */
-    JLUST_FN_RELU = 7       /* max(v, 0), NaN kept      */
+    JLUST_FN_RELU = 7,      /* max(v, 0), NaN kept      */
+    JLUST_FN_GELU = 8,      /* v * Phi(v), Phi the normal distribution's integral */
+    JLUST_FN_SILU = 9       /* v / (1 + exp(-v))        */
 };
 
 /*
@@ -1131,6 +1133,107 @@ int jlust_hip_shifted_diag_spmm_f32(int64_t m, int64_t n, int64_t k,
                                     const float *B, int64_t ldb, float beta,
                                     float *C, int64_t ldc,
                                     jlust_stream_t stream);
+
+/* ------------------------------------- a layer's products and normalisation */
+
+/*
+ * The dense parts of a network's layer, next to the sparse products (no
+ * counterpart in the reference, whose GPU paths leave them to the caller's
+ * array library): a column is one node of a graph, one token or one sample.
+ * Values are Float64, Float32, Float16 or BFloat16, one type for all operands
+ * of a call; sums and statistics are Float32 (Float64 for Float64).
+ */
+enum jlust_value_type {
+    JLUST_VALUE_F64 = 0,
+    JLUST_VALUE_F32 = 1,
+    JLUST_VALUE_F16 = 2,
+    JLUST_VALUE_BF16 = 3
+};
+
+/*
+ * The columns of a batch by group: a plan is 32-bit integers in device memory
+ * of the caller, offsets[groups + 1], then the columns 0 .. n-1 in stable order
+ * of their group, those whose id names no group last, and, for copies > 1, the
+ * columns of X they stand for (column / copies).  ids are Int32 or Int64 (64
+ * set) and count from `origin`.  At most 4,095 groups.  plan_ints gives the
+ * plan's length.  Stream-ordered, nothing is read back.
+ */
+int jlust_hip_group_plan_ints(int64_t n, int64_t groups, int64_t copies, int64_t *ints);
+int jlust_hip_group_plan_build(int64_t n, int64_t groups, int64_t copies, int32_t origin,
+                               const void *ids, int ids64, int32_t *plan, jlust_stream_t stream);
+
+/*
+ * Y = act.(W*X .+ bias) .+ R for out x inp W, inp x cols X and out x cols Y
+ * and R (column-major, leading dimensions ld*); Z, where it is given, gets
+ * W*X .+ bias.  w_layout 0: W is column-major, ldw >= out; 1: W is the
+ * transpose of a column-major inp x out matrix, ldw >= inp.  act is
+ * JLUST_FN_IDENTITY, _RELU, _GELU or _SILU.  bias, R and Z may be null.  R may
+ * be Y.
+ * With groups > 0, `plan` sorts the cols columns of Y; column p takes the
+ * matrix W + g*w_stride and the bias + g*bias_stride of its group g and column
+ * p / copies of X, which has cols / copies columns.  A column of no group gets
+ * 0 .+ R, and 0 in Z.
+ */
+typedef struct jlust_linear {
+    int32_t value_type, act, w_layout, reserved;
+    int64_t out, inp, cols;
+    const void *W; int64_t ldw;
+    const void *X; int64_t ldx;
+    void *Y; int64_t ldy;
+    const void *bias;
+    const void *R; int64_t ldr;
+    void *Z; int64_t ldz;
+    int64_t groups, copies;
+    const int32_t *plan;
+    int64_t w_stride, bias_stride;
+} jlust_linear;
+int jlust_hip_linear(const jlust_linear *op, jlust_stream_t stream);
+
+/*
+ * Its gradients: with G = dY .* act'.(Z), dX = W'*G, dW = G*X' and dbias =
+ * G's row sums, each where its pointer is not null (dW laid out as W, dbias as
+ * bias; groups: each column to its own group's, and the copies' sum in dX; a
+ * group without columns gets zeros).  Z is what the forward call kept; unused
+ * for JLUST_FN_IDENTITY.  G is rounded to the value type once, for the two
+ * products; dbias sums it as it is.
+ */
+typedef struct jlust_linear_grad {
+    int32_t value_type, act, w_layout, reserved;
+    int64_t out, inp, cols;
+    const void *W; int64_t ldw;
+    const void *X; int64_t ldx;
+    const void *dY; int64_t lddy;
+    const void *Z; int64_t ldz;
+    void *dX; int64_t lddx;
+    void *dW; int64_t lddw;
+    void *dbias;
+    int64_t groups, copies;
+    const int32_t *plan;
+    int64_t w_stride, dw_stride, dbias_stride;
+} jlust_linear_grad;
+int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t stream);
+
+/*
+ * Layer norm of the columns of a d x cols X: y = (x - mean) * rstd .* weight
+ * .+ bias with rstd = 1/sqrt(variance + eps) over the column's d values
+ * (weight, bias: d values or null).  stats (or null) gets mean and rstd of
+ * each column, 2 x cols with leading dimension lds >= 2, Float32 (Float64 for
+ * Float64).  Y may be X.
+ */
+int jlust_hip_layer_norm(int32_t value_type, int64_t d, int64_t cols, const void *X, int64_t ldx,
+                         const void *weight, const void *bias, double eps, void *Y, int64_t ldy,
+                         void *stats, int64_t lds, jlust_stream_t stream);
+
+/*
+ * Its gradients from X, dY and the stats of the forward call: with h = (x -
+ * mean)*rstd and g = dY .* weight, dX = rstd*(g - mean(g) - h*mean(g.*h)) by
+ * column, dweight = sum of dY.*h and dbias = sum of dY over the columns; each
+ * where its pointer is not null.  dX may be dY.
+ */
+int jlust_hip_layer_norm_grad(int32_t value_type, int64_t d, int64_t cols, const void *X, int64_t ldx,
+                              const void *dY, int64_t lddy, const void *stats, int64_t lds,
+                              const void *weight, void *dX, int64_t lddx, void *dweight, void *dbias,
+                              jlust_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -18,13 +18,15 @@ from .errors import (DeviceMismatch, HIPError, IncompatibleExtents, IndexOriginM
 from .formats import (CompressedLevel, DenseLevel, Formats, PeriodicLevel, ShiftedDiagLevel,
                       SingletonLevel, TensorFormat, dim2lvl, lvl2dim)
 from .ops import (AbstractKernelHandle, AbstractUSTBackend, BBMSpMVOp, BlockSpMMOp, BlockSpMVOp,
-                  HIPBackend, Op, OpType, SDDMMOp, SpMMOp, SpMVOp, default_backend, execute,
+                  GroupedLinearGradOp, GroupedLinearOp, HIPBackend, LayerNormGradOp, LayerNormOp,
+                  LinearGradOp, LinearOp, Op, OpType, SDDMMOp, SpMMOp, SpMVOp, default_backend, execute,
                   matmul, mul_, prepare, supports_backend, update_values_)
 from .block_sparse import (BlockSparseMatrix, BlockStructureError, batch_mul, batch_mul_,
                            update_block_values_)
 from .block_banded import BlockBandedMatrix
-from .elementwise import (ElementwiseFn, abs_fn, affine_fn, exp_fn, identity_fn, log_fn, relu_fn,
-                          sqrt_fn, square_fn)
+from .elementwise import (ElementwiseFn, abs_fn, affine_fn, exp_fn, gelu_fn, identity_fn, log_fn,
+                          relu_fn, silu_fn, sqrt_fn, square_fn)
+from .layers import GroupPlan
 from .convert import (convert_format, convert_index_type, convert_value_type, csc_tensor,
                       dcsr_tensor, sparse_to_dense)
 from ._lib import preload

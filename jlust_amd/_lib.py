@@ -169,6 +169,13 @@ SIGNATURES = {
     "jlust_hip_gather_rows_f32": (_INT, [_I64, _I64, _I32, _P, _I64, _P, _I64, _P, _I64, _P]),
     "jlust_hip_scatter_rows_f64": (_INT, [_I64, _I64, _I32, _P, _I64, _P, _I64, _P, _I64, _P]),
     "jlust_hip_scatter_rows_f32": (_INT, [_I64, _I64, _I32, _P, _I64, _P, _I64, _P, _I64, _P]),
+    "jlust_hip_group_plan_ints": (_INT, [_I64, _I64, _I64, ctypes.POINTER(_I64)]),
+    "jlust_hip_group_plan_build": (_INT, [_I64, _I64, _I64, _I32, _P, _INT, _P, _P]),
+    "jlust_hip_linear": (_INT, [_P, _P]),
+    "jlust_hip_linear_grad": (_INT, [_P, _P]),
+    "jlust_hip_layer_norm": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _P, _D, _P, _I64, _P, _I64, _P]),
+    "jlust_hip_layer_norm_grad": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P,
+                                         _P]),
 }
 
 STATUS = {

@@ -22,7 +22,7 @@ BUILD = os.path.join(HERE, "_build")
 HIP_LIB = os.path.join(HERE, "libjlust_hip.so")
 WL_LIB = os.path.join(HERE, "libjlust_workloads.so")
 
-HIP_SOURCES = ["capi.hip", "scan.hip", "spmv.hip", "coo_spmv.hip", "spmm.hip", "sddmm.hip",
+HIP_SOURCES = ["linear_half.hip", "linear_wide.hip", "layer_norm.hip", "linear.hip", "capi.hip", "scan.hip", "spmv.hip", "coo_spmv.hip", "spmm.hip", "sddmm.hip",
                "bsr_spmm.hip", "bsr_small.hip", "convert.hip", "assemble.hip", "fn.hip", "dcsr.hip", "coo_plan.hip",
                "periodic.hip", "spmv_binned.hip", "coo_csc.hip"]
 

@@ -178,6 +178,10 @@ int preload_dcsr();
 int preload_fn();
 int preload_periodic();
 int preload_scan();
+int preload_linear();
+int preload_linear_half();
+int preload_linear_wide();
+int preload_layer_norm();
 
 #define JLUST_PRELOAD_KERNEL(KERNEL)                                                        \
     do {                                                                                    \

@@ -12,6 +12,7 @@
 // are exact, so the result equals the fused form's; the extra passes move
 // O(n + m) bytes next to the O(nnz) of the product.  Products and sums are
 // not contracted into FMAs, as in the reference's generic Julia code.
+#include "activation.hpp"
 #include "common.hpp"
 
 #include <cmath>
@@ -33,6 +34,8 @@ __device__ __forceinline__ T apply(int kind, T a, T b, T v)
     case JLUST_FN_EXP: return exp(v);
     case JLUST_FN_LOG: return log(v);
     case JLUST_FN_RELU: return v > T(0) ? v : (v != v ? v : T(0));
+    case JLUST_FN_GELU:
+    case JLUST_FN_SILU: return activate<false>(kind, v);
     default: return v;
     }
 }
@@ -54,7 +57,7 @@ int apply_fn(int64_t n, int32_t kind, T a, T b, const T *src, T alpha, T beta, T
 {
     clear_error();
     if (n < 0) return fail(JLUST_STATUS_INVALID_ARGUMENT, "apply_fn: negative length");
-    if (kind < JLUST_FN_IDENTITY || kind > JLUST_FN_RELU)
+    if (kind < JLUST_FN_IDENTITY || kind > JLUST_FN_SILU)
         return fail(JLUST_STATUS_INVALID_ARGUMENT, "apply_fn: unknown function kind %d", kind);
     if (bad_ptr(src, n) || bad_ptr(dst, n)) return fail(JLUST_STATUS_INVALID_ARGUMENT, "apply_fn: null device pointer");
     if (int st = require_device(nullptr)) return st;

@@ -1,0 +1,620 @@
+// linear.hip -- a layer's dense products, Y = act.(W*X .+ b) .+ R, with one W or
+// one per group of columns, and their gradients; the plan that sorts the columns
+// by group.  The products run in tile_kernel.hpp; here are their arguments, the
+// gradient's first pass over dY, and the small sums.
+#include <initializer_list>
+
+#include "tile_product.hpp"
+
+namespace jlust {
+namespace {
+
+// ---------------------------------------------------------------- group plans
+
+constexpr int64_t MAX_GROUPS = 4095;           // 4 waves' counters of a workgroup fit 64 KB of LDS
+constexpr int PLAN_WAVES = 4, PLAN_IDS = 1024; // of a wave of the plan kernels on many columns
+constexpr int SMALL_WAVES = 16;
+constexpr int64_t SMALL_COLUMNS = 8192, SMALL_GROUPS = 1000;
+
+// The bin of column p: its group, `groups` if it names none.
+__device__ __forceinline__ int bin_of(const void *ids, int ids64, int64_t p, int origin, int groups)
+{
+    const int64_t id = (ids64 ? ((const int64_t *)ids)[p] : (int64_t)((const int32_t *)ids)[p]) - origin;
+    return id >= 0 && id < groups ? (int)id : groups;
+}
+
+// The lanes of the wave that hold the same bin as this one (bits: those of a
+// bin); lanes without one pass active = false and get 0.
+__device__ __forceinline__ uint64_t same_bin(int bin, bool active, int bits)
+{
+    uint64_t mask = __ballot(active);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t set = __ballot(bin >> b & 1);
+        mask &= bin >> b & 1 ? set : ~set;
+    }
+    return active ? mask : 0;
+}
+
+// Counts a wave's ids [p0, p1) per bin, or (PLACE) writes every column at its
+// bin's next place: 64 columns at a time, a column's place among its own 64 by
+// the lanes before it, so equal bins keep their order.
+template <bool PLACE>
+__device__ __forceinline__ void walk_ids(const void *ids, int ids64, int64_t p0, int64_t p1, int origin, int groups,
+                                         int bits, int32_t *cnt, int32_t *perm, int32_t *src, int copies)
+{
+    const int lane = lane_id();
+    for (int64_t base = p0; base < p1; base += 64) {
+        const int64_t p = base + lane;
+        const bool active = p < p1;
+        const int bin = active ? bin_of(ids, ids64, p, origin, groups) : 0;
+        const uint64_t mask = same_bin(bin, active, bits);
+        const int before = __popcll(mask & ((1ull << lane) - 1));
+        const int at = active ? cnt[bin] : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (active && before == 0) cnt[bin] = at + __popcll(mask);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (PLACE && active) {
+            perm[at + before] = (int32_t)p;
+            if (src) src[at + before] = (int32_t)(p / copies);
+        }
+    }
+}
+
+// The whole plan in one workgroup: a few columns cost a launch, not six.
+__global__ __launch_bounds__(SMALL_WAVES * 64) void group_plan_small_kernel(int64_t n, int groups, int copies, int origin,
+                                                                            const void *ids, int ids64, int bits,
+                                                                            int32_t *offsets, int32_t *perm, int32_t *src)
+{
+    extern __shared__ int32_t cnt[];               // [waves][groups + 1]
+    __shared__ int32_t waves[SMALL_WAVES + 1];
+    const int wave = threadIdx.x >> 6, bins = groups + 1;
+    for (int i = threadIdx.x; i < SMALL_WAVES * bins; i += SMALL_WAVES * 64) cnt[i] = 0;
+    __syncthreads();
+    const int64_t per = ((n + SMALL_WAVES - 1) / SMALL_WAVES + 63) / 64 * 64;
+    const int64_t p0 = per * wave < n ? per * wave : n, p1 = p0 + per < n ? p0 + per : n;
+    walk_ids<false>(ids, ids64, p0, p1, origin, groups, bits, cnt + wave * bins, nullptr, nullptr, 1);
+    __syncthreads();
+    // bins <= 1,024: one a thread.
+    const int b = threadIdx.x, lane = lane_id();
+    int32_t total = 0;
+    if (b < bins)
+        for (int w = 0; w < SMALL_WAVES; ++w) total += cnt[w * bins + b];
+    int32_t incl = total;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int32_t t = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += t;
+    }
+    if (lane == 63) waves[wave] = incl;
+    __syncthreads();
+    if (b < bins) {
+        int32_t run = incl - total;
+        for (int w = 0; w < wave; ++w) run += waves[w];
+        offsets[b] = run;
+        for (int w = 0; w < SMALL_WAVES; ++w) {
+            const int32_t c = cnt[w * bins + b];
+            cnt[w * bins + b] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+    walk_ids<true>(ids, ids64, p0, p1, origin, groups, bits, cnt + wave * bins, perm, src, copies);
+}
+
+// Many columns: counts[bin][wave] of runs of PLAN_IDS columns, which a scan
+// turns into each wave's first place in every bin.
+template <bool PLACE>
+__global__ __launch_bounds__(PLAN_WAVES * 64) void group_plan_kernel(int64_t n, int groups, int copies, int origin,
+                                                                     const void *ids, int ids64, int bits, int64_t runs,
+                                                                     int32_t *counts, int32_t *offsets, int32_t *perm,
+                                                                     int32_t *src)
+{
+    extern __shared__ int32_t cnt[];
+    const int wave = threadIdx.x >> 6, lane = lane_id(), bins = groups + 1;
+    const int64_t run = (int64_t)blockIdx.x * PLAN_WAVES + wave;
+    int32_t *mine = cnt + wave * bins;
+    for (int b = lane; b < bins; b += 64) mine[b] = PLACE && run < runs ? counts[b * runs + run] : 0;
+    __syncthreads();
+    const int64_t p0 = run * PLAN_IDS < n ? run * PLAN_IDS : n, p1 = p0 + PLAN_IDS < n ? p0 + PLAN_IDS : n;
+    if (PLACE && run == 0)
+        for (int b = lane; b < bins; b += 64) offsets[b] = counts[b * runs];
+    walk_ids<PLACE>(ids, ids64, p0, p1, origin, groups, bits, mine, perm, src, copies);
+    __syncthreads();
+    if (!PLACE && run < runs)
+        for (int b = lane; b < bins; b += 64) counts[b * runs + run] = mine[b];
+}
+
+int check_groups(const char *who, int64_t n, int64_t groups, int64_t copies)
+{
+    if (n < 0 || n >= (int64_t)1 << 31)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: %lld columns are not within [0, 2^31)", who, (long long)n);
+    if (groups < 1 || groups > MAX_GROUPS)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: %lld groups are not within [1, %lld]", who, (long long)groups,
+                    (long long)MAX_GROUPS);
+    if (copies < 1 || copies >= (int64_t)1 << 31 || n % copies)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: %lld columns are not %lld copies of some", who, (long long)n,
+                    (long long)copies);
+    return JLUST_STATUS_SUCCESS;
+}
+
+// ------------------------------------------------------- the gradient's first pass
+
+// Runs of rows that one workgroup takes; 256 threads are 32 vectors along m by
+// 8 rows.
+template <typename T>
+struct Prepass {
+    static constexpr int V = 16 / sizeof(T), COLS = 32 * V;
+};
+
+// G = dY .* act'(Z) in the order of the groups (row p of G is column perm[p]),
+// rounded to T, and the sums of its unrounded rows over a run of `per` columns:
+// sums[run][m].  dY and Z are read once; G and dbias would each read them again.
+template <typename T>
+__global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m, const T *__restrict__ dY, int64_t lddy,
+                                                           const T *__restrict__ Z, int64_t ldz, int act, T *__restrict__ G,
+                                                           int64_t ldg, const int32_t *__restrict__ offsets,
+                                                           const int32_t *__restrict__ perm, int groups, int per, int blocks_m,
+                                                           typename Elem<T>::Acc *__restrict__ sums)
+{
+    using A = typename Elem<T>::Acc;
+    constexpr int V = Prepass<T>::V, COLS = Prepass<T>::COLS;
+    __shared__ A s_sum[8][COLS + 1];
+    const int64_t run = blockIdx.x / blocks_m;
+    const int64_t m0 = (int64_t)(blockIdx.x % blocks_m) * COLS;
+    GroupRun r;
+    if (offsets) {
+        if (!find_run(offsets, groups, n, run, per, &r) || r.group == groups) return;
+    } else {
+        r.begin = run * per;
+        r.end = r.begin + per < n ? r.begin + per : n;
+    }
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = m0 + (int64_t)tx * V, left = m - c;
+    A acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = A(0);
+    if (left > 0)
+        for (int64_t p = r.begin + ty; p < r.end; p += 8) {
+            const int64_t col = perm ? (int64_t)perm[p] : p;
+            T y[V], z[V];
+            const uint32x4 vy = left >= V ? load_chunk(dY + col * lddy + c) : load_chunk_part(dY + col * lddy + c, left);
+            __builtin_memcpy(y, &vy, 16);
+            if (Z) {
+                const uint32x4 vz = left >= V ? load_chunk(Z + col * ldz + c) : load_chunk_part(Z + col * ldz + c, left);
+                __builtin_memcpy(z, &vz, 16);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                A g = A(y[e]);
+                if (Z) g *= activate_slope<sizeof(T) == 2>(act, A(z[e]));
+                acc[e] += g;
+                y[e] = T(g);
+            }
+            if (G) {
+                if (left >= V) store_vec<V>(G + p * ldg + c, y);
+                else
+                    for (int e = 0; e < V; ++e)
+                        if (e < left) G[p * ldg + c + e] = y[e];
+            }
+        }
+    if (!sums) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_sum[ty][tx * V + e] = acc[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < COLS; i += 256) {
+        A s = A(0);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += s_sum[q][i];
+        if (m0 + i < m) sums[run * m + m0 + i] = s;
+    }
+}
+
+// dbias of a group: the sums of its runs, in order; 32 m by 32 runs at a time.
+template <typename T>
+__global__ __launch_bounds__(1024) void grad_bias_kernel(int64_t n, int64_t m, const int32_t *__restrict__ offsets, int per,
+                                                         const typename Elem<T>::Acc *__restrict__ sums, T *__restrict__ dbias,
+                                                         int64_t stride)
+{
+    using A = typename Elem<T>::Acc;
+    __shared__ A s_sum[32][33];
+    __shared__ int64_t s_first;
+    const int group = blockIdx.y, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    int64_t first = 0, count = (n + per - 1) / per;
+    if (offsets) {
+        if (threadIdx.x < 64) {                    // the runs of the groups before
+            int64_t before = 0;
+            for (int g = lane_id(); g < group; g += 64) before += (offsets[g + 1] - offsets[g] + per - 1) / per;
+            for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d, 64);
+            if (threadIdx.x == 0) s_first = before;
+        }
+        __syncthreads();
+        first = s_first;
+        count = (offsets[group + 1] - offsets[group] + per - 1) / per;
+    }
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+    A s = A(0);
+    if (c < m) {
+#pragma unroll 8
+        for (int64_t i = ty; i < count; i += 32) s += sums[(first + i) * m + c];
+    }
+    s_sum[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < m) {
+        A t = A(0);
+#pragma unroll
+        for (int q = 0; q < 32; ++q) t += s_sum[q][tx];
+        dbias[group * stride + c] = T(t);
+    }
+}
+
+// dX's column t: the sum of its copies' columns of the product.
+template <typename T>
+__global__ __launch_bounds__(256) void sum_copies_kernel(int64_t cols, int64_t d, int copies,
+                                                         const typename Elem<T>::Acc *__restrict__ src, T *__restrict__ dX,
+                                                         int64_t ldx)
+{
+    using A = typename Elem<T>::Acc;
+    constexpr int V = 4;
+    const int64_t per = (d + V - 1) / V, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= cols * per) return;
+    const int64_t t = at / per, c = (at - t * per) * V;
+    const A *p = src + t * copies * d + c;
+    A s[V] = {0, 0, 0, 0};
+    T o[V];
+    if (c + V <= d) {
+        for (int q = 0; q < copies; ++q, p += d) {
+            A v[V];
+            load_vec<V>(p, v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = T(s[e]);
+        store_vec<V>(dX + t * ldx + c, o);
+        return;
+    }
+    for (int e = 0; c + e < d; ++e) {
+        A v = A(0);
+        for (int q = 0; q < copies; ++q) v += p[q * d + e];
+        dX[t * ldx + c + e] = T(v);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void fill_zero_kernel(int64_t rows, int64_t d, T *__restrict__ out, int64_t ld)
+{
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at < rows * d) out[at / d * ld + at % d] = T(0);
+}
+
+template <typename T>
+int fill_zero(int64_t rows, int64_t d, void *out, int64_t ld, hipStream_t s)
+{
+    if (rows * d == 0) return JLUST_STATUS_SUCCESS;
+    hipLaunchKernelGGL((fill_zero_kernel<T>), dim3((unsigned)((rows * d + 255) / 256)), dim3(256), 0, s, rows, d, (T *)out, ld);
+    return check_launch("fill_zero_kernel");
+}
+
+// ---------------------------------------------------------------------- checks
+
+struct Operand { const char *name; const void *p; int64_t rows, cols, ld; bool needed; };
+
+int check_operands(const char *who, std::initializer_list<Operand> ops)
+{
+    for (const Operand &o : ops) {
+        const bool empty = o.rows == 0 || o.cols == 0;
+        if (!o.p) {
+            if (o.needed && !empty) return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: %s is null", who, o.name);
+            continue;
+        }
+        if (o.cols > 1 && o.ld < o.rows)
+            return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: %s has leading dimension %lld, its columns %lld rows", who,
+                        o.name, (long long)o.ld, (long long)o.rows);
+    }
+    return JLUST_STATUS_SUCCESS;
+}
+
+int check_common(const char *who, int32_t value_type, int32_t act, int32_t w_layout, int64_t out, int64_t inp, int64_t cols,
+                 int64_t groups, int64_t copies, const int32_t *plan)
+{
+    if (value_type < JLUST_VALUE_F64 || value_type > JLUST_VALUE_BF16)
+        return fail(JLUST_STATUS_UNSUPPORTED_VALUE_TYPE, "%s: unknown value type %d", who, value_type);
+    if (act != JLUST_FN_IDENTITY && act != JLUST_FN_RELU && act != JLUST_FN_GELU && act != JLUST_FN_SILU)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: function kind %d is no activation of this call", who, act);
+    if (w_layout != 0 && w_layout != 1) return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: w_layout is %d", who, w_layout);
+    if (out < 0 || inp < 0 || cols < 0) return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: negative extent", who);
+    if (out >= (int64_t)1 << 31 || inp >= (int64_t)1 << 31 || cols >= (int64_t)1 << 31)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: an extent of 2^31 or more", who);
+    if (groups) {
+        if (int st = check_groups(who, cols, groups, copies)) return st;
+        if (!plan && cols) return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: groups without a plan", who);
+    } else if (copies > 1) {
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: copies without groups", who);
+    }
+    return JLUST_STATUS_SUCCESS;
+}
+
+struct PlanParts { const int32_t *offsets, *perm, *src; };
+
+PlanParts plan_parts(const int32_t *plan, int64_t n, int64_t groups, int64_t copies)
+{
+    if (!groups) return {nullptr, nullptr, nullptr};
+    const int32_t *perm = plan + groups + 1;
+    return {plan, perm, copies > 1 ? perm + n : perm};
+}
+
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
+template <typename F>
+int by_type(int32_t value_type, F &&f)
+{
+    switch (value_type) {
+    case JLUST_VALUE_F64: return f(double());
+    case JLUST_VALUE_F32: return f(float());
+    case JLUST_VALUE_F16: return f((_Float16)0);
+    default: return f((__bf16)0.0f);
+    }
+}
+
+// --------------------------------------------------------------------- forward
+
+template <typename T>
+int linear(const jlust_linear &op, jlust_stream_t stream)
+{
+    const PlanParts pl = plan_parts(op.plan, op.cols, op.groups, op.copies);
+    TileArgs a;
+    a.m = op.out;
+    a.n = op.cols;
+    a.k = op.inp;
+    a.P = op.W;
+    a.ldp = op.ldw;
+    a.gp = op.w_stride;
+    a.Q = op.X;
+    a.ldq = op.ldx;
+    a.qrow = pl.src;
+    a.crow = pl.perm;
+    a.offsets = pl.offsets;
+    a.groups = (int)op.groups;
+    a.C = op.Y;
+    a.ldc = op.ldy;
+    a.bias = op.bias;
+    a.gb = op.bias_stride;
+    a.R = op.R;
+    a.ldr = op.ldr;
+    a.Z = op.Z;
+    a.ldz = op.ldz;
+    a.act = op.act;
+    const bool pkc = op.w_layout == 1;
+    int shape = 0;
+    size_t bytes = 0;
+    plan_tile_product<T>(&a, pkc, true, &shape, &bytes);
+    if (bytes)
+        if (int st = scratch(stream, bytes, &a.part)) return st;
+    return launch_tile_product<T>(a, pkc, true, shape, (hipStream_t)stream);
+}
+
+// ------------------------------------------------------------------- gradients
+
+template <typename T>
+int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
+{
+    using A = typename Elem<T>::Acc;
+    hipStream_t s = (hipStream_t)stream;
+    const PlanParts pl = plan_parts(op.plan, op.cols, op.groups, op.copies);
+    const bool slope = op.act != JLUST_FN_IDENTITY, products = op.dX || op.dW;
+    const bool make_g = slope && products;
+    const int64_t n = op.cols, out = op.out, inp = op.inp;
+    const bool wide = op.dX && op.groups && op.copies > 1;
+
+    // G's columns are the groups' in order where it is made, dY's own where not.
+    const T *G = (const T *)op.dY;
+    int64_t ldg = op.lddy;
+    const int32_t *grow = pl.perm;
+    if (make_g) {
+        ldg = (out + 7) / 8 * 8;
+        grow = nullptr;
+    }
+
+    TileArgs x;
+    int shape_x = 0;
+    size_t part_x = 0;
+    const bool x_kc = op.w_layout == 0;
+    if (op.dX) {
+        x.m = inp;
+        x.n = n;
+        x.k = out;
+        x.P = op.W;
+        x.ldp = op.ldw;
+        x.gp = op.w_stride;
+        x.ldq = ldg;
+        x.qrow = grow;
+        x.crow = pl.perm;
+        x.offsets = pl.offsets;
+        x.groups = (int)op.groups;
+        x.C = op.dX;
+        x.ldc = wide ? inp : op.lddx;
+        x.c_wide = wide;
+        plan_tile_product<T>(&x, x_kc, true, &shape_x, &part_x);
+    }
+    TileArgs w;
+    int shape_w = 0;
+    size_t part_w = 0;
+    if (op.dW) {
+        w.m = op.w_layout ? inp : out;
+        w.n = op.w_layout ? out : inp;
+        w.k = n;
+        (op.w_layout ? w.P : w.Q) = op.X;
+        (op.w_layout ? w.ldp : w.ldq) = op.ldx;
+        (op.w_layout ? w.prow : w.qrow) = pl.src;
+        (op.w_layout ? w.ldq : w.ldp) = ldg;
+        (op.w_layout ? w.qrow : w.prow) = grow;
+        w.offsets = pl.offsets;
+        w.groups = (int)op.groups;
+        w.C = op.dW;
+        w.ldc = op.lddw;
+        w.gc = op.dw_stride;
+        plan_tile_product<T>(&w, false, false, &shape_w, &part_w);
+    }
+
+    const int64_t blocks_m = (out + Prepass<T>::COLS - 1) / Prepass<T>::COLS;
+    int64_t per = (n * blocks_m + 2047) / 2048;                // about 2,048 workgroups
+    per = per < 64 ? 64 : (per + 7) / 8 * 8;
+    const int64_t runs = (n + per - 1) / per + (op.groups ? (op.groups < n ? op.groups : n) : 0);
+    const size_t g_bytes = make_g ? align256(sizeof(T) * n * ldg) : 0;
+    const size_t wide_bytes = wide ? align256(sizeof(A) * n * inp) : 0;
+    const size_t part = align256(part_x > part_w ? part_x : part_w);
+    const size_t sum_bytes = op.dbias ? sizeof(A) * runs * out : 0;
+    void *ws = nullptr;
+    if (g_bytes + wide_bytes + part + sum_bytes)
+        if (int st = scratch(stream, g_bytes + wide_bytes + part + sum_bytes, &ws)) return st;
+    char *at = (char *)ws;
+    T *g_buf = make_g ? (T *)at : nullptr;
+    A *wide_buf = (A *)(at + g_bytes);
+    x.part = w.part = at + g_bytes + wide_bytes;
+    A *sums = op.dbias ? (A *)(at + g_bytes + wide_bytes + part) : nullptr;
+    if (make_g) G = g_buf;
+
+    if (make_g || op.dbias) {
+        if (n > 0) {
+            hipLaunchKernelGGL((grad_prepass_kernel<T>), dim3((unsigned)(runs * blocks_m)), dim3(256), 0, s, n, out,
+                               (const T *)op.dY, op.lddy, slope ? (const T *)op.Z : nullptr, op.ldz, op.act, g_buf, ldg,
+                               pl.offsets, pl.perm, (int)op.groups, (int)per, (int)blocks_m, sums);
+            if (int st = check_launch("grad_prepass_kernel")) return st;
+        }
+        if (op.dbias) {
+            hipLaunchKernelGGL((grad_bias_kernel<T>), dim3((unsigned)((out + 31) / 32), (unsigned)(op.groups ? op.groups : 1)),
+                               dim3(1024), 0, s, n, out, n ? pl.offsets : nullptr, (int)per, sums, (T *)op.dbias,
+                               op.dbias_stride);
+            if (int st = check_launch("grad_bias_kernel")) return st;
+        }
+    }
+    if (op.dX && n > 0 && inp > 0) {
+        x.Q = G;
+        if (wide) x.C = wide_buf;
+        if (int st = launch_tile_product<T>(x, x_kc, true, shape_x, s)) return st;
+        if (wide) {
+            const int64_t cols = n / op.copies, items = cols * ((inp + 3) / 4);
+            hipLaunchKernelGGL((sum_copies_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, cols, inp,
+                               (int)op.copies, wide_buf, (T *)op.dX, op.lddx);
+            if (int st = check_launch("sum_copies_kernel")) return st;
+        }
+    }
+    if (op.dW && inp > 0) {
+        if (n == 0) {
+            const int64_t rows = op.w_layout ? out : inp, d = op.w_layout ? inp : out;
+            for (int64_t g = 0; g < (op.groups ? op.groups : 1); ++g)
+                if (int st = fill_zero<T>(rows, d, (T *)op.dW + g * op.dw_stride, op.lddw, s)) return st;
+        } else {
+            (op.w_layout ? w.Q : w.P) = G;
+            if (int st = launch_tile_product<T>(w, false, false, shape_w, s)) return st;
+        }
+    }
+    return JLUST_STATUS_SUCCESS;
+}
+
+}  // namespace
+}  // namespace jlust
+
+using namespace jlust;
+
+extern "C" int jlust_hip_group_plan_ints(int64_t n, int64_t groups, int64_t copies, int64_t *ints)
+{
+    clear_error();
+    if (int st = check_groups("group_plan", n, groups, copies)) return st;
+    if (!ints) return fail(JLUST_STATUS_INVALID_ARGUMENT, "group_plan: null result");
+    *ints = groups + 1 + n * (copies > 1 ? 2 : 1);
+    return JLUST_STATUS_SUCCESS;
+}
+
+extern "C" int jlust_hip_group_plan_build(int64_t n, int64_t groups, int64_t copies, int32_t origin, const void *ids,
+                                          int ids64, int32_t *plan, jlust_stream_t stream)
+{
+    clear_error();
+    if (int st = check_groups("group_plan", n, groups, copies)) return st;
+    if (int st = check_origin(origin)) return st;
+    if (bad_ptr(ids, n) || !plan) return fail(JLUST_STATUS_INVALID_ARGUMENT, "group_plan: null device pointer");
+    if (int st = require_device(nullptr)) return st;
+    hipStream_t s = (hipStream_t)stream;
+    int bits = 1;
+    while ((groups >> bits) != 0) ++bits;
+    int32_t *perm = plan + groups + 1, *src = copies > 1 ? perm + n : nullptr;
+    if (n <= SMALL_COLUMNS && groups <= SMALL_GROUPS) {
+        hipLaunchKernelGGL(group_plan_small_kernel, dim3(1), dim3(SMALL_WAVES * 64),
+                           SMALL_WAVES * (groups + 1) * sizeof(int32_t), s, n, (int)groups, (int)copies, (int)origin, ids,
+                           ids64, bits, plan, perm, src);
+        return check_launch("group_plan_small_kernel");
+    }
+    const int64_t runs = (n + PLAN_IDS - 1) / PLAN_IDS > 0 ? (n + PLAN_IDS - 1) / PLAN_IDS : 1;
+    const int64_t counts_n = (groups + 1) * runs;
+    const size_t first = (exclusive_scan_scratch_bytes(counts_n) + 255) / 256 * 256;
+    void *ws = nullptr;
+    if (int st = scratch(stream, first + sizeof(int32_t) * counts_n, &ws)) return st;
+    int32_t *counts = (int32_t *)((char *)ws + first);
+    const dim3 grid((unsigned)((runs + PLAN_WAVES - 1) / PLAN_WAVES)), block(PLAN_WAVES * 64);
+    const size_t lds = PLAN_WAVES * (groups + 1) * sizeof(int32_t);
+    hipLaunchKernelGGL((group_plan_kernel<false>), grid, block, lds, s, n, (int)groups, (int)copies, (int)origin, ids, ids64,
+                       bits, runs, counts, plan, perm, src);
+    if (int st = check_launch("group_plan_kernel")) return st;
+    if (int st = exclusive_scan_i32(counts, counts, counts_n, stream)) return st;
+    hipLaunchKernelGGL((group_plan_kernel<true>), grid, block, lds, s, n, (int)groups, (int)copies, (int)origin, ids, ids64,
+                       bits, runs, counts, plan, perm, src);
+    return check_launch("group_plan_kernel");
+}
+
+extern "C" int jlust_hip_linear(const jlust_linear *op, jlust_stream_t stream)
+{
+    clear_error();
+    if (!op) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: null argument");
+    const char *who = "linear";
+    if (int st = check_common(who, op->value_type, op->act, op->w_layout, op->out, op->inp, op->cols, op->groups, op->copies,
+                              op->plan))
+        return st;
+    const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
+    const int64_t wr = op->w_layout ? op->inp : op->out, wc = op->w_layout ? op->out : op->inp;
+    if (int st = check_operands(who, {{"W", op->W, wr, wc, op->ldw, true},
+                                      {"X", op->X, op->inp, xcols, op->ldx, true},
+                                      {"Y", op->Y, op->out, op->cols, op->ldy, true},
+                                      {"R", op->R, op->out, op->cols, op->ldr, false},
+                                      {"Z", op->Z, op->out, op->cols, op->ldz, false}}))
+        return st;
+    if (int st = require_device(nullptr)) return st;
+    if (op->out == 0 || op->cols == 0) return JLUST_STATUS_SUCCESS;
+    return by_type(op->value_type, [&](auto t) { return linear<decltype(t)>(*op, stream); });
+}
+
+extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t stream)
+{
+    clear_error();
+    if (!op) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_grad: null argument");
+    const char *who = "linear_grad";
+    if (int st = check_common(who, op->value_type, op->act, op->w_layout, op->out, op->inp, op->cols, op->groups, op->copies,
+                              op->plan))
+        return st;
+    const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
+    const int64_t wr = op->w_layout ? op->inp : op->out, wc = op->w_layout ? op->out : op->inp;
+    if (int st = check_operands(who, {{"W", op->W, wr, wc, op->ldw, op->dX != nullptr},
+                                      {"X", op->X, op->inp, xcols, op->ldx, op->dW != nullptr},
+                                      {"dY", op->dY, op->out, op->cols, op->lddy, true},
+                                      {"Z", op->Z, op->out, op->cols, op->ldz, op->act != JLUST_FN_IDENTITY},
+                                      {"dX", op->dX, op->inp, xcols, op->lddx, false},
+                                      {"dW", op->dW, wr, wc, op->lddw, false}}))
+        return st;
+    if (int st = require_device(nullptr)) return st;
+    if (op->out == 0) {
+        if (!op->dX) return JLUST_STATUS_SUCCESS;
+        return by_type(op->value_type, [&](auto t) {
+            return fill_zero<decltype(t)>(xcols, op->inp, op->dX, op->lddx, (hipStream_t)stream);
+        });
+    }
+    return by_type(op->value_type, [&](auto t) { return linear_grad<decltype(t)>(*op, stream); });
+}
+
+namespace jlust {
+int preload_linear()
+{
+    JLUST_PRELOAD_KERNEL(group_plan_small_kernel);
+    return JLUST_STATUS_SUCCESS;
+}
+}  // namespace jlust

@@ -1,0 +1,17 @@
+// linear_half.hip -- the dense products of 16-bit values.
+#include "tile_kernel.hpp"
+
+namespace jlust {
+
+template void plan_tile_product<_Float16>(TileArgs *, bool, bool, int *, size_t *);
+template int launch_tile_product<_Float16>(const TileArgs &, bool, bool, int, hipStream_t);
+template void plan_tile_product<__bf16>(TileArgs *, bool, bool, int *, size_t *);
+template int launch_tile_product<__bf16>(const TileArgs &, bool, bool, int, hipStream_t);
+
+int preload_linear_half()
+{
+    JLUST_PRELOAD_KERNEL((tile_product_kernel<__bf16, true, true, 128, 128, 2, 2, false>));
+    return JLUST_STATUS_SUCCESS;
+}
+
+}  // namespace jlust

@@ -7,7 +7,7 @@ The reference compiles the two Julia functions into its kernel.  Here a
 transform is either
 
   * an ElementwiseFn (identity, affine a*v + b, abs, square, sqrt, exp, log,
-    relu), applied on the device by jlust_hip_apply_fn_{f64,f32}; or
+    relu, gelu, silu), applied on the device by jlust_hip_apply_fn_{f64,f32}; or
   * any Python callable, called once on the whole device vector (a torch
     tensor) and expected to return a tensor of the same shape and dtype, the
     counterpart of the reference's arbitrary `input_fn::IF`.
@@ -26,9 +26,9 @@ import torch
 
 from . import _lib
 
-FN_IDENTITY, FN_AFFINE, FN_ABS, FN_SQUARE, FN_SQRT, FN_EXP, FN_LOG, FN_RELU = range(8)
+FN_IDENTITY, FN_AFFINE, FN_ABS, FN_SQUARE, FN_SQRT, FN_EXP, FN_LOG, FN_RELU, FN_GELU, FN_SILU = range(10)
 _NAMES = {FN_IDENTITY: "identity", FN_AFFINE: "affine", FN_ABS: "abs", FN_SQUARE: "square",
-          FN_SQRT: "sqrt", FN_EXP: "exp", FN_LOG: "log", FN_RELU: "relu"}
+          FN_SQRT: "sqrt", FN_EXP: "exp", FN_LOG: "log", FN_RELU: "relu", FN_GELU: "gelu", FN_SILU: "silu"}
 
 
 @dataclass(frozen=True)
@@ -56,6 +56,8 @@ sqrt_fn = ElementwiseFn(FN_SQRT)
 exp_fn = ElementwiseFn(FN_EXP)
 log_fn = ElementwiseFn(FN_LOG)
 relu_fn = ElementwiseFn(FN_RELU)
+gelu_fn = ElementwiseFn(FN_GELU)      # v * Phi(v), Phi the normal distribution's integral
+silu_fn = ElementwiseFn(FN_SILU)      # v / (1 + exp(-v))
 
 
 def affine_fn(a: float, b: float = 0.0) -> ElementwiseFn:

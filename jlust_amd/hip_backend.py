@@ -20,7 +20,7 @@ from .errors import (DeviceMismatch, IncompatibleExtents, NonCanonicalStorage,
                      UnsupportedFormat, UnsupportedIndexType, UnsupportedValueType)
 from .formats import (Formats, bsr_blocksize, is_bsr, is_coo_shaped, is_csc_shaped, is_csr_shaped,
                       is_periodic_csr, is_shifted_diag)
-from .ops import AbstractKernelHandle, HIPBackend, Op, SDDMMOp, SpMMOp, SpMVOp
+from .ops import _LAYER_TAGS, AbstractKernelHandle, HIPBackend, Op, SDDMMOp, SpMMOp, SpMVOp
 from .tensor import USTensor, dense_matrix, leading_dim, nnz, nonzeros, ust
 
 _BE = HIPBackend()
@@ -70,6 +70,8 @@ def _supports(op: Op) -> bool:
     if op.tag == "SDDMM" and len(f) == 3:
         return _dense_fmt(f[0]) and _dense_fmt(f[1]) and \
             (is_csr_shaped(f[2]) or is_coo_shaped(f[2]) or is_csc_shaped(f[2]) or f[2] == Formats.DCSR)
+    if op.tag in _LAYER_TAGS:
+        return all(_dense_fmt(x) for x in f)
     return False
 
 

@@ -48,6 +48,15 @@ BlockSpMVOp = OpType("BlockSpMV")    # src/ops.jl (Op{:BlockSpMV})
 BlockSpMMOp = OpType("BlockSpMM")    # src/ops.jl:111
 BBMSpMVOp = OpType("BBMSpMV")        # src/ops.jl:115
 _AGGREGATE_TAGS = ("BlockSpMV", "BlockSpMM", "BBMSpMV")
+# A layer's dense products and normalisation (layers.py; not in the reference).
+LinearOp = OpType("Linear")
+LinearGradOp = OpType("LinearGrad")
+GroupedLinearOp = OpType("GroupedLinear")
+GroupedLinearGradOp = OpType("GroupedLinearGrad")
+LayerNormOp = OpType("LayerNorm")
+LayerNormGradOp = OpType("LayerNormGrad")
+_LAYER_TAGS = frozenset(("Linear", "LinearGrad", "GroupedLinear", "GroupedLinearGrad", "LayerNorm",
+                         "LayerNormGrad"))
 
 
 # ------------------------------------------------------------------ backends
@@ -114,6 +123,9 @@ def execute(optype, *args, backend=None, **kw):
             r = hip_backend.spmv_fast(A, x, y, kw.get("alpha", 1.0), kw.get("beta", 0.0))
             if r is not None:
                 return r
+    if type(optype) is OpType and optype.tag in _LAYER_TAGS:
+        from . import layers
+        return layers.execute(optype, args, backend, kw)
     if isinstance(optype, AbstractKernelHandle) or (args and isinstance(args[0], AbstractKernelHandle)):
         h, rest = (optype, args) if isinstance(optype, AbstractKernelHandle) else (args[0], args[1:])
         if getattr(h, "takes_raw", False):
@@ -160,6 +172,9 @@ def prepare(backend, optype: OpType, u_A, *more, **kw):
     """prepare(backend, OpType, A; kw...) -> handle (src/ops.jl:179);
     prepare(backend, SDDMMOp, A, B, C) as the cuSPARSE SDDMM handle takes it
     (ext/CUDAExt/ops/sddmm.jl:24-26)."""
+    if optype is GroupedLinearOp and isinstance(backend, HIPBackend):
+        from . import layers
+        return layers.GroupPlan(u_A, *more, **kw)
     u_A = _wrap(u_A)
     if not isinstance(backend, HIPBackend):
         raise UnsupportedFormat(u_A.format, backend, "prepare is implemented for HIPBackend")
