@@ -54,6 +54,27 @@ __device__ __forceinline__ A activate(int act, A z)
     }
 }
 
+// V of them, the kind asked for once.
+template <bool FAST, int V, typename A>
+__device__ __forceinline__ void activate_all(int act, A *z)
+{
+    switch (act) {
+    case JLUST_FN_RELU:
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] = activate<FAST>(JLUST_FN_RELU, z[e]);
+        break;
+    case JLUST_FN_GELU:
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] = activate<FAST>(JLUST_FN_GELU, z[e]);
+        break;
+    case JLUST_FN_SILU:
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] = activate<FAST>(JLUST_FN_SILU, z[e]);
+        break;
+    default: break;
+    }
+}
+
 // The activation's derivative at z.
 template <bool FAST, typename A>
 __device__ __forceinline__ A activate_slope(int act, A z)
