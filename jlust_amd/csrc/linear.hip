@@ -5,6 +5,7 @@
 #include <initializer_list>
 
 #include "tile_product.hpp"
+#include "wave.hpp"
 
 namespace jlust {
 namespace {
@@ -12,9 +13,11 @@ namespace {
 // ---------------------------------------------------------------- group plans
 
 constexpr int64_t MAX_GROUPS = 4095;           // 4 waves' counters of a workgroup fit 64 KB of LDS
-constexpr int PLAN_WAVES = 4, PLAN_IDS = 1024; // of a wave of the plan kernels on many columns
-constexpr int SMALL_WAVES = 16;
-constexpr int64_t SMALL_COLUMNS = 8192, SMALL_GROUPS = 1000;
+constexpr int PLAN_WAVES = 4;                  // of a workgroup of the plan kernels on many columns
+constexpr int PLAN_ROUNDS = 4;                 // of 64 ids a wave holds in registers
+constexpr int SMALL_WAVES = 16, SMALL_ROUNDS = 4;
+constexpr int64_t SMALL_COLUMNS = SMALL_WAVES * SMALL_ROUNDS * 64, SMALL_GROUPS = 1000;
+constexpr int64_t SCAN_COUNTS = 1 << 16;       // that one workgroup scans
 
 // The bin of column p: its group, `groups` if it names none.
 __device__ __forceinline__ int bin_of(const void *ids, int ids64, int64_t p, int origin, int groups)
@@ -35,27 +38,39 @@ __device__ __forceinline__ uint64_t same_bin(int bin, bool active, int bits)
     return active ? mask : 0;
 }
 
-// Counts a wave's ids [p0, p1) per bin, or (PLACE) writes every column at its
-// bin's next place: 64 columns at a time, a column's place among its own 64 by
-// the lanes before it, so equal bins keep their order.
-template <bool PLACE>
-__device__ __forceinline__ void walk_ids(const void *ids, int ids64, int64_t p0, int64_t p1, int origin, int groups,
-                                         int bits, int32_t *cnt, int32_t *perm, int32_t *src, int copies)
+// A wave's ids, 64 a round, all read before the first is used (a round of its own
+// reads took 0.7 us): the bins of [p0, p1), -1 past the end.
+template <int ROUNDS>
+__device__ __forceinline__ void read_bins(const void *ids, int ids64, int64_t p0, int64_t p1, int origin, int groups,
+                                          int (&bin)[ROUNDS])
+{
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int64_t p = p0 + r * 64 + lane_id();
+        bin[r] = p < p1 ? bin_of(ids, ids64, p, origin, groups) : -1;
+    }
+}
+
+// Counts them, or (PLACE) writes every column at its bin's next place: a column's
+// place among its own 64 by the lanes before it, so equal bins keep their order.
+template <bool PLACE, int ROUNDS>
+__device__ __forceinline__ void walk_bins(const int (&bins)[ROUNDS], int64_t p0, int bits, int32_t *cnt, int32_t *perm,
+                                          int32_t *src, int copies)
 {
     const int lane = lane_id();
-    for (int64_t base = p0; base < p1; base += 64) {
-        const int64_t p = base + lane;
-        const bool active = p < p1;
-        const int bin = active ? bin_of(ids, ids64, p, origin, groups) : 0;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const bool active = bins[r] >= 0;
+        if (__ballot(active) == 0) break;
+        const int bin = active ? bins[r] : 0;
         const uint64_t mask = same_bin(bin, active, bits);
         const int before = __popcll(mask & ((1ull << lane) - 1));
         const int at = active ? cnt[bin] : 0;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         if (active && before == 0) cnt[bin] = at + __popcll(mask);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         if (PLACE && active) {
+            const int64_t p = p0 + r * 64 + lane;
             perm[at + before] = (int32_t)p;
             if (src) src[at + before] = (int32_t)(p / copies);
         }
@@ -74,7 +89,9 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void group_plan_small_kernel(int6
     __syncthreads();
     const int64_t per = ((n + SMALL_WAVES - 1) / SMALL_WAVES + 63) / 64 * 64;
     const int64_t p0 = per * wave < n ? per * wave : n, p1 = p0 + per < n ? p0 + per : n;
-    walk_ids<false>(ids, ids64, p0, p1, origin, groups, bits, cnt + wave * bins, nullptr, nullptr, 1);
+    int bin[SMALL_ROUNDS];
+    read_bins(ids, ids64, p0, p1, origin, groups, bin);
+    walk_bins<false>(bin, p0, bits, cnt + wave * bins, nullptr, nullptr, 1);
     __syncthreads();
     // bins <= 1,024: one a thread.
     const int b = threadIdx.x, lane = lane_id();
@@ -100,14 +117,15 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void group_plan_small_kernel(int6
         }
     }
     __syncthreads();
-    walk_ids<true>(ids, ids64, p0, p1, origin, groups, bits, cnt + wave * bins, perm, src, copies);
+    walk_bins<true>(bin, p0, bits, cnt + wave * bins, perm, src, copies);
 }
 
-// Many columns: counts[bin][wave] of runs of PLAN_IDS columns, which a scan
-// turns into each wave's first place in every bin.
+// Many columns: counts[bin][run] of a wave's runs of columns, which a scan turns
+// into each run's first place in every bin.  More groups have longer runs, so that
+// the counts stay below the ids.
 template <bool PLACE>
 __global__ __launch_bounds__(PLAN_WAVES * 64) void group_plan_kernel(int64_t n, int groups, int copies, int origin,
-                                                                     const void *ids, int ids64, int bits, int64_t runs,
+                                                                     const void *ids, int ids64, int bits, int64_t runs, int per,
                                                                      int32_t *counts, int32_t *offsets, int32_t *perm,
                                                                      int32_t *src)
 {
@@ -117,13 +135,54 @@ __global__ __launch_bounds__(PLAN_WAVES * 64) void group_plan_kernel(int64_t n, 
     int32_t *mine = cnt + wave * bins;
     for (int b = lane; b < bins; b += 64) mine[b] = PLACE && run < runs ? counts[b * runs + run] : 0;
     __syncthreads();
-    const int64_t p0 = run * PLAN_IDS < n ? run * PLAN_IDS : n, p1 = p0 + PLAN_IDS < n ? p0 + PLAN_IDS : n;
+    const int64_t p0 = run * per < n ? run * per : n, p1 = p0 + per < n ? p0 + per : n;
     if (PLACE && run == 0)
         for (int b = lane; b < bins; b += 64) offsets[b] = counts[b * runs];
-    walk_ids<PLACE>(ids, ids64, p0, p1, origin, groups, bits, mine, perm, src, copies);
+    for (int64_t p = p0; p < p1; p += PLAN_ROUNDS * 64) {
+        int bin[PLAN_ROUNDS];
+        read_bins(ids, ids64, p, p1, origin, groups, bin);
+        walk_bins<PLACE>(bin, p, bits, mine, perm, src, copies);
+    }
     __syncthreads();
     if (!PLACE && run < runs)
         for (int b = lane; b < bins; b += 64) counts[b * runs + run] = mine[b];
+}
+
+// Exclusive scan of n counts in one workgroup, 4 a thread and round.
+__global__ __launch_bounds__(1024) void group_scan_kernel(int n, int32_t *counts)
+{
+    __shared__ int32_t s_wave[16];
+    const int wave = threadIdx.x >> 6, lane = lane_id();
+    int32_t base = 0;
+    for (int i0 = 0; i0 < n; i0 += 4096) {
+        const int i = i0 + (int)threadIdx.x * 4;
+        int32_t v[4], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = i + e < n ? counts[i + e] : 0;
+            sum += v[e];
+        }
+        int32_t incl = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int32_t t = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += t;
+        }
+        __syncthreads();
+        if (lane == 63) s_wave[wave] = incl;
+        __syncthreads();
+        int32_t run = base + incl - sum;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) run += s_wave[w];
+            base += s_wave[w];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i + e < n) counts[i + e] = run;
+            run += v[e];
+        }
+    }
 }
 
 int check_groups(const char *who, int64_t n, int64_t groups, int64_t copies)
@@ -546,7 +605,9 @@ extern "C" int jlust_hip_group_plan_build(int64_t n, int64_t groups, int64_t cop
                            ids64, bits, plan, perm, src);
         return check_launch("group_plan_small_kernel");
     }
-    const int64_t runs = (n + PLAN_IDS - 1) / PLAN_IDS > 0 ? (n + PLAN_IDS - 1) / PLAN_IDS : 1;
+    int64_t per = (groups + 256) / 256 * 256;
+    int64_t runs = (n + per - 1) / per;
+    if (runs < 1) runs = 1;
     const int64_t counts_n = (groups + 1) * runs;
     const size_t first = (exclusive_scan_scratch_bytes(counts_n) + 255) / 256 * 256;
     void *ws = nullptr;
@@ -555,11 +616,16 @@ extern "C" int jlust_hip_group_plan_build(int64_t n, int64_t groups, int64_t cop
     const dim3 grid((unsigned)((runs + PLAN_WAVES - 1) / PLAN_WAVES)), block(PLAN_WAVES * 64);
     const size_t lds = PLAN_WAVES * (groups + 1) * sizeof(int32_t);
     hipLaunchKernelGGL((group_plan_kernel<false>), grid, block, lds, s, n, (int)groups, (int)copies, (int)origin, ids, ids64,
-                       bits, runs, counts, plan, perm, src);
+                       bits, runs, (int)per, counts, plan, perm, src);
     if (int st = check_launch("group_plan_kernel")) return st;
-    if (int st = exclusive_scan_i32(counts, counts, counts_n, stream)) return st;
+    if (counts_n <= SCAN_COUNTS) {
+        hipLaunchKernelGGL(group_scan_kernel, dim3(1), dim3(1024), 0, s, (int)counts_n, counts);
+        if (int st = check_launch("group_scan_kernel")) return st;
+    } else if (int st = exclusive_scan_i32(counts, counts, counts_n, stream)) {
+        return st;
+    }
     hipLaunchKernelGGL((group_plan_kernel<true>), grid, block, lds, s, n, (int)groups, (int)copies, (int)origin, ids, ids64,
-                       bits, runs, counts, plan, perm, src);
+                       bits, runs, (int)per, counts, plan, perm, src);
     return check_launch("group_plan_kernel");
 }
 

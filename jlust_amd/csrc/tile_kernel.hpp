@@ -4,6 +4,8 @@
 #include "tile_product.hpp"
 #include "wave.hpp"
 
+#include <type_traits>
+
 namespace jlust {
 
 typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
@@ -159,10 +161,9 @@ struct Stage {
         }
     }
 
-    // 32- and 64-bit operands: the values of 16-row tiles [0, TILES) from row
-    // r0 for the CH steps of half s of the k range: f[tile][j] is lane (lr, g)'s
-    // for k = CH*(g + 4s) + j.  kc: tile i's row lr is r0 + 16 i + lr; sc: it is
-    // r0 + 16 CH (i/CH) + CH lr + i%CH, CH tiles from one read.
+    // 32- and 64-bit operands: the values of 16-row tiles [0, TILES) from row r0
+    // for the CH steps of half s of the k range: f[i][j] is lane (lr, g)'s, row
+    // r0 + 16 i + lr at k = CH*(g + 4s) + j.
     template <int TILES>
     __device__ __forceinline__ static void frag(const char *lds, int r0, int lr, int g, int s, T (&f)[TILES][CH])
     {
@@ -173,19 +174,11 @@ struct Stage {
                 __builtin_memcpy(f[i], &c, 16);
             }
         } else {
-            static_assert(TILES % CH == 0, "sc tiles come CH at a time");
+            const T *q = (const T *)lds + CH * (g + 4 * s) * R + r0 + lr;
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const char *q = lds + (CH * (g + 4 * s) + j) * R * (int)sizeof(T);
+            for (int j = 0; j < CH; ++j)
 #pragma unroll
-                for (int i = 0; i < TILES; i += CH) {
-                    T e[CH];
-                    const uint32x4 c = *reinterpret_cast<const uint32x4 *>(q + (r0 + 16 * i + CH * lr) * sizeof(T));
-                    __builtin_memcpy(e, &c, 16);
-#pragma unroll
-                    for (int u = 0; u < CH; ++u) f[i + u][j] = e[u];
-                }
-            }
+                for (int i = 0; i < TILES; ++i) f[i][j] = q[j * R + 16 * i];
         }
     }
 };
@@ -247,9 +240,9 @@ __device__ __forceinline__ void load_bias(const TileArgs &a, int group, int64_t 
     load_some<V>((const T *)a.bias + group * a.gb + m, some ? a.m - m : 0, b);
 }
 
-// V sums of row `row` of C, columns mm ..: the epilogue.
+// V sums of row `row` of C, columns mm ..: the epilogue; res: R's there.
 template <int V, typename T, typename A>
-__device__ __forceinline__ void finish(const TileArgs &a, const T *bias, int64_t row, int64_t mm, A *s)
+__device__ __forceinline__ void finish(const TileArgs &a, const T *bias, const T *res, int64_t row, int64_t mm, A *s)
 {
     const int64_t left = a.m - mm;
     if (left <= 0) return;
@@ -267,61 +260,112 @@ __device__ __forceinline__ void finish(const TileArgs &a, const T *bias, int64_t
     }
     activate_all<sizeof(T) == 2, V>(a.act, s);
     if (a.R) {
-        load_some<V>((const T *)a.R + row * a.ldr + mm, left, t);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[e] += A(t[e]);
+        for (int e = 0; e < V; ++e) s[e] += A(res[e]);
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) t[e] = T(s[e]);
     store_some<V>((T *)a.C + row * a.ldc + mm, left, t);
 }
 
-// This workgroup's tile.  Tiles lie in bands of 8 along n, m after m inside a
-// band, each XCD a run of its own: the workgroups that run at once on one XCD
-// share P and Q tiles in its L2.
-__device__ __forceinline__ bool tile_of(const TileArgs &a, int *tm, int *tn)
-{
-    const int64_t total = (int64_t)a.tiles_m * a.tiles_n, per = (total + NUM_XCD - 1) / NUM_XCD;
-    const int64_t t = (int64_t)(blockIdx.x % NUM_XCD) * per + blockIdx.x / NUM_XCD;
-    if (t >= total) return false;
-    const int64_t band = t / (8 * (int64_t)a.tiles_m);
-    const int in = (int)(t - band * 8 * a.tiles_m);
-    const int wide = a.tiles_n - (int)band * 8 < 8 ? a.tiles_n - (int)band * 8 : 8;
-    *tm = in / wide;
-    *tn = (int)band * 8 + in % wide;
-    return true;
-}
-
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The rows of n, the k range and the group of a tile (extents are below 2^31);
-// false if it has none.
-struct TileRange { int group, n0, nend, k0, kend; };
+// What a workgroup does: its tile, the piece of k, the group, the rows of n and the
+// k range.  Extents are below 2^31, and so are a launch's workgroups.
+struct Work { int tm, piece, group, n0, nend, k0, kend; };
 
-template <bool KSUM, int BN, int BK>
-__device__ __forceinline__ bool tile_range(const TileArgs &a, int tn, TileRange *t)
+// Tile t of tiles_m x tiles_n: bands of 8 along n, m after m inside a band, so that
+// neighbours share P and Q tiles.
+__device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_n, uint32_t tiles_m, int *tm, int *tn)
 {
-    *t = TileRange{0, tn * BN, (int)a.n, 0, (int)a.k};
-    if (a.offsets) {
-        if constexpr (KSUM) {
-            t->group = blockIdx.z;
-            t->k0 = a.offsets[t->group];
-            t->kend = a.offsets[t->group + 1];
+    const uint32_t band = t / (8 * tiles_m), in = t - band * 8 * tiles_m;
+    const uint32_t wide = tiles_n - band * 8 < 8 ? tiles_n - band * 8 : 8;
+    *tm = in / wide;
+    *tn = band * 8 + in % wide;
+}
+
+// A launch's work in order: groups, pieces of k, tiles.  Each XCD takes a run of its
+// own, the workgroups that run at once on one sharing tiles in its L2.  Groups of
+// rows: first the tiles of columns in groups, by their number and not by the bound
+// that the launch is sized for (with the empty ones at its end one XCD had nothing
+// to do: 32 groups, a quarter of the columns in none, 187 us and 152), then those of
+// the columns in none, which only store.  False where there is none.
+template <bool KSUM, int BN, int BK>
+__device__ __forceinline__ bool find_work(const TileArgs &a, Work *w)
+{
+    const uint32_t xcd = blockIdx.x % NUM_XCD, i = blockIdx.x / NUM_XCD, tiles_m = a.tiles_m, split = a.split;
+    int tn;
+    *w = Work{0, 0, 0, 0, (int)a.n, 0, (int)a.k};
+    if (!KSUM && a.offsets) {
+        // A lane holds every 64th group's rows; up to 63 groups are read once.
+        const int lane = lane_id();
+        const bool few = a.groups < 64;
+        int lo = 0, hi = 0, live = 0;
+        for (int g = lane; g <= a.groups; g += 64) {
+            lo = a.offsets[g];
+            hi = g < a.groups ? a.offsets[g + 1] : (int)a.n;
+            if (g < a.groups) live += (hi - lo + BN - 1) / BN;
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) live += __shfl_xor(live, d, 64);
+        live = uniform(live);
+        const uint32_t tiles = live * tiles_m, total = tiles * split, per = (total + NUM_XCD - 1) / NUM_XCD;
+        uint32_t t = xcd * per + i;
+        if (i < per) {
+            if (t >= total) return false;
+            w->piece = t / tiles;
+            tile_at(t % tiles, live, tiles_m, &w->tm, &tn);
+        } else {
+            t = (i - per) * NUM_XCD + xcd;
+            w->piece = t % split;
+            t /= split;
+            w->tm = t % tiles_m;
+            tn = live + t / tiles_m;
+        }
+        if (few) {
+            const int runs = (hi - lo + BN - 1) / BN;
+            int incl = runs;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int v = __shfl_up(incl, d, 64);
+                if (lane >= d) incl += v;
+            }
+            const uint64_t mask = __ballot(tn < incl);
+            if (mask == 0) return false;
+            const int g = __ffsll((unsigned long long)mask) - 1;
+            w->group = g;
+            w->n0 = __shfl(lo + (tn - incl + runs) * BN, g, 64);
+            w->nend = __shfl(hi, g, 64);
         } else {
             GroupRun r;
             if (!find_run(a.offsets, a.groups, a.n, tn, BN, &r)) return false;
-            t->group = r.group;
-            t->n0 = (int)r.begin;
-            t->nend = (int)r.end;
-            if (t->group == a.groups) t->kend = 0;
+            w->group = r.group;
+            w->n0 = (int)r.begin;
+            w->nend = (int)r.group_end;
+        }
+        if (w->group == a.groups) w->kend = 0;
+    } else {
+        const uint32_t tiles = tiles_m * (uint32_t)a.tiles_n;
+        const uint32_t total = tiles * split * (KSUM && a.offsets ? a.groups : 1), per = (total + NUM_XCD - 1) / NUM_XCD;
+        const uint32_t t = xcd * per + i;
+        if (i >= per || t >= total) return false;
+        tile_at(t % tiles, a.tiles_n, tiles_m, &w->tm, &tn);
+        w->piece = t / tiles % split;
+        w->n0 = tn * BN;
+        if (KSUM && a.offsets) {
+            w->group = t / tiles / split;
+            w->k0 = a.offsets[w->group];
+            w->kend = a.offsets[w->group + 1];
         }
     }
-    if (a.split > 1) {
-        const int piece = ((t->kend - t->k0 + a.split - 1) / a.split + BK - 1) / BK * BK;
-        const int lo = t->k0 + piece * (int)blockIdx.y;
-        t->kend = lo + (int64_t)piece < t->kend ? lo + piece : t->kend;
-        t->k0 = lo;
+    if (split > 1) {
+        const int piece = ((w->kend - w->k0 + a.split - 1) / a.split + BK - 1) / BK * BK;
+        const int64_t lo = w->k0 + (int64_t)piece * w->piece, end = w->kend;
+        w->k0 = (int)(lo < end ? lo : end);
+        w->kend = (int)(lo + piece < end ? lo + piece : end);
     }
+    *w = Work{uniform(w->tm), uniform(w->piece), uniform(w->group), uniform(w->n0), uniform(w->nend), uniform(w->k0),
+              uniform(w->kend)};
     return true;
 }
 
@@ -329,21 +373,22 @@ __device__ __forceinline__ bool tile_range(const TileArgs &a, int tn, TileRange 
 // leave a lane 4 values of a row; 16 rows at a time go through the wave's part of
 // the LDS tile (put(run, its place) writes them, chunk c of row r at chunk c ^
 // (r & FLIP)), so that a lane ends 16 bytes of C and a row's lanes a whole line.
-// row_of(run, r) is their place along n.
 template <typename A, int TM> struct SumRows {
-    static constexpr int CHUNKS = TM * (int)sizeof(A) / 16, FLIP = CHUNKS < 16 ? CHUNKS - 1 : 15;
+    static constexpr int USED = TM * (int)sizeof(A) / 16;
+    static constexpr int CHUNKS = USED <= 4 ? 4 : USED <= 8 ? 8 : USED <= 16 ? 16 : USED <= 32 ? 32 : 64;
+    static constexpr int FLIP = CHUNKS < 16 ? CHUNKS - 1 : 15, BYTES = 16 * CHUNKS * 16;
     __device__ __forceinline__ static int at(int r, int c) { return r * CHUNKS * 16 + ((c ^ (r & FLIP)) << 4); }
 };
 
-template <typename T, bool KSUM, int TM, int RUNS, typename Put, typename RowOf>
-__device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int group, int n0, int nend, int64_t m0, Put &&put,
-                                            RowOf &&row_of)
+template <typename T, bool KSUM, int TM, int RUNS, typename Put>
+__device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int piece, int group, int n0, int nend, int64_t m0, Put &&put)
 {
     using A = typename Elem<T>::Acc;
     using SR = SumRows<A, TM>;
-    constexpr int CH = 16 / sizeof(T), ACH = 16 / sizeof(A), LANES = TM / CH, ROWS = 64 / LANES;
+    constexpr int CH = 16 / sizeof(T), ACH = 16 / sizeof(A), LANES = TM / CH, ROWS = 64 / LANES, ITER = (16 + ROWS - 1) / ROWS;
     const int lane = threadIdx.x & 63;
-    char *mine = lds + (threadIdx.x >> 6) * (16 * TM * (int)sizeof(A));
+    const int r0 = lane < LANES * ROWS ? lane / LANES : 16;
+    char *mine = lds + (threadIdx.x >> 6) * SR::BYTES;
     const int64_t m = m0 + lane % LANES * CH, left = a.m - m;
     TileArgs b = a;
     if constexpr (KSUM) b.C = (T *)a.C + group * a.gc;
@@ -351,26 +396,56 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int gr
     T bias[CH];
     load_bias<CH>(b, group, m, bias);
     const int64_t part_rows = KSUM && a.offsets ? a.n * a.groups : a.n;
-    const int64_t part_row = blockIdx.y * part_rows + (KSUM ? group * a.n : 0);
+    const int64_t part_row = piece * part_rows + (KSUM ? group * a.n : 0);
 #pragma unroll
     for (int run = 0; run < RUNS; ++run) {
+        // What the rows need from memory, all of it before the first is used.
+        int row[ITER];
+        T res[ITER][CH];
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            const int r = r0 + it * ROWS, n = n0 + 16 * run + r;
+            row[it] = r < 16 && n < nend && left > 0 ? n : -1;
+        }
+        if (!a.part && a.crow) {
+#pragma unroll
+            for (int it = 0; it < ITER; ++it) row[it] = row[it] >= 0 ? a.crow[row[it]] : -1;
+        }
+        if (a.R && !a.part) {
+#pragma unroll
+            for (int it = 0; it < ITER; ++it) load_some<CH>((const T *)a.R + row[it] * a.ldr + m, row[it] >= 0 ? left : 0, res[it]);
+        }
         wave_sync();
         put(run, mine);
         wave_sync();
-#pragma unroll 1
-        for (int r = lane / LANES; r < 16; r += ROWS) {
-            const int64_t n = n0 + row_of(run, r);
-            if (n >= nend || left <= 0) continue;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            if (row[it] < 0) continue;
+            const int r = r0 + it * ROWS;
             A v[CH];
 #pragma unroll
             for (int e = 0; e < CH; e += ACH) __builtin_memcpy(v + e, mine + SR::at(r, (lane % LANES * CH + e) / ACH), 16);
-            if (a.part) {
-                store_some<CH>((A *)a.part + (part_row + n) * a.m + m, left, v);
-            } else {
-                finish<CH, T, A>(b, bias, a.crow ? (int64_t)a.crow[n] : n, m, v);
-            }
+            if (a.part) store_some<CH>((A *)a.part + (part_row + row[it]) * a.m + m, left, v);
+            else finish<CH, T, A>(b, bias, res[it], row[it], m, v);
         }
     }
+}
+
+// A 16-row run of 16 x 16 tiles: lane (li, g) holds rows 4g .. 4g+3 of column li.
+template <typename A, int MT, int NTL, int TM, typename A4>
+__device__ __forceinline__ void put_rows(const A4 (&acc)[MT][NTL], int j, char *to)
+{
+    constexpr int ACH = 16 / sizeof(A);
+    const int li = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; w += ACH) {
+            A v[ACH];
+#pragma unroll
+            for (int e = 0; e < ACH; ++e) v[e] = acc[i][j][w + e];
+            __builtin_memcpy(to + SumRows<A, TM>::at(li, (16 * i + 4 * g + w) / ACH), v, 16);
+        }
 }
 
 // A workgroup of WM x WN waves makes BM x BN sums; a wave (BM/WM) x (BN/WN) in
@@ -383,16 +458,16 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
     using A4 = typename Elem<T>::Acc4;
     constexpr int NT = WM * WN * 64, BK = 128 / sizeof(T), CH = 16 / sizeof(T);
     constexpr int TM = BM / WM, TN = BN / WN, MT = TM / 16, NTL = TN / 16;
+    constexpr int LM = BM > 64 && BM < 128 ? 128 : BM;  // rows of P in LDS
     constexpr bool KSUM = !PKC && !QKC;                 // groups cut k, not n
-    constexpr int TILE = (BM + BN) * 128, SUMS = WM * WN * 16 * TM * (int)sizeof(typename Elem<T>::Acc);
+    constexpr int TILE = (LM + BN) * 128, SUMS = WM * WN * SumRows<typename Elem<T>::Acc, TM>::BYTES;
     __shared__ __align__(16) char lds[TILE > SUMS ? TILE : SUMS];
-    char *lp = lds, *lq = lds + BM * 128;
+    char *lp = lds, *lq = lds + LM * 128;
 
-    int tm, tn;
-    TileRange r;
-    if (!tile_of(a, &tm, &tn) || !tile_range<KSUM, BN, BK>(a, tn, &r)) return;
-    const int group = uniform(r.group), n0 = uniform(r.n0), nend = uniform(r.nend), k0 = uniform(r.k0), kend = uniform(r.kend);
-    const int64_t m0 = (int64_t)tm * BM;
+    Work w;
+    if (!find_work<KSUM, BN, BK>(a, &w)) return;
+    const int group = w.group, n0 = w.n0, nend = w.nend, k0 = w.k0, kend = w.kend;
+    const int64_t m0 = (int64_t)w.tm * BM;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     const int wm0 = wave % WM * TM, wn0 = wave / WM * TN;
     // The f64 step leaves rows g, g+4, g+8, g+12 in lane (j, g); fed with A's
@@ -406,7 +481,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
         for (int j = 0; j < NTL; ++j) acc[i][j] = A4{0, 0, 0, 0};
 
     if (k0 < kend) {
-        using SP = Stage<T, PKC, BM, NT, IDX>;
+        using SP = Stage<T, PKC, LM, NT, IDX>;
         using SQ = Stage<T, QKC, BN, NT, IDX>;
         SP sp;
         SQ sq;
@@ -426,6 +501,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
+                if (s && k + BK / 2 >= kend) break;
                 if constexpr (sizeof(T) == 2) {
                     uint32x4 p[MT], q[NTL];
 #pragma unroll
@@ -452,29 +528,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
     }
 
     __syncthreads();
-    // Lane (li, g) holds rows 4g .. 4g+3 of every 16 x 16 tile's column li.  Tiles of
-    // an sc P in 32 and 64 bits interleave (Stage::frag): neighbours in m are
-    // neighbouring tiles' values, else the four of one tile; the same along n.
-    constexpr bool MIX = sizeof(T) > 2 && !PKC, MIXN = sizeof(T) > 2 && !QKC;
-    constexpr int ACH = 16 / sizeof(typename Elem<T>::Acc);
-    auto put = [&](int j, char *to) {
-#pragma unroll
-        for (int i = 0; i < MT; i += MIX ? CH : 1)
-#pragma unroll
-            for (int w = 0; w < 4; w += MIX ? 1 : ACH) {
-                typename Elem<T>::Acc v[ACH];
-#pragma unroll
-                for (int e = 0; e < ACH; ++e) v[e] = MIX ? acc[i + (MIX ? e : 0)][j][w] : acc[i][j][(w + (MIX ? 0 : e)) & 3];
-                const int at = 16 * i + (MIX ? CH * (4 * g + w) : 4 * g + w);       // in m
-                __builtin_memcpy(to + SumRows<typename Elem<T>::Acc, TM>::at(li, at / ACH), v, 16);
-            }
-    };
-    finish_tile<T, KSUM, TM, NTL>(a, lds, group, n0 + wn0, nend, m0 + wm0, put, [](int j, int r) {
-        return MIXN ? 16 * CH * (j / CH) + CH * r + j % CH : 16 * j + r;
-    });
+    auto put = [&](int j, char *to) { put_rows<typename Elem<T>::Acc, MT, NTL, TM>(acc, j, to); };
+    finish_tile<T, KSUM, TM, NTL>(a, lds, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
 }
 
-// ----------------------------------------------- 16-bit tiles by copies to LDS
+// ----------------------------------------------- tiles by copies to LDS
 
 __device__ uint32_t tile_zeros[4];             // what a copy reads for k past the end
 
@@ -485,8 +543,10 @@ __device__ uint32_t tile_zeros[4];             // what a copy reads for k past t
 // them making one pass over the banks), sc rows their segments.
 template <typename T, bool KC, int R, int NT, int BK, bool IDX>
 struct Copy {
-    static constexpr int PER = KC ? BK / 8 : R / 8, CNT = R * BK / 8 / NT, BYTES = R * BK * 2, STEP = NT / PER;
-    static_assert(R * BK / 8 % NT == 0 && NT % PER == 0, "whole copies");
+    static constexpr int SZ = sizeof(T), CH = 16 / SZ, RB = BK * SZ;   // a chunk's elements, a kc row's bytes
+    static constexpr int PER = KC ? BK / CH : R / CH, CNT = R * BK / CH / NT, BYTES = R * RB, STEP = NT / PER;
+    static_assert(R * BK / CH % NT == 0 && NT % PER == 0, "whole copies");
+    static_assert(R / 16 >= (SZ == 2 ? 8 : 4), "segments to permute");
     // kc rows may lie anywhere (qrow), so each slot has its address; sc slots lie
     // at 32-bit distances from the step's first row, or IDX finds their rows.
     const T *base;
@@ -499,19 +559,20 @@ struct Copy {
     __device__ __forceinline__ static int lds_row(int i) { return threadIdx.x / PER + i * STEP; }
     __device__ __forceinline__ static int flip(int r)
     {
-        return BK == 64 ? (r >> 1 & 7) ^ (r & 1) << 2 : (r >> 2 & 3) ^ (r & 2);
+        return RB == 128 ? (r >> 1 & 7) ^ (r & 1) << 2 : (r >> 2 & 3) ^ (r & 2);
     }
+    // Where 16 elements of an sc row lie: a transposed 16-bit read takes 4 rows at
+    // two of them at once, a 32- or 64-bit read 4 rows 16 bytes of k apart.
     __device__ __forceinline__ static int segment(int seg, int k)
     {
-        static_assert(R / 16 >= 8, "rows of 256 bytes at least");
-        return seg ^ (k & 3) << 1;
+        return SZ == 2 ? seg ^ (k & 3) << 1 : seg ^ (k / CH & 3);
     }
-    // The first of the 8 elements along its row that slot i reads.
+    // The first of the elements along its row that slot i reads.
     __device__ __forceinline__ static int first(int i)
     {
         const int c = threadIdx.x % PER, r = lds_row(i);
-        if constexpr (KC) return (c ^ flip(r)) * 8;
-        else return segment(c >> 1, r) * 16 + (c & 1) * 8;
+        if constexpr (KC) return (c ^ flip(r)) * CH;
+        else return segment(c / (16 / CH), r) * 16 + c % (16 / CH) * CH;
     }
 
     __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx_, int r0, int rend, int k0, int kend)
@@ -575,10 +636,17 @@ struct Copy {
     // Where a lane reads what it feeds to a 32x32x16 step: row 32 tile + lane % 32,
     // k = 8 (lane / 32) .. + 7; the other tiles and steps lie at flips of its bits
     // and at fixed distances.
+    template <bool PERMUTE = false>
     __device__ __forceinline__ static int place(int tile)
     {
         const int lane = threadIdx.x & 63, li = lane & 15;
-        if constexpr (KC) return (32 * tile + (lane & 31)) * BK * 2 + (((lane >> 5) ^ flip(lane & 31)) << 4);
+        if constexpr (SZ > 2) {
+            // A 16x16x4 step: row 16 tile + lr, k = CH g + j.
+            const int g = lane >> 4, lr = SZ == 8 ? 4 * (li & 3) + (li >> 2) : li, row = PERMUTE ? lr : li;
+            if constexpr (KC) return (16 * tile + row) * RB + ((g ^ flip(row)) << 4);
+            return CH * g * R * SZ + (segment(tile, CH * g) * 16 + row) * SZ;
+        }
+        if constexpr (KC) return (32 * tile + (lane & 31)) * RB + (((lane >> 5) ^ flip(lane & 31)) << 4);
         const int k = 8 * (lane >> 5) + (li >> 2);
         return k * R * 2 + (segment(2 * tile + (lane >> 4 & 1), k) << 5) + ((li & 3) << 3);
     }
@@ -588,7 +656,7 @@ struct Copy {
     __device__ __forceinline__ static uint32x4 frag(const char *lds, int at, int i, int s)
     {
         if constexpr (KC) {
-            return *reinterpret_cast<const uint32x4 *>(lds + (at ^ s << 5) + i * 64 * BK);
+            return *reinterpret_cast<const uint32x4 *>(lds + (at ^ s << 5) + i * 32 * RB);
         } else {
             uint32x4 out;
 #pragma unroll
@@ -600,6 +668,18 @@ struct Copy {
                 out[2 * h + 1] = u[1];
             }
             return out;
+        }
+    }
+
+    // The same of a 16x16x4 step's: f[j] is its value at k = CH (g + 4 s) + j.
+    __device__ __forceinline__ static void frag_wide(const char *lds, int at, int i, int s, T (&f)[CH])
+    {
+        if constexpr (KC) {
+            __builtin_memcpy(f, lds + (at ^ s << 6) + i * 16 * RB, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+                f[j] = *reinterpret_cast<const T *>(lds + (at ^ i * 16 * SZ) + (4 * CH * s + j) * R * SZ);
         }
     }
 };
@@ -615,34 +695,38 @@ __device__ __forceinline__ void copies_done()
     asm volatile("" ::: "memory");
 }
 
-// As tile_product_kernel for 16-bit values whose chunks lie whole and aligned, NB
+// As tile_product_kernel for operands whose chunks lie whole and aligned, NB
 // LDS tiles in turn: while one is multiplied, the copies of the next NB - 1 are
 // under way, and a step has one barrier.
 template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB, bool IDX>
-__global__ __launch_bounds__(WM *WN * 64, BM == 128 && BK == 32 ? 3 : 2) void tile_copy_kernel(const TileArgs a)
+__global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 32 ? 3 : 2) void tile_copy_kernel(const TileArgs a)
 {
-    constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MT = TM / 32, NTL = TN / 32;
+    constexpr bool HALF = sizeof(T) == 2;
+    constexpr int STEP = HALF ? 32 : 16;                // rows and columns of a matrix step
+    constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MT = TM / STEP, NTL = TN / STEP;
+    constexpr int LM = BM > 64 && BM < 128 ? 128 : BM;  // rows of P in LDS
     constexpr bool KSUM = !PKC && !QKC;
-    using CP = Copy<T, PKC, BM, NT, BK, IDX>;
+    using A = typename Elem<T>::Acc;
+    using Sum = std::conditional_t<HALF, floatx16, typename Elem<T>::Acc4>;
+    using CP = Copy<T, PKC, LM, NT, BK, IDX>;
     using CQ = Copy<T, QKC, BN, NT, BK, IDX>;
     // Arrays of their own: the compiler then knows which copies an LDS read waits for.
-    constexpr int TILE = CP::BYTES + CQ::BYTES, SUMS = WM * WN * 16 * TM * 4;
+    constexpr int TILE = CP::BYTES + CQ::BYTES, SUMS = WM * WN * SumRows<A, TM>::BYTES;
     __shared__ __align__(16) char lds0[TILE > SUMS ? TILE : SUMS];
     __shared__ __align__(16) char lds1[TILE];
     __shared__ __align__(16) char lds2[NB > 2 ? TILE : 16];
-    int tm, tn;
-    TileRange r;
-    if (!tile_of(a, &tm, &tn) || !tile_range<KSUM, BN, BK>(a, tn, &r)) return;
-    const int group = uniform(r.group), n0 = uniform(r.n0), nend = uniform(r.nend), k0 = uniform(r.k0), kend = uniform(r.kend);
-    const int m0 = tm * BM;
+    Work w;
+    if (!find_work<KSUM, BN, BK>(a, &w)) return;
+    const int group = w.group, n0 = w.n0, nend = w.nend, k0 = w.k0, kend = w.kend;
+    const int m0 = w.tm * BM;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm0 = wave % WM * TM, wn0 = wave / WM * TN;
 
-    floatx16 acc[MT][NTL];
+    Sum acc[MT][NTL];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NTL; ++j) acc[i][j] = floatx16{0};
+        for (int j = 0; j < NTL; ++j) acc[i][j] = Sum{0};
 
     if (k0 < kend) {
         CP cp;
@@ -659,21 +743,41 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 128 && BK == 32 ? 3 : 2) void ti
                 cq.template start<true>(to + CP::BYTES, k, kend);
             }
         };
-        const int at_p = CP::place(wm0 / 32), at_q = CQ::place(wn0 / 32);
-        auto multiply = [&](const char *from) {
+        const int at_p = CP::template place<true>(wm0 / STEP), at_q = CQ::template place<false>(wn0 / STEP);
+        auto multiply = [&](const char *from, int left) {
             int pa = at_p, qa = at_q;
             asm("" : "+v"(pa), "+v"(qa));          // its flips are made here, not held in registers over the loop
+            if constexpr (HALF) {
 #pragma unroll
-            for (int s = 0; s < BK / 16; ++s) {
-                uint32x4 p[MT], q[NTL];
+                for (int s = 0; s < BK / 16; ++s) {
+                    uint32x4 p[MT], q[NTL];
 #pragma unroll
-                for (int j = 0; j < NTL; ++j) q[j] = CQ::frag(from + CP::BYTES, qa, j, s);
+                    for (int j = 0; j < NTL; ++j) q[j] = CQ::frag(from + CP::BYTES, qa, j, s);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) p[i] = CP::frag(from, pa, i, s);
+                    for (int i = 0; i < MT; ++i) p[i] = CP::frag(from, pa, i, s);
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < NTL; ++j) acc[i][j] = mma(p[i], q[j], acc[i][j], T());
+                        for (int j = 0; j < NTL; ++j) acc[i][j] = mma(p[i], q[j], acc[i][j], T());
+                }
+            } else {
+                constexpr int CH = 16 / sizeof(T);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (s == 0 || left > BK / 2) {
+                    T p[MT][CH], q[NTL][CH];
+#pragma unroll
+                    for (int j = 0; j < NTL; ++j) CQ::frag_wide(from + CP::BYTES, qa, j, s, q[j]);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) CP::frag_wide(from, pa, i, s, p[i]);
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int j = 0; j < NTL; ++j) acc[i][j] = mma(p[i][c], q[j][c], acc[i][j]);
+                    }
+                }
             }
         };
         // One step: its tile is there once all but the later tiles' copies are.
@@ -681,7 +785,7 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 128 && BK == 32 ? 3 : 2) void ti
             if (NB > 2 && !IDX && k + BK < kend) copies_done<(NB - 2) * EACH>();
             else copies_done<0>();
             if (k + (NB - 1) * BK < kend) start(to, k + (NB - 1) * BK);
-            multiply(from);
+            multiply(from, kend - k);
         };
         // The same where that tile's copies, and the next's, are whole.
         auto copy = [&](char *to, int k) {
@@ -692,7 +796,7 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 128 && BK == 32 ? 3 : 2) void ti
         auto steady = [&](const char *from, char *to, int k) {
             copies_done<IDX ? 0 : (NB - 2) * EACH>();
             copy(to, k + (NB - 1) * BK);
-            multiply(from);
+            multiply(from, BK);
         };
         char *const last = NB == 2 ? lds1 : lds2;
         int k = k0;
@@ -722,45 +826,64 @@ __global__ __launch_bounds__(WM *WN * 64, BM == 128 && BK == 32 ? 3 : 2) void ti
         }
     }
     __syncthreads();
-    // Lane l holds m = 8 q + 4 (l / 32) .. + 3 of column l % 32 in its values 4 q .. + 3.
     auto put = [&](int run, char *to) {
         const int lane = threadIdx.x & 63;
-        if ((lane >> 4 & 1) != (run & 1)) return;
+        if constexpr (HALF) {
+            // Lane l holds m = 8 q + 4 (l / 32) .. + 3 of column l % 32 in its values 4 q .. + 3.
+            if ((lane >> 4 & 1) != (run & 1)) return;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float v[4];
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][run / 2][4 * q + e];
-                __builtin_memcpy(to + SumRows<float, TM>::at(lane & 15, 8 * i + 2 * q + (lane >> 5)), v, 16);
-            }
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][run / 2][4 * q + e];
+                    __builtin_memcpy(to + SumRows<A, TM>::at(lane & 15, 8 * i + 2 * q + (lane >> 5)), v, 16);
+                }
+        } else {
+            put_rows<A, MT, NTL, TM>(acc, run, to);
+        }
     };
-    finish_tile<T, KSUM, TM, 2 * NTL>(a, lds0, group, n0 + wn0, nend, m0 + wm0, put, [](int run, int r) { return 16 * run + r; });
+    finish_tile<T, KSUM, TM, TN / 16>(a, lds0, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
 }
 
-// Adds the split partial sums in order and ends as the kernel above would.
-template <typename T, bool KSUM>
+// Adds the split partial sums and ends as the kernels above would.  256 threads are
+// 256/LANES items of 4 values by LANES shares of the splits, each share added in
+// order and then the shares in theirs.
+template <typename T, bool KSUM, int LANES>
 __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
 {
     using A = typename Elem<T>::Acc;
-    constexpr int V = 4;
+    constexpr int V = 4, ITEMS = 256 / LANES;
+    __shared__ A s_sum[LANES > 1 ? LANES : 1][ITEMS][V];
     const int64_t per = (a.m + V - 1) / V;
     const int64_t rows = KSUM && a.offsets ? a.n * a.groups : a.n;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= rows * per) return;
-    const int64_t pr = at / per, m = (at - pr * per) * V;
+    const int item = threadIdx.x % ITEMS, share = threadIdx.x / ITEMS;
+    const int64_t at = (int64_t)blockIdx.x * ITEMS + item;
+    const bool live = at < rows * per;
+    const int64_t pr = live ? at / per : 0, m = live ? (at - pr * per) * V : 0;
     A s[V] = {0, 0, 0, 0};
-    const A *p = (const A *)a.part + pr * a.m + m;
-    for (int q = 0; q < a.split; ++q, p += rows * a.m) {
-        A t[V] = {0, 0, 0, 0};
-        if (m + V <= a.m) load_vec<V>(p, t);
-        else
-            for (int e = 0; e < V; ++e)
-                if (m + e < a.m) t[e] = p[e];
+    if (live) {
+        const A *p = (const A *)a.part + (share * rows + pr) * a.m + m;
+#pragma unroll 4
+        for (int q = share; q < a.split; q += LANES, p += LANES * rows * a.m) {
+            A t[V];
+            load_some<V>(p, a.m - m, t);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[e] += t[e];
+            for (int e = 0; e < V; ++e) s[e] += t[e];
+        }
     }
+    if constexpr (LANES > 1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s_sum[share][item][e] = s[e];
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (int q = 1; q < LANES; ++q)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += s_sum[q][item][e];
+    }
+    if (!live) return;
     TileArgs b = a;
     int group = 0;
     int64_t n = pr;
@@ -779,24 +902,31 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
     } else {
         b.groups = 1;
     }
-    T bias[V];
+    T bias[V], res[V];
     load_bias<V>(b, group, m, bias);
-    finish<V, T, A>(b, bias, a.crow ? (int64_t)a.crow[n] : n, m, s);
+    const int64_t row = a.crow ? (int64_t)a.crow[n] : n;
+    if (a.R) load_some<V>((const T *)a.R + row * a.ldr + m, a.m - m, res);
+    finish<V, T, A>(b, bias, res, row, m, s);
 }
 
 // ------------------------------------------------------------------- host
 
 struct TileShape { int bm, bn; };
-enum { REG_128, REG_32, REG_16, COPY_256, COPY_TALL, COPY_128 };
-constexpr TileShape TILE_SHAPES[] = {{128, 128}, {128, 32}, {128, 16}, {256, 256}, {256, 128}, {128, 128}};
+enum { REG_128, REG_32, REG_16, COPY_256, COPY_TALL, COPY_128, REG_M112, REG_M96, REG_M80, REG_M64,
+       COPY_M112, COPY_M96, COPY_M80, COPY_M64 };
+constexpr TileShape TILE_SHAPES[] = {{128, 128}, {128, 32}, {128, 16}, {256, 256}, {256, 128}, {128, 128},
+                                     {112, 128}, {96, 128}, {80, 128}, {64, 128},
+                                     {112, 128}, {96, 128}, {80, 128}, {64, 128}};
 
 // Whether every chunk that a copy reads lies whole in the operands, 16 bytes aligned.
-inline bool copies_fit(const TileArgs &a, bool pkc, bool qkc)
+template <typename T>
+bool copies_fit(const TileArgs &a, bool pkc, bool qkc)
 {
-    const uintptr_t bits = (uintptr_t)a.P | (uintptr_t)a.Q | (uintptr_t)(a.ldp * 2) | (uintptr_t)(a.ldq * 2) |
-                           (uintptr_t)(a.gp * 2) | (uintptr_t)(a.gq * 2);
+    const int64_t z = sizeof(T);
+    const uintptr_t bits = (uintptr_t)a.P | (uintptr_t)a.Q | (uintptr_t)(a.ldp * z) | (uintptr_t)(a.ldq * z) |
+                           (uintptr_t)(a.gp * z) | (uintptr_t)(a.gq * z);
     const int64_t k = pkc || qkc ? a.k : 0, m = pkc ? 0 : a.m, n = qkc ? 0 : a.n;
-    return (bits & 15) == 0 && (k | m | n) % 8 == 0 && a.ldp < (1 << 22) && a.ldq < (1 << 22);
+    return (bits & 15) == 0 && (k | m | n) * z % 16 == 0 && a.ldp < (1 << 22) && a.ldq < (1 << 22);
 }
 
 template <typename T>
@@ -818,9 +948,21 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
     int s = REG_128;
     if (!ksum && share <= 16) s = REG_16;
     else if (!ksum && share <= 48) s = REG_32;
-    else if (sizeof(T) == 2 && copies_fit(*a, pkc, qkc)) {
-        if (!ksum && tiles(COPY_256) >= 512) s = COPY_256;
+    else if (sizeof(T) == 2 && copies_fit<T>(*a, pkc, qkc)) {
+        if (!ksum && (!a->offsets || share >= 1024) && tiles(COPY_256) >= 512) s = COPY_256;
         else s = tiles(COPY_TALL) >= 512 ? COPY_TALL : COPY_128;
+    }
+    if (sizeof(T) == 4 && s == REG_128) {
+        const bool fit = copies_fit<T>(*a, pkc, qkc);
+        if (ksum) {
+            s = fit ? COPY_128 : REG_128;
+        } else {
+            const int64_t each = (a->m + (a->m + 127) / 128 - 1) / ((a->m + 127) / 128);
+            const int over = each <= 64 ? 0 : each <= 80 ? 1 : each <= 96 ? 2 : each <= 112 ? 3 : 4;
+            const int reg[] = {REG_M64, REG_M80, REG_M96, REG_M112, REG_128};
+            const int copy[] = {COPY_M64, COPY_M80, COPY_M96, COPY_M112, COPY_128};
+            s = fit ? copy[over] : reg[over];
+        }
     }
     const int64_t count = tiles(s);
     // k is cut where fewer tiles than two a CU would run, into pieces of 4 steps at least.
@@ -829,7 +971,8 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
     if (count < 512) {
         split = (512 + count - 1) / count;
         if (split > k / (4 * BK)) split = k / (4 * BK);
-        if (split > 64) split = 64;
+        const int64_t most = ((int64_t)1 << 28) / (a->n * a->m * batch * (int64_t)sizeof(typename Elem<T>::Acc));   // 256 MB of sums
+        if (split > most) split = most;
         if (split < 1) split = 1;
     }
     a->split = (int)split;
@@ -837,23 +980,26 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
     *part_bytes = split > 1 ? (size_t)split * a->n * a->m * batch * sizeof(typename Elem<T>::Acc) : 0;
 }
 
+// The workgroups that find_work counts on.
+inline unsigned work_groups(const TileArgs &a, bool ksum)
+{
+    const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.split * (ksum && a.offsets ? a.groups : 1);
+    return (unsigned)(((total + NUM_XCD - 1) / NUM_XCD + (a.offsets && !ksum ? 1 : 0)) * NUM_XCD);
+}
+
 template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, bool IDX>
 int launch_shape(const TileArgs &a, hipStream_t s)
 {
-    const int64_t per = ((int64_t)a.tiles_m * a.tiles_n + NUM_XCD - 1) / NUM_XCD;
-    const unsigned z = !PKC && !QKC && a.offsets ? (unsigned)a.groups : 1u;
     hipLaunchKernelGGL((tile_product_kernel<T, PKC, QKC, BM, BN, WM, WN, IDX>),
-                       dim3((unsigned)(per * NUM_XCD), (unsigned)a.split, z), dim3(WM * WN * 64), 0, s, a);
+                       dim3(work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("tile_product_kernel");
 }
 
 template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB, bool IDX>
 int launch_copies(const TileArgs &a, hipStream_t s)
 {
-    const int64_t per = ((int64_t)a.tiles_m * a.tiles_n + NUM_XCD - 1) / NUM_XCD;
-    const unsigned z = !PKC && !QKC && a.offsets ? (unsigned)a.groups : 1u;
     hipLaunchKernelGGL((tile_copy_kernel<T, PKC, QKC, BM, BN, WM, WN, BK, NB, IDX>),
-                       dim3((unsigned)(per * NUM_XCD), (unsigned)a.split, z), dim3(WM * WN * 64), 0, s, a);
+                       dim3(work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("tile_copy_kernel");
 }
 
@@ -871,6 +1017,17 @@ int launch_columns(const TileArgs &a, int shape, hipStream_t s)
         case REG_32: return launch_shape<T, PKC, true, 128, 32, 2, 2, false>(a, s);
         case REG_16: return launch_shape<T, PKC, true, 128, 16, 2, 1, false>(a, s);
         }
+    if constexpr (sizeof(T) == 4) switch (shape) {
+        case REG_M112: return launch_shape<T, PKC, true, 112, 128, 1, 4, false>(a, s);
+        case REG_M96: return launch_shape<T, PKC, true, 96, 128, 1, 4, false>(a, s);
+        case REG_M80: return launch_shape<T, PKC, true, 80, 128, 1, 4, false>(a, s);
+        case REG_M64: return launch_shape<T, PKC, true, 64, 128, 1, 4, false>(a, s);
+        case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 32, 2, false>(a, s);
+        case COPY_M112: return launch_copies<T, PKC, true, 112, 128, 1, 4, 32, 2, false>(a, s);
+        case COPY_M96: return launch_copies<T, PKC, true, 96, 128, 1, 4, 32, 2, false>(a, s);
+        case COPY_M80: return launch_copies<T, PKC, true, 80, 128, 1, 4, 32, 2, false>(a, s);
+        case COPY_M64: return launch_copies<T, PKC, true, 64, 128, 1, 4, 32, 2, false>(a, s);
+        }
     return launch_shape<T, PKC, true, 128, 128, 2, 2, false>(a, s);
 }
 
@@ -881,6 +1038,8 @@ int launch_sums(const TileArgs &a, int shape, hipStream_t s)
         if (shape == COPY_TALL) return launch_copies<T, false, false, 256, 128, 2, 2, 32, 3, IDX>(a, s);
         if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 3, IDX>(a, s);
     }
+    if constexpr (sizeof(T) == 4)
+        if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 2, IDX>(a, s);
     return launch_shape<T, false, false, 128, 128, 2, 2, IDX>(a, s);
 }
 
@@ -891,13 +1050,19 @@ int launch_tile_product(const TileArgs &args, bool pkc, bool qkc, int shape, hip
     if (a.split == 1) a.part = nullptr;
     const bool ksum = !pkc && !qkc;
     int st;
+    if ((int64_t)a.tiles_m * a.tiles_n * a.split * (ksum && a.offsets ? a.groups : 1) >= (int64_t)1 << 23)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: a product of %d x %d tiles is more than one launch takes", a.tiles_m,
+                    a.tiles_n);
     if (ksum) st = a.prow || a.qrow ? launch_sums<T, true>(a, shape, s) : launch_sums<T, false>(a, shape, s);
     else st = pkc ? launch_columns<T, true>(a, shape, s) : launch_columns<T, false>(a, shape, s);
     if (st || a.split == 1) return st;
     const int64_t rows = a.n * (ksum && a.offsets ? a.groups : 1), items = rows * ((a.m + 3) / 4);
-    const dim3 grid((unsigned)((items + 255) / 256));
-    if (ksum) hipLaunchKernelGGL((split_reduce_kernel<T, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((split_reduce_kernel<T, false>), grid, dim3(256), 0, s, a);
+    const bool shares = a.split > 16;
+    const dim3 grid((unsigned)((items + (shares ? 15 : 255)) / (shares ? 16 : 256)));
+    if (ksum && shares) hipLaunchKernelGGL((split_reduce_kernel<T, true, 16>), grid, dim3(256), 0, s, a);
+    else if (ksum) hipLaunchKernelGGL((split_reduce_kernel<T, true, 1>), grid, dim3(256), 0, s, a);
+    else if (shares) hipLaunchKernelGGL((split_reduce_kernel<T, false, 16>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((split_reduce_kernel<T, false, 1>), grid, dim3(256), 0, s, a);
     return check_launch("split_reduce_kernel");
 }
 
