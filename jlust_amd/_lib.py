@@ -203,6 +203,17 @@ def stream_handle(dev: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of device `index` as an address."""
+    if _RAW_STREAM is not None:
+        return _RAW_STREAM(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def current_device() -> int:
+    return _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
+
+
 def on_device(dev: torch.device):
     """torch.cuda.device(dev), or no guard when dev is already current."""
     if _CUR_DEVICE is not None and dev.index is not None and _CUR_DEVICE() == dev.index:

@@ -15,7 +15,7 @@
 namespace jlust {
 namespace {
 
-constexpr int64_t LN_BLOCKS = 1024;            // workgroups of the kernels that walk over columns
+constexpr int64_t LN_BLOCKS = 2048;            // workgroups that walk over the columns, forward
 
 template <typename A>
 __device__ __forceinline__ A inv_sqrt(A v)
@@ -49,16 +49,38 @@ __device__ __forceinline__ void column_sum(A (&v)[K], A *lds)
     }
 }
 
-// Chunk i of this lane: elements [at, at + CH) of a column of d.
+// A chunk as it lies in memory (zeros past the column's end), and its values.
+template <typename T>
+__device__ __forceinline__ uint32x4 read_raw(const T *p, int64_t left)
+{
+    constexpr int CH = 16 / sizeof(T);
+    const uint32x4 zero = {0, 0, 0, 0};
+    return left >= CH ? load_chunk(p) : left > 0 ? load_chunk_part(p, left) : zero;
+}
+
 template <typename T, typename A>
-__device__ __forceinline__ void read_chunk(const T *p, int64_t left, A (&f)[16 / sizeof(T)])
+__device__ __forceinline__ void values(uint32x4 v, A (&f)[16 / sizeof(T)])
 {
     constexpr int CH = 16 / sizeof(T);
     T e[CH];
-    const uint32x4 v = left >= CH ? load_chunk(p) : load_chunk_part(p, left);
     __builtin_memcpy(e, &v, 16);
 #pragma unroll
     for (int j = 0; j < CH; ++j) f[j] = A(e[j]);
+}
+
+// Its values again: without this the compiler keeps those of an earlier pass, two
+// or four times the registers of the packed chunk.
+template <typename T, typename A>
+__device__ __forceinline__ void values_again(uint32x4 &v, A (&f)[16 / sizeof(T)])
+{
+    asm("" : "+v"(v));
+    values<T>(v, f);
+}
+
+template <typename T, typename A>
+__device__ __forceinline__ void read_chunk(const T *p, int64_t left, A (&f)[16 / sizeof(T)])
+{
+    values<T>(read_raw(p, left), f);
 }
 
 template <typename T, typename A>
@@ -77,6 +99,9 @@ __device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 
     }
 }
 
+// Lane l of a column's LANES holds its chunks l, l + LANES, ..., packed as they are
+// read: the few registers leave room for the waves that hide the reads.  weight and
+// bias stay in registers over the columns that a workgroup takes.
 template <typename T, int LANES, int VPL>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_kernel(
     int64_t d, int64_t cols, const T *X, int64_t ldx, const T *__restrict__ weight, const T *__restrict__ bias,
@@ -87,21 +112,28 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_kernel(
     __shared__ A s_red[NT / 64];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const A len = A(d);                            // divided by: a constant column's mean is exact
+    uint32x4 w[VPL], b[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int64_t at = (int64_t)(lane + LANES * i) * CH;
+        w[i] = read_raw(weight + at, weight ? d - at : 0);
+        b[i] = read_raw(bias + at, bias ? d - at : 0);
+    }
     for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < cols; c0 += (int64_t)gridDim.x * COLS) {
         const int64_t c = c0 + sub;
         const bool live = c < cols;
-        A x[VPL][CH], sum[1] = {A(0)};
+        uint32x4 x[VPL];
+        A f[CH], sum[1] = {A(0)};
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int64_t at = (int64_t)(lane + LANES * i) * CH;
-            if (live && at < d) {
-                read_chunk(X + c * ldx + at, d - at, x[i]);
-            } else {
+            x[i] = read_raw(X + c * ldx + at, live ? d - at : 0);
+        }
 #pragma unroll
-                for (int j = 0; j < CH; ++j) x[i][j] = A(0);
-            }
+        for (int i = 0; i < VPL; ++i) {
+            values<T>(x[i], f);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) sum[0] += x[i][j];
+            for (int j = 0; j < CH; ++j) sum[0] += f[j];
         }
         column_sum<LANES>(sum, s_red);
         const A mean = sum[0] / len;
@@ -109,11 +141,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_kernel(
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int64_t left = d - (int64_t)(lane + LANES * i) * CH;
+            values_again<T>(x[i], f);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                x[i][j] -= mean;
-                if (j < left) sq[0] += x[i][j] * x[i][j];
-            }
+            for (int j = 0; j < CH; ++j)
+                if (j < left) sq[0] += (f[j] - mean) * (f[j] - mean);
         }
         column_sum<LANES>(sq, s_red);
         const A rstd = inv_sqrt(sq[0] / len + eps);
@@ -126,20 +157,21 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_kernel(
         for (int i = 0; i < VPL; ++i) {
             const int64_t at = (int64_t)(lane + LANES * i) * CH, left = d - at;
             if (left <= 0) continue;
-            A w[CH];
+            A v[CH];
+            values_again<T>(x[i], f);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) x[i][j] *= rstd;
+            for (int j = 0; j < CH; ++j) f[j] = (f[j] - mean) * rstd;
             if (weight) {
-                read_chunk(weight + at, left, w);
+                values_again<T>(w[i], v);
 #pragma unroll
-                for (int j = 0; j < CH; ++j) x[i][j] *= w[j];
+                for (int j = 0; j < CH; ++j) f[j] *= v[j];
             }
             if (bias) {
-                read_chunk(bias + at, left, w);
+                values_again<T>(b[i], v);
 #pragma unroll
-                for (int j = 0; j < CH; ++j) x[i][j] += w[j];
+                for (int j = 0; j < CH; ++j) f[j] += v[j];
             }
-            write_chunk(Y + c * ldy + at, left, x[i]);
+            write_chunk(Y + c * ldy + at, left, f);
         }
     }
 }
@@ -217,51 +249,60 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_grad_ker
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
         for (int j = 0; j < CH; ++j) dw[i][j] = db[i][j] = A(0);
+    uint32x4 w[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int64_t at = (int64_t)(lane + LANES * i) * CH;
+        w[i] = read_raw(weight + at, weight ? d - at : 0);
+    }
     for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < cols; c0 += (int64_t)gridDim.x * COLS) {
         const int64_t c = c0 + sub;
         const bool live = c < cols;
         const A mean = live ? stats[c * lds_] : A(0), rstd = live ? stats[c * lds_ + 1] : A(0);
-        A h[VPL][CH], g[VPL][CH], sum[2] = {A(0), A(0)};
+        uint32x4 x[VPL], y[VPL];
+        A sum[2] = {A(0), A(0)};
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int64_t at = (int64_t)(lane + LANES * i) * CH, left = d - at;
-            if (live && left > 0) {
-                read_chunk(X + c * ldx + at, left, h[i]);
-                read_chunk(dY + c * lddy + at, left, g[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < CH; ++j) h[i][j] = g[i][j] = A(0);
-            }
+            const int64_t at = (int64_t)(lane + LANES * i) * CH, left = live ? d - at : 0;
+            x[i] = read_raw(X + c * ldx + at, left);
+            y[i] = read_raw(dY + c * lddy + at, left);
         }
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int64_t at = (int64_t)(lane + LANES * i) * CH, left = d - at;
-            if (!live || left <= 0) continue;
-            A w[CH];
-            if (weight) read_chunk(weight + at, left, w);
+            const int64_t left = live ? d - (int64_t)(lane + LANES * i) * CH : 0;
+            A h[CH], g[CH], v[CH];
+            values<T>(x[i], h);
+            values<T>(y[i], g);
+            if (weight) values_again<T>(w[i], v);
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
-                h[i][j] = (h[i][j] - mean) * rstd;
-                dw[i][j] += g[i][j] * h[i][j];
-                db[i][j] += g[i][j];
-                if (weight) g[i][j] *= w[j];
-                if (j < left) {
-                    sum[0] += g[i][j];
-                    sum[1] += g[i][j] * h[i][j];
-                }
+                if (j >= left) continue;
+                h[j] = (h[j] - mean) * rstd;
+                dw[i][j] += g[j] * h[j];
+                db[i][j] += g[j];
+                if (weight) g[j] *= v[j];
+                sum[0] += g[j];
+                sum[1] += g[j] * h[j];
             }
         }
         if (!dX) continue;
         column_sum<LANES>(sum, s_red);
         if (!live) continue;
-        const A a = sum[0] / len, b = sum[1] / len;
+        const A m0 = sum[0] / len, m1 = sum[1] / len;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int64_t at = (int64_t)(lane + LANES * i) * CH, left = d - at;
             if (left <= 0) continue;
+            A h[CH], g[CH], v[CH];
+            values_again<T>(x[i], h);
+            values_again<T>(y[i], g);
+            if (weight) values_again<T>(w[i], v);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) g[i][j] = rstd * (g[i][j] - a - h[i][j] * b);
-            write_chunk(dX + c * lddx + at, left, g[i]);
+            for (int j = 0; j < CH; ++j) {
+                if (weight) g[j] *= v[j];
+                g[j] = rstd * (g[j] - m0 - (h[j] - mean) * rstd * m1);
+            }
+            write_chunk(dX + c * lddx + at, left, g);
         }
     }
     if (!parts) return;
@@ -399,7 +440,7 @@ __global__ __launch_bounds__(1024) void layer_norm_parts_kernel(int64_t d, int64
 // false if it is too long for the registers.
 template <int L, int V> struct Span { static constexpr int lanes = L, vpl = V; };
 
-template <typename T, typename F>
+template <bool GRAD, typename T, typename F>
 bool by_span(int64_t d, F &&f)
 {
     const int64_t chunks = (d * (int64_t)sizeof(T) + 15) / 16;
@@ -407,10 +448,10 @@ bool by_span(int64_t d, F &&f)
     else if (chunks <= 32) f(Span<32, 1>());
     else if (chunks <= 64) f(Span<64, 1>());
     else if (chunks <= 128) f(Span<64, 2>());
-    else if (chunks <= 256) f(Span<256, 1>());
-    else if (chunks <= 512) f(Span<256, 2>());
-    else if (chunks <= 1024) f(Span<512, 2>());
-    else if (chunks <= 2048) f(Span<1024, 2>());
+    else if (chunks <= 256) f(Span<64, 4>());
+    else if (chunks <= 512) f(Span<GRAD ? 256 : 64, GRAD ? 2 : 8>());
+    else if (chunks <= 1024) f(Span<256, 4>());
+    else if (chunks <= 2048) f(Span<512, 4>());
     else return false;
     return true;
 }
@@ -420,10 +461,10 @@ int layer_norm(int64_t d, int64_t cols, const void *X, int64_t ldx, const void *
                int64_t ldy, void *stats, int64_t lds, hipStream_t s)
 {
     using A = typename Elem<T>::Acc;
-    const bool held = by_span<T>(d, [&](auto span) {
+    const bool held = by_span<false, T>(d, [&](auto span) {
         constexpr int L = decltype(span)::lanes, V = decltype(span)::vpl, NT = L > 256 ? L : 256;
         const int64_t blocks = (cols + NT / L - 1) / (NT / L);
-        hipLaunchKernelGGL((layer_norm_kernel<T, L, V>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(NT), 0, s, d, cols,
+        hipLaunchKernelGGL((layer_norm_kernel<T, L, V>), dim3((unsigned)(blocks < LN_BLOCKS ? blocks : LN_BLOCKS)), dim3(NT), 0, s, d, cols,
                            (const T *)X, ldx, (const T *)weight, (const T *)bias, (A)eps, (T *)Y, ldy, (A *)stats, lds);
     });
     if (!held)
@@ -447,10 +488,14 @@ int layer_norm_grad(int64_t d, int64_t cols, const void *X, int64_t ldx, const v
         if (sums && n) st = scratch(stream, sizeof(A) * 2 * d * n, &ws);
         return st;
     };
-    const bool held = by_span<T>(d, [&](auto span) {
+    const bool held = by_span<true, T>(d, [&](auto span) {
         constexpr int L = decltype(span)::lanes, V = decltype(span)::vpl, NT = L > 256 ? L : 256;
         int64_t blocks = (cols + NT / L - 1) / (NT / L);
-        if (blocks > LN_BLOCKS) blocks = LN_BLOCKS;
+        // As many as the CUs hold: each adds a share of 2 d sums to write and read
+        // (9,001 x 2,047 half: 43 us with 512, 51 with 1,024, 62 with 2,048; 200,003 x
+        // 100 Float32: 75, 51, 58).
+        const int64_t most = V * 16 / (int64_t)sizeof(T) >= 32 ? 512 : 1024;
+        if (blocks > most) blocks = most;
         if (parts(blocks) || !blocks) return;
         hipLaunchKernelGGL((layer_norm_grad_kernel<T, L, V>), dim3((unsigned)blocks), dim3(NT), 0, s, d, cols, (const T *)X, ldx,
                            (const T *)dY, lddy, (const A *)stats, lds, (const T *)weight, (T *)dX, lddx, (A *)ws);
@@ -459,7 +504,7 @@ int layer_norm_grad(int64_t d, int64_t cols, const void *X, int64_t ldx, const v
     if (!held && cols) {
         if (sums) {                                // before dX, which may be dY
             const int64_t span = 256 * 16 / (int64_t)sizeof(T), blocks_d = (d + span - 1) / span;
-            int64_t per = (cols * blocks_d + LN_BLOCKS - 1) / LN_BLOCKS;
+            int64_t per = (cols * blocks_d + 1023) / 1024;
             if (per < 16) per = 16;
             if (!parts((cols + per - 1) / per)) {
                 hipLaunchKernelGGL((layer_norm_weight_kernel<T>), dim3((unsigned)blocks_d, (unsigned)count), dim3(256), 0, s, d,

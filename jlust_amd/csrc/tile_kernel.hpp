@@ -911,12 +911,22 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
 
 // ------------------------------------------------------------------- host
 
+// The shapes.  REG_* go through registers at any alignment, COPY_* copy to LDS.
+// 256 x 256 and 256 x 128 carry the large products, 128 x 128 and 64 x 64 what
+// leaves CUs idle in larger tiles, 128 x 32 and 128 x 16 few columns.  Float32's
+// matrix steps bound it, so its widths of 64 to 128 fit m instead (100 of 128 rows
+// would be a fifth of the steps for nothing) at 64 columns, where a CU holds
+// enough workgroups to hide the rows it reads and stores.
 struct TileShape { int bm, bn; };
-enum { REG_128, REG_32, REG_16, COPY_256, COPY_TALL, COPY_128, REG_M112, REG_M96, REG_M80, REG_M64,
-       COPY_M112, COPY_M96, COPY_M80, COPY_M64 };
-constexpr TileShape TILE_SHAPES[] = {{128, 128}, {128, 32}, {128, 16}, {256, 256}, {256, 128}, {128, 128},
-                                     {112, 128}, {96, 128}, {80, 128}, {64, 128},
-                                     {112, 128}, {96, 128}, {80, 128}, {64, 128}};
+enum Shape { REG_128, REG_32, REG_16, REG_M128, REG_M112, REG_M96, REG_M80, REG_M64, COPY_256, COPY_TALL, COPY_128 };
+constexpr TileShape TILE_SHAPES[] = {{128, 128}, {128, 32}, {128, 16}, {128, 64}, {112, 64}, {96, 64}, {80, 64}, {64, 64},
+                                     {256, 256}, {256, 128}, {128, 128}};
+
+// What a shape costs: its rate with a CU full of it (Tflop/s a CU), the time of 64 of
+// k where latency bounds it (us), workgroups a CU.  Measured on products of 64 to
+// 8,192 columns and 512 to 8,192 rows and k; the estimate below picks within 10 %
+// of the best of them but for three (up to 20 %).
+struct ShapeCost { Shape shape; double rate, latency; int held; };
 
 // Whether every chunk that a copy reads lies whole in the operands, 16 bytes aligned.
 template <typename T>
@@ -932,52 +942,80 @@ bool copies_fit(const TileArgs &a, bool pkc, bool qkc)
 template <typename T>
 void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes)
 {
-    constexpr int64_t BK = 128 / sizeof(T);
-    const bool ksum = !pkc && !qkc;
+    const bool ksum = !pkc && !qkc, grouped = a->offsets && !ksum;
     const int64_t batch = ksum && a->offsets ? a->groups : 1;
+    const int64_t runs = grouped ? (a->groups < a->n ? a->groups : a->n) : 0;
+    // Columns that share a matrix, and k of one sum, on average.
+    const int64_t share = grouped ? (a->n + a->groups - 1) / a->groups : a->n;
+    const int64_t k = ksum && a->offsets ? (a->k + a->groups - 1) / a->groups : a->k;
+    const int64_t sums = a->n * a->m * batch;
+    const bool fit = copies_fit<T>(*a, pkc, qkc);
     auto tiles = [&](int s) {
         const int64_t tm = (a->m + TILE_SHAPES[s].bm - 1) / TILE_SHAPES[s].bm;
-        int64_t tn = (a->n + TILE_SHAPES[s].bn - 1) / TILE_SHAPES[s].bn;
-        if (a->offsets && !ksum) tn += a->groups < a->n ? a->groups : a->n;   // every group's last run may be short
-        a->tiles_m = (int)tm;
-        a->tiles_n = (int)tn;
-        return tm * tn * batch;
+        const int64_t tn = (a->n + TILE_SHAPES[s].bn - 1) / TILE_SHAPES[s].bn;
+        return tm * (tn + runs / 2) * batch;           // half the groups' last runs short, on average
     };
-    // Columns that share a matrix, on average.
-    const int64_t share = a->offsets && !ksum ? (a->n + a->groups - 1) / a->groups : a->n;
-    int s = REG_128;
-    if (!ksum && share <= 16) s = REG_16;
-    else if (!ksum && share <= 48) s = REG_32;
-    else if (sizeof(T) == 2 && copies_fit<T>(*a, pkc, qkc)) {
-        if (!ksum && (!a->offsets || share >= 1024) && tiles(COPY_256) >= 512) s = COPY_256;
-        else s = tiles(COPY_TALL) >= 512 ? COPY_TALL : COPY_128;
-    }
-    if (sizeof(T) == 4 && s == REG_128) {
-        const bool fit = copies_fit<T>(*a, pkc, qkc);
-        if (ksum) {
-            s = fit ? COPY_128 : REG_128;
+
+    ShapeCost some[4];
+    int count = 0;
+    if (!ksum && share <= 48) {
+        some[count++] = share <= 16 ? ShapeCost{REG_16, 1.0, 0.5, 6} : ShapeCost{REG_32, 1.5, 0.5, 5};
+        if (sizeof(T) > 2) some[0].rate = sizeof(T) == 4 ? 0.4 : 0.2, some[0].latency = 1.0;
+    } else if constexpr (sizeof(T) == 2) {
+        // 256 x 256 where there is more than one round of it and columns fill it:
+        // 8,192 columns 2048 -> 8192 with gelu 284 us, 322 by 256 x 128.
+        if (fit && !ksum && (!a->offsets || share >= 1024) && tiles(COPY_256) >= 512 && k > 192) {
+            some[count++] = {COPY_256, 4.5, 1.3, 1};
         } else {
-            const int64_t each = (a->m + (a->m + 127) / 128 - 1) / ((a->m + 127) / 128);
-            const int over = each <= 64 ? 0 : each <= 80 ? 1 : each <= 96 ? 2 : each <= 112 ? 3 : 4;
-            const int reg[] = {REG_M64, REG_M80, REG_M96, REG_M112, REG_128};
-            const int copy[] = {COPY_M64, COPY_M80, COPY_M96, COPY_M112, COPY_128};
-            s = fit ? copy[over] : reg[over];
+            if (fit && k > 192) {
+                some[count++] = {COPY_TALL, 4.5, 0.95, 2};
+                some[count++] = {COPY_128, 4.2, 0.62, 2};
+            } else {
+                some[count++] = {REG_128, 3.1, 0.75, 2};
+            }
+            some[count++] = {REG_M64, 2.2, 0.57, 5};
+        }
+    } else if constexpr (sizeof(T) == 4) {
+        const int64_t each = (a->m + (a->m + 127) / 128 - 1) / ((a->m + 127) / 128);
+        if (ksum || (fit && k > 256 && each > 112)) {
+            some[count++] = fit ? ShapeCost{COPY_128, 0.55, 1.2, 2} : ShapeCost{REG_128, 0.48, 1.4, 2};
+            some[count++] = {REG_M64, 0.45, 1.9, 4};
+        } else {
+            const Shape fits = each <= 64 ? REG_M64 : each <= 80 ? REG_M80 : each <= 96 ? REG_M96 : each <= 112 ? REG_M112 : REG_M128;
+            some[count++] = {fits, 0.48, 1.2, 3};
+        }
+    } else {
+        some[count++] = {REG_128, 0.25, 1.6, 2};
+    }
+
+    // Rounds of workgroups, each its steps of 64 of k; k cut in pieces costs a second
+    // launch and its sums written and read.
+    double best = 0;
+    int best_shape = -1;
+    int64_t split = 1;
+    for (int i = 0; i < count; ++i) {
+        const ShapeCost &o = some[i];
+        const int64_t n = tiles(o.shape);
+        const double work = 2e-6 * 64 * TILE_SHAPES[o.shape].bm * TILE_SHAPES[o.shape].bn / o.rate;
+        for (int64_t p = 1; p == 1 || (p <= k / 128 && p * sums * (int64_t)sizeof(typename Elem<T>::Acc) <= (int64_t)1 << 28); p *= 2) {
+            const int64_t groups = n * p, slots = 256 * o.held;
+            const int64_t held = (groups + 255) / 256 < o.held ? (groups + 255) / 256 : o.held;
+            double rounds = (double)groups / slots;
+            rounds = rounds <= 1 ? 1 : rounds < 3 ? (double)((groups + slots - 1) / slots) : rounds;
+            const double step = held * work > o.latency ? held * work : o.latency;
+            const double us = rounds * ((double)((k + 64 * p - 1) / (64 * p)) * step + 2) + (p > 1 ? 8 + 1e-6 * p * sums : 0);
+            if (best_shape < 0 || us < best) {
+                best = us;
+                best_shape = o.shape;
+                split = p;
+            }
         }
     }
-    const int64_t count = tiles(s);
-    // k is cut where fewer tiles than two a CU would run, into pieces of 4 steps at least.
-    const int64_t k = ksum && a->offsets ? (a->k + a->groups - 1) / a->groups : a->k;
-    int64_t split = 1;
-    if (count < 512) {
-        split = (512 + count - 1) / count;
-        if (split > k / (4 * BK)) split = k / (4 * BK);
-        const int64_t most = ((int64_t)1 << 28) / (a->n * a->m * batch * (int64_t)sizeof(typename Elem<T>::Acc));   // 256 MB of sums
-        if (split > most) split = most;
-        if (split < 1) split = 1;
-    }
+    *shape = best_shape;
     a->split = (int)split;
-    *shape = s;
-    *part_bytes = split > 1 ? (size_t)split * a->n * a->m * batch * sizeof(typename Elem<T>::Acc) : 0;
+    a->tiles_m = (int)((a->m + TILE_SHAPES[best_shape].bm - 1) / TILE_SHAPES[best_shape].bm);
+    a->tiles_n = (int)((a->n + TILE_SHAPES[best_shape].bn - 1) / TILE_SHAPES[best_shape].bn + runs);
+    *part_bytes = split > 1 ? (size_t)split * sums * sizeof(typename Elem<T>::Acc) : 0;
 }
 
 // The workgroups that find_work counts on.
@@ -1010,6 +1048,7 @@ int launch_columns(const TileArgs &a, int shape, hipStream_t s)
         case COPY_256: return launch_copies<T, PKC, true, 256, 256, 2, 4, 64, 2, false>(a, s);
         case COPY_TALL: return launch_copies<T, PKC, true, 256, 128, 2, 2, 32, 3, false>(a, s);
         case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 64, 2, false>(a, s);
+        case REG_M64: return launch_shape<T, PKC, true, 64, 64, 2, 2, false>(a, s);
         case REG_32: return launch_shape<T, PKC, true, 128, 32, 4, 1, false>(a, s);
         case REG_16: return launch_shape<T, PKC, true, 128, 16, 4, 1, false>(a, s);
         }
@@ -1018,15 +1057,12 @@ int launch_columns(const TileArgs &a, int shape, hipStream_t s)
         case REG_16: return launch_shape<T, PKC, true, 128, 16, 2, 1, false>(a, s);
         }
     if constexpr (sizeof(T) == 4) switch (shape) {
-        case REG_M112: return launch_shape<T, PKC, true, 112, 128, 1, 4, false>(a, s);
-        case REG_M96: return launch_shape<T, PKC, true, 96, 128, 1, 4, false>(a, s);
-        case REG_M80: return launch_shape<T, PKC, true, 80, 128, 1, 4, false>(a, s);
-        case REG_M64: return launch_shape<T, PKC, true, 64, 128, 1, 4, false>(a, s);
+        case REG_M128: return launch_shape<T, PKC, true, 128, 64, 1, 4, false>(a, s);
+        case REG_M112: return launch_shape<T, PKC, true, 112, 64, 1, 4, false>(a, s);
+        case REG_M96: return launch_shape<T, PKC, true, 96, 64, 1, 4, false>(a, s);
+        case REG_M80: return launch_shape<T, PKC, true, 80, 64, 1, 4, false>(a, s);
+        case REG_M64: return launch_shape<T, PKC, true, 64, 64, 1, 4, false>(a, s);
         case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 32, 2, false>(a, s);
-        case COPY_M112: return launch_copies<T, PKC, true, 112, 128, 1, 4, 32, 2, false>(a, s);
-        case COPY_M96: return launch_copies<T, PKC, true, 96, 128, 1, 4, 32, 2, false>(a, s);
-        case COPY_M80: return launch_copies<T, PKC, true, 80, 128, 1, 4, 32, 2, false>(a, s);
-        case COPY_M64: return launch_copies<T, PKC, true, 64, 128, 1, 4, 32, 2, false>(a, s);
         }
     return launch_shape<T, PKC, true, 128, 128, 2, 2, false>(a, s);
 }
@@ -1040,6 +1076,8 @@ int launch_sums(const TileArgs &a, int shape, hipStream_t s)
     }
     if constexpr (sizeof(T) == 4)
         if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 2, IDX>(a, s);
+    if constexpr (sizeof(T) <= 4)
+        if (shape == REG_M64) return launch_shape<T, false, false, 64, 64, 2, 2, IDX>(a, s);
     return launch_shape<T, false, false, 128, 128, 2, 2, IDX>(a, s);
 }
 

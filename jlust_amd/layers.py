@@ -22,7 +22,7 @@ column.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -36,26 +36,13 @@ from .tensor import OneBased, USTensor
 _BE = HIPBackend()
 _TYPES = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
 _ACTS = (FN_IDENTITY, FN_RELU, FN_GELU, FN_SILU)
-_I32, _I64, _P = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 
 
-class _Linear(ctypes.Structure):
-    """jlust_linear of include/jlust_hip.h."""
-    _fields_ = [("value_type", _I32), ("act", _I32), ("w_layout", _I32), ("reserved", _I32),
-                ("out", _I64), ("inp", _I64), ("cols", _I64),
-                ("W", _P), ("ldw", _I64), ("X", _P), ("ldx", _I64), ("Y", _P), ("ldy", _I64),
-                ("bias", _P), ("R", _P), ("ldr", _I64), ("Z", _P), ("ldz", _I64),
-                ("groups", _I64), ("copies", _I64), ("plan", _P), ("w_stride", _I64), ("bias_stride", _I64)]
-
-
-class _LinearGrad(ctypes.Structure):
-    """jlust_linear_grad of include/jlust_hip.h."""
-    _fields_ = [("value_type", _I32), ("act", _I32), ("w_layout", _I32), ("reserved", _I32),
-                ("out", _I64), ("inp", _I64), ("cols", _I64),
-                ("W", _P), ("ldw", _I64), ("X", _P), ("ldx", _I64), ("dY", _P), ("lddy", _I64),
-                ("Z", _P), ("ldz", _I64), ("dX", _P), ("lddx", _I64), ("dW", _P), ("lddw", _I64), ("dbias", _P),
-                ("groups", _I64), ("copies", _I64), ("plan", _P), ("w_stride", _I64), ("dw_stride", _I64),
-                ("dbias_stride", _I64)]
+# jlust_linear and jlust_linear_grad of include/jlust_hip.h: four 32-bit fields,
+# then 64-bit ones.  Packed bytes cost a third of a ctypes structure, which counts
+# in a call of a few microseconds.
+_LINEAR = struct.Struct("@4i19q").pack
+_LINEAR_GRAD = struct.Struct("@4i22q").pack
 
 
 # --------------------------------------------------------------------- checks
@@ -71,77 +58,91 @@ def _raw(t, name):
     raise TypeError(f"{name}: expected a dense tensor, got {type(t).__name__}")
 
 
-def _first(t, name, dev, T):
-    if T not in _TYPES:
-        raise UnsupportedValueType(T, _BE)
-    if dev.type != "cuda":
-        raise DeviceMismatch(f"HIPBackend needs GPU buffers, {name} is on {dev}")
-    return _TYPES[T]
+def _first(t, name):
+    """(value type, device index) of the call, from its first operand."""
+    vt, index = _TYPES.get(t.dtype), t.get_device()
+    if vt is None:
+        raise UnsupportedValueType(t.dtype, _BE)
+    if index < 0:
+        raise DeviceMismatch(f"HIPBackend needs GPU buffers, {name} is on {t.device}")
+    return vt, index
 
 
-def _same(t, name, dev, T):
+def _same(t, name, index, T):
     if t.dtype != T:
         raise UnsupportedValueType(t.dtype, _BE, f"operands must share the value type {T}; {name} does not")
-    if t.device != dev:
-        raise DeviceMismatch(f"operands on several devices: {name} is on {t.device}, others on {dev}")
+    if t.get_device() != index:
+        raise DeviceMismatch(f"operands on several devices: {name} is on {t.device}, others on cuda:{index}")
 
 
-def _matrix(t, name, rows, cols, dev, T):
+def _matrix(t, name, rows, cols, index, T):
     """(address, leading dimension) of a rows x cols column-major operand, a
     vector standing for one column; None stands for no operand."""
     if t is None:
         return 0, 0
-    t = _raw(t, name)
-    _same(t, name, dev, T)
-    if t.dim() == 1:
-        r, c, s0, ld = t.shape[0], 1, t.stride(0), t.shape[0]
-    elif t.dim() == 2:
-        (r, c), (s0, ld) = t.shape, t.stride()
+    if type(t) is not torch.Tensor:
+        t = _raw(t, name)
+    if t.dtype is not T or t.get_device() != index:
+        _same(t, name, index, T)
+    shape = t.shape
+    if len(shape) == 2:
+        s0, ld = t.stride()
+        if shape[0] == rows and shape[1] == cols and (s0 == 1 or rows <= 1):
+            if cols <= 1:
+                return t.data_ptr(), rows
+            if ld >= rows:
+                return t.data_ptr(), ld
+    elif len(shape) == 1:
+        if cols == 1 and shape[0] == rows and (t.stride(0) == 1 or rows <= 1):
+            return t.data_ptr(), rows
     else:
         raise IncompatibleExtents(f"{name}: {t.dim()}-D arrays are not supported")
-    if r != rows or c != cols:
-        raise IncompatibleExtents(f"{name} is {r}x{c}, expected {rows}x{cols}")
-    if (s0 != 1 and rows > 1) or (ld < rows and cols > 1):
-        raise NonCanonicalStorage(f"{name}: dense matrices are column-major (Julia layout): expected stride(0) == 1 "
-                                  f"and columns apart, got strides {tuple(t.stride())}")
-    return t.data_ptr(), ld if cols > 1 else rows
+    if tuple(shape) != (rows, cols) and not (len(shape) == 1 and cols == 1 and shape[0] == rows):
+        raise IncompatibleExtents(f"{name} is {'x'.join(map(str, shape))}, expected {rows}x{cols}")
+    raise NonCanonicalStorage(f"{name}: dense matrices are column-major (Julia layout): expected stride(0) == 1 "
+                              f"and columns apart, got strides {tuple(t.stride())}")
 
 
 def _extents(t, name):
-    if t.dim() == 2:
-        return t.shape
-    if t.dim() == 1:
-        return t.shape[0], 1
+    shape = t.shape
+    if len(shape) == 2:
+        return shape
+    if len(shape) == 1:
+        return shape[0], 1
     raise IncompatibleExtents(f"{name}: {t.dim()}-D arrays are not supported")
 
 
-def _weights(t, name, groups, dev, T):
+def _weights(t, name, groups, index, T):
     """(address, layout, leading dimension, group stride, out, inp) of a weight
     matrix, or of one per group: contiguous along either side."""
-    _same(t, name, dev, T)
-    if t.dim() != (3 if groups else 2):
+    if t.dtype is not T or t.get_device() != index:
+        _same(t, name, index, T)
+    shape, strides = t.shape, t.stride()
+    if len(shape) != (3 if groups else 2):
         raise IncompatibleExtents(f"{name}: expected {'out x inp x groups' if groups else 'out x inp'}, got "
                                   f"{t.dim()} dimensions")
-    out, inp = t.shape[0], t.shape[1]
-    if groups and t.shape[2] != groups:
-        raise IncompatibleExtents(f"{name} holds {t.shape[2]} matrices, expected {groups}")
-    s0, s1 = t.stride(0), t.stride(1)
+    out, inp = shape[0], shape[1]
+    if groups and shape[2] != groups:
+        raise IncompatibleExtents(f"{name} holds {shape[2]} matrices, expected {groups}")
+    s0, s1 = strides[0], strides[1]
     if (s0 == 1 or out <= 1) and (s1 >= out or inp <= 1) and not (out <= 1 and s1 == 1):
         layout, ld = 0, s1 if inp > 1 else max(out, 1)
     elif (s1 == 1 or inp <= 1) and (s0 >= inp or out <= 1):
         layout, ld = 1, s0 if out > 1 else max(inp, 1)
     else:
         raise NonCanonicalStorage(f"{name}: a matrix is column-major or the transpose of one, got strides "
-                                  f"{tuple(t.stride())}")
-    return t.data_ptr(), layout, ld, t.stride(2) if groups else 0, out, inp
+                                  f"{strides}")
+    return t.data_ptr(), layout, ld, strides[2] if groups else 0, out, inp
 
 
-def _bias(t, name, out, groups, dev, T):
+def _bias(t, name, out, groups, index, T):
     """(address, stride between groups)."""
     if t is None:
         return 0, 0
-    t = _raw(t, name)
-    _same(t, name, dev, T)
+    if type(t) is not torch.Tensor:
+        t = _raw(t, name)
+    if t.dtype is not T or t.get_device() != index:
+        _same(t, name, index, T)
     if tuple(t.shape) != ((out, groups) if groups else (out,)):
         raise IncompatibleExtents(f"{name} is {tuple(t.shape)}, expected {(out, groups) if groups else (out,)}")
     if out > 1 and t.stride(0) != 1:
@@ -180,9 +181,9 @@ class GroupPlan(AbstractKernelHandle):
         if n_groups is None:
             raise TypeError("prepare(GroupedLinearOp, ids): n_groups is needed")
         ids = _raw(ids, "ids")
-        self.shape = tuple(ids.shape)
+        self.shape = ids.shape
         self.groups, self.origin = int(n_groups), (OneBased() if origin is None else origin).offset
-        self.dev, self.n = ids.device, ids.numel()
+        self.dev, self.index, self.n = ids.device, ids.get_device(), ids.numel()
         if ids.dim() == 1:
             self.copies = 1
         elif ids.dim() == 2:
@@ -197,20 +198,17 @@ class GroupPlan(AbstractKernelHandle):
     def _check_ids(self, ids):
         if ids.dtype != torch.int32 and ids.dtype != torch.int64:
             raise UnsupportedIndexType(ids.dtype, _BE)
-        if ids.device.type != "cuda" or ids.device != self.dev:
+        if ids.get_device() != self.index or self.index < 0:
             raise DeviceMismatch(f"HIPBackend needs GPU buffers, ids are on {ids.device}")
-        if tuple(ids.shape) != self.shape:
-            raise IncompatibleExtents(f"ids are {tuple(ids.shape)}, the plan's {self.shape}")
-        if not (ids if ids.dim() == 1 else ids.t()).is_contiguous():
+        if ids.shape != self.shape:
+            raise IncompatibleExtents(f"ids are {tuple(ids.shape)}, the plan's {tuple(self.shape)}")
+        if not (ids if len(self.shape) == 1 else ids.t()).is_contiguous():
             raise NonCanonicalStorage(f"ids must be contiguous columns, got strides {tuple(ids.stride())}")
 
     def _build(self, ids):
-        with _lib.on_device(self.dev):
-            self._stream = _lib.stream_handle(self.dev).value
-            st = _lib.lib().jlust_hip_group_plan_build(
-                self.n, self.groups, self.copies, self.origin, ids.data_ptr(), int(ids.dtype == torch.int64),
-                self._plan.data_ptr(), self._stream)
-        _lib.check(st, "group_plan", None, _BE, ids.dtype)
+        self._stream = _run(_lib.lib().jlust_hip_group_plan_build, self.index, "group_plan", ids.dtype, self.n,
+                            self.groups, self.copies, self.origin, ids.data_ptr(), ids.dtype is torch.int64,
+                            self._plan.data_ptr())
 
     def update(self, ids):
         """New groups for the same columns."""
@@ -219,9 +217,10 @@ class GroupPlan(AbstractKernelHandle):
         self._build(ids)
         return self
 
-    def use(self, stream):
-        """The plan's address, its memory kept until `stream` is done with it."""
-        if stream != self._stream:
+    def use(self):
+        """The plan's address, its memory kept until the current stream is done
+        with it."""
+        if _lib.raw_stream(self.index) != self._stream:
             self._plan.record_stream(torch.cuda.current_stream(self.dev))
         return self._plan.data_ptr()
 
@@ -238,6 +237,20 @@ class GroupPlan(AbstractKernelHandle):
         return _linear(self, W, X, Y, **kw)
 
 
+def _run(f, index, what, T, *args):
+    """f(*args, stream) on the operands' device; returns the stream."""
+    if _lib.current_device() == index:
+        s = _lib.raw_stream(index)
+        st = f(*args, s)
+    else:
+        with torch.cuda.device(index):
+            s = _lib.raw_stream(index)
+            st = f(*args, s)
+    if st:
+        _lib.check(st, what, None, _BE, T)
+    return s
+
+
 def _columns(X, Y, h):
     """Checks the batch against the plan; returns Y's columns."""
     (_, xc), (_, yc) = _extents(X, "X"), _extents(Y, "Y")
@@ -250,79 +263,75 @@ def _columns(X, Y, h):
 
 
 def _linear(h, W, X, Y, bias=None, act=None, residual=None, preact=None):
-    w, x, y = _raw(W, "W"), _raw(X, "X"), _raw(Y, "Y")
-    T, dev = w.dtype, w.device
-    vt, groups = _first(w, "W", dev, T), 0 if h is None else h.groups
-    wp, layout, ldw, ws, out, inp = _weights(w, "W", groups, dev, T)
+    w = W if type(W) is torch.Tensor else _raw(W, "W")
+    x = X if type(X) is torch.Tensor else _raw(X, "X")
+    y = Y if type(Y) is torch.Tensor else _raw(Y, "Y")
+    T = w.dtype
+    vt, index = _first(w, "W")
+    groups, copies, plan = 0, 1, 0
+    if h is not None:
+        if h.index != index:
+            raise DeviceMismatch(f"the plan is on {h.dev}, W on {w.device}")
+        groups, copies, plan = h.groups, h.copies, h.use()
+    wp, layout, ldw, ws, out, inp = _weights(w, "W", groups, index, T)
     n, xc = _columns(x, y, h)
-    xp, ldx = _matrix(x, "X", inp, xc, dev, T)
-    yp, ldy = _matrix(y, "Y", out, n, dev, T)
-    bp, bs = _bias(bias, "bias", out, groups, dev, T)
-    rp, ldr = _matrix(residual, "residual", out, n, dev, T)
-    zp, ldz = _matrix(preact, "preact", out, n, dev, T)
-    if h is not None and h.dev != dev:
-        raise DeviceMismatch(f"the plan is on {h.dev}, W on {dev}")
-    kind = _act(act)
-    with _lib.on_device(dev):
-        s = _lib.stream_handle(dev).value
-        op = _Linear(vt, kind, layout, 0, out, inp, n, wp, ldw, xp, ldx, yp, ldy, bp, rp, ldr, zp, ldz,
-                     groups, 1 if h is None else h.copies, 0 if h is None else h.use(s), ws, bs)
-        st = _lib.lib().jlust_hip_linear(ctypes.byref(op), s)
-    if st:
-        _lib.check(st, "linear", None, _BE, T)
+    xp, ldx = _matrix(x, "X", inp, xc, index, T)
+    yp, ldy = _matrix(y, "Y", out, n, index, T)
+    bp, bs = _bias(bias, "bias", out, groups, index, T) if bias is not None else (0, 0)
+    rp, ldr = _matrix(residual, "residual", out, n, index, T)
+    zp, ldz = _matrix(preact, "preact", out, n, index, T)
+    _run(_lib.lib().jlust_hip_linear, index, "linear", T,
+         _LINEAR(vt, _act(act), layout, 0, out, inp, n, wp, ldw, xp, ldx, yp, ldy, bp, rp, ldr, zp, ldz, groups, copies,
+                 plan, ws, bs))
     return Y
 
 
 def _linear_grad(h, W, X, dY, act=None, preact=None, dX=None, dW=None, dbias=None):
     w, x, dy = _raw(W, "W"), _raw(X, "X"), _raw(dY, "dY")
-    T, dev = w.dtype, w.device
-    vt, groups = _first(w, "W", dev, T), 0 if h is None else h.groups
-    wp, layout, ldw, ws, out, inp = _weights(w, "W", groups, dev, T)
+    T = w.dtype
+    vt, index = _first(w, "W")
+    groups, copies, plan = 0, 1, 0
+    if h is not None:
+        if h.index != index:
+            raise DeviceMismatch(f"the plan is on {h.dev}, W on {w.device}")
+        groups, copies, plan = h.groups, h.copies, h.use()
+    wp, layout, ldw, ws, out, inp = _weights(w, "W", groups, index, T)
     n, xc = _columns(x, dy, h)
     kind = _act(act)
     if kind != FN_IDENTITY and preact is None:
         raise TypeError(f"the gradient of {act!r} needs preact, the pre-activation that the forward call kept")
-    xp, ldx = _matrix(x, "X", inp, xc, dev, T)
-    dyp, lddy = _matrix(dy, "dY", out, n, dev, T)
-    zp, ldz = _matrix(preact, "preact", out, n, dev, T) if kind != FN_IDENTITY else (0, 0)
-    dxp, lddx = _matrix(dX, "dX", inp, xc, dev, T)
+    xp, ldx = _matrix(x, "X", inp, xc, index, T)
+    dyp, lddy = _matrix(dy, "dY", out, n, index, T)
+    zp, ldz = _matrix(preact, "preact", out, n, index, T) if kind != FN_IDENTITY else (0, 0)
+    dxp, lddx = _matrix(dX, "dX", inp, xc, index, T)
     dwp, wlayout, lddw, dws = 0, layout, 0, 0
     if dW is not None:
-        dwp, wlayout, lddw, dws, o, i = _weights(_raw(dW, "dW"), "dW", groups, dev, T)
+        dwp, wlayout, lddw, dws, o, i = _weights(_raw(dW, "dW"), "dW", groups, index, T)
         if (o, i) != (out, inp):
             raise IncompatibleExtents(f"dW is {o}x{i}, expected {out}x{inp}")
         _apart(dws, out * inp, groups, "dW")
-    dbp, dbs = _bias(dbias, "dbias", out, groups, dev, T)
+    dbp, dbs = _bias(dbias, "dbias", out, groups, index, T)
     if dbp:
         _apart(dbs, out, groups, "dbias")
-    if h is not None and h.dev != dev:
-        raise DeviceMismatch(f"the plan is on {h.dev}, W on {dev}")
-    copies = 1 if h is None else h.copies
-    L = _lib.lib()
-    with _lib.on_device(dev):
-        s = _lib.stream_handle(dev).value
-        plan = 0 if h is None else h.use(s)
-        # dW beside dX in one call where they are laid out alike.
-        calls = [(layout, dxp, dwp, dbp)] if wlayout == layout or not (dxp and dwp) else \
-            [(layout, dxp, 0, dbp), (wlayout, 0, dwp, 0)]
-        for lay, a, b, c in calls:
-            if not a:
-                lay = wlayout
-            op = _LinearGrad(vt, kind, lay, 0, out, inp, n, wp, ldw, xp, ldx, dyp, lddy, zp, ldz, a, lddx, b, lddw, c,
-                             groups, copies, plan, ws, dws, dbs)
-            st = L.jlust_hip_linear_grad(ctypes.byref(op), s)
-            if st:
-                _lib.check(st, "linear_grad", None, _BE, T)
+    # dW beside dX in one call where they are laid out alike.
+    calls = [(layout if dxp else wlayout, dxp, dwp, dbp)] if wlayout == layout or not (dxp and dwp) else \
+        [(layout, dxp, 0, dbp), (wlayout, 0, dwp, 0)]
+    for lay, a, b, c in calls:
+        _run(_lib.lib().jlust_hip_linear_grad, index, "linear_grad", T,
+             _LINEAR_GRAD(vt, kind, lay, 0, out, inp, n, wp, ldw, xp, ldx, dyp, lddy, zp, ldz, a, lddx, b, lddw, c, groups,
+                          copies, plan, ws, dws, dbs))
     return dX if dX is not None else dW if dW is not None else dbias
 
 
 # -------------------------------------------------------------- normalisation
 
-def _norm_vector(t, name, d, dev, T):
+def _norm_vector(t, name, d, index, T):
     if t is None:
         return 0
-    t = _raw(t, name)
-    _same(t, name, dev, T)
+    if type(t) is not torch.Tensor:
+        t = _raw(t, name)
+    if t.dtype is not T or t.get_device() != index:
+        _same(t, name, index, T)
     if tuple(t.shape) != (d,):
         raise IncompatibleExtents(f"{name} is {tuple(t.shape)}, expected ({d},)")
     if d > 1 and t.stride(0) != 1:
@@ -331,38 +340,31 @@ def _norm_vector(t, name, d, dev, T):
 
 
 def _layer_norm(X, Y, weight=None, bias=None, eps=1e-5, stats=None):
-    x = _raw(X, "X")
-    T, dev = x.dtype, x.device
-    vt = _first(x, "X", dev, T)
+    x = X if type(X) is torch.Tensor else _raw(X, "X")
+    T = x.dtype
+    vt, index = _first(x, "X")
     d, cols = _extents(x, "X")
-    xp, ldx = _matrix(x, "X", d, cols, dev, T)
-    yp, ldy = _matrix(Y, "Y", d, cols, dev, T)
-    wp, bp = _norm_vector(weight, "weight", d, dev, T), _norm_vector(bias, "bias", d, dev, T)
-    sp, lds = _matrix(stats, "stats", 2, cols, dev, torch.float64 if T == torch.float64 else torch.float32)
-    with _lib.on_device(dev):
-        st = _lib.lib().jlust_hip_layer_norm(vt, d, cols, xp, ldx, wp, bp, float(eps), yp, ldy, sp, lds,
-                                             _lib.stream_handle(dev).value)
-    if st:
-        _lib.check(st, "layer_norm", None, _BE, T)
+    xp, ldx = _matrix(x, "X", d, cols, index, T)
+    yp, ldy = _matrix(Y, "Y", d, cols, index, T)
+    wp, bp = _norm_vector(weight, "weight", d, index, T), _norm_vector(bias, "bias", d, index, T)
+    sp, lds = _matrix(stats, "stats", 2, cols, index, torch.float64 if vt == 0 else torch.float32)
+    _run(_lib.lib().jlust_hip_layer_norm, index, "layer_norm", T, vt, d, cols, xp, ldx, wp, bp, eps, yp, ldy, sp, lds)
     return Y
 
 
 def _layer_norm_grad(X, dY, stats, weight=None, dX=None, dweight=None, dbias=None):
     x = _raw(X, "X")
-    T, dev = x.dtype, x.device
-    vt = _first(x, "X", dev, T)
+    T = x.dtype
+    vt, index = _first(x, "X")
     d, cols = _extents(x, "X")
-    xp, ldx = _matrix(x, "X", d, cols, dev, T)
-    dyp, lddy = _matrix(dY, "dY", d, cols, dev, T)
-    sp, lds = _matrix(stats, "stats", 2, cols, dev, torch.float64 if T == torch.float64 else torch.float32)
-    dxp, lddx = _matrix(dX, "dX", d, cols, dev, T)
-    wp = _norm_vector(weight, "weight", d, dev, T)
-    dwp, dbp = _norm_vector(dweight, "dweight", d, dev, T), _norm_vector(dbias, "dbias", d, dev, T)
-    with _lib.on_device(dev):
-        st = _lib.lib().jlust_hip_layer_norm_grad(vt, d, cols, xp, ldx, dyp, lddy, sp, lds, wp, dxp, lddx, dwp, dbp,
-                                                  _lib.stream_handle(dev).value)
-    if st:
-        _lib.check(st, "layer_norm_grad", None, _BE, T)
+    xp, ldx = _matrix(x, "X", d, cols, index, T)
+    dyp, lddy = _matrix(dY, "dY", d, cols, index, T)
+    sp, lds = _matrix(stats, "stats", 2, cols, index, torch.float64 if vt == 0 else torch.float32)
+    dxp, lddx = _matrix(dX, "dX", d, cols, index, T)
+    wp = _norm_vector(weight, "weight", d, index, T)
+    dwp, dbp = _norm_vector(dweight, "dweight", d, index, T), _norm_vector(dbias, "dbias", d, index, T)
+    _run(_lib.lib().jlust_hip_layer_norm_grad, index, "layer_norm_grad", T, vt, d, cols, xp, ldx, dyp, lddy, sp, lds, wp, dxp,
+         lddx, dwp, dbp)
     return dX if dX is not None else dweight if dweight is not None else dbias
 
 
@@ -374,18 +376,19 @@ def _plan(args, what):
     return args
 
 
-_RUN = {
-    "Linear": lambda args, kw: _linear(None, *args, **kw),
-    "LinearGrad": lambda args, kw: _linear_grad(None, *args, **kw),
-    "GroupedLinear": lambda args, kw: _linear(*_plan(args, "GroupedLinearOp"), **kw),
-    "GroupedLinearGrad": lambda args, kw: _linear_grad(*_plan(args, "GroupedLinearGradOp"), **kw),
-    "LayerNorm": lambda args, kw: _layer_norm(*args, **kw),
-    "LayerNormGrad": lambda args, kw: _layer_norm_grad(*args, **kw),
-}
-
-
 def execute(optype, args, backend, kw):
     """execute(LinearOp, ...) and the others of this module (ops.execute)."""
     if backend is not None and not isinstance(backend, HIPBackend):
         raise UnsupportedFormat(optype.tag, backend, "no such backend in jlust_amd")
-    return _RUN[optype.tag](args, kw)
+    tag = optype.tag
+    if tag == "Linear":
+        return _linear(None, *args, **kw)
+    if tag == "GroupedLinear":
+        return _linear(*_plan(args, "GroupedLinearOp"), **kw)
+    if tag == "LayerNorm":
+        return _layer_norm(*args, **kw)
+    if tag == "LinearGrad":
+        return _linear_grad(None, *args, **kw)
+    if tag == "GroupedLinearGrad":
+        return _linear_grad(*_plan(args, "GroupedLinearGradOp"), **kw)
+    return _layer_norm_grad(*args, **kw)
