@@ -198,6 +198,8 @@ int check_groups(const char *who, int64_t n, int64_t groups, int64_t copies)
     return JLUST_STATUS_SUCCESS;
 }
 
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
 // ------------------------------------------------------- the gradient's first pass
 
 // Runs of rows that one workgroup takes; 256 threads are 32 vectors along m by
@@ -208,8 +210,8 @@ struct Prepass {
 };
 
 // G = dY .* act'(Z) in the order of the groups (row p of G is column perm[p]),
-// rounded to T, and the sums of its unrounded rows over a run of `per` columns:
-// sums[run][m].  dY and Z are read once; G and dbias would each read them again.
+// rounded to T, its rows ldg apart (a whole number of 16 bytes, zeros at their ends),
+// and the sums of its unrounded rows over a run of `per` columns: sums[run][m].  dY and Z are read once; G and dbias would each read them again.
 template <typename T>
 __global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m, const T *__restrict__ dY, int64_t lddy,
                                                            const T *__restrict__ Z, int64_t ldz, int act, T *__restrict__ G,
@@ -251,12 +253,7 @@ __global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m,
                 acc[e] += g;
                 y[e] = T(g);
             }
-            if (G) {
-                if (left >= V) store_vec<V>(G + p * ldg + c, y);
-                else
-                    for (int e = 0; e < V; ++e)
-                        if (e < left) G[p * ldg + c + e] = y[e];
-            }
+            if (G) store_vec<V>(G + p * ldg + c, y);           // zeros past m
         }
     if (!sums) return;
 #pragma unroll
@@ -268,6 +265,63 @@ __global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m,
         for (int q = 0; q < 8; ++q) s += s_sum[q][i];
         if (m0 + i < m) sums[run * m + m0 + i] = s;
     }
+}
+
+// Rows src[idx[p]] (or src[p]) of `len` values for p < rows (or offsets[groups]),
+// 16-byte aligned and `ld` apart, zeros at their ends: what the copies of
+// tile_kernel.hpp take.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(int64_t rows, int64_t len, const T *__restrict__ src, int64_t lds_,
+                                                        int64_t per, int64_t stride, const int32_t *__restrict__ idx,
+                                                        const int32_t *__restrict__ limit, T *__restrict__ out, int64_t ld)
+{
+    constexpr int V = 16 / sizeof(T);
+    const int64_t chunks = ld / V, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= rows * chunks) return;
+    const int64_t p = at / chunks, c = (at - p * chunks) * V, left = len - c;
+    if (limit && p >= *limit) return;
+    const int64_t r = idx ? (int64_t)idx[p] : p;
+    const T *q = src + r / per * stride + r % per * lds_ + c;
+    const uint32x4 v = left >= V ? load_chunk(q) : load_chunk_part(q, left);
+    __builtin_memcpy(out + p * ld + c, &v, 16);
+}
+
+// rows in runs of `per`, `stride` apart (the groups' matrices; else one run).
+template <typename T>
+int pack_rows(int64_t rows, int64_t len, const void *src, int64_t lds, int64_t per, int64_t stride, const int32_t *idx,
+              const int32_t *limit, void *out, int64_t ld, hipStream_t s)
+{
+    const int64_t items = rows * (ld / (16 / (int64_t)sizeof(T)));
+    if (items == 0) return JLUST_STATUS_SUCCESS;
+    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, rows, len, (const T *)src, lds,
+                       per, stride, idx, limit, (T *)out, ld);
+    return check_launch("pack_rows_kernel");
+}
+
+template <typename T>
+int64_t padded(int64_t len)
+{
+    constexpr int64_t V = 16 / sizeof(T);
+    return (len + V - 1) / V * V;
+}
+
+// Whether rows of `len` values can be copied to LDS as they lie.
+template <typename T>
+bool lies_well(const void *p, int64_t len, int64_t ld, int64_t stride)
+{
+    return (((uintptr_t)p | (uintptr_t)(len * sizeof(T)) | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(stride * sizeof(T))) & 15) == 0;
+}
+
+// Whether 16-bit operands of `values` values are better packed first: the product
+// through registers runs at 550 Tflop/s where rows along its sides lie badly and 800
+// where rows along k do, at 1,000 from copies (8,191 columns 2047 -> 8191: 482 and 334
+// us against 257), and packing reads and writes them at 3 TB/s.
+template <typename T>
+bool worth_packing(int64_t m, int64_t n, int64_t k, int64_t values, bool sides)
+{
+    if (sizeof(T) != 2 || values == 0) return false;
+    const double us = 2e-6 * m * n * k * (sides ? 1 / 550.0 - 1 / 1000.0 : 1 / 800.0 - 1 / 1000.0);
+    return us > 3 + values * 1.3e-6;
 }
 
 // dbias of a group: the sums of its runs, in order; 32 m by 32 runs at a time.
@@ -404,8 +458,6 @@ PlanParts plan_parts(const int32_t *plan, int64_t n, int64_t groups, int64_t cop
     return {plan, perm, copies > 1 ? perm + n : perm};
 }
 
-size_t align256(size_t b) { return (b + 255) / 256 * 256; }
-
 template <typename F>
 int by_type(int32_t value_type, F &&f)
 {
@@ -446,12 +498,46 @@ int linear(const jlust_linear &op, jlust_stream_t stream)
     a.ldz = op.ldz;
     a.act = op.act;
     const bool pkc = op.w_layout == 1;
+    const int64_t batch = op.groups ? op.groups : 1, w_rows = pkc ? op.out : op.inp, w_len = pkc ? op.inp : op.out;
+    const int64_t x_rows = op.cols / (op.groups ? op.copies : 1), ldw = padded<T>(w_len), ldx = padded<T>(op.inp);
+    const bool bad_w = !lies_well<T>(op.W, w_len, op.ldw, op.groups ? op.w_stride : 0), bad_x = !lies_well<T>(op.X, op.inp, op.ldx, 0);
+    const int64_t w_values = bad_w ? batch * w_rows * ldw : 0, x_values = bad_x ? x_rows * ldx : 0;
+    size_t pack = 0;
+    if (op.cols > 48 * batch && worth_packing<T>(op.out, op.cols, op.inp, w_values + x_values, bad_w && !pkc)) {
+        if (bad_w) {
+            a.P = nullptr;
+            a.ldp = ldw;
+            a.gp = w_rows * ldw;
+            a.p_pad = true;
+        }
+        if (bad_x) {
+            a.Q = nullptr;
+            a.ldq = ldx;
+            a.q_pad = true;
+        }
+        pack = align256(sizeof(T) * w_values) + align256(sizeof(T) * x_values);
+    }
     int shape = 0;
     size_t bytes = 0;
     plan_tile_product<T>(&a, pkc, true, &shape, &bytes);
-    if (bytes)
-        if (int st = scratch(stream, bytes, &a.part)) return st;
-    return launch_tile_product<T>(a, pkc, true, shape, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    if (pack + bytes) {
+        void *ws = nullptr;
+        if (int st = scratch(stream, pack + bytes, &ws)) return st;
+        char *at = (char *)ws;
+        if (a.p_pad) {
+            if (int st = pack_rows<T>(batch * w_rows, w_len, op.W, op.ldw, w_rows, op.w_stride, nullptr, nullptr, at, ldw, s)) return st;
+            a.P = at;
+            at += align256(sizeof(T) * w_values);
+        }
+        if (a.q_pad) {
+            if (int st = pack_rows<T>(x_rows, op.inp, op.X, op.ldx, x_rows, 0, nullptr, nullptr, at, ldx, s)) return st;
+            a.Q = at;
+            at += align256(sizeof(T) * x_values);
+        }
+        a.part = at;
+    }
+    return launch_tile_product<T>(a, pkc, true, shape, s);
 }
 
 // ------------------------------------------------------------------- gradients
@@ -462,32 +548,59 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
     using A = typename Elem<T>::Acc;
     hipStream_t s = (hipStream_t)stream;
     const PlanParts pl = plan_parts(op.plan, op.cols, op.groups, op.copies);
-    const bool slope = op.act != JLUST_FN_IDENTITY, products = op.dX || op.dW;
-    const bool make_g = slope && products;
-    const int64_t n = op.cols, out = op.out, inp = op.inp;
+    const bool slope = op.act != JLUST_FN_IDENTITY;
+    const int64_t n = op.cols, out = op.out, inp = op.inp, batch = op.groups ? op.groups : 1;
     const bool wide = op.dX && op.groups && op.copies > 1;
+
+    // What is packed.  G is made where there is a slope, and where dW's columns are
+    // sorted by group: its sums then walk rows in order (found through the plan, their
+    // copies waited for the indexes: 262 us of 573 in the gradients of 32 experts).
+    // X is sorted with it.  Else what lies badly, where it pays.
+    const bool x_kc = op.w_layout == 0;
+    const int64_t x_rows = n / (op.groups ? op.copies : 1), w_rows = x_kc ? inp : out, w_len = x_kc ? out : inp;
+    const int64_t ldg_made = padded<T>(out), ldx_made = padded<T>(inp), ldw_made = padded<T>(w_len);
+    bool make_g = (slope && (op.dX || op.dW)) || (op.groups && op.dW), make_x = op.groups && op.dW, make_w = false;
+    {
+        const bool bad_g = !lies_well<T>(op.dY, out, op.lddy, 0), bad_x = !lies_well<T>(op.X, inp, op.ldx, 0);
+        const bool bad_w = !lies_well<T>(op.W, w_len, op.ldw, op.groups ? op.w_stride : 0);
+        const int64_t g_values = bad_g && !make_g ? n * ldg_made : 0;
+        const int64_t w_values = bad_w ? batch * w_rows * ldw_made : 0, x_values = bad_x && !make_x ? n * ldx_made : 0;
+        if (op.dX && n > 48 * batch && worth_packing<T>(inp, n, out, g_values + w_values, bad_w && !x_kc)) {
+            make_g |= g_values > 0;
+            make_w = bad_w;
+        }
+        if (op.dW && worth_packing<T>(inp, n, out, (make_g ? 0 : g_values) + x_values, true)) {
+            make_g |= g_values > 0;
+            make_x |= bad_x;
+        }
+    }
+    make_g = make_g && n > 0;
+    make_x = make_x && n > 0;
 
     // G's columns are the groups' in order where it is made, dY's own where not.
     const T *G = (const T *)op.dY;
     int64_t ldg = op.lddy;
     const int32_t *grow = pl.perm;
     if (make_g) {
-        ldg = (out + 7) / 8 * 8;
+        G = nullptr;
+        ldg = ldg_made;
         grow = nullptr;
     }
 
     TileArgs x;
     int shape_x = 0;
     size_t part_x = 0;
-    const bool x_kc = op.w_layout == 0;
     if (op.dX) {
         x.m = inp;
         x.n = n;
         x.k = out;
-        x.P = op.W;
-        x.ldp = op.ldw;
-        x.gp = op.w_stride;
+        x.P = make_w ? nullptr : op.W;             // the plan goes by alignment: what is made has any
+        x.ldp = make_w ? ldw_made : op.ldw;
+        x.gp = make_w ? w_rows * ldw_made : op.w_stride;
+        x.p_pad = make_w;
+        x.Q = G;
         x.ldq = ldg;
+        x.q_pad = make_g;
         x.qrow = grow;
         x.crow = pl.perm;
         x.offsets = pl.offsets;
@@ -504,11 +617,12 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         w.m = op.w_layout ? inp : out;
         w.n = op.w_layout ? out : inp;
         w.k = n;
-        (op.w_layout ? w.P : w.Q) = op.X;
-        (op.w_layout ? w.ldp : w.ldq) = op.ldx;
-        (op.w_layout ? w.prow : w.qrow) = pl.src;
+        (op.w_layout ? w.P : w.Q) = make_x ? nullptr : op.X;
+        (op.w_layout ? w.ldp : w.ldq) = make_x ? ldx_made : op.ldx;
+        (op.w_layout ? w.p_pad : w.q_pad) = make_x;
+        (op.w_layout ? w.Q : w.P) = G;
         (op.w_layout ? w.ldq : w.ldp) = ldg;
-        (op.w_layout ? w.qrow : w.prow) = grow;
+        (op.w_layout ? w.q_pad : w.p_pad) = make_g;
         w.offsets = pl.offsets;
         w.groups = (int)op.groups;
         w.C = op.dW;
@@ -522,18 +636,34 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
     per = per < 64 ? 64 : (per + 7) / 8 * 8;
     const int64_t runs = (n + per - 1) / per + (op.groups ? (op.groups < n ? op.groups : n) : 0);
     const size_t g_bytes = make_g ? align256(sizeof(T) * n * ldg) : 0;
+    const size_t x_bytes = make_x ? align256(sizeof(T) * n * ldx_made) : 0;
+    const size_t w_bytes = make_w ? align256(sizeof(T) * batch * w_rows * ldw_made) : 0, made = g_bytes + x_bytes + w_bytes;
     const size_t wide_bytes = wide ? align256(sizeof(A) * n * inp) : 0;
     const size_t part = align256(part_x > part_w ? part_x : part_w);
     const size_t sum_bytes = op.dbias ? sizeof(A) * runs * out : 0;
     void *ws = nullptr;
-    if (g_bytes + wide_bytes + part + sum_bytes)
-        if (int st = scratch(stream, g_bytes + wide_bytes + part + sum_bytes, &ws)) return st;
+    if (made + wide_bytes + part + sum_bytes)
+        if (int st = scratch(stream, made + wide_bytes + part + sum_bytes, &ws)) return st;
     char *at = (char *)ws;
-    T *g_buf = make_g ? (T *)at : nullptr;
-    A *wide_buf = (A *)(at + g_bytes);
-    x.part = w.part = at + g_bytes + wide_bytes;
-    A *sums = op.dbias ? (A *)(at + g_bytes + wide_bytes + part) : nullptr;
-    if (make_g) G = g_buf;
+    T *g_buf = make_g ? (T *)at : nullptr, *x_buf = (T *)(at + g_bytes), *w_buf = (T *)(at + g_bytes + x_bytes);
+    A *wide_buf = (A *)(at + made);
+    x.part = w.part = at + made + wide_bytes;
+    A *sums = op.dbias ? (A *)(at + made + wide_bytes + part) : nullptr;
+    if (make_g) {
+        x.Q = g_buf;
+        (op.w_layout ? w.Q : w.P) = g_buf;
+    }
+    if (make_x) {
+        if (int st = pack_rows<T>(n, inp, op.X, op.ldx, x_rows, 0, pl.src, pl.offsets ? pl.offsets + op.groups : nullptr, x_buf,
+                                  ldx_made, s))
+            return st;
+        (op.w_layout ? w.P : w.Q) = x_buf;
+    }
+    if (make_w) {
+        if (int st = pack_rows<T>(batch * w_rows, w_len, op.W, op.ldw, w_rows, op.w_stride, nullptr, nullptr, w_buf, ldw_made, s))
+            return st;
+        x.P = w_buf;
+    }
 
     if (make_g || op.dbias) {
         if (n > 0) {
@@ -550,7 +680,6 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         }
     }
     if (op.dX && n > 0 && inp > 0) {
-        x.Q = G;
         if (wide) x.C = wide_buf;
         if (int st = launch_tile_product<T>(x, x_kc, true, shape_x, s)) return st;
         if (wide) {
@@ -566,7 +695,6 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
             for (int64_t g = 0; g < (op.groups ? op.groups : 1); ++g)
                 if (int st = fill_zero<T>(rows, d, (T *)op.dW + g * op.dw_stride, op.lddw, s)) return st;
         } else {
-            (op.w_layout ? w.Q : w.P) = G;
             if (int st = launch_tile_product<T>(w, false, false, shape_w, s)) return st;
         }
     }

@@ -10,7 +10,7 @@ template int launch_tile_product<__bf16>(const TileArgs &, bool, bool, int, hipS
 
 int preload_linear_half()
 {
-    JLUST_PRELOAD_KERNEL((tile_product_kernel<__bf16, true, true, 128, 128, 2, 2, false>));
+    JLUST_PRELOAD_KERNEL((tile_product_kernel<__bf16, true, true, 128, 128, 2, 2>));
     return JLUST_STATUS_SUCCESS;
 }
 

@@ -10,7 +10,7 @@ template int launch_tile_product<double>(const TileArgs &, bool, bool, int, hipS
 
 int preload_linear_wide()
 {
-    JLUST_PRELOAD_KERNEL((tile_product_kernel<double, true, true, 128, 128, 2, 2, false>));
+    JLUST_PRELOAD_KERNEL((tile_product_kernel<double, true, true, 128, 128, 2, 2>));
     return JLUST_STATUS_SUCCESS;
 }
 

@@ -19,7 +19,7 @@ typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 // 16 rows that a wave reads at one k lie in different banks.  sc: LDS row k
 // holds R elements; 16-bit ones have their 32-byte segments permuted by k, see
 // `segment`.
-template <typename T, bool KC, int R, int NT, bool IDX>
+template <typename T, bool KC, int R, int NT>
 struct Stage {
     static constexpr int CH = 16 / sizeof(T);
     static constexpr int BK = 128 / sizeof(T);
@@ -30,12 +30,9 @@ struct Stage {
     static constexpr bool WHOLE = CHUNKS % NT == 0;
     static_assert(NT % PER == 0, "a thread keeps its place in a row");
 
-    const T *base;
     const T *p[KC ? CNT : 1];
     int64_t ld;
-    int32_t row[IDX && !KC ? CNT : 1];
     int64_t avail;                       // sc: elements from this thread's first one to the edge
-    const int32_t *idx;
     uint32x4 v[CNT];
 
     __device__ __forceinline__ static bool mine(int i) { return WHOLE || (int)threadIdx.x + i * NT < CHUNKS; }
@@ -51,12 +48,9 @@ struct Stage {
         return seg ^ (((k & 3) | (k >> 1 & 4)) & MASK);
     }
 
-    __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx_, int64_t r0, int64_t rend,
-                                         int64_t k0, int64_t kend)
+    __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx, int64_t r0, int64_t rend)
     {
-        base = b;
         ld = ld_;
-        idx = idx_;
         if constexpr (KC) {
 #pragma unroll
             for (int i = 0; i < CNT; ++i) {
@@ -69,20 +63,7 @@ struct Stage {
             const int64_t c = r0 + (int64_t)place() * CH;
             avail = rend - c;
             p[0] = b + c;
-            rows(k0, kend);
         }
-    }
-
-    __device__ __forceinline__ void rows(int64_t k0, int64_t kend)
-    {
-        if constexpr (IDX && !KC)
-            if (idx) {
-#pragma unroll
-                for (int i = 0; i < CNT; ++i) {
-                    const int64_t k = k0 + lds_row(i);
-                    row[i] = k < kend ? idx[k] : 0;
-                }
-            }
     }
 
     // Reads the tile of [k0, k0 + BK); what lies past kend is zero.
@@ -108,13 +89,10 @@ struct Stage {
                 const int64_t k = k0 + lds_row(i);
                 v[i] = zero;
                 if (mine(i) && k < kend && avail > 0) {
-                    int64_t r = k;
-                    if constexpr (IDX) r = idx ? (int64_t)row[i] : k;
-                    const T *q = p[0] + r * ld;
+                    const T *q = p[0] + k * ld;
                     v[i] = avail >= CH ? load_chunk(q) : load_chunk_part(q, avail);
                 }
             }
-            rows(k0 + BK, kend);
         }
     }
 
@@ -452,7 +430,7 @@ __device__ __forceinline__ void put_rows(const A4 (&acc)[MT][NTL], int j, char *
 // registers.  One LDS tile of 128 bytes of k per row: while the waves multiply
 // it, their loads of the next one are in flight to registers, and two
 // workgroups a CU fill each other's waits.
-template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, bool IDX>
+template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const TileArgs a)
 {
     using A4 = typename Elem<T>::Acc4;
@@ -481,13 +459,13 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
         for (int j = 0; j < NTL; ++j) acc[i][j] = A4{0, 0, 0, 0};
 
     if (k0 < kend) {
-        using SP = Stage<T, PKC, LM, NT, IDX>;
-        using SQ = Stage<T, QKC, BN, NT, IDX>;
+        using SP = Stage<T, PKC, LM, NT>;
+        using SQ = Stage<T, QKC, BN, NT>;
         SP sp;
         SQ sq;
         const int64_t sg = KSUM ? 0 : group;
-        sp.init((const T *)a.P + sg * a.gp, a.ldp, PKC ? nullptr : a.prow, m0, a.m, k0, kend);
-        sq.init((const T *)a.Q, a.ldq, a.qrow, n0, nend, k0, kend);
+        sp.init((const T *)a.P + sg * a.gp, a.ldp, nullptr, m0, a.m);
+        sq.init((const T *)a.Q, a.ldq, a.qrow, n0, nend);
         sp.load(k0, kend);
         sq.load(k0, kend);
         for (int64_t k = k0; k < kend; k += BK) {
@@ -541,20 +519,18 @@ __device__ uint32_t tile_zeros[4];             // what a copy reads for k past t
 // order, so the order that the LDS reads want is given by what each lane reads.
 // kc rows have their chunks permuted as in Stage (64-byte rows: by r / 4, four of
 // them making one pass over the banks), sc rows their segments.
-template <typename T, bool KC, int R, int NT, int BK, bool IDX>
+template <typename T, bool KC, int R, int NT, int BK>
 struct Copy {
     static constexpr int SZ = sizeof(T), CH = 16 / SZ, RB = BK * SZ;   // a chunk's elements, a kc row's bytes
     static constexpr int PER = KC ? BK / CH : R / CH, CNT = R * BK / CH / NT, BYTES = R * RB, STEP = NT / PER;
     static_assert(R * BK / CH % NT == 0 && NT % PER == 0, "whole copies");
     static_assert(R / 16 >= (SZ == 2 ? 8 : 4), "segments to permute");
     // kc rows may lie anywhere (qrow), so each slot has its address; sc slots lie
-    // at 32-bit distances from the step's first row, or IDX finds their rows.
+    // at 32-bit distances from the step's first row.
     const T *base;
     const T *p[KC ? CNT : 1];
     uint32_t off[KC ? 1 : CNT];
     int64_t ld;
-    const int32_t *idx;
-    int32_t row[IDX && !KC ? CNT : 1];
 
     __device__ __forceinline__ static int lds_row(int i) { return threadIdx.x / PER + i * STEP; }
     __device__ __forceinline__ static int flip(int r)
@@ -575,10 +551,9 @@ struct Copy {
         else return segment(c / (16 / CH), r) * 16 + c % (16 / CH) * CH;
     }
 
-    __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx_, int r0, int rend, int k0, int kend)
+    __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx, int r0, int rend, int k0)
     {
         ld = ld_;
-        idx = idx_;
         base = b;
         if constexpr (KC) {
 #pragma unroll
@@ -589,25 +564,14 @@ struct Copy {
                 p[i] = b + (int64_t)r * ld + first(i) + k0;
             }
         } else {
-            if constexpr (!IDX) base += k0 * ld;
+            base += k0 * ld;
 #pragma unroll
             for (int i = 0; i < CNT; ++i) {
                 int c = r0 + first(i);
                 c = c < rend ? c : r0;             // columns past the edge are computed and not stored
-                off[i] = c + (IDX ? 0 : lds_row(i) * (uint32_t)ld);
+                off[i] = c + lds_row(i) * (uint32_t)ld;
             }
-            rows(k0, kend);
         }
-    }
-
-    __device__ __forceinline__ void rows(int k0, int kend)
-    {
-        if constexpr (IDX && !KC)
-#pragma unroll
-            for (int i = 0; i < CNT; ++i) {
-                const int k = k0 + lds_row(i);
-                row[i] = k < kend ? (idx ? idx[k] : k) : 0;
-            }
     }
 
     // Starts the copies of [k0, k0 + BK) and steps on.
@@ -619,7 +583,6 @@ struct Copy {
         for (int i = 0; i < CNT; ++i) {
             const T *q;
             if constexpr (KC) q = p[i];
-            else if constexpr (IDX) q = base + ((int64_t)row[i] * ld + off[i]);
             else q = base + off[i];
             if constexpr (TAIL) {
                 const int k = k0 + (KC ? first(i) : lds_row(i));
@@ -629,8 +592,7 @@ struct Copy {
                                              (__attribute__((address_space(3))) void *)(lds + (i * NT + wave * 64) * 16), 16, 0, 0);
             if constexpr (KC) p[i] += BK;
         }
-        if constexpr (!KC && !IDX) base += BK * ld;
-        rows(k0 + BK, kend);
+        if constexpr (!KC) base += BK * ld;
     }
 
     // Where a lane reads what it feeds to a 32x32x16 step: row 32 tile + lane % 32,
@@ -698,7 +660,7 @@ __device__ __forceinline__ void copies_done()
 // As tile_product_kernel for operands whose chunks lie whole and aligned, NB
 // LDS tiles in turn: while one is multiplied, the copies of the next NB - 1 are
 // under way, and a step has one barrier.
-template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB, bool IDX>
+template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB>
 __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 32 ? 3 : 2) void tile_copy_kernel(const TileArgs a)
 {
     constexpr bool HALF = sizeof(T) == 2;
@@ -708,8 +670,8 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
     constexpr bool KSUM = !PKC && !QKC;
     using A = typename Elem<T>::Acc;
     using Sum = std::conditional_t<HALF, floatx16, typename Elem<T>::Acc4>;
-    using CP = Copy<T, PKC, LM, NT, BK, IDX>;
-    using CQ = Copy<T, QKC, BN, NT, BK, IDX>;
+    using CP = Copy<T, PKC, LM, NT, BK>;
+    using CQ = Copy<T, QKC, BN, NT, BK>;
     // Arrays of their own: the compiler then knows which copies an LDS read waits for.
     constexpr int TILE = CP::BYTES + CQ::BYTES, SUMS = WM * WN * SumRows<A, TM>::BYTES;
     __shared__ __align__(16) char lds0[TILE > SUMS ? TILE : SUMS];
@@ -731,8 +693,8 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
     if (k0 < kend) {
         CP cp;
         CQ cq;
-        cp.init((const T *)a.P + (KSUM ? 0 : group * a.gp), a.ldp, PKC ? nullptr : a.prow, m0, a.m, k0, kend);
-        cq.init((const T *)a.Q, a.ldq, a.qrow, n0, nend, k0, kend);
+        cp.init((const T *)a.P + (KSUM ? 0 : group * a.gp), a.ldp, nullptr, m0, a.m, k0);
+        cq.init((const T *)a.Q, a.ldq, a.qrow, n0, nend, k0);
         constexpr int EACH = CP::CNT + CQ::CNT;
         auto start = [&](char *to, int k) {
             if (k + BK <= kend) {
@@ -782,7 +744,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
         };
         // One step: its tile is there once all but the later tiles' copies are.
         auto step = [&](const char *from, char *to, int k) {
-            if (NB > 2 && !IDX && k + BK < kend) copies_done<(NB - 2) * EACH>();
+            if (NB > 2 && k + BK < kend) copies_done<(NB - 2) * EACH>();
             else copies_done<0>();
             if (k + (NB - 1) * BK < kend) start(to, k + (NB - 1) * BK);
             multiply(from, kend - k);
@@ -794,7 +756,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
             __builtin_amdgcn_sched_barrier(0);      // not after the products, where they would be late
         };
         auto steady = [&](const char *from, char *to, int k) {
-            copies_done<IDX ? 0 : (NB - 2) * EACH>();
+            copies_done<(NB - 2) * EACH>();
             copy(to, k + (NB - 1) * BK);
             multiply(from, BK);
         };
@@ -935,7 +897,7 @@ bool copies_fit(const TileArgs &a, bool pkc, bool qkc)
     const int64_t z = sizeof(T);
     const uintptr_t bits = (uintptr_t)a.P | (uintptr_t)a.Q | (uintptr_t)(a.ldp * z) | (uintptr_t)(a.ldq * z) |
                            (uintptr_t)(a.gp * z) | (uintptr_t)(a.gq * z);
-    const int64_t k = pkc || qkc ? a.k : 0, m = pkc ? 0 : a.m, n = qkc ? 0 : a.n;
+    const int64_t k = (pkc && !a.p_pad) || (qkc && !a.q_pad) ? a.k : 0, m = pkc || a.p_pad ? 0 : a.m, n = qkc || a.q_pad ? 0 : a.n;
     return (bits & 15) == 0 && (k | m | n) * z % 16 == 0 && a.ldp < (1 << 22) && a.ldq < (1 << 22);
 }
 
@@ -1025,18 +987,18 @@ inline unsigned work_groups(const TileArgs &a, bool ksum)
     return (unsigned)(((total + NUM_XCD - 1) / NUM_XCD + (a.offsets && !ksum ? 1 : 0)) * NUM_XCD);
 }
 
-template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, bool IDX>
+template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN>
 int launch_shape(const TileArgs &a, hipStream_t s)
 {
-    hipLaunchKernelGGL((tile_product_kernel<T, PKC, QKC, BM, BN, WM, WN, IDX>),
+    hipLaunchKernelGGL((tile_product_kernel<T, PKC, QKC, BM, BN, WM, WN>),
                        dim3(work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("tile_product_kernel");
 }
 
-template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB, bool IDX>
+template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB>
 int launch_copies(const TileArgs &a, hipStream_t s)
 {
-    hipLaunchKernelGGL((tile_copy_kernel<T, PKC, QKC, BM, BN, WM, WN, BK, NB, IDX>),
+    hipLaunchKernelGGL((tile_copy_kernel<T, PKC, QKC, BM, BN, WM, WN, BK, NB>),
                        dim3(work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("tile_copy_kernel");
 }
@@ -1045,40 +1007,40 @@ template <typename T, bool PKC>
 int launch_columns(const TileArgs &a, int shape, hipStream_t s)
 {
     if constexpr (sizeof(T) == 2) switch (shape) {
-        case COPY_256: return launch_copies<T, PKC, true, 256, 256, 2, 4, 64, 2, false>(a, s);
-        case COPY_TALL: return launch_copies<T, PKC, true, 256, 128, 2, 2, 32, 3, false>(a, s);
-        case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 64, 2, false>(a, s);
-        case REG_M64: return launch_shape<T, PKC, true, 64, 64, 2, 2, false>(a, s);
-        case REG_32: return launch_shape<T, PKC, true, 128, 32, 4, 1, false>(a, s);
-        case REG_16: return launch_shape<T, PKC, true, 128, 16, 4, 1, false>(a, s);
+        case COPY_256: return launch_copies<T, PKC, true, 256, 256, 2, 4, 64, 2>(a, s);
+        case COPY_TALL: return launch_copies<T, PKC, true, 256, 128, 2, 2, 32, 3>(a, s);
+        case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 64, 2>(a, s);
+        case REG_M64: return launch_shape<T, PKC, true, 64, 64, 2, 2>(a, s);
+        case REG_32: return launch_shape<T, PKC, true, 128, 32, 4, 1>(a, s);
+        case REG_16: return launch_shape<T, PKC, true, 128, 16, 4, 1>(a, s);
         }
     else switch (shape) {
-        case REG_32: return launch_shape<T, PKC, true, 128, 32, 2, 2, false>(a, s);
-        case REG_16: return launch_shape<T, PKC, true, 128, 16, 2, 1, false>(a, s);
+        case REG_32: return launch_shape<T, PKC, true, 128, 32, 2, 2>(a, s);
+        case REG_16: return launch_shape<T, PKC, true, 128, 16, 2, 1>(a, s);
         }
     if constexpr (sizeof(T) == 4) switch (shape) {
-        case REG_M128: return launch_shape<T, PKC, true, 128, 64, 1, 4, false>(a, s);
-        case REG_M112: return launch_shape<T, PKC, true, 112, 64, 1, 4, false>(a, s);
-        case REG_M96: return launch_shape<T, PKC, true, 96, 64, 1, 4, false>(a, s);
-        case REG_M80: return launch_shape<T, PKC, true, 80, 64, 1, 4, false>(a, s);
-        case REG_M64: return launch_shape<T, PKC, true, 64, 64, 1, 4, false>(a, s);
-        case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 32, 2, false>(a, s);
+        case REG_M128: return launch_shape<T, PKC, true, 128, 64, 1, 4>(a, s);
+        case REG_M112: return launch_shape<T, PKC, true, 112, 64, 1, 4>(a, s);
+        case REG_M96: return launch_shape<T, PKC, true, 96, 64, 1, 4>(a, s);
+        case REG_M80: return launch_shape<T, PKC, true, 80, 64, 1, 4>(a, s);
+        case REG_M64: return launch_shape<T, PKC, true, 64, 64, 1, 4>(a, s);
+        case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 32, 2>(a, s);
         }
-    return launch_shape<T, PKC, true, 128, 128, 2, 2, false>(a, s);
+    return launch_shape<T, PKC, true, 128, 128, 2, 2>(a, s);
 }
 
-template <typename T, bool IDX>
+template <typename T>
 int launch_sums(const TileArgs &a, int shape, hipStream_t s)
 {
     if constexpr (sizeof(T) == 2) {
-        if (shape == COPY_TALL) return launch_copies<T, false, false, 256, 128, 2, 2, 32, 3, IDX>(a, s);
-        if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 3, IDX>(a, s);
+        if (shape == COPY_TALL) return launch_copies<T, false, false, 256, 128, 2, 2, 32, 3>(a, s);
+        if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 3>(a, s);
     }
     if constexpr (sizeof(T) == 4)
-        if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 2, IDX>(a, s);
+        if (shape == COPY_128) return launch_copies<T, false, false, 128, 128, 2, 2, 32, 2>(a, s);
     if constexpr (sizeof(T) <= 4)
-        if (shape == REG_M64) return launch_shape<T, false, false, 64, 64, 2, 2, IDX>(a, s);
-    return launch_shape<T, false, false, 128, 128, 2, 2, IDX>(a, s);
+        if (shape == REG_M64) return launch_shape<T, false, false, 64, 64, 2, 2>(a, s);
+    return launch_shape<T, false, false, 128, 128, 2, 2>(a, s);
 }
 
 template <typename T>
@@ -1091,7 +1053,7 @@ int launch_tile_product(const TileArgs &args, bool pkc, bool qkc, int shape, hip
     if ((int64_t)a.tiles_m * a.tiles_n * a.split * (ksum && a.offsets ? a.groups : 1) >= (int64_t)1 << 23)
         return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: a product of %d x %d tiles is more than one launch takes", a.tiles_m,
                     a.tiles_n);
-    if (ksum) st = a.prow || a.qrow ? launch_sums<T, true>(a, shape, s) : launch_sums<T, false>(a, shape, s);
+    if (ksum) st = launch_sums<T>(a, shape, s);
     else st = pkc ? launch_columns<T, true>(a, shape, s) : launch_columns<T, false>(a, shape, s);
     if (st || a.split == 1) return st;
     const int64_t rows = a.n * (ksum && a.offsets ? a.groups : 1), items = rows * ((a.m + 3) / 4);

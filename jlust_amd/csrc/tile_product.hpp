@@ -17,12 +17,12 @@ namespace jlust {
 // One product.  P and Q are each contiguous along k ("kc": element (r, k) at
 // base[r * ld + k]) or along their own side ("sc": base[k * ld + r]).
 struct TileArgs {
-    int64_t m, n, k;
-    const void *P, *Q;
-    int64_t ldp, ldq;
+    int64_t m = 0, n = 0, k = 0;
+    const void *P = nullptr, *Q = nullptr;
+    int64_t ldp = 0, ldq = 0;
     int64_t gp = 0, gq = 0;             // elements between the matrices of two groups
-    const int32_t *prow = nullptr;      // sc: the row of P that k stands for (null: k itself)
-    const int32_t *qrow = nullptr;      // sc: as prow; kc: the row of Q that n stands for
+    bool p_pad = false, q_pad = false;  // rows lie in buffers of their own, zeros after them to the next 16 bytes
+    const int32_t *qrow = nullptr;      // kc: the row of Q that n stands for (null: n itself)
     const int32_t *crow = nullptr;      // the row of C, R and Z that n stands for
     void *C = nullptr;
     int64_t ldc = 0, gc = 0;

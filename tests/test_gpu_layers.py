@@ -114,6 +114,17 @@ def test_linear_large_tiles(J, T, layout):
     check_grad(J, s)
 
 
+@pytest.mark.parametrize("layout", ["out", "inp"])
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("out,inp,cols,pad,skip", [(2053, 1029, 4100, 0, 0), (1024, 1032, 4096, 8, 3), (1160, 2048, 1200, 1, 0)])
+def test_linear_packed(J, layout, act, out, inp, cols, pad, skip):
+    """Products large enough that rows that lie badly (odd lengths, starts or
+    distances) are packed first, the gradient's dY among them."""
+    s = case(out, torch.bfloat16, out, inp, cols, layout, act, True, False, pad=pad, skip=skip)
+    check_forward(J, s)
+    check_grad(J, s)
+
+
 @pytest.mark.parametrize("T", L.TYPES)
 def test_linear_gradient_against_differences(J, T):
     """The gradients of sum(Y .* D) by central differences of the 64-bit form:
@@ -267,6 +278,17 @@ def test_grouped(J, T, layout, i):
     h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
     check_forward(J, s, ids, copies, h)
     check_grad(J, s, ids, copies, h, seed=i)
+
+
+@pytest.mark.parametrize("layout", ["out", "inp"])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_grouped_packed(J, layout, act):
+    """As test_linear_packed, with columns in no group and two copies."""
+    s = case(3, torch.float16, 1531, 1029, 2050, layout, act, True, False, 3, 2, pad=1)
+    ids = torch.from_numpy(some_ids(4100, 3, 9, 0.1)).cuda().view(2050, 2).t()
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=3)
+    check_forward(J, s, ids, 2, h)
+    check_grad(J, s, ids, 2, h)
 
 
 @pytest.mark.parametrize("T", [torch.bfloat16, torch.float32])
