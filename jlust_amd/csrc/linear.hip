@@ -276,14 +276,17 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(int64_t rows, int64_t le
                                                         const int32_t *__restrict__ limit, T *__restrict__ out, int64_t ld)
 {
     constexpr int V = 16 / sizeof(T);
-    const int64_t chunks = ld / V, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= rows * chunks) return;
-    const int64_t p = at / chunks, c = (at - p * chunks) * V, left = len - c;
-    if (limit && p >= *limit) return;
+    // 32 chunks along a row by 8 rows.
+    const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (p >= rows || (limit && p >= *limit)) return;
     const int64_t r = idx ? (int64_t)idx[p] : p;
-    const T *q = src + r / per * stride + r % per * lds_ + c;
-    const uint32x4 v = left >= V ? load_chunk(q) : load_chunk_part(q, left);
-    __builtin_memcpy(out + p * ld + c, &v, 16);
+    const T *from = src + (stride ? r / per * stride + r % per * lds_ : r * lds_);
+    for (int64_t c = (int64_t)(threadIdx.x & 31) * V; c < ld; c += 32 * V) {
+        const int64_t left = len - c;
+        const T *q = from + c;
+        const uint32x4 v = left >= V ? load_chunk(q) : load_chunk_part(q, left);
+        __builtin_memcpy(out + p * ld + c, &v, 16);
+    }
 }
 
 // rows in runs of `per`, `stride` apart (the groups' matrices; else one run).
@@ -291,9 +294,8 @@ template <typename T>
 int pack_rows(int64_t rows, int64_t len, const void *src, int64_t lds, int64_t per, int64_t stride, const int32_t *idx,
               const int32_t *limit, void *out, int64_t ld, hipStream_t s)
 {
-    const int64_t items = rows * (ld / (16 / (int64_t)sizeof(T)));
-    if (items == 0) return JLUST_STATUS_SUCCESS;
-    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, rows, len, (const T *)src, lds,
+    if (rows == 0 || ld == 0) return JLUST_STATUS_SUCCESS;
+    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, rows, len, (const T *)src, lds,
                        per, stride, idx, limit, (T *)out, ld);
     return check_launch("pack_rows_kernel");
 }
@@ -324,14 +326,15 @@ bool worth_packing(int64_t m, int64_t n, int64_t k, int64_t values, bool sides)
     return us > 3 + values * 1.3e-6;
 }
 
-// dbias of a group: the sums of its runs, in order; 32 m by 32 runs at a time.
-template <typename T>
-__global__ __launch_bounds__(1024) void grad_bias_kernel(int64_t n, int64_t m, const int32_t *__restrict__ offsets, int per,
+// dbias of a group: the sums of its runs, in order; 32 m by LANES runs at a time (8
+// where groups have few: 13 us by 32 and 5 by 8 for 32 groups of 8 runs).
+template <typename T, int LANES>
+__global__ __launch_bounds__(32 * LANES) void grad_bias_kernel(int64_t n, int64_t m, const int32_t *__restrict__ offsets, int per,
                                                          const typename Elem<T>::Acc *__restrict__ sums, T *__restrict__ dbias,
                                                          int64_t stride)
 {
     using A = typename Elem<T>::Acc;
-    __shared__ A s_sum[32][33];
+    __shared__ A s_sum[LANES][33];
     __shared__ int64_t s_first;
     const int group = blockIdx.y, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     int64_t first = 0, count = (n + per - 1) / per;
@@ -350,14 +353,14 @@ __global__ __launch_bounds__(1024) void grad_bias_kernel(int64_t n, int64_t m, c
     A s = A(0);
     if (c < m) {
 #pragma unroll 8
-        for (int64_t i = ty; i < count; i += 32) s += sums[(first + i) * m + c];
+        for (int64_t i = ty; i < count; i += LANES) s += sums[(first + i) * m + c];
     }
     s_sum[ty][tx] = s;
     __syncthreads();
     if (ty == 0 && c < m) {
         A t = A(0);
 #pragma unroll
-        for (int q = 0; q < 32; ++q) t += s_sum[q][tx];
+        for (int q = 0; q < LANES; ++q) t += s_sum[q][tx];
         dbias[group * stride + c] = T(t);
     }
 }
@@ -673,9 +676,14 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
             if (int st = check_launch("grad_prepass_kernel")) return st;
         }
         if (op.dbias) {
-            hipLaunchKernelGGL((grad_bias_kernel<T>), dim3((unsigned)((out + 31) / 32), (unsigned)(op.groups ? op.groups : 1)),
-                               dim3(1024), 0, s, n, out, n ? pl.offsets : nullptr, (int)per, sums, (T *)op.dbias,
-                               op.dbias_stride);
+            const dim3 grid((unsigned)((out + 31) / 32), (unsigned)(op.groups ? op.groups : 1));
+            const int32_t *offsets = n ? pl.offsets : nullptr;
+            if (runs <= 32 * (op.groups ? op.groups : 1))
+                hipLaunchKernelGGL((grad_bias_kernel<T, 8>), grid, dim3(256), 0, s, n, out, offsets, (int)per, sums,
+                                   (T *)op.dbias, op.dbias_stride);
+            else
+                hipLaunchKernelGGL((grad_bias_kernel<T, 32>), grid, dim3(1024), 0, s, n, out, offsets, (int)per, sums,
+                                   (T *)op.dbias, op.dbias_stride);
             if (int st = check_launch("grad_bias_kernel")) return st;
         }
     }

@@ -812,85 +812,100 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
 // ------------------------------------------------------------ few columns
 
 // 16-bit products of at most 16 columns a run, where reading P is all the work: a
-// workgroup makes 16 m by a run's columns over the whole k, its 8 waves taking 128 of
-// k each in turn straight to registers, 64 bytes a lane ahead, and adds their sums in
-// LDS in order.  One launch, no sums in memory (k cut over workgroups and added by
-// a second launch: 12.9 us for 4096 x 4096 and one column).  An sc P's 16 x 32 pieces
-// are transposed through a kilobyte of LDS that the wave keeps to itself.
-constexpr int FEW_WAVES = 8, FEW_STEPS = 4;
+// workgroup makes 16 TILES of m by a run's columns over the whole k, its waves taking
+// 32 STEPS of k each in turn straight to registers, the next ones read ahead, and adds
+// their sums in LDS in order.  One launch, no sums in memory (k cut over workgroups and
+// added by a second launch: 12.9 us for 4096 x 4096 and one column).  kc: 16 m, 64 bytes
+// a row and step, 8.9 us at 3.8 TB/s with P in no cache.  sc: 32 m where that makes
+// enough workgroups, for 64 bytes of a row (2048 -> 8192: 11.3 us, 16.3 with 16 m),
+// else 16 (4096 -> 4096: 16.2 us, 17.6 with 32); its pieces are transposed through LDS
+// that the wave keeps to itself.
+template <int TILES> struct Few {
+    static constexpr int WAVES = TILES == 1 ? 8 : 16, STEPS = TILES == 1 ? 4 : 2;
+};
 
-template <typename T, bool PKC>
-__global__ __launch_bounds__(FEW_WAVES * 64) void few_columns_kernel(const TileArgs a)
+template <typename T, bool PKC, int TILES>
+__global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(const TileArgs a)
 {
-    constexpr int CH = 8, SPAN = 32 * FEW_STEPS;
-    __shared__ __align__(16) float s_sum[FEW_WAVES][16][16];
-    __shared__ __align__(16) char s_turn[PKC ? 16 : FEW_WAVES * FEW_STEPS * 1024];
+    using F = Few<TILES>;
+    constexpr int CH = 8, WAVES = F::WAVES, STEPS = F::STEPS, M = 16 * TILES, SPAN = 32 * STEPS;
+    constexpr int LANES = M / CH, ROWS = 64 / LANES;       // sc: lanes of a row of k, rows of one read
+    static_assert(PKC || ROWS * TILES == 32, "TILES reads make a step");
+    __shared__ __align__(16) float s_sum[WAVES][16][M];
+    __shared__ __align__(16) char s_turn[PKC ? 16 : WAVES * STEPS * 32 * M * 2];
     Work w;
     if (!find_work<false, 16, 64>(a, &w)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int64_t m0 = (int64_t)w.tm * 16;
+    const int64_t m0 = (int64_t)w.tm * M;
     const T *P = (const T *)a.P + w.group * a.gp;
 
-    // What a lane reads of each 32 of k: kc, 16 bytes of row m0 + li from 8 g; sc, of
-    // row lane / 2 its half of the 16 m.
+    // kc: 16 bytes of row m0 + li from k = 8 g; sc: 16 bytes of m of every ROWS'th row.
     const T *p;
     int64_t avail = CH;
     if constexpr (PKC) {
         p = P + (m0 + li < a.m ? m0 + li : a.m - 1) * a.ldp + 8 * g;
     } else {
-        const int64_t m = m0 + 8 * (lane & 1);
+        const int64_t m = m0 + CH * (lane % LANES);
         avail = a.m - m;
-        p = P + (int64_t)(lane >> 1) * a.ldp + m;
+        p = P + (int64_t)(lane / LANES) * a.ldp + m;
     }
     int col = w.n0 + li < w.nend ? w.n0 + li : w.nend - 1;
     if (a.qrow) col = a.qrow[col];
     const T *q = (const T *)a.Q + (int64_t)col * a.ldq + 8 * g;
 
     const uint32x4 zero = {0, 0, 0, 0};
-    auto read = [&](int k, uint32x4 (&pv)[FEW_STEPS], uint32x4 (&qv)[FEW_STEPS]) {
+    auto read = [&](int k, uint32x4 (&pv)[STEPS][TILES], uint32x4 (&qv)[STEPS]) {
 #pragma unroll
-        for (int s = 0; s < FEW_STEPS; ++s) {
+        for (int s = 0; s < STEPS; ++s) {
             const int at = k + 32 * s, left = w.kend - at - 8 * g;
             qv[s] = left >= CH ? load_chunk(q + at) : left > 0 ? load_chunk_part(q + at, left) : zero;
-            if constexpr (PKC) {
-                pv[s] = left >= CH ? load_chunk(p + at) : left > 0 ? load_chunk_part(p + at, left) : zero;
-            } else {
-                const T *r = p + (int64_t)at * a.ldp;
-                const bool in = at + (lane >> 1) < w.kend;
-                pv[s] = !in || avail <= 0 ? zero : avail >= CH ? load_chunk(r) : load_chunk_part(r, avail);
+#pragma unroll
+            for (int u = 0; u < TILES; ++u) {
+                if constexpr (PKC) {
+                    pv[s][u] = left >= CH ? load_chunk(p + at) : left > 0 ? load_chunk_part(p + at, left) : zero;
+                } else {
+                    const int row = at + lane / LANES + u * ROWS;
+                    const T *r = p + (int64_t)(at + u * ROWS) * a.ldp;
+                    pv[s][u] = row >= w.kend || avail <= 0 ? zero : avail >= CH ? load_chunk(r) : load_chunk_part(r, avail);
+                }
             }
         }
     };
-    floatx4 acc = {0, 0, 0, 0};
-    auto multiply = [&](uint32x4 (&pv)[FEW_STEPS], uint32x4 (&qv)[FEW_STEPS]) {
+    floatx4 acc[TILES];
+#pragma unroll
+    for (int u = 0; u < TILES; ++u) acc[u] = floatx4{0, 0, 0, 0};
+    auto multiply = [&](uint32x4 (&pv)[STEPS][TILES], uint32x4 (&qv)[STEPS]) {
         if constexpr (!PKC) {
-            // Row k lies at k * 32, its halves changed over by k / 4: 16 lanes' 4 rows
-            // by 16 columns read from different banks.
-            char *turn = s_turn + wave * FEW_STEPS * 1024;
-            const int row = lane >> 1, half = lane & 1;
+            char *turn = s_turn + wave * STEPS * 32 * M * 2;
             wave_sync();
 #pragma unroll
-            for (int s = 0; s < FEW_STEPS; ++s)
-                *reinterpret_cast<uint32x4 *>(turn + s * 1024 + row * 32 + half * 16) = pv[s];
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int u = 0; u < TILES; ++u)
+                    *reinterpret_cast<uint32x4 *>(turn + (s * 32 + u * ROWS) * M * 2 + lane * 16) = pv[s][u];
             wave_sync();
 #pragma unroll
-            for (int s = 0; s < FEW_STEPS; ++s)
+            for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = 8 * g + 4 * h + (li >> 2);
-                    const shortx4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) shortx4 *)(turn + s * 1024 + k * 32 + (li & 3) * 8));
-                    const uint32x2 u = __builtin_bit_cast(uint32x2, t);
-                    pv[s][2 * h] = u[0];
-                    pv[s][2 * h + 1] = u[1];
-                }
+                for (int u = 0; u < TILES; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int k = 32 * s + 8 * g + 4 * h + (li >> 2);
+                        const shortx4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) shortx4 *)(turn + k * M * 2 + u * 32 + (li & 3) * 8));
+                        const uint32x2 v = __builtin_bit_cast(uint32x2, t);
+                        pv[s][u][2 * h] = v[0];
+                        pv[s][u][2 * h + 1] = v[1];
+                    }
         }
 #pragma unroll
-        for (int s = 0; s < FEW_STEPS; ++s) acc = mma(pv[s], qv[s], acc, T());
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int u = 0; u < TILES; ++u) acc[u] = mma(pv[s][u], qv[s], acc[u], T());
     };
-    uint32x4 pa[FEW_STEPS], qa[FEW_STEPS], pb[FEW_STEPS], qb[FEW_STEPS];
+    uint32x4 pa[STEPS][TILES], qa[STEPS], pb[STEPS][TILES], qb[STEPS];
     int k = w.k0 + wave * SPAN;
-    constexpr int ROUND = FEW_WAVES * SPAN;
+    constexpr int ROUND = WAVES * SPAN;
     if (k < w.kend) read(k, pa, qa);
     while (k < w.kend) {
         if (k + ROUND < w.kend) read(k + ROUND, pb, qb);
@@ -902,14 +917,16 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_columns_kernel(const TileA
         k += ROUND;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s_sum[wave][li][4 * g + e] = acc[e];
+    for (int u = 0; u < TILES; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_sum[wave][li][16 * u + 4 * g + e] = acc[u][e];
     __syncthreads();
-    const int n = w.n0 + (threadIdx.x >> 4);
-    const int64_t m = m0 + (threadIdx.x & 15);
-    if (threadIdx.x >= 256 || n >= w.nend || m >= a.m) return;
+    const int i = threadIdx.x / M, j = threadIdx.x % M, n = w.n0 + i;
+    const int64_t m = m0 + j;
+    if (i >= 16 || n >= w.nend || m >= a.m) return;
     float v[1] = {0};
 #pragma unroll
-    for (int u = 0; u < FEW_WAVES; ++u) v[0] += s_sum[u][threadIdx.x >> 4][threadIdx.x & 15];
+    for (int u = 0; u < WAVES; ++u) v[0] += s_sum[u][i][j];
     TileArgs b = a;
     if (!a.offsets) b.groups = 1;
     const int64_t row = a.crow ? (int64_t)a.crow[n] : n;
@@ -990,9 +1007,9 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
 // would be a fifth of the steps for nothing) at 64 columns, where a CU holds
 // enough workgroups to hide the rows it reads and stores.
 struct TileShape { int bm, bn; };
-enum Shape { REG_128, REG_32, REG_16, REG_M128, REG_M112, REG_M96, REG_M80, REG_M64, COPY_256, COPY_TALL, COPY_128, FEW };
+enum Shape { REG_128, REG_32, REG_16, REG_M128, REG_M112, REG_M96, REG_M80, REG_M64, COPY_256, COPY_TALL, COPY_128, FEW_16, FEW_32 };
 constexpr TileShape TILE_SHAPES[] = {{128, 128}, {128, 32}, {128, 16}, {128, 64}, {112, 64}, {96, 64}, {80, 64}, {64, 64},
-                                     {256, 256}, {256, 128}, {128, 128}, {16, 16}};
+                                     {256, 256}, {256, 128}, {128, 128}, {16, 16}, {32, 16}};
 
 // What a shape costs: its rate with a CU full of it (Tflop/s a CU), the time of 64 of
 // k where latency bounds it (us), workgroups a CU.  Measured on products of 64 to
@@ -1030,10 +1047,14 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
 
     ShapeCost some[4];
     int count = 0;
-    bool alone = false;                                // k is not cut
     if (sizeof(T) == 2 && !ksum && share <= 16) {
-        some[count++] = {FEW, 1.0, 0.06, 2};
-        alone = true;
+        if (pkc) {
+            some[count++] = {FEW_16, 0.25, 0.07, 4};
+        } else {
+            some[count++] = {FEW_16, 0.2, 0.17, 4};
+            some[count++] = {FEW_32, 0.25, 0.21, 2};
+            some[count++] = {REG_16, 1.0, 0.5, 6};
+        }
     } else if (!ksum && share <= 48) {
         some[count++] = share <= 16 ? ShapeCost{REG_16, 1.0, 0.5, 6} : ShapeCost{REG_32, 1.5, 0.5, 5};
         if (sizeof(T) > 2) some[0].rate = sizeof(T) == 4 ? 0.4 : 0.2, some[0].latency = 1.0;
@@ -1073,7 +1094,7 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
         const ShapeCost &o = some[i];
         const int64_t n = tiles(o.shape);
         const double work = 2e-6 * 64 * TILE_SHAPES[o.shape].bm * TILE_SHAPES[o.shape].bn / o.rate;
-        for (int64_t p = 1; p == 1 || (!alone && p <= k / 128 && p * sums * (int64_t)sizeof(typename Elem<T>::Acc) <= (int64_t)1 << 28); p *= 2) {
+        for (int64_t p = 1; p == 1 || (o.shape != FEW_16 && o.shape != FEW_32 && p <= k / 128 && p * sums * (int64_t)sizeof(typename Elem<T>::Acc) <= (int64_t)1 << 28); p *= 2) {
             const int64_t groups = n * p, slots = 256 * o.held;
             const int64_t held = (groups + 255) / 256 < o.held ? (groups + 255) / 256 : o.held;
             double rounds = (double)groups / slots;
@@ -1121,8 +1142,12 @@ template <typename T, bool PKC>
 int launch_columns(const TileArgs &a, int shape, hipStream_t s)
 {
     if constexpr (sizeof(T) == 2) switch (shape) {
-        case FEW:
-            hipLaunchKernelGGL((few_columns_kernel<T, PKC>), dim3(work_groups(a, false)), dim3(FEW_WAVES * 64), 0, s, a);
+        case FEW_16:
+        case FEW_32:
+            if (PKC || shape == FEW_16)
+                hipLaunchKernelGGL((few_columns_kernel<T, PKC, 1>), dim3(work_groups(a, false)), dim3(Few<1>::WAVES * 64), 0, s, a);
+            else
+                hipLaunchKernelGGL((few_columns_kernel<T, false, 2>), dim3(work_groups(a, false)), dim3(Few<2>::WAVES * 64), 0, s, a);
             return check_launch("few_columns_kernel");
         case COPY_256: return launch_copies<T, PKC, true, 256, 256, 2, 4, 64, 2>(a, s);
         case COPY_TALL: return launch_copies<T, PKC, true, 256, 128, 2, 2, 32, 3>(a, s);
