@@ -1,0 +1,92 @@
+"""Argument checks of the layer operators' C entries and Python surface that are
+made on the host, before anything reaches a device (no GPU needed)."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+import jlust_amd as J
+from jlust_amd import _lib, layers
+from jlust_amd.elementwise import FN_EXP, FN_GELU
+
+
+def linear(**kw):
+    f = dict(value_type=1, act=0, w_layout=0, reserved=0, out=4, inp=3, cols=2, W=64, ldw=4, X=64, ldx=3, Y=64, ldy=4,
+             bias=0, R=0, ldr=0, Z=0, ldz=0, groups=0, copies=1, plan=0, w_stride=0, bias_stride=0)
+    assert set(kw) <= set(f)
+    f.update(kw)
+    return _lib.lib().jlust_hip_linear(layers._LINEAR(*f.values()), 0)
+
+
+def grad(**kw):
+    f = dict(value_type=1, act=0, w_layout=0, reserved=0, out=4, inp=3, cols=2, W=64, ldw=4, X=64, ldx=3, dY=64, lddy=4, Z=0,
+             ldz=0, dX=64, lddx=3, dW=0, lddw=0, dbias=0, groups=0, copies=1, plan=0, w_stride=0, dw_stride=0, dbias_stride=0)
+    assert set(kw) <= set(f)
+    f.update(kw)
+    return _lib.lib().jlust_hip_linear_grad(layers._LINEAR_GRAD(*f.values()), 0)
+
+
+def test_packed_arguments_match_the_header():
+    """The packed bytes are as long as the header's structures."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "jlust_hip.h")).read()
+    for name, pack in (("jlust_linear", "@4i19q"), ("jlust_linear_grad", "@4i22q")):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        words = sum(len(d.split(",")) * (4 if "int32_t" in d and "*" not in d else 8) for d in body.split(";") if d.strip())
+        assert words == struct.calcsize(pack)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(value_type=4), 2), (dict(value_type=-1), 2), (dict(act=FN_EXP), 1), (dict(w_layout=2), 1), (dict(out=-1), 1),
+    (dict(cols=1 << 31), 1), (dict(ldw=3), 1), (dict(ldx=2), 1), (dict(ldy=3), 1), (dict(W=0), 1), (dict(X=0), 1), (dict(Y=0), 1),
+    (dict(R=64, ldr=3), 1), (dict(Z=64, ldz=1), 1), (dict(groups=2), 1), (dict(groups=5000, plan=64), 1), (dict(copies=2), 1),
+    (dict(groups=2, plan=64, copies=3), 1)])
+def test_linear_refuses(bad, status):
+    assert linear(**bad) == status
+    assert _lib.last_error()
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(value_type=9), 2), (dict(act=FN_GELU), 1), (dict(dY=0), 1), (dict(lddx=2), 1), (dict(dW=64, lddw=1), 1), (dict(W=0), 1),
+    (dict(dW=64, lddw=4, X=0), 1), (dict(groups=1), 1)])
+def test_linear_grad_refuses(bad, status):
+    assert grad(**bad) == status
+
+
+def test_group_plan_and_layer_norm_refuse():
+    L, n = _lib.lib(), ctypes.c_int64()
+    assert L.jlust_hip_group_plan_ints(10, 3, 1, ctypes.byref(n)) == 0 and n.value == 14
+    assert L.jlust_hip_group_plan_ints(10, 3, 2, ctypes.byref(n)) == 0 and n.value == 24
+    for bad in ((-1, 3, 1), (10, 0, 1), (10, 4096, 1), (10, 3, 3), (10, 3, 0), (1 << 31, 3, 1)):
+        assert L.jlust_hip_group_plan_ints(*bad, ctypes.byref(n)) == 1, bad
+    assert L.jlust_hip_group_plan_build(4, 2, 1, 2, 64, 0, 64, 0) == 5          # the origin
+    assert L.jlust_hip_group_plan_build(4, 2, 1, 1, 0, 0, 64, 0) == 1
+    norm = lambda vt=1, d=8, cols=2, X=64, ldx=8, eps=1e-5, Y=64, ldy=8, S=0, lds=2: L.jlust_hip_layer_norm(  # noqa: E731
+        vt, d, cols, X, ldx, 0, 0, eps, Y, ldy, S, lds, 0)
+    assert norm(vt=7) == 2
+    for bad in (dict(d=-1), dict(X=0), dict(Y=0), dict(ldx=7), dict(ldy=1), dict(eps=-1.0), dict(eps=float("nan")),
+                dict(S=64, lds=1)):
+        assert norm(**bad) == 1, bad
+    assert L.jlust_hip_layer_norm_grad(1, 8, 2, 64, 8, 64, 8, 0, 2, 0, 64, 8, 0, 0, 0) == 1      # no stats
+
+
+def test_host_memory_is_refused():
+    x = torch.zeros((4, 3)).t()
+    with pytest.raises(J.DeviceMismatch):
+        J.execute(J.LinearOp, torch.zeros((3, 5)).t(), x, torch.zeros((4, 5)).t())
+    with pytest.raises(J.DeviceMismatch):
+        J.execute(J.LayerNormOp, x, x)
+    with pytest.raises(J.DeviceMismatch):
+        J.prepare(J.HIPBackend(), J.GroupedLinearOp, torch.ones(4, dtype=torch.int32), n_groups=2)
+    with pytest.raises(TypeError):
+        J.prepare(J.HIPBackend(), J.GroupedLinearOp, torch.ones(4, dtype=torch.int32))
+    with pytest.raises(J.UnsupportedFormat):
+        J.execute(J.LinearOp, x, x, x, backend=object())
+
+
+def test_capability_table():
+    dense = J.Formats.DensedRight(2)
+    assert J.supports_backend(J.HIPBackend(), J.LinearOp(dense, dense, dense))
+    assert not J.supports_backend(J.HIPBackend(), J.LinearOp(J.Formats.CSR, dense, dense))
