@@ -314,16 +314,18 @@ bool lies_well(const void *p, int64_t len, int64_t ld, int64_t stride)
     return (((uintptr_t)p | (uintptr_t)(len * sizeof(T)) | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(stride * sizeof(T))) & 15) == 0;
 }
 
-// Whether 16-bit operands of `values` values are better packed first: the product
-// through registers runs at 550 Tflop/s where rows along its sides lie badly and 800
-// where rows along k do, at 1,000 from copies (8,191 columns 2047 -> 8191: 482 and 334
-// us against 257), and packing reads and writes them at 3 TB/s.
+// Whether operands of `values` values are better packed first: the product through
+// registers runs at 550 Tflop/s where rows along its sides lie badly and 800 where rows
+// along k do, at 1,000 from copies (8,191 columns 2047 -> 8191: 482 and 334 us against
+// 257), Float32's at 108 against 127 (8,191 columns 2047 -> 2047: 636 us and 558; 4,600
+// columns 1001 -> 1001: 126 and 131).  Packing reads and writes them at 3 TB/s.
+// Float32 with k of 256 and less runs through registers all the same.
 template <typename T>
 bool worth_packing(int64_t m, int64_t n, int64_t k, int64_t values, bool sides)
 {
-    if (sizeof(T) != 2 || values == 0) return false;
-    const double us = 2e-6 * m * n * k * (sides ? 1 / 550.0 - 1 / 1000.0 : 1 / 800.0 - 1 / 1000.0);
-    return us > 3 + values * 1.3e-6;
+    if (sizeof(T) > 4 || values == 0 || (sizeof(T) == 4 && k <= 256)) return false;
+    const double gain = sizeof(T) == 4 ? 1 / 108.0 - 1 / 127.0 : sides ? 1 / 550.0 - 1 / 1000.0 : 1 / 800.0 - 1 / 1000.0;
+    return 2e-6 * m * n * k * gain > 3 + values * (sizeof(T) * 0.65e-6);
 }
 
 // dbias of a group: the sums of its runs, in order; 32 m by LANES runs at a time (8

@@ -33,6 +33,7 @@ struct Stage {
     const T *p[KC ? CNT : 1];
     int64_t ld;
     int64_t avail;                       // sc: elements from this thread's first one to the edge
+    int64_t over;                        // sc: rows of k below this one may be read past the edge
     uint32x4 v[CNT];
 
     __device__ __forceinline__ static bool mine(int i) { return WHOLE || (int)threadIdx.x + i * NT < CHUNKS; }
@@ -48,7 +49,8 @@ struct Stage {
         return seg ^ (((k & 3) | (k >> 1 & 4)) & MASK);
     }
 
-    __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx, int64_t r0, int64_t rend)
+    // `ks`: the operand's extent along k.
+    __device__ __forceinline__ void init(const T *b, int64_t ld_, const int32_t *idx, int64_t r0, int64_t rend, int64_t ks)
     {
         ld = ld_;
         if constexpr (KC) {
@@ -62,11 +64,16 @@ struct Stage {
         } else {
             const int64_t c = r0 + (int64_t)place() * CH;
             avail = rend - c;
+            over = rend >= CH ? ks - 1 : 0;
             p[0] = b + c;
         }
     }
 
-    // Reads the tile of [k0, k0 + BK); what lies past kend is zero.
+    // Reads the tile of [k0, k0 + BK); what lies past kend is zero.  sc: a chunk
+    // over the edge takes the start of the next row with it (those columns are not
+    // stored), and only the last row's is read by elements: with both kinds in a wave
+    // every chunk waited for the one before (dW of 7168 x 111 over 4,600 columns,
+    // Float32: 144 us and 111).
     __device__ __forceinline__ void load(int64_t k0, int64_t kend)
     {
         const uint32x4 zero = {0, 0, 0, 0};
@@ -90,7 +97,7 @@ struct Stage {
                 v[i] = zero;
                 if (mine(i) && k < kend && avail > 0) {
                     const T *q = p[0] + k * ld;
-                    v[i] = avail >= CH ? load_chunk(q) : load_chunk_part(q, avail);
+                    v[i] = avail >= CH || k < over ? load_chunk(q) : load_chunk_part(q, avail);
                 }
             }
         }
@@ -464,8 +471,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
         SP sp;
         SQ sq;
         const int64_t sg = KSUM ? 0 : group;
-        sp.init((const T *)a.P + sg * a.gp, a.ldp, nullptr, m0, a.m);
-        sq.init((const T *)a.Q, a.ldq, a.qrow, n0, nend);
+        sp.init((const T *)a.P + sg * a.gp, a.ldp, nullptr, m0, a.m, a.k);
+        sq.init((const T *)a.Q, a.ldq, a.qrow, n0, nend, a.k);
         sp.load(k0, kend);
         sq.load(k0, kend);
         for (int64_t k = k0; k < kend; k += BK) {
@@ -849,6 +856,7 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
         avail = a.m - m;
         p = P + (int64_t)(lane / LANES) * a.ldp + m;
     }
+    const int64_t over = a.m >= CH ? a.k - 1 : 0;          // as in Stage
     int col = w.n0 + li < w.nend ? w.n0 + li : w.nend - 1;
     if (a.qrow) col = a.qrow[col];
     const T *q = (const T *)a.Q + (int64_t)col * a.ldq + 8 * g;
@@ -866,7 +874,7 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
                 } else {
                     const int row = at + lane / LANES + u * ROWS;
                     const T *r = p + (int64_t)(at + u * ROWS) * a.ldp;
-                    pv[s][u] = row >= w.kend || avail <= 0 ? zero : avail >= CH ? load_chunk(r) : load_chunk_part(r, avail);
+                    pv[s][u] = row >= w.kend || avail <= 0 ? zero : avail >= CH || row < over ? load_chunk(r) : load_chunk_part(r, avail);
                 }
             }
         }
@@ -1075,7 +1083,7 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
     } else if constexpr (sizeof(T) == 4) {
         const int64_t each = (a->m + (a->m + 127) / 128 - 1) / ((a->m + 127) / 128);
         if (ksum || (fit && k > 256 && each > 112)) {
-            some[count++] = fit ? ShapeCost{COPY_128, 0.55, 1.2, 2} : ShapeCost{REG_128, 0.48, 1.4, 2};
+            some[count++] = fit ? ShapeCost{COPY_128, 0.55, 1.2, 2} : ShapeCost{REG_128, 0.48, 5.5, 2};
             some[count++] = {REG_M64, 0.45, 1.9, 4};
         } else {
             const Shape fits = each <= 64 ? REG_M64 : each <= 80 ? REG_M80 : each <= 96 ? REG_M96 : each <= 112 ? REG_M112 : REG_M128;
