@@ -193,6 +193,7 @@ class GroupPlan(AbstractKernelHandle):
         self._check_ids(ids)
         ints = self.groups + 1 + self.n * (2 if self.copies > 1 else 1)
         self._plan = torch.empty(max(ints, 1), dtype=torch.int32, device=self.dev)
+        self._home = _lib.raw_stream(self.index)       # the stream that its memory goes back to
         self._build(ids)
 
     def _check_ids(self, ids):
@@ -206,9 +207,8 @@ class GroupPlan(AbstractKernelHandle):
             raise NonCanonicalStorage(f"ids must be contiguous columns, got strides {tuple(ids.stride())}")
 
     def _build(self, ids):
-        self._stream = _run(_lib.lib().jlust_hip_group_plan_build, self.index, "group_plan", ids.dtype, self.n,
-                            self.groups, self.copies, self.origin, ids.data_ptr(), ids.dtype is torch.int64,
-                            self._plan.data_ptr())
+        _run(_lib.lib().jlust_hip_group_plan_build, self.index, "group_plan", ids.dtype, self.n, self.groups,
+             self.copies, self.origin, ids.data_ptr(), ids.dtype is torch.int64, self.use())
 
     def update(self, ids):
         """New groups for the same columns."""
@@ -220,7 +220,7 @@ class GroupPlan(AbstractKernelHandle):
     def use(self):
         """The plan's address, its memory kept until the current stream is done
         with it."""
-        if _lib.raw_stream(self.index) != self._stream:
+        if _lib.raw_stream(self.index) != self._home:
             self._plan.record_stream(torch.cuda.current_stream(self.dev))
         return self._plan.data_ptr()
 

@@ -485,6 +485,27 @@ def test_streams_and_graphs(J):
     del keep
 
 
+def test_plan_memory_on_other_streams(J, monkeypatch):
+    """A plan updated or used on a stream other than the one it was made on tells
+    the allocator, also when both happen on the same other stream."""
+    ids = torch.tensor([1, 2, 0, 2], dtype=torch.int32, device="cuda")
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=2)
+    seen = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "record_stream", lambda t, s: seen.append((t.data_ptr(), s)))
+        h.use()
+        h.update(ids)
+        assert not seen
+        with torch.cuda.stream(side):
+            h.update(ids)
+            h.use()
+    assert seen == [(h.offsets().data_ptr(), side)] * 2
+    torch.cuda.current_stream().wait_stream(side)
+    assert h.order().tolist() == [0, 1, 3, 2]
+
+
 def test_refusals(J):
     T = torch.float32
     gen = torch.Generator().manual_seed(0)
