@@ -86,15 +86,31 @@ __device__ __forceinline__ void read_chunk(const T *p, int64_t left, A (&f)[16 /
     values<T>(read_raw(p, left), f);
 }
 
+// 16 bytes past the caches.  Results that the eight L2s of 4 MB do not hold would only
+// push out what is still read (16,384 bfloat16 columns of 4,096: 71.4 us by plain stores
+// and 63.9; backward, 200,003 Float32 columns of 100: 51.6 and 49.2; products' results
+// gain nothing: 8,192 columns 2048 -> 8192, 305 and 307 us).
+constexpr int64_t STREAMED = 32 << 20;         // bytes of a result from which it is stored so
+typedef uint32_t uint32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
+
+template <typename T>
+__device__ __forceinline__ void stream_chunk(T *p, const T *v)
+{
+    uint32x4 u;
+    __builtin_memcpy(&u, v, 16);
+    __builtin_nontemporal_store((uint32x4_any)u, reinterpret_cast<uint32x4_any *>(p));
+}
+
 template <typename T, typename A>
-__device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 / sizeof(T)])
+__device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 / sizeof(T)], bool streamed = false)
 {
     constexpr int CH = 16 / sizeof(T);
     T e[CH];
 #pragma unroll
     for (int j = 0; j < CH; ++j) e[j] = T(f[j]);
     if (left >= CH) {
-        store_vec<CH>(p, e);
+        if (streamed) stream_chunk(p, e);
+        else store_vec<CH>(p, e);
     } else {
 #pragma unroll
         for (int j = 0; j < CH; ++j)
@@ -108,7 +124,7 @@ __device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 
 template <typename T, int LANES, int VPL>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_kernel(
     int64_t d, int64_t cols, const T *X, int64_t ldx, const T *__restrict__ weight, const T *__restrict__ bias,
-    typename Elem<T>::Acc eps, T *Y, int64_t ldy, typename Elem<T>::Acc *__restrict__ stats, int64_t lds_)
+    typename Elem<T>::Acc eps, T *Y, int64_t ldy, typename Elem<T>::Acc *__restrict__ stats, int64_t lds_, bool streamed)
 {
     using A = typename Elem<T>::Acc;
     constexpr int CH = 16 / sizeof(T), NT = LANES > 256 ? LANES : 256, COLS = NT / LANES;
@@ -176,7 +192,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_kernel(
 #pragma unroll
                 for (int j = 0; j < CH; ++j) f[j] += v[j];
             }
-            write_chunk(Y + c * ldy + at, left, f);
+            write_chunk(Y + c * ldy + at, left, f, streamed);
         }
     }
 }
@@ -241,7 +257,7 @@ template <typename T, int LANES, int VPL>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_grad_kernel(
     int64_t d, int64_t cols, const T *__restrict__ X, int64_t ldx, const T *dY, int64_t lddy,
     const typename Elem<T>::Acc *__restrict__ stats, int64_t lds_, const T *__restrict__ weight, T *dX, int64_t lddx,
-    typename Elem<T>::Acc *__restrict__ parts)
+    typename Elem<T>::Acc *__restrict__ parts, bool streamed)
 {
     using A = typename Elem<T>::Acc;
     constexpr int CH = 16 / sizeof(T), NT = LANES > 256 ? LANES : 256, COLS = NT / LANES, SPAN = LANES * VPL * CH;
@@ -307,7 +323,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layer_norm_grad_ker
                 if (weight) g[j] *= v[j];
                 g[j] = rstd * (g[j] - m0 - (h[j] - mean) * rstd * m1);
             }
-            write_chunk(dX + c * lddx + at, left, g);
+            write_chunk(dX + c * lddx + at, left, g, streamed);
         }
     }
     if (!parts) return;
@@ -470,7 +486,8 @@ int layer_norm(int64_t d, int64_t cols, const void *X, int64_t ldx, const void *
         constexpr int L = decltype(span)::lanes, V = decltype(span)::vpl, NT = L > 256 ? L : 256;
         const int64_t blocks = (cols + NT / L - 1) / (NT / L);
         hipLaunchKernelGGL((layer_norm_kernel<T, L, V>), dim3((unsigned)(blocks < LN_BLOCKS ? blocks : LN_BLOCKS)), dim3(NT), 0, s, d, cols,
-                           (const T *)X, ldx, (const T *)weight, (const T *)bias, (A)eps, (T *)Y, ldy, (A *)stats, lds);
+                           (const T *)X, ldx, (const T *)weight, (const T *)bias, (A)eps, (T *)Y, ldy, (A *)stats, lds,
+                           d * cols * (int64_t)sizeof(T) > STREAMED);
     });
     if (!held)
         hipLaunchKernelGGL((layer_norm_long_kernel<T>), dim3((unsigned)(cols < 8192 ? cols : 8192)), dim3(1024), 0, s, d, cols,
@@ -503,7 +520,8 @@ int layer_norm_grad(int64_t d, int64_t cols, const void *X, int64_t ldx, const v
         if (blocks > most) blocks = most;
         if (parts(blocks) || !blocks) return;
         hipLaunchKernelGGL((layer_norm_grad_kernel<T, L, V>), dim3((unsigned)blocks), dim3(NT), 0, s, d, cols, (const T *)X, ldx,
-                           (const T *)dY, lddy, (const A *)stats, lds, (const T *)weight, (T *)dX, lddx, (A *)ws);
+                           (const T *)dY, lddy, (const A *)stats, lds, (const T *)weight, (T *)dX, lddx, (A *)ws,
+                           d * cols * (int64_t)sizeof(T) > STREAMED);
         st = check_launch("layer_norm_grad_kernel");
     });
     if (!held && cols) {
