@@ -399,6 +399,36 @@ def test_layer_norm_many_columns(J, T, d, cols):
     assert torch.equal(again, dw)                         # the same sums in the same order
 
 
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("d,cols,pad,skip", [(2047, 9001, 0, 0), (1024, 17_000, 3, 1), (4096, 4200, 0, 0)])
+def test_layer_norm_large_results(J, T, d, cols, pad, skip):
+    """Results past the caches' size are those of the same columns in small calls, to
+    the bit, and what lies between their columns stays as it was."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+
+    def matrix(fill=None):
+        t = torch.empty(cols * (d + pad) + skip, dtype=T, device="cuda")
+        t.normal_(generator=gen) if fill is None else t.fill_(fill)
+        return t, t[skip:].view(cols, d + pad)[:, :d].t()
+
+    X, dY = matrix()[1], matrix()[1]
+    ybuf, Y = matrix(7.0)
+    dbuf, dX = matrix(7.0)
+    w = torch.randn(d, generator=gen, device="cuda").to(T)
+    S = torch.empty((cols, 2), dtype=torch.float64 if T == torch.float64 else torch.float32, device="cuda").t()
+    J.execute(J.LayerNormOp, X, Y, weight=w, bias=w, stats=S)
+    J.execute(J.LayerNormGradOp, X, dY, S, weight=w, dX=dX)
+    step = 500
+    for c in range(0, cols, step):
+        at = slice(c, c + step)
+        y, dx = torch.empty_like(Y[:, at]), torch.empty_like(Y[:, at])
+        J.execute(J.LayerNormOp, X[:, at], y, weight=w, bias=w)
+        J.execute(J.LayerNormGradOp, X[:, at], dY[:, at], S[:, at], weight=w, dX=dx)
+        assert torch.equal(Y[:, at], y) and torch.equal(dX[:, at], dx), c
+    for buf in (ybuf, dbuf):
+        assert torch.all(buf[:skip] == 7) and torch.all(buf[skip:].view(cols, d + pad)[:, d:] == 7)
+
+
 def test_layer_norm_gradient_against_differences(J):
     """Central differences (step 1e-5) of the 64-bit form, 1e-8 for their error."""
     T, d, cols = torch.float64, 9, 4
