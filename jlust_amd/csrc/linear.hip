@@ -267,38 +267,40 @@ __global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m,
     }
 }
 
-// Rows src[idx[p]] (or src[p]) of `len` values for p < rows (or offsets[groups]),
-// 16-byte aligned and `ld` apart, zeros at their ends: what the copies of
-// tile_kernel.hpp take.
+// Rows src[idx[p]] (or src[p]) of `len` values for p < rows (or offsets[groups]) of
+// each of the blockIdx.y matrices, `stride` apart, 16-byte aligned and `ld` apart,
+// zeros at their ends: what the copies of tile_kernel.hpp take.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(int64_t rows, int64_t len, const T *__restrict__ src, int64_t lds_,
-                                                        int64_t per, int64_t stride, const int32_t *__restrict__ idx,
+                                                        int64_t stride, const int32_t *__restrict__ idx,
                                                         const int32_t *__restrict__ limit, T *__restrict__ out, int64_t ld)
 {
     constexpr int V = 16 / sizeof(T);
     // 32 chunks along a row by 8 rows.
     const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (p >= rows || (limit && p >= *limit)) return;
-    const int64_t r = idx ? (int64_t)idx[p] : p;
-    const T *from = src + (stride ? r / per * stride + r % per * lds_ : r * lds_);
+    const T *from = src + blockIdx.y * stride + (idx ? (int64_t)idx[p] : p) * lds_;
+    T *to = out + (blockIdx.y * rows + p) * ld;
     for (int64_t c = (int64_t)(threadIdx.x & 31) * V; c < ld; c += 32 * V) {
         const int64_t left = len - c;
         const T *q = from + c;
         const uint32x4 v = left >= V ? load_chunk(q) : load_chunk_part(q, left);
-        __builtin_memcpy(out + p * ld + c, &v, 16);
+        __builtin_memcpy(to + c, &v, 16);
     }
 }
 
-// rows in runs of `per`, `stride` apart (the groups' matrices; else one run).
 template <typename T>
-int pack_rows(int64_t rows, int64_t len, const void *src, int64_t lds, int64_t per, int64_t stride, const int32_t *idx,
+int pack_rows(int64_t rows, int64_t len, const void *src, int64_t lds, int64_t matrices, int64_t stride, const int32_t *idx,
               const int32_t *limit, void *out, int64_t ld, hipStream_t s)
 {
     if (rows == 0 || ld == 0) return JLUST_STATUS_SUCCESS;
-    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, rows, len, (const T *)src, lds,
-                       per, stride, idx, limit, (T *)out, ld);
+    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)((rows + 7) / 8), (unsigned)matrices), dim3(256), 0, s, rows, len,
+                       (const T *)src, lds, stride, idx, limit, (T *)out, ld);
     return check_launch("pack_rows_kernel");
 }
+
+// The matrices that groups' packed weights take: one where the groups share it.
+int64_t packed_matrices(int64_t groups, int64_t w_stride) { return groups && w_stride ? groups : 1; }
 
 template <typename T>
 int64_t padded(int64_t len)
@@ -506,13 +508,14 @@ int linear(const jlust_linear &op, jlust_stream_t stream)
     const int64_t batch = op.groups ? op.groups : 1, w_rows = pkc ? op.out : op.inp, w_len = pkc ? op.inp : op.out;
     const int64_t x_rows = op.cols / (op.groups ? op.copies : 1), ldw = padded<T>(w_len), ldx = padded<T>(op.inp);
     const bool bad_w = !lies_well<T>(op.W, w_len, op.ldw, op.groups ? op.w_stride : 0), bad_x = !lies_well<T>(op.X, op.inp, op.ldx, 0);
-    const int64_t w_values = bad_w ? batch * w_rows * ldw : 0, x_values = bad_x ? x_rows * ldx : 0;
+    const int64_t matrices = packed_matrices(op.groups, op.w_stride);
+    const int64_t w_values = bad_w ? matrices * w_rows * ldw : 0, x_values = bad_x ? x_rows * ldx : 0;
     size_t pack = 0;
     if (op.cols > 48 * batch && worth_packing<T>(op.out, op.cols, op.inp, w_values + x_values, bad_w && !pkc)) {
         if (bad_w) {
             a.P = nullptr;
             a.ldp = ldw;
-            a.gp = w_rows * ldw;
+            a.gp = matrices > 1 ? w_rows * ldw : 0;
             a.p_pad = true;
         }
         if (bad_x) {
@@ -531,12 +534,12 @@ int linear(const jlust_linear &op, jlust_stream_t stream)
         if (int st = scratch(stream, pack + bytes, &ws)) return st;
         char *at = (char *)ws;
         if (a.p_pad) {
-            if (int st = pack_rows<T>(batch * w_rows, w_len, op.W, op.ldw, w_rows, op.w_stride, nullptr, nullptr, at, ldw, s)) return st;
+            if (int st = pack_rows<T>(w_rows, w_len, op.W, op.ldw, matrices, op.w_stride, nullptr, nullptr, at, ldw, s)) return st;
             a.P = at;
             at += align256(sizeof(T) * w_values);
         }
         if (a.q_pad) {
-            if (int st = pack_rows<T>(x_rows, op.inp, op.X, op.ldx, x_rows, 0, nullptr, nullptr, at, ldx, s)) return st;
+            if (int st = pack_rows<T>(x_rows, op.inp, op.X, op.ldx, 1, 0, nullptr, nullptr, at, ldx, s)) return st;
             a.Q = at;
             at += align256(sizeof(T) * x_values);
         }
@@ -562,14 +565,14 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
     // copies waited for the indexes: 262 us of 573 in the gradients of 32 experts).
     // X is sorted with it.  Else what lies badly, where it pays.
     const bool x_kc = op.w_layout == 0;
-    const int64_t x_rows = n / (op.groups ? op.copies : 1), w_rows = x_kc ? inp : out, w_len = x_kc ? out : inp;
+    const int64_t w_rows = x_kc ? inp : out, w_len = x_kc ? out : inp, matrices = packed_matrices(op.groups, op.w_stride);
     const int64_t ldg_made = padded<T>(out), ldx_made = padded<T>(inp), ldw_made = padded<T>(w_len);
     bool make_g = (slope && (op.dX || op.dW)) || (op.groups && op.dW), make_x = op.groups && op.dW, make_w = false;
     {
         const bool bad_g = !lies_well<T>(op.dY, out, op.lddy, 0), bad_x = !lies_well<T>(op.X, inp, op.ldx, 0);
         const bool bad_w = !lies_well<T>(op.W, w_len, op.ldw, op.groups ? op.w_stride : 0);
         const int64_t g_values = bad_g && !make_g ? n * ldg_made : 0;
-        const int64_t w_values = bad_w ? batch * w_rows * ldw_made : 0, x_values = bad_x && !make_x ? n * ldx_made : 0;
+        const int64_t w_values = bad_w ? matrices * w_rows * ldw_made : 0, x_values = bad_x && !make_x ? n * ldx_made : 0;
         if (op.dX && n > 48 * batch && worth_packing<T>(inp, n, out, g_values + w_values, bad_w && !x_kc)) {
             make_g |= g_values > 0;
             make_w = bad_w;
@@ -601,7 +604,7 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         x.k = out;
         x.P = make_w ? nullptr : op.W;             // the plan goes by alignment: what is made has any
         x.ldp = make_w ? ldw_made : op.ldw;
-        x.gp = make_w ? w_rows * ldw_made : op.w_stride;
+        x.gp = make_w ? (matrices > 1 ? w_rows * ldw_made : 0) : op.w_stride;
         x.p_pad = make_w;
         x.Q = G;
         x.ldq = ldg;
@@ -642,7 +645,7 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
     const int64_t runs = (n + per - 1) / per + (op.groups ? (op.groups < n ? op.groups : n) : 0);
     const size_t g_bytes = make_g ? align256(sizeof(T) * n * ldg) : 0;
     const size_t x_bytes = make_x ? align256(sizeof(T) * n * ldx_made) : 0;
-    const size_t w_bytes = make_w ? align256(sizeof(T) * batch * w_rows * ldw_made) : 0, made = g_bytes + x_bytes + w_bytes;
+    const size_t w_bytes = make_w ? align256(sizeof(T) * matrices * w_rows * ldw_made) : 0, made = g_bytes + x_bytes + w_bytes;
     const size_t wide_bytes = wide ? align256(sizeof(A) * n * inp) : 0;
     const size_t part = align256(part_x > part_w ? part_x : part_w);
     const size_t sum_bytes = op.dbias ? sizeof(A) * runs * out : 0;
@@ -659,13 +662,13 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         (op.w_layout ? w.Q : w.P) = g_buf;
     }
     if (make_x) {
-        if (int st = pack_rows<T>(n, inp, op.X, op.ldx, x_rows, 0, pl.src, pl.offsets ? pl.offsets + op.groups : nullptr, x_buf,
+        if (int st = pack_rows<T>(n, inp, op.X, op.ldx, 1, 0, pl.src, pl.offsets ? pl.offsets + op.groups : nullptr, x_buf,
                                   ldx_made, s))
             return st;
         (op.w_layout ? w.P : w.Q) = x_buf;
     }
     if (make_w) {
-        if (int st = pack_rows<T>(batch * w_rows, w_len, op.W, op.ldw, w_rows, op.w_stride, nullptr, nullptr, w_buf, ldw_made, s))
+        if (int st = pack_rows<T>(w_rows, w_len, op.W, op.ldw, matrices, op.w_stride, nullptr, nullptr, w_buf, ldw_made, s))
             return st;
         x.P = w_buf;
     }

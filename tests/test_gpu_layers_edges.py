@@ -1,0 +1,55 @@
+"""Layer operators on the GPU where they went wrong once, or where the chosen
+kernel has to be named: against the plain 64-bit forms of tests/_layers.py."""
+import pytest
+import torch
+
+from tests import _layers as L
+from tests.test_gpu_layers import case, some_ids, weights
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def J():
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    import jlust_amd
+    return jlust_amd
+
+
+@pytest.mark.parametrize("T", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", ["out", "inp"])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_groups_that_share_a_matrix(J, T, layout, act):
+    """W.expand over the groups, its rows off any alignment, in products large enough
+    to pack it first: the bits of the same call on a matrix per group, and the 64-bit
+    form at some columns."""
+    out, inp, cols, groups = 1000, 1024, 16384, 3
+    s = case(1, T, out, inp, cols, layout, act, True, False, groups, pad=0)
+    one = weights(out, inp, 1, T, torch.Generator().manual_seed(9), layout, pad=1, skip=1)
+    shared, apart = one.expand(out, inp, groups), weights(out, inp, groups, T, torch.Generator(), layout, pad=1, skip=1)
+    assert shared.stride(2) == 0
+    apart.copy_(shared)
+    ids = torch.from_numpy(some_ids(cols, groups, 4, 0.1)).cuda()
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
+    fn = {None: None, "gelu": J.gelu_fn}[act]
+    Y = torch.empty_like(s["Y"])
+    J.execute(h, apart, s["X"], Y, bias=s["b"], act=fn)
+    J.execute(h, shared, s["X"], s["Y"], bias=s["b"], act=fn, preact=s["Z"])
+    assert torch.equal(s["Y"], Y)
+    at = list(range(0, cols, 97)) + [cols - 1]
+    ref, refz, ey, ez = L.forward(apart, s["X"][:, at], s["b"], act, None, ids[at], 1)
+    L.close(s["Y"][:, at], ref, ey, "Y")
+    L.close(s["Z"][:, at], refz, ez, "Z")
+
+    dY = torch.randn((cols, out), generator=torch.Generator().manual_seed(5)).to(T).cuda().t()
+    got = []
+    for W in (apart, shared):
+        dX, dW = torch.empty_like(s["X"]), torch.empty_like(apart)
+        J.execute(J.GroupedLinearGradOp, h, W, s["X"], dY, act=fn, preact=s["Z"] if act else None, dX=dX, dW=dW)
+        only = torch.empty_like(dX)
+        J.execute(J.GroupedLinearGradOp, h, W, s["X"], dY, act=fn, preact=s["Z"] if act else None, dX=only)
+        got.append((dX, dW, only))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    ref = L.gradients(apart, s["X"][:, at], dY[:, at], s["Z"][:, at], act, ids[at], 1)["dX"]
+    for i in (0, 2):
+        L.close(got[1][i][:, at], *ref, "dX")
