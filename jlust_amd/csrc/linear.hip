@@ -801,8 +801,9 @@ extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t
         return st;
     const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
     const int64_t wr = op->w_layout ? op->inp : op->out, wc = op->w_layout ? op->out : op->inp;
-    if (int st = check_operands(who, {{"W", op->W, wr, wc, op->ldw, op->dX != nullptr},
-                                      {"X", op->X, op->inp, xcols, op->ldx, op->dW != nullptr},
+    // W is read for dX alone (it may be laid out otherwise beside a dW), X for dW alone.
+    if (int st = check_operands(who, {{"W", op->dX ? op->W : nullptr, wr, wc, op->ldw, op->dX != nullptr},
+                                      {"X", op->dW ? op->X : nullptr, op->inp, xcols, op->ldx, op->dW != nullptr},
                                       {"dY", op->dY, op->out, op->cols, op->lddy, true},
                                       {"Z", op->Z, op->out, op->cols, op->ldz, op->act != JLUST_FN_IDENTITY},
                                       {"dX", op->dX, op->inp, xcols, op->lddx, false},

@@ -53,3 +53,34 @@ def test_groups_that_share_a_matrix(J, T, layout, act):
     ref = L.gradients(apart, s["X"][:, at], dY[:, at], s["Z"][:, at], act, ids[at], 1)["dX"]
     for i in (0, 2):
         L.close(got[1][i][:, at], *ref, "dX")
+
+
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("layout", ["out", "inp"])
+@pytest.mark.parametrize("out,inp", [(40, 70), (70, 40), (1, 9), (9, 1)])
+@pytest.mark.parametrize("groups", [None, 3])
+def test_gradient_of_the_other_layout(J, T, layout, out, inp, groups):
+    """dW contiguous along the other side than W, with dX and dbias and alone: the
+    64-bit form, and dX and dbias as in the call with dW laid out as W."""
+    s = case(2, T, out, inp, 50, layout, "relu", True, False, groups)
+    gen = torch.Generator().manual_seed(3)
+    dY, Z = (L.colmajor(out, 50, T, gen) for _ in range(2))
+    ids = h = None
+    if groups:
+        ids = torch.from_numpy(some_ids(50, groups, 4, 0.1)).cuda()
+        h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
+    ref = L.gradients(s["W"], s["X"], dY, Z, "relu", ids, 1)
+
+    def run(**out):
+        for v in out.values():
+            v.fill_(float("nan"))
+        op = (J.LinearGradOp,) if h is None else (J.GroupedLinearGradOp, h)
+        J.execute(*op, s["W"], s["X"], dY, act=J.relu_fn, preact=Z, **out)
+        return out
+
+    same = run(dX=torch.empty_like(s["X"]), dW=torch.empty_like(s["W"]), dbias=torch.empty_like(s["b"]))
+    other = lambda: weights(out, inp, groups, T, gen, "inp" if layout == "out" else "out")  # noqa: E731
+    full, alone = run(dX=torch.empty_like(s["X"]), dW=other(), dbias=torch.empty_like(s["b"])), run(dW=other())
+    assert torch.equal(full["dX"], same["dX"]) and torch.equal(full["dbias"], same["dbias"])
+    for got in (full, alone):
+        L.close(got["dW"], *ref["dW"], "dW")

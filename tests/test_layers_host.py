@@ -55,6 +55,16 @@ def test_linear_grad_refuses(bad, status):
     assert grad(**bad) == status
 
 
+@pytest.mark.parametrize("only", [dict(dX=0, dW=64, W=64, ldw=64, lddw=128, dbias=64),      # W 64 x 128 beside dW's transpose
+                                  dict(dX=0, dW=64, W=0, ldw=0, lddw=128),
+                                  dict(dX=64, lddx=128, dW=0, ldw=128, X=64, ldx=1),
+                                  dict(dX=0, dW=0, ldw=0, ldx=0, dbias=64)])
+def test_linear_grad_checks_what_it_reads(only):
+    """W is read for dX alone and X for dW alone; the null dY is what is refused."""
+    assert grad(out=64, inp=128, w_layout=1, **{**dict(lddy=64, ldx=128), **only}, dY=0) == 1
+    assert "dY is null" in _lib.last_error()
+
+
 def test_group_plan_and_layer_norm_refuse():
     L, n = _lib.lib(), ctypes.c_int64()
     assert L.jlust_hip_group_plan_ints(10, 3, 1, ctypes.byref(n)) == 0 and n.value == 14
