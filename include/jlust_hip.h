@@ -1193,7 +1193,8 @@ int jlust_hip_linear(const jlust_linear *op, jlust_stream_t stream);
  * Its gradients: with G = dY .* act'.(Z), dX = W'*G, dW = G*X' and dbias =
  * G's row sums, each where its pointer is not null (dW laid out as W, dbias as
  * bias; groups: each column to its own group's, and the copies' sum in dX; a
- * group without columns gets zeros).  Z is what the forward call kept; unused
+ * group without columns gets zeros; groups' matrices that overlap in dW or dbias
+ * are NONCANONICAL_STORAGE).  Z is what the forward call kept; unused
  * for JLUST_FN_IDENTITY.  W is read for dX alone and X for dW alone, so a dW
  * laid out otherwise than W takes a call of its own.  G is rounded to the value
  * type once, for the two products; dbias sums it as it is.

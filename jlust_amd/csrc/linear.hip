@@ -436,6 +436,19 @@ int check_operands(const char *who, std::initializer_list<Operand> ops)
     return JLUST_STATUS_SUCCESS;
 }
 
+// The matrices of a result's groups must not share memory: each lies behind the one
+// before, or all of them within one's leading dimension.
+int check_apart(const char *who, const char *name, const void *p, int64_t rows, int64_t cols, int64_t ld, int64_t groups,
+                int64_t stride)
+{
+    if (!p || groups < 2 || rows == 0 || cols == 0) return JLUST_STATUS_SUCCESS;
+    const int64_t by = stride < 0 ? -stride : stride;
+    const bool behind = by >= (cols > 1 ? (cols - 1) * ld : 0) + rows, within = by >= rows && ld >= (groups - 1) * by + rows;
+    if (behind || within) return JLUST_STATUS_SUCCESS;
+    return fail(JLUST_STATUS_NONCANONICAL_STORAGE, "%s: the groups' matrices of %s overlap (%lld x %lld, leading dimension %lld, "
+                "%lld elements from one to the next)", who, name, (long long)rows, (long long)cols, (long long)ld, (long long)stride);
+}
+
 int check_common(const char *who, int32_t value_type, int32_t act, int32_t w_layout, int64_t out, int64_t inp, int64_t cols,
                  int64_t groups, int64_t copies, const int32_t *plan)
 {
@@ -801,6 +814,8 @@ extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t
         return st;
     const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
     const int64_t wr = op->w_layout ? op->inp : op->out, wc = op->w_layout ? op->out : op->inp;
+    if (int st = check_apart(who, "dW", op->dW, wr, wc, op->lddw, op->groups, op->dw_stride)) return st;
+    if (int st = check_apart(who, "dbias", op->dbias, op->out, 1, op->out, op->groups, op->dbias_stride)) return st;
     // W is read for dX alone (it may be laid out otherwise beside a dW), X for dW alone.
     if (int st = check_operands(who, {{"W", op->dX ? op->W : nullptr, wr, wc, op->ldw, op->dX != nullptr},
                                       {"X", op->dW ? op->X : nullptr, op->inp, xcols, op->ldx, op->dW != nullptr},

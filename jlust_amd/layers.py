@@ -150,12 +150,6 @@ def _bias(t, name, out, groups, index, T):
     return t.data_ptr(), t.stride(1) if groups else 0
 
 
-def _apart(stride, per, groups, name):
-    """A result's groups must not share memory."""
-    if groups > 1 and abs(stride) < per:
-        raise NonCanonicalStorage(f"{name}: the groups' matrices overlap (stride {stride}, {per} elements each)")
-
-
 def _act(act):
     if act is None:
         return FN_IDENTITY
@@ -309,13 +303,11 @@ def _linear_grad(h, W, X, dY, act=None, preact=None, dX=None, dW=None, dbias=Non
         dwp, wlayout, lddw, dws, o, i = _weights(_raw(dW, "dW"), "dW", groups, index, T)
         if (o, i) != (out, inp):
             raise IncompatibleExtents(f"dW is {o}x{i}, expected {out}x{inp}")
-        _apart(dws, out * inp, groups, "dW")
     dbp, dbs = _bias(dbias, "dbias", out, groups, index, T)
-    if dbp:
-        _apart(dbs, out, groups, "dbias")
-    # dW beside dX in one call where they are laid out alike.
+    # dW beside dX in one call where they are laid out alike; else first what the call
+    # may refuse, groups that overlap.
     calls = [(layout if dxp else wlayout, dxp, dwp, dbp)] if wlayout == layout or not (dxp and dwp) else \
-        [(layout, dxp, 0, dbp), (wlayout, 0, dwp, 0)]
+        [(wlayout, 0, dwp, dbp), (layout, dxp, 0, 0)]
     for lay, a, b, c in calls:
         _run(_lib.lib().jlust_hip_linear_grad, index, "linear_grad", T,
              _LINEAR_GRAD(vt, kind, lay, 0, out, inp, n, wp, ldw, xp, ldx, dyp, lddy, zp, ldz, a, lddx, b, lddw, c, groups,

@@ -84,3 +84,33 @@ def test_gradient_of_the_other_layout(J, T, layout, out, inp, groups):
     assert torch.equal(full["dX"], same["dX"]) and torch.equal(full["dbias"], same["dbias"])
     for got in (full, alone):
         L.close(got["dW"], *ref["dW"], "dW")
+
+
+@pytest.mark.parametrize("T", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [60, 3000])
+@pytest.mark.parametrize("other", [False, True])
+def test_gradient_of_interleaved_groups(J, T, cols, other):
+    """dW and dbias whose groups lie within each other's leading dimension (an inp x
+    groups x out array, or its transpose's), beside W as it is usual; what overlaps
+    is refused before anything is written."""
+    out, inp, groups = 72, 40, 3
+    s = case(6, T, out, inp, cols, "out", None, True, False, groups)
+    dY = L.colmajor(out, cols, T, torch.Generator().manual_seed(1))
+    ids = torch.from_numpy(some_ids(cols, groups, 4, 0.1)).cuda()
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
+    ref = L.gradients(s["W"], s["X"], dY, None, None, ids, 1)
+    a, b = (inp, out) if other else (out, inp)
+    dW = torch.full((b, groups, a), float("nan"), dtype=T, device="cuda").permute(2, 0, 1)
+    dW = dW.transpose(0, 1) if other else dW
+    dX, db = torch.full_like(s["X"], float("nan")), torch.full_like(s["b"], float("nan"))
+    J.execute(J.GroupedLinearGradOp, h, s["W"], s["X"], dY, dX=dX, dW=dW, dbias=db)
+    for k, v in (("dX", dX), ("dW", dW), ("dbias", db)):
+        L.close(v, *ref[k], k)
+    buf = torch.zeros(groups * (a + 1) * b + 64, dtype=T, device="cuda")
+    over = torch.as_strided(buf, (a, b, groups), (1, a + 1, a * b))
+    over = over.transpose(0, 1) if other else over
+    dX.fill_(5)
+    for bad in (dict(dW=over, dbias=db), dict(dW=dW, dbias=db[:, :1].expand(out, groups))):
+        with pytest.raises(J.NonCanonicalStorage):
+            J.execute(J.GroupedLinearGradOp, h, s["W"], s["X"], dY, dX=dX, **bad)
+    assert (dX == 5).all() and (buf == 0).all()

@@ -65,6 +65,21 @@ def test_linear_grad_checks_what_it_reads(only):
     assert "dY is null" in _lib.last_error()
 
 
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("rows,cols,ld,stride", [(4, 6, 4, 24), (4, 6, 4, 26), (4, 6, 12, 4), (4, 6, 5, 24), (4, 6, 5, 29), (4, 6, 5, 28),
+                                                 (4, 6, 11, 4), (4, 6, 12, 3), (4, 6, 4, 0), (4, 6, 4, -24), (4, 6, 4, -23),
+                                                 (4, 1, 4, 4), (4, 1, 4, 3), (1, 6, 3, 1), (1, 6, 2, 1)])
+def test_groups_of_a_gradient_do_not_overlap(layout, rows, cols, ld, stride):
+    """dW of three groups: refused just where two of them hold the same element, the
+    null dY being what is refused otherwise."""
+    at = [g * stride + j * ld + i for g in range(3) for j in range(cols) for i in range(rows)]
+    out, inp = (rows, cols) if layout == 0 else (cols, rows)
+    st = grad(out=out, inp=inp, cols=6, w_layout=layout, dX=0, dW=1 << 20, lddw=ld, dw_stride=stride, ldx=inp, lddy=out, groups=3,
+              plan=64, dY=0)
+    assert st == (4 if len(set(at)) < len(at) else 1)
+    assert ("overlap" if st == 4 else "dY is null") in _lib.last_error()
+
+
 def test_group_plan_and_layer_norm_refuse():
     L, n = _lib.lib(), ctypes.c_int64()
     assert L.jlust_hip_group_plan_ints(10, 3, 1, ctypes.byref(n)) == 0 and n.value == 14
