@@ -1141,7 +1141,9 @@ int jlust_hip_shifted_diag_spmm_f32(int64_t m, int64_t n, int64_t k,
  * counterpart in the reference, whose GPU paths leave them to the caller's
  * array library): a column is one node of a graph, one token or one sample.
  * Values are Float64, Float32, Float16 or BFloat16, one type for all operands
- * of a call; sums and statistics are Float32 (Float64 for Float64).
+ * of a call; sums and statistics are Float32 (Float64 for Float64).  Extents are
+ * below 2^31; a product of some 2^24 tiles or more (of 64 x 64 sums, or 128 x 16
+ * for few columns) is INVALID_ARGUMENT: one launch does not take it.
  */
 enum jlust_value_type {
     JLUST_VALUE_F64 = 0,

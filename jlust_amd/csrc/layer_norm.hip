@@ -440,20 +440,24 @@ __global__ __launch_bounds__(1024) void layer_norm_parts_kernel(int64_t d, int64
     T *out = blockIdx.y ? dbias : dweight;
     if (!out) return;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t at = (int64_t)blockIdx.x * 32 + tx;
-    const A *p = parts + blockIdx.y * d + at;
-    A s = A(0);
-    if (at < d) {
+    // In turn where a launch would not take 32 threads for each of d (2^32 in all).
+    for (int64_t at0 = (int64_t)blockIdx.x * 32; at0 < d; at0 += (int64_t)gridDim.x * 32) {
+        const int64_t at = at0 + tx;
+        const A *p = parts + blockIdx.y * d + at;
+        A s = A(0);
+        if (at < d) {
 #pragma unroll 8
-        for (int64_t i = ty; i < count; i += 32) s += p[i * 2 * d];
-    }
-    s_sum[ty][tx] = s;
-    __syncthreads();
-    if (ty == 0 && at < d) {
-        A t = A(0);
+            for (int64_t i = ty; i < count; i += 32) s += p[i * 2 * d];
+        }
+        __syncthreads();
+        s_sum[ty][tx] = s;
+        __syncthreads();
+        if (ty == 0 && at < d) {
+            A t = A(0);
 #pragma unroll
-        for (int q = 0; q < 32; ++q) t += s_sum[q][tx];
-        out[at] = T(t);
+            for (int q = 0; q < 32; ++q) t += s_sum[q][tx];
+            out[at] = T(t);
+        }
     }
 }
 
@@ -543,7 +547,7 @@ int layer_norm_grad(int64_t d, int64_t cols, const void *X, int64_t ldx, const v
         }
     }
     if (st || !sums) return st;
-    hipLaunchKernelGGL((layer_norm_parts_kernel<T>), dim3((unsigned)((d + 31) / 32), 2), dim3(1024), 0, s, d, count,
+    hipLaunchKernelGGL((layer_norm_parts_kernel<T>), dim3((unsigned)(d < 1 << 26 ? (d + 31) / 32 : 1 << 21), 2), dim3(1024), 0, s, d, count,
                        (const A *)ws, (T *)dweight, (T *)dbias);
     return check_launch("layer_norm_parts_kernel");
 }

@@ -267,6 +267,14 @@ __global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m,
     }
 }
 
+// A launch takes fewer than 2^32 threads (of more it runs their number modulo 2^32,
+// without an error): at most 2^21 workgroups, which walk over the items in turn.
+unsigned blocks_for(int64_t items, int64_t each)
+{
+    const int64_t blocks = (items + each - 1) / each;
+    return (unsigned)(blocks < 1 << 21 ? blocks : 1 << 21);
+}
+
 // Rows src[idx[p]] (or src[p]) of `len` values for p < rows (or offsets[groups]) of
 // each of the blockIdx.y matrices, `stride` apart, 16-byte aligned and `ld` apart,
 // zeros at their ends: what the copies of tile_kernel.hpp take.
@@ -276,16 +284,17 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(int64_t rows, int64_t le
                                                         const int32_t *__restrict__ limit, T *__restrict__ out, int64_t ld)
 {
     constexpr int V = 16 / sizeof(T);
+    const int64_t end = limit && *limit < rows ? *limit : rows;
     // 32 chunks along a row by 8 rows.
-    const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (p >= rows || (limit && p >= *limit)) return;
-    const T *from = src + blockIdx.y * stride + (idx ? (int64_t)idx[p] : p) * lds_;
-    T *to = out + (blockIdx.y * rows + p) * ld;
-    for (int64_t c = (int64_t)(threadIdx.x & 31) * V; c < ld; c += 32 * V) {
-        const int64_t left = len - c;
-        const T *q = from + c;
-        const uint32x4 v = left >= V ? load_chunk(q) : load_chunk_part(q, left);
-        __builtin_memcpy(to + c, &v, 16);
+    for (int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); p < end; p += (int64_t)gridDim.x * 8) {
+        const T *from = src + blockIdx.y * stride + (idx ? (int64_t)idx[p] : p) * lds_;
+        T *to = out + (blockIdx.y * rows + p) * ld;
+        for (int64_t c = (int64_t)(threadIdx.x & 31) * V; c < ld; c += 32 * V) {
+            const int64_t left = len - c;
+            const T *q = from + c;
+            const uint32x4 v = left >= V ? load_chunk(q) : load_chunk_part(q, left);
+            __builtin_memcpy(to + c, &v, 16);
+        }
     }
 }
 
@@ -294,7 +303,7 @@ int pack_rows(int64_t rows, int64_t len, const void *src, int64_t lds, int64_t m
               const int32_t *limit, void *out, int64_t ld, hipStream_t s)
 {
     if (rows == 0 || ld == 0) return JLUST_STATUS_SUCCESS;
-    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3((unsigned)((rows + 7) / 8), (unsigned)matrices), dim3(256), 0, s, rows, len,
+    hipLaunchKernelGGL((pack_rows_kernel<T>), dim3(blocks_for(rows, 8), (unsigned)matrices), dim3(256), 0, s, rows, len,
                        (const T *)src, lds, stride, idx, limit, (T *)out, ld);
     return check_launch("pack_rows_kernel");
 }
@@ -353,19 +362,22 @@ __global__ __launch_bounds__(32 * LANES) void grad_bias_kernel(int64_t n, int64_
         first = s_first;
         count = (offsets[group + 1] - offsets[group] + per - 1) / per;
     }
-    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
-    A s = A(0);
-    if (c < m) {
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < m; c0 += (int64_t)gridDim.x * 32) {
+        const int64_t c = c0 + tx;
+        A s = A(0);
+        if (c < m) {
 #pragma unroll 8
-        for (int64_t i = ty; i < count; i += LANES) s += sums[(first + i) * m + c];
-    }
-    s_sum[ty][tx] = s;
-    __syncthreads();
-    if (ty == 0 && c < m) {
-        A t = A(0);
+            for (int64_t i = ty; i < count; i += LANES) s += sums[(first + i) * m + c];
+        }
+        __syncthreads();
+        s_sum[ty][tx] = s;
+        __syncthreads();
+        if (ty == 0 && c < m) {
+            A t = A(0);
 #pragma unroll
-        for (int q = 0; q < LANES; ++q) t += s_sum[q][tx];
-        dbias[group * stride + c] = T(t);
+            for (int q = 0; q < LANES; ++q) t += s_sum[q][tx];
+            dbias[group * stride + c] = T(t);
+        }
     }
 }
 
@@ -377,43 +389,44 @@ __global__ __launch_bounds__(256) void sum_copies_kernel(int64_t cols, int64_t d
 {
     using A = typename Elem<T>::Acc;
     constexpr int V = 4;
-    const int64_t per = (d + V - 1) / V, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= cols * per) return;
-    const int64_t t = at / per, c = (at - t * per) * V;
-    const A *p = src + t * copies * d + c;
-    A s[V] = {0, 0, 0, 0};
-    T o[V];
-    if (c + V <= d) {
-        for (int q = 0; q < copies; ++q, p += d) {
-            A v[V];
-            load_vec<V>(p, v);
+    const int64_t per = (d + V - 1) / V;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < cols * per; at += (int64_t)gridDim.x * 256) {
+        const int64_t t = at / per, c = (at - t * per) * V;
+        const A *p = src + t * copies * d + c;
+        if (c + V <= d) {
+            A s[V] = {0, 0, 0, 0};
+            T o[V];
+            for (int q = 0; q < copies; ++q, p += d) {
+                A v[V];
+                load_vec<V>(p, v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) s[e] += v[e];
+                for (int e = 0; e < V; ++e) s[e] += v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = T(s[e]);
+            store_vec<V>(dX + t * ldx + c, o);
+            continue;
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = T(s[e]);
-        store_vec<V>(dX + t * ldx + c, o);
-        return;
-    }
-    for (int e = 0; c + e < d; ++e) {
-        A v = A(0);
-        for (int q = 0; q < copies; ++q) v += p[q * d + e];
-        dX[t * ldx + c + e] = T(v);
+        for (int e = 0; c + e < d; ++e) {
+            A v = A(0);
+            for (int q = 0; q < copies; ++q) v += p[q * d + e];
+            dX[t * ldx + c + e] = T(v);
+        }
     }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void fill_zero_kernel(int64_t rows, int64_t d, T *__restrict__ out, int64_t ld)
 {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at < rows * d) out[at / d * ld + at % d] = T(0);
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < rows * d; at += (int64_t)gridDim.x * 256)
+        out[at / d * ld + at % d] = T(0);
 }
 
 template <typename T>
 int fill_zero(int64_t rows, int64_t d, void *out, int64_t ld, hipStream_t s)
 {
     if (rows * d == 0) return JLUST_STATUS_SUCCESS;
-    hipLaunchKernelGGL((fill_zero_kernel<T>), dim3((unsigned)((rows * d + 255) / 256)), dim3(256), 0, s, rows, d, (T *)out, ld);
+    hipLaunchKernelGGL((fill_zero_kernel<T>), dim3(blocks_for(rows * d, 256)), dim3(256), 0, s, rows, d, (T *)out, ld);
     return check_launch("fill_zero_kernel");
 }
 
@@ -540,7 +553,7 @@ int linear(const jlust_linear &op, jlust_stream_t stream)
     }
     int shape = 0;
     size_t bytes = 0;
-    plan_tile_product<T>(&a, pkc, true, &shape, &bytes);
+    if (int st = plan_tile_product<T>(&a, pkc, true, &shape, &bytes)) return st;
     hipStream_t s = (hipStream_t)stream;
     if (pack + bytes) {
         void *ws = nullptr;
@@ -629,7 +642,7 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         x.C = op.dX;
         x.ldc = wide ? inp : op.lddx;
         x.c_wide = wide;
-        plan_tile_product<T>(&x, x_kc, true, &shape_x, &part_x);
+        if (int st = plan_tile_product<T>(&x, x_kc, true, &shape_x, &part_x)) return st;
     }
     TileArgs w;
     int shape_w = 0;
@@ -649,13 +662,16 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         w.C = op.dW;
         w.ldc = op.lddw;
         w.gc = op.dw_stride;
-        plan_tile_product<T>(&w, false, false, &shape_w, &part_w);
+        if (int st = plan_tile_product<T>(&w, false, false, &shape_w, &part_w)) return st;
     }
 
     const int64_t blocks_m = (out + Prepass<T>::COLS - 1) / Prepass<T>::COLS;
     int64_t per = (n * blocks_m + 2047) / 2048;                // about 2,048 workgroups
     per = per < 64 ? 64 : (per + 7) / 8 * 8;
     const int64_t runs = (n + per - 1) / per + (op.groups ? (op.groups < n ? op.groups : n) : 0);
+    if ((make_g || op.dbias) && runs * blocks_m >= 1 << 24)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_grad: dY of %lld x %lld (%lld groups) is more than one launch takes",
+                    (long long)out, (long long)n, (long long)op.groups);
     const size_t g_bytes = make_g ? align256(sizeof(T) * n * ldg) : 0;
     const size_t x_bytes = make_x ? align256(sizeof(T) * n * ldx_made) : 0;
     const size_t w_bytes = make_w ? align256(sizeof(T) * matrices * w_rows * ldw_made) : 0, made = g_bytes + x_bytes + w_bytes;
@@ -694,7 +710,7 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
             if (int st = check_launch("grad_prepass_kernel")) return st;
         }
         if (op.dbias) {
-            const dim3 grid((unsigned)((out + 31) / 32), (unsigned)(op.groups ? op.groups : 1));
+            const dim3 grid(blocks_for(out, 32), (unsigned)(op.groups ? op.groups : 1));
             const int32_t *offsets = n ? pl.offsets : nullptr;
             if (runs <= 32 * (op.groups ? op.groups : 1))
                 hipLaunchKernelGGL((grad_bias_kernel<T, 8>), grid, dim3(256), 0, s, n, out, offsets, (int)per, sums,
@@ -710,7 +726,7 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
         if (int st = launch_tile_product<T>(x, x_kc, true, shape_x, s)) return st;
         if (wide) {
             const int64_t cols = n / op.copies, items = cols * ((inp + 3) / 4);
-            hipLaunchKernelGGL((sum_copies_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, cols, inp,
+            hipLaunchKernelGGL((sum_copies_kernel<T>), dim3(blocks_for(items, 256)), dim3(256), 0, s, cols, inp,
                                (int)op.copies, wide_buf, (T *)op.dX, op.lddx);
             if (int st = check_launch("sum_copies_kernel")) return st;
         }

@@ -3,9 +3,9 @@
 
 namespace jlust {
 
-template void plan_tile_product<_Float16>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<_Float16>(TileArgs *, bool, bool, int *, size_t *);
 template int launch_tile_product<_Float16>(const TileArgs &, bool, bool, int, hipStream_t);
-template void plan_tile_product<__bf16>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<__bf16>(TileArgs *, bool, bool, int *, size_t *);
 template int launch_tile_product<__bf16>(const TileArgs &, bool, bool, int, hipStream_t);
 
 int preload_linear_half()

@@ -3,9 +3,9 @@
 
 namespace jlust {
 
-template void plan_tile_product<float>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<float>(TileArgs *, bool, bool, int *, size_t *);
 template int launch_tile_product<float>(const TileArgs &, bool, bool, int, hipStream_t);
-template void plan_tile_product<double>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<double>(TileArgs *, bool, bool, int *, size_t *);
 template int launch_tile_product<double>(const TileArgs &, bool, bool, int, hipStream_t);
 
 int preload_linear_wide()

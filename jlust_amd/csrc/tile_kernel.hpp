@@ -1014,10 +1014,11 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
 // matrix steps bound it, so its widths of 64 to 128 fit m instead (100 of 128 rows
 // would be a fifth of the steps for nothing) at 64 columns, where a CU holds
 // enough workgroups to hide the rows it reads and stores.
-struct TileShape { int bm, bn; };
+struct TileShape { int bm, bn, threads; };
 enum Shape { REG_128, REG_32, REG_16, REG_M128, REG_M112, REG_M96, REG_M80, REG_M64, COPY_256, COPY_TALL, COPY_128, FEW_16, FEW_32 };
-constexpr TileShape TILE_SHAPES[] = {{128, 128}, {128, 32}, {128, 16}, {128, 64}, {112, 64}, {96, 64}, {80, 64}, {64, 64},
-                                     {256, 256}, {256, 128}, {128, 128}, {16, 16}, {32, 16}};
+constexpr TileShape TILE_SHAPES[] = {{128, 128, 256}, {128, 32, 256}, {128, 16, 256}, {128, 64, 256}, {112, 64, 256},
+                                     {96, 64, 256}, {80, 64, 256}, {64, 64, 256}, {256, 256, 512}, {256, 128, 256},
+                                     {128, 128, 256}, {16, 16, Few<1>::WAVES * 64}, {32, 16, Few<2>::WAVES * 64}};
 
 // What a shape costs: its rate with a CU full of it (Tflop/s a CU), the time of 64 of
 // k where latency bounds it (us), workgroups a CU.  Measured on products of 64 to
@@ -1036,8 +1037,15 @@ bool copies_fit(const TileArgs &a, bool pkc, bool qkc)
     return (bits & 15) == 0 && (k | m | n) * z % 16 == 0 && a.ldp < (1 << 22) && a.ldq < (1 << 22);
 }
 
+// The workgroups that find_work counts on.
+inline int64_t work_groups(const TileArgs &a, bool ksum)
+{
+    const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.split * (ksum && a.offsets ? a.groups : 1);
+    return ((total + NUM_XCD - 1) / NUM_XCD + (a.offsets && !ksum ? 1 : 0)) * NUM_XCD;
+}
+
 template <typename T>
-void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes)
+int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes)
 {
     const bool ksum = !pkc && !qkc, grouped = a->offsets && !ksum;
     const int64_t batch = ksum && a->offsets ? a->groups : 1;
@@ -1052,11 +1060,22 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
         const int64_t tn = (a->n + TILE_SHAPES[s].bn - 1) / TILE_SHAPES[s].bn;
         return tm * (tn + runs / 2) * batch;           // half the groups' last runs short, on average
     };
+    // Sets a shape and its pieces of k; whether a launch, of fewer than 2^32 threads, takes it.
+    auto set = [&](int s, int64_t p) {
+        const TileShape &t = TILE_SHAPES[s];
+        *shape = s;
+        a->split = (int)p;
+        a->tiles_m = (int)((a->m + t.bm - 1) / t.bm);
+        a->tiles_n = (int)((a->n + t.bn - 1) / t.bn + runs);
+        return work_groups(*a, ksum) < ((int64_t)1 << 32) / t.threads;
+    };
 
     ShapeCost some[4];
     int count = 0;
     if (sizeof(T) == 2 && !ksum && share <= 16) {
-        if (pkc) {
+        if (!set(FEW_16, 1)) {
+            some[count++] = {REG_16, 1.0, 0.5, 6};
+        } else if (pkc) {
             some[count++] = {FEW_16, 0.25, 0.07, 4};
         } else {
             some[count++] = {FEW_16, 0.2, 0.17, 4};
@@ -1103,6 +1122,7 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
         const int64_t n = tiles(o.shape);
         const double work = 2e-6 * 64 * TILE_SHAPES[o.shape].bm * TILE_SHAPES[o.shape].bn / o.rate;
         for (int64_t p = 1; p == 1 || (o.shape != FEW_16 && o.shape != FEW_32 && p <= k / 128 && p * sums * (int64_t)sizeof(typename Elem<T>::Acc) <= (int64_t)1 << 28); p *= 2) {
+            if (!set(o.shape, p)) break;
             const int64_t groups = n * p, slots = 256 * o.held;
             const int64_t held = (groups + 255) / 256 < o.held ? (groups + 255) / 256 : o.held;
             double rounds = (double)groups / slots;
@@ -1116,25 +1136,19 @@ void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part
             }
         }
     }
-    *shape = best_shape;
-    a->split = (int)split;
-    a->tiles_m = (int)((a->m + TILE_SHAPES[best_shape].bm - 1) / TILE_SHAPES[best_shape].bm);
-    a->tiles_n = (int)((a->n + TILE_SHAPES[best_shape].bn - 1) / TILE_SHAPES[best_shape].bn + runs);
+    if (best_shape < 0)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: %lld x %lld sums (%lld groups) are more tiles than one launch takes",
+                    (long long)a->m, (long long)a->n, (long long)a->groups);
+    set(best_shape, split);
     *part_bytes = split > 1 ? (size_t)split * sums * sizeof(typename Elem<T>::Acc) : 0;
-}
-
-// The workgroups that find_work counts on.
-inline unsigned work_groups(const TileArgs &a, bool ksum)
-{
-    const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.split * (ksum && a.offsets ? a.groups : 1);
-    return (unsigned)(((total + NUM_XCD - 1) / NUM_XCD + (a.offsets && !ksum ? 1 : 0)) * NUM_XCD);
+    return JLUST_STATUS_SUCCESS;
 }
 
 template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN>
 int launch_shape(const TileArgs &a, hipStream_t s)
 {
     hipLaunchKernelGGL((tile_product_kernel<T, PKC, QKC, BM, BN, WM, WN>),
-                       dim3(work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
+                       dim3((unsigned)work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("tile_product_kernel");
 }
 
@@ -1142,7 +1156,7 @@ template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK
 int launch_copies(const TileArgs &a, hipStream_t s)
 {
     hipLaunchKernelGGL((tile_copy_kernel<T, PKC, QKC, BM, BN, WM, WN, BK, NB>),
-                       dim3(work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
+                       dim3((unsigned)work_groups(a, !PKC && !QKC)), dim3(WM * WN * 64), 0, s, a);
     return check_launch("tile_copy_kernel");
 }
 
@@ -1153,9 +1167,9 @@ int launch_columns(const TileArgs &a, int shape, hipStream_t s)
         case FEW_16:
         case FEW_32:
             if (PKC || shape == FEW_16)
-                hipLaunchKernelGGL((few_columns_kernel<T, PKC, 1>), dim3(work_groups(a, false)), dim3(Few<1>::WAVES * 64), 0, s, a);
+                hipLaunchKernelGGL((few_columns_kernel<T, PKC, 1>), dim3((unsigned)work_groups(a, false)), dim3(Few<1>::WAVES * 64), 0, s, a);
             else
-                hipLaunchKernelGGL((few_columns_kernel<T, false, 2>), dim3(work_groups(a, false)), dim3(Few<2>::WAVES * 64), 0, s, a);
+                hipLaunchKernelGGL((few_columns_kernel<T, false, 2>), dim3((unsigned)work_groups(a, false)), dim3(Few<2>::WAVES * 64), 0, s, a);
             return check_launch("few_columns_kernel");
         case COPY_256: return launch_copies<T, PKC, true, 256, 256, 2, 4, 64, 2>(a, s);
         case COPY_TALL: return launch_copies<T, PKC, true, 256, 128, 2, 2, 32, 3>(a, s);
@@ -1200,9 +1214,6 @@ int launch_tile_product(const TileArgs &args, bool pkc, bool qkc, int shape, hip
     if (a.split == 1) a.part = nullptr;
     const bool ksum = !pkc && !qkc;
     int st;
-    if ((int64_t)a.tiles_m * a.tiles_n * a.split * (ksum && a.offsets ? a.groups : 1) >= (int64_t)1 << 23)
-        return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: a product of %d x %d tiles is more than one launch takes", a.tiles_m,
-                    a.tiles_n);
     if (ksum) st = launch_sums<T>(a, shape, s);
     else st = pkc ? launch_columns<T, true>(a, shape, s) : launch_columns<T, false>(a, shape, s);
     if (st || a.split == 1) return st;

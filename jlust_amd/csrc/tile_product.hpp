@@ -134,9 +134,10 @@ __device__ __forceinline__ bool find_run(const int32_t *__restrict__ offsets, in
 }
 
 // Chooses the tile shape and the split of k and sets them in `a`; *part_bytes of
-// partial sums are to be at a->part when it is launched.
+// partial sums are to be at a->part when it is launched.  INVALID_ARGUMENT where one
+// launch does not take all the tiles.
 template <typename T>
-void plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes);
+int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes);
 template <typename T>
 int launch_tile_product(const TileArgs &a, bool pkc, bool qkc, int shape, hipStream_t s);
 

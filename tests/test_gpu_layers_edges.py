@@ -114,3 +114,51 @@ def test_gradient_of_interleaved_groups(J, T, cols, other):
         with pytest.raises(J.NonCanonicalStorage):
             J.execute(J.GroupedLinearGradOp, h, s["W"], s["X"], dY, dX=dX, **bad)
     assert (dX == 5).all() and (buf == 0).all()
+
+
+def test_more_rows_than_a_launch_has_threads_for(J):
+    """134 million columns: a launch of 32 threads for each would pass 2^32 threads.
+    All but a few columns are zero, so that the 64-bit form takes those alone."""
+    T, inp, out, cols = torch.float16, 8, 8, (1 << 27) + 40
+    gen = torch.Generator().manual_seed(0)
+    at = [0, 5, (1 << 26) + 3, (1 << 27) - 1, 1 << 27, cols - 1]
+    W, X, dY = (weights(out, inp, 2, T, gen, "out"), torch.zeros((cols, inp), dtype=T, device="cuda").t(),
+                torch.zeros((cols, out), dtype=T, device="cuda").t())
+    X[:, at], dY[:, at] = (torch.randn((8, len(at)), generator=gen).to(T).cuda() for _ in range(2))
+    ids = torch.ones(cols, dtype=torch.int32, device="cuda")
+    ids[at[1::2]] = 2
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=2)
+    dX, dW = torch.full((cols, inp), 7.0, dtype=T, device="cuda").t(), torch.empty_like(W)
+    J.execute(J.GroupedLinearGradOp, h, W, X, dY, dX=dX, dW=dW)
+    ref = L.gradients(W, X[:, at], dY[:, at], None, None, ids[at], 1)
+    L.close(dX[:, at], *ref["dX"], "dX")
+    L.close(dW, *ref["dW"], "dW")
+    assert int(torch.count_nonzero(dX)) == int(torch.count_nonzero(dX[:, at]))
+
+
+def test_longest_columns_sums(J):
+    """dweight and dbias of a column of 134 million values, and zeros without columns."""
+    T, d = torch.float16, (1 << 27) + 40
+    X = torch.empty((1, d), dtype=T, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1)).t()
+    dY, S = X.flip(0).t().contiguous().t(), torch.tensor([[0.25, 2.0]], device="cuda").t()
+    dw, db = torch.full((d,), 7.0, dtype=T, device="cuda"), torch.full((d,), 7.0, dtype=T, device="cuda")
+    J.execute(J.LayerNormGradOp, X, dY, S, dweight=dw, dbias=db)
+    assert torch.equal(db, dY[:, 0])
+    assert torch.equal(dw, (dY[:, 0].float() * ((X[:, 0].float() - 0.25) * 2.0)).to(T))
+    none = torch.empty((0, d), dtype=T, device="cuda").t()
+    J.execute(J.LayerNormGradOp, none, none, torch.empty((0, 2), device="cuda").t(), dweight=dw, dbias=db)
+    assert not dw.any() and not db.any()
+
+
+def test_bias_of_the_longest_columns(J):
+    """dbias of columns of 134 million values, by groups and without."""
+    T, out = torch.float16, (1 << 27) + 40
+    dY = torch.empty((2, out), dtype=T, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1)).t()
+    W, X = torch.zeros((1, out), dtype=T, device="cuda").t(), torch.zeros((2, 1), dtype=T, device="cuda").t()
+    db = torch.full((out,), 7.0, dtype=T, device="cuda")
+    J.execute(J.LinearGradOp, W, X, dY, dbias=db)
+    assert torch.equal(db, (dY[:, 0].float() + dY[:, 1].float()).to(T))
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, torch.tensor([2, 0], dtype=torch.int32, device="cuda"), n_groups=2)
+    db = torch.full((2, out), 7.0, dtype=T, device="cuda").t()
+    J.execute(J.GroupedLinearGradOp, h, W[:, :, None].expand(out, 1, 2), X, dY, dbias=db)
+    assert torch.equal(db[:, 1], dY[:, 0]) and not db[:, 0].any()
