@@ -1218,6 +1218,21 @@ typedef struct jlust_linear_grad {
 int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t stream);
 
 /*
+ * What those calls run for the same arguments (for diagnostics and tests; no GPU
+ * needed, the operands' addresses are only looked at): the sums a workgroup makes,
+ * whether it copies its operands to LDS or takes them through registers, the pieces
+ * that k is cut into, what is packed first (bits of jlust_packed), and the call's
+ * scratch, of which the largest per stream is kept.  linear_grad_info fills info[0]
+ * for dX and info[1] for dW, zeros for what is not asked.
+ */
+enum jlust_packed { JLUST_PACKED_W = 1, JLUST_PACKED_X = 2, JLUST_PACKED_DY = 4 };
+typedef struct jlust_product_info {
+    int64_t tile_rows, tile_cols, copies, pieces, packed, scratch_bytes;
+} jlust_product_info;
+int jlust_hip_linear_info(const jlust_linear *op, jlust_product_info *info);
+int jlust_hip_linear_grad_info(const jlust_linear_grad *op, jlust_product_info *info);
+
+/*
  * Layer norm of the columns of a d x cols X: y = (x - mean) * rstd .* weight
  * .+ bias with rstd = 1/sqrt(variance + eps) over the column's d values
  * (weight, bias: d values or null).  stats (or null) gets mean and rstd of

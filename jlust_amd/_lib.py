@@ -173,6 +173,8 @@ SIGNATURES = {
     "jlust_hip_group_plan_build": (_INT, [_I64, _I64, _I64, _I32, _P, _INT, _P, _P]),
     "jlust_hip_linear": (_INT, [_P, _P]),
     "jlust_hip_linear_grad": (_INT, [_P, _P]),
+    "jlust_hip_linear_info": (_INT, [_P, ctypes.POINTER(_I64)]),
+    "jlust_hip_linear_grad_info": (_INT, [_P, ctypes.POINTER(_I64)]),
     "jlust_hip_layer_norm": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _P, _D, _P, _I64, _P, _I64, _P]),
     "jlust_hip_layer_norm_grad": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P,
                                          _P]),

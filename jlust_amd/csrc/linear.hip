@@ -504,8 +504,16 @@ int by_type(int32_t value_type, F &&f)
 
 // --------------------------------------------------------------------- forward
 
+// What is planned, for the info entries.
+jlust_product_info info_of(const TileArgs &a, int shape, bool w, bool x, bool g, size_t scratch_bytes)
+{
+    const TileForm f = tile_form(shape);
+    return {f.m, f.n, f.copies, a.split, (w ? JLUST_PACKED_W : 0) | (x ? JLUST_PACKED_X : 0) | (g ? JLUST_PACKED_DY : 0),
+            (int64_t)scratch_bytes};
+}
+
 template <typename T>
-int linear(const jlust_linear &op, jlust_stream_t stream)
+int linear(const jlust_linear &op, jlust_stream_t stream, jlust_product_info *info = nullptr)
 {
     const PlanParts pl = plan_parts(op.plan, op.cols, op.groups, op.copies);
     TileArgs a;
@@ -554,6 +562,10 @@ int linear(const jlust_linear &op, jlust_stream_t stream)
     int shape = 0;
     size_t bytes = 0;
     if (int st = plan_tile_product<T>(&a, pkc, true, &shape, &bytes)) return st;
+    if (info) {
+        *info = info_of(a, shape, a.p_pad, a.q_pad, false, pack + bytes);
+        return JLUST_STATUS_SUCCESS;
+    }
     hipStream_t s = (hipStream_t)stream;
     if (pack + bytes) {
         void *ws = nullptr;
@@ -577,7 +589,7 @@ int linear(const jlust_linear &op, jlust_stream_t stream)
 // ------------------------------------------------------------------- gradients
 
 template <typename T>
-int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
+int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream, jlust_product_info *info = nullptr)
 {
     using A = typename Elem<T>::Acc;
     hipStream_t s = (hipStream_t)stream;
@@ -678,6 +690,11 @@ int linear_grad(const jlust_linear_grad &op, jlust_stream_t stream)
     const size_t wide_bytes = wide ? align256(sizeof(A) * n * inp) : 0;
     const size_t part = align256(part_x > part_w ? part_x : part_w);
     const size_t sum_bytes = op.dbias ? sizeof(A) * runs * out : 0;
+    if (info) {
+        info[0] = op.dX ? info_of(x, shape_x, make_w, false, make_g, made + wide_bytes + part + sum_bytes) : jlust_product_info{};
+        info[1] = op.dW ? info_of(w, shape_w, false, make_x, make_g, made + wide_bytes + part + sum_bytes) : jlust_product_info{};
+        return JLUST_STATUS_SUCCESS;
+    }
     void *ws = nullptr;
     if (made + wide_bytes + part + sum_bytes)
         if (int st = scratch(stream, made + wide_bytes + part + sum_bytes, &ws)) return st;
@@ -799,7 +816,9 @@ extern "C" int jlust_hip_group_plan_build(int64_t n, int64_t groups, int64_t cop
     return check_launch("group_plan_kernel");
 }
 
-extern "C" int jlust_hip_linear(const jlust_linear *op, jlust_stream_t stream)
+namespace {
+
+int check_linear(const jlust_linear *op)
 {
     clear_error();
     if (!op) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: null argument");
@@ -809,18 +828,14 @@ extern "C" int jlust_hip_linear(const jlust_linear *op, jlust_stream_t stream)
         return st;
     const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
     const int64_t wr = op->w_layout ? op->inp : op->out, wc = op->w_layout ? op->out : op->inp;
-    if (int st = check_operands(who, {{"W", op->W, wr, wc, op->ldw, true},
-                                      {"X", op->X, op->inp, xcols, op->ldx, true},
-                                      {"Y", op->Y, op->out, op->cols, op->ldy, true},
-                                      {"R", op->R, op->out, op->cols, op->ldr, false},
-                                      {"Z", op->Z, op->out, op->cols, op->ldz, false}}))
-        return st;
-    if (int st = require_device(nullptr)) return st;
-    if (op->out == 0 || op->cols == 0) return JLUST_STATUS_SUCCESS;
-    return by_type(op->value_type, [&](auto t) { return linear<decltype(t)>(*op, stream); });
+    return check_operands(who, {{"W", op->W, wr, wc, op->ldw, true},
+                                {"X", op->X, op->inp, xcols, op->ldx, true},
+                                {"Y", op->Y, op->out, op->cols, op->ldy, true},
+                                {"R", op->R, op->out, op->cols, op->ldr, false},
+                                {"Z", op->Z, op->out, op->cols, op->ldz, false}});
 }
 
-extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t stream)
+int check_linear_grad(const jlust_linear_grad *op)
 {
     clear_error();
     if (!op) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_grad: null argument");
@@ -833,21 +848,54 @@ extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t
     if (int st = check_apart(who, "dW", op->dW, wr, wc, op->lddw, op->groups, op->dw_stride)) return st;
     if (int st = check_apart(who, "dbias", op->dbias, op->out, 1, op->out, op->groups, op->dbias_stride)) return st;
     // W is read for dX alone (it may be laid out otherwise beside a dW), X for dW alone.
-    if (int st = check_operands(who, {{"W", op->dX ? op->W : nullptr, wr, wc, op->ldw, op->dX != nullptr},
-                                      {"X", op->dW ? op->X : nullptr, op->inp, xcols, op->ldx, op->dW != nullptr},
-                                      {"dY", op->dY, op->out, op->cols, op->lddy, true},
-                                      {"Z", op->Z, op->out, op->cols, op->ldz, op->act != JLUST_FN_IDENTITY},
-                                      {"dX", op->dX, op->inp, xcols, op->lddx, false},
-                                      {"dW", op->dW, wr, wc, op->lddw, false}}))
-        return st;
+    return check_operands(who, {{"W", op->dX ? op->W : nullptr, wr, wc, op->ldw, op->dX != nullptr},
+                                {"X", op->dW ? op->X : nullptr, op->inp, xcols, op->ldx, op->dW != nullptr},
+                                {"dY", op->dY, op->out, op->cols, op->lddy, true},
+                                {"Z", op->Z, op->out, op->cols, op->ldz, op->act != JLUST_FN_IDENTITY},
+                                {"dX", op->dX, op->inp, xcols, op->lddx, false},
+                                {"dW", op->dW, wr, wc, op->lddw, false}});
+}
+
+}  // namespace
+
+extern "C" int jlust_hip_linear(const jlust_linear *op, jlust_stream_t stream)
+{
+    if (int st = check_linear(op)) return st;
+    if (int st = require_device(nullptr)) return st;
+    if (op->out == 0 || op->cols == 0) return JLUST_STATUS_SUCCESS;
+    return by_type(op->value_type, [&](auto t) { return linear<decltype(t)>(*op, stream); });
+}
+
+extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t stream)
+{
+    if (int st = check_linear_grad(op)) return st;
     if (int st = require_device(nullptr)) return st;
     if (op->out == 0) {
         if (!op->dX) return JLUST_STATUS_SUCCESS;
         return by_type(op->value_type, [&](auto t) {
+            const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
             return fill_zero<decltype(t)>(xcols, op->inp, op->dX, op->lddx, (hipStream_t)stream);
         });
     }
     return by_type(op->value_type, [&](auto t) { return linear_grad<decltype(t)>(*op, stream); });
+}
+
+extern "C" int jlust_hip_linear_info(const jlust_linear *op, jlust_product_info *info)
+{
+    if (int st = check_linear(op)) return st;
+    if (!info) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_info: null result");
+    *info = jlust_product_info{};
+    if (op->out == 0 || op->cols == 0) return JLUST_STATUS_SUCCESS;
+    return by_type(op->value_type, [&](auto t) { return linear<decltype(t)>(*op, nullptr, info); });
+}
+
+extern "C" int jlust_hip_linear_grad_info(const jlust_linear_grad *op, jlust_product_info *info)
+{
+    if (int st = check_linear_grad(op)) return st;
+    if (!info) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_grad_info: null result");
+    info[0] = info[1] = jlust_product_info{};
+    if (op->out == 0) return JLUST_STATUS_SUCCESS;
+    return by_type(op->value_type, [&](auto t) { return linear_grad<decltype(t)>(*op, nullptr, info); });
 }
 
 namespace jlust {

@@ -141,4 +141,8 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
 template <typename T>
 int launch_tile_product(const TileArgs &a, bool pkc, bool qkc, int shape, hipStream_t s);
 
+// What a shape is: its tile, and whether its operands are copied to LDS.
+struct TileForm { int m, n, copies; };
+TileForm tile_form(int shape);
+
 }  // namespace jlust

@@ -3,10 +3,13 @@ kernel has to be named: against the plain 64-bit forms of tests/_layers.py."""
 import pytest
 import torch
 
+from tests import _layer_cases as C
 from tests import _layers as L
-from tests.test_gpu_layers import case, some_ids, weights
+from tests.test_gpu_layers import case, check_forward, check_grad, some_ids, weights
 
 pytestmark = pytest.mark.gpu
+
+TYPES = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
 
 @pytest.fixture(scope="module")
@@ -162,3 +165,35 @@ def test_bias_of_the_longest_columns(J):
     db = torch.full((2, out), 7.0, dtype=T, device="cuda").t()
     J.execute(J.GroupedLinearGradOp, h, W[:, :, None].expand(out, 1, 2), X, dY, dbias=db)
     assert torch.equal(db[:, 1], dY[:, 0]) and not db[:, 0].any()
+
+
+@pytest.mark.parametrize("i", range(len(C.PLANNED)))
+def test_planned(J, monkeypatch, i):
+    """The products of tests/_layer_cases.py, in the kernels that they are there for."""
+    T, out, inp, cols, layout, groups, pad, act, forward, dX, dW = C.PLANNED[i]
+    s = case(i, TYPES[T], out, inp, cols, layout, act, True, i % 2 == 0, groups or None, pad=pad)
+    ids = h = None
+    if groups:
+        ids = torch.from_numpy(some_ids(cols, groups, i, 0.1)).cuda()
+        h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
+    made = []
+    for name in ("_LINEAR", "_LINEAR_GRAD"):
+        pack = getattr(C.layers, name)
+        monkeypatch.setattr(C.layers, name, lambda *a, pack=pack: made.append(pack(*a)) or made[-1])
+    check_forward(J, s, ids, 1, h)
+    check_grad(J, s, ids, 1, h, seed=i)
+    assert C.info(made[0])[:5] == forward
+    assert tuple(v[:5] for v in C.info(made[1], True)) == (dX, dW)
+
+
+@pytest.mark.parametrize("n", [4095, 4096, 4097, 8191])
+@pytest.mark.parametrize("groups", [999, 1000, 1001])
+def test_group_plan_of_one_workgroup(J, n, groups):
+    """About the most columns and groups that one workgroup sorts."""
+    import numpy as np
+    ids = some_ids(n, groups, n + groups)
+    h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, torch.from_numpy(ids).cuda(), n_groups=groups)
+    bins = np.where((ids >= 1) & (ids <= groups), ids - 1, groups)
+    assert np.array_equal(h.order().cpu().numpy(), np.argsort(bins, kind="stable"))
+    want = np.concatenate([[0], np.cumsum(np.bincount(bins, minlength=groups + 1))])[: groups + 1]
+    assert np.array_equal(h.offsets().cpu().numpy(), want)

@@ -9,6 +9,7 @@ import torch
 import jlust_amd as J
 from jlust_amd import _lib, layers
 from jlust_amd.elementwise import FN_EXP, FN_GELU
+from tests import _layer_cases as C
 
 
 def linear(**kw):
@@ -115,3 +116,61 @@ def test_capability_table():
     dense = J.Formats.DensedRight(2)
     assert J.supports_backend(J.HIPBackend(), J.LinearOp(dense, dense, dense))
     assert not J.supports_backend(J.HIPBackend(), J.LinearOp(J.Formats.CSR, dense, dense))
+
+
+def test_planned_products():
+    """The kernels that tests/_layer_cases.py says its cases reach."""
+    for *args, forward, dX, dW in C.PLANNED:
+        f, g = C.arguments(*args)
+        assert C.info(f)[:5] == forward, args
+        assert tuple(i[:5] for i in C.info(g, True)) == (dX, dW), args
+    kinds = {(c[0] if c[0] == "f32" else "half", i, c[4] == ("inp" if i == 0 else "out") if i < 2 else None, c[8 + i][:3])
+             for c in C.PLANNED for i in range(3)}
+    for kc in (True, False):                       # every tile by copies, in each direction
+        for tile in ((256, 256, 1), (256, 128, 1), (128, 128, 1)):
+            assert any(k[0] == "half" and k[1] < 2 and k[2] == kc and k[3] == tile for k in kinds), (kc, tile)
+        assert any(k[0] == "f32" and k[1] < 2 and k[2] == kc and k[3] == (128, 128, 1) for k in kinds)
+    for want in (("half", (256, 128, 1)), ("half", (128, 128, 1)), ("half", (128, 128, 0)), ("f32", (128, 128, 1)), ("f32", (128, 128, 0))):
+        assert (want[0], 2, None, want[1]) in kinds, want
+
+
+@pytest.mark.parametrize("T", ["bf16", "f32"])
+@pytest.mark.parametrize("layout", ["out", "inp"])
+def test_a_shared_matrix_is_packed_once(T, layout):
+    """tests/test_gpu_layers_edges.py's groups that share a matrix: W is packed in both
+    directions, shared or not, and takes one matrix's scratch where it is."""
+    size = 4 if T == "f32" else 2
+    scratch = []
+    for shared in (True, False):
+        f, g = (bytearray(b) for b in C.arguments(T, 1000, 1024, 16384, layout, 3, 0, None))
+        a, b = (1000, 1024) if layout == "out" else (1024, 1000)
+        for buf in (f, g):
+            struct.pack_into("@q", buf, 16 + 8 * 4, a + 1)                              # ldw
+            struct.pack_into("@q", buf, len(buf) - (16 if buf is f else 24), 0 if shared else (a + 1) * b)
+        (dX, _), Y = C.info(bytes(g), True), C.info(bytes(f))
+        assert Y[4] == 1 and dX[4] == 5
+        scratch.append((Y[5], dX[5]))
+    a, b = (1000, 1024) if layout == "out" else (1024, 1000)
+    ld = (a * size + 15) // 16 * 16
+    extra = lambda v: (v + 255) // 256 * 256  # noqa: E731
+    assert all(apart - shared == extra(3 * ld * b) - extra(ld * b) for shared, apart in zip(*scratch))
+
+
+def test_a_product_that_one_launch_does_not_take():
+    """2^31 - 1 columns of 64 Float32 sums are 2^25 tiles; the gradient is refused too,
+    before anything of it runs.  What few columns' tiles would pass takes wider ones."""
+    n = (1 << 31) - 1
+    big = dict(T="f32", out=64, inp=4, cols=n, layout="out", groups=0, pad=0, act=None)
+    f, _ = C.arguments(**big)
+    assert _lib.lib().jlust_hip_linear_info(f, (ctypes.c_int64 * 6)()) == 1 and "one launch" in _lib.last_error()
+    _, g = C.arguments(**{**big, "inp": 64, "out": 4})
+    assert _lib.lib().jlust_hip_linear_grad_info(g, (ctypes.c_int64 * 12)()) == 1 and "one launch" in _lib.last_error()
+    few = dict(T="bf16", out=1 << 20, inp=64, cols=4000, layout="inp", pad=0, act=None)
+    assert C.info(C.arguments(**few, groups=300)[0])[:2] == (128, 16)
+    assert C.info(C.arguments(**{**few, "out": 1 << 16}, groups=300)[0])[:2] == (16, 16)
+
+
+def test_info_of_nothing():
+    f, g = C.arguments("bf16", 0, 5, 3, "out", 0, 0, None)
+    assert C.info(f) == (0,) * 6 and C.info(g, True) == ((0,) * 6,) * 2
+    assert _lib.lib().jlust_hip_linear_info(f, None) == 1 and _lib.lib().jlust_hip_linear_grad_info(None, (ctypes.c_int64 * 12)()) == 1
