@@ -545,7 +545,7 @@ struct Copy {
         return RB == 128 ? (r >> 1 & 7) ^ (r & 1) << 2 : (r >> 2 & 3) ^ (r & 2);
     }
     // Where 16 elements of an sc row lie: a transposed 16-bit read takes 4 rows at
-    // two of them at once, a 32- or 64-bit read 4 rows 16 bytes of k apart.
+    // two of them at once, a 32-bit read 4 rows 16 bytes of k apart.
     __device__ __forceinline__ static int segment(int seg, int k)
     {
         return SZ == 2 ? seg ^ (k & 3) << 1 : seg ^ (k / CH & 3);
@@ -605,15 +605,14 @@ struct Copy {
     // Where a lane reads what it feeds to a 32x32x16 step: row 32 tile + lane % 32,
     // k = 8 (lane / 32) .. + 7; the other tiles and steps lie at flips of its bits
     // and at fixed distances.
-    template <bool PERMUTE = false>
     __device__ __forceinline__ static int place(int tile)
     {
         const int lane = threadIdx.x & 63, li = lane & 15;
         if constexpr (SZ > 2) {
-            // A 16x16x4 step: row 16 tile + lr, k = CH g + j.
-            const int g = lane >> 4, lr = SZ == 8 ? 4 * (li & 3) + (li >> 2) : li, row = PERMUTE ? lr : li;
-            if constexpr (KC) return (16 * tile + row) * RB + ((g ^ flip(row)) << 4);
-            return CH * g * R * SZ + (segment(tile, CH * g) * 16 + row) * SZ;
+            // A 16x16x4 step: row 16 tile + li, k = CH g + j.
+            const int g = lane >> 4;
+            if constexpr (KC) return (16 * tile + li) * RB + ((g ^ flip(li)) << 4);
+            return CH * g * R * SZ + (segment(tile, CH * g) * 16 + li) * SZ;
         }
         if constexpr (KC) return (32 * tile + (lane & 31)) * RB + (((lane >> 5) ^ flip(lane & 31)) << 4);
         const int k = 8 * (lane >> 5) + (li >> 2);
@@ -676,7 +675,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
     constexpr int LM = BM > 64 && BM < 128 ? 128 : BM;  // rows of P in LDS
     constexpr bool KSUM = !PKC && !QKC;
     using A = typename Elem<T>::Acc;
-    using Sum = std::conditional_t<HALF, floatx16, typename Elem<T>::Acc4>;
+    using Sum = std::conditional_t<HALF, floatx16, floatx4>;
     using CP = Copy<T, PKC, LM, NT, BK>;
     using CQ = Copy<T, QKC, BN, NT, BK>;
     // Arrays of their own: the compiler then knows which copies an LDS read waits for.
@@ -712,7 +711,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
                 cq.template start<true>(to + CP::BYTES, k, kend);
             }
         };
-        const int at_p = CP::template place<true>(wm0 / STEP), at_q = CQ::template place<false>(wn0 / STEP);
+        const int at_p = CP::place(wm0 / STEP), at_q = CQ::place(wn0 / STEP);
         auto multiply = [&](const char *from, int left) {
             int pa = at_p, qa = at_q;
             asm("" : "+v"(pa), "+v"(qa));          // its flips are made here, not held in registers over the loop
@@ -1032,7 +1031,7 @@ bool copies_fit(const TileArgs &a, bool pkc, bool qkc)
 {
     const int64_t z = sizeof(T);
     const uintptr_t bits = (uintptr_t)a.P | (uintptr_t)a.Q | (uintptr_t)(a.ldp * z) | (uintptr_t)(a.ldq * z) |
-                           (uintptr_t)(a.gp * z) | (uintptr_t)(a.gq * z);
+                           (uintptr_t)(a.gp * z);
     const int64_t k = (pkc && !a.p_pad) || (qkc && !a.q_pad) ? a.k : 0, m = pkc || a.p_pad ? 0 : a.m, n = qkc || a.q_pad ? 0 : a.n;
     return (bits & 15) == 0 && (k | m | n) * z % 16 == 0 && a.ldp < (1 << 22) && a.ldq < (1 << 22);
 }
@@ -1183,14 +1182,14 @@ int launch_columns(const TileArgs &a, int shape, hipStream_t s)
         case REG_16: return launch_shape<T, PKC, true, 128, 16, 2, 1>(a, s);
         }
     if constexpr (sizeof(T) == 4) switch (shape) {
-        case REG_M128: return launch_shape<T, PKC, true, 128, 64, 1, 4>(a, s);
         case REG_M112: return launch_shape<T, PKC, true, 112, 64, 1, 4>(a, s);
         case REG_M96: return launch_shape<T, PKC, true, 96, 64, 1, 4>(a, s);
         case REG_M80: return launch_shape<T, PKC, true, 80, 64, 1, 4>(a, s);
         case REG_M64: return launch_shape<T, PKC, true, 64, 64, 1, 4>(a, s);
         case COPY_128: return launch_copies<T, PKC, true, 128, 128, 2, 2, 32, 2>(a, s);
         }
-    return launch_shape<T, PKC, true, 128, 128, 2, 2>(a, s);
+    if constexpr (sizeof(T) == 4) return launch_shape<T, PKC, true, 128, 64, 1, 4>(a, s);     // REG_M128
+    else return launch_shape<T, PKC, true, 128, 128, 2, 2>(a, s);
 }
 
 template <typename T>

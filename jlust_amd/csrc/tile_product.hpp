@@ -20,7 +20,7 @@ struct TileArgs {
     int64_t m = 0, n = 0, k = 0;
     const void *P = nullptr, *Q = nullptr;
     int64_t ldp = 0, ldq = 0;
-    int64_t gp = 0, gq = 0;             // elements between the matrices of two groups
+    int64_t gp = 0;                     // elements between the P of two groups
     bool p_pad = false, q_pad = false;  // rows lie in buffers of their own, zeros after them to the next 16 bytes
     const int32_t *qrow = nullptr;      // kc: the row of Q that n stands for (null: n itself)
     const int32_t *crow = nullptr;      // the row of C, R and Z that n stands for
@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32x4 load_chunk_part(const T *p, int64_t count)
 // [offsets[g], offsets[g+1]) are cut into such runs, group after group, and
 // those from offsets[groups] to n as group `groups`.  False past the last.
 // Every lane of a wave calls it with the same arguments.
-struct GroupRun { int group; int64_t begin, end, group_begin, group_end; int64_t first; };
+struct GroupRun { int group; int64_t begin, end, group_end; };
 
 __device__ __forceinline__ bool find_run(const int32_t *__restrict__ offsets, int groups, int64_t n, int64_t tile,
                                          int per, GroupRun *out)
@@ -121,9 +121,7 @@ __device__ __forceinline__ bool find_run(const int32_t *__restrict__ offsets, in
             const int64_t first = base + __shfl(incl - tiles, l, 64);
             const int64_t b = __shfl(lo, l, 64), e = __shfl(hi, l, 64);
             out->group = g0 + l;
-            out->group_begin = b;
             out->group_end = e;
-            out->first = first;
             out->begin = b + (tile - first) * per;
             out->end = out->begin + per < e ? out->begin + per : e;
             return true;
