@@ -25,7 +25,8 @@
  *  - Work is enqueued on `stream` (a hipStream_t; NULL = the null stream) and
  *    returns without synchronising.  Entry points are reentrant.  The library
  *    keeps one scratch buffer per (device, stream) for the SpMV/SpMM partial
- *    results and copies of B, so concurrent calls must use different streams
+ *    results and copies of B and the layer operators' partial sums and packed
+ *    operands, so concurrent calls must use different streams
  *    (the COO and CSC SDDMM have one of their own and order themselves).  The
  *    buffer grows on demand and an outgrown one is kept, never freed, so work already
  *    queued and HIP graphs that captured a call stay valid.  Capturing a call

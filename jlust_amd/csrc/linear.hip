@@ -211,7 +211,13 @@ struct Prepass {
 
 // G = dY .* act'(Z) in the order of the groups (row p of G is column perm[p]),
 // rounded to T, its rows ldg apart (a whole number of 16 bytes, zeros at their ends),
-// and the sums of its unrounded rows over a run of `per` columns: sums[run][m].  dY and Z are read once; G and dbias would each read them again.
+// and the sums of its unrounded rows over a run of `per` columns: sums[run][m].  dY
+// and Z are read once; G and dbias would each read them again.
+// The rounding is one to the type of dY, W and X, which the 16-bit matrix steps take:
+// the results' error goes from 0.0017 to 0.0023 in bfloat16.  G as the sum of two
+// 16-bit values would take both products twice (8,192 columns 2048 -> 8192: dX 248 us
+// and 486, dW 230 and 460, of 566 in all); Float32 operands, which a caller who needs
+// more can pass, take 4,257.
 template <typename T>
 __global__ __launch_bounds__(256) void grad_prepass_kernel(int64_t n, int64_t m, const T *__restrict__ dY, int64_t lddy,
                                                            const T *__restrict__ Z, int64_t ldz, int act, T *__restrict__ G,

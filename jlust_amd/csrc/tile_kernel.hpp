@@ -1022,7 +1022,9 @@ constexpr TileShape TILE_SHAPES[] = {{128, 128, 256}, {128, 32, 256}, {128, 16, 
 // What a shape costs: its rate with a CU full of it (Tflop/s a CU), the time of 64 of
 // k where latency bounds it (us), workgroups a CU.  Measured on products of 64 to
 // 8,192 columns and 512 to 8,192 rows and k; the estimate below picks within 10 %
-// of the best of them but for three (up to 20 %).
+// of the best of them but for three (up to 20 %).  Of groups' products it only ranks
+// the shapes (32 groups, 16,384 columns 2816 -> 1024: 138 us estimated, 194 measured;
+// the sums over columns 93 and 181).
 struct ShapeCost { Shape shape; double rate, latency; int held; };
 
 // Whether every chunk that a copy reads lies whole in the operands, 16 bytes aligned.
@@ -1049,7 +1051,12 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
     const bool ksum = !pkc && !qkc, grouped = a->offsets && !ksum;
     const int64_t batch = ksum && a->offsets ? a->groups : 1;
     const int64_t runs = grouped ? (a->groups < a->n ? a->groups : a->n) : 0;
-    // Columns that share a matrix, and k of one sum, on average.
+    // Columns that share a matrix, and k of one sum, on average: the groups' sizes are
+    // known on the device alone.  Worst where the average is just below a shape's limit
+    // (64 groups, 2048 -> 1024, columns spread evenly and all in one group, us).  16:
+    // bfloat16 with W along inp 115 and 87 for 1,024 columns, by wider tiles 43 and 24
+    // for 1,025; along out 50 and 28, 44 and 29; Float32 131 and 84, 133 and 67.  48:
+    // 57 and 33 for 3,071 columns, 55 and 43 for 3,100; Float32 184 and 130, 196 and 151.
     const int64_t share = grouped ? (a->n + a->groups - 1) / a->groups : a->n;
     const int64_t k = ksum && a->offsets ? (a->k + a->groups - 1) / a->groups : a->k;
     const int64_t sums = a->n * a->m * batch;
