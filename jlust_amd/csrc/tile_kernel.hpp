@@ -824,7 +824,8 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
 // added by a second launch: 12.9 us for 4096 x 4096 and one column).  kc: 16 m, 64 bytes
 // a row and step, 8.9 us at 3.8 TB/s with P in no cache.  sc: 32 m where that makes
 // enough workgroups, for 64 bytes of a row (2048 -> 8192: 11.3 us, 16.3 with 16 m),
-// else 16 (4096 -> 4096: 16.2 us, 17.6 with 32); its pieces are transposed through LDS
+// else 16 (4096 -> 4096: 16.2 us, 17.6 with 32; 12.2 by 128 x 16 tiles and 16 pieces
+// of k, which the estimate takes there); its pieces are transposed through LDS
 // that the wave keeps to itself.
 template <int TILES> struct Few {
     static constexpr int WAVES = TILES == 1 ? 8 : 16, STEPS = TILES == 1 ? 4 : 2;
