@@ -1255,6 +1255,111 @@ int jlust_hip_layer_norm_grad(int32_t value_type, int64_t d, int64_t cols, const
                               const void *weight, void *dX, int64_t lddx, void *dweight, void *dbias,
                               jlust_stream_t stream);
 
+/*
+ * The products of a layer in 8 bits.  quantize_columns: scales[j] = max |X[:, j]| /
+ * 127, rounded to Float32, and Q[:, j] = X[:, j] / scales[j] to the nearest whole
+ * number, halves to the even one, within 127 of 0 (zeros where the scale is 0).  A
+ * column that holds an infinity or NaN gets the scale NaN and zeros.  X is Float32,
+ * Float16 or BFloat16.
+ */
+int jlust_hip_quantize_columns(int32_t value_type, int64_t d, int64_t cols, const void *X, int64_t ldx,
+                               int8_t *Q, int64_t ldq, float *scales, jlust_stream_t stream);
+
+/*
+ * jlust_hip_linear of 8-bit integers: (W*X)[m, n] times w_scale[m] * x_scale[n].  W is
+ * the transpose of a column-major inp x out matrix, ldw >= inp (w_layout 1); the
+ * scales of group g are at w_scale + g*w_scale_stride, those of X go by X's columns.
+ * value_type is that of Y, bias, R and Z: Float32, Float16 or BFloat16.  Sums are
+ * Int32 and exact: inp is at most 131,071.  A column of no group gets 0 .+ R.
+ */
+typedef struct jlust_linear_int8 {
+    int32_t value_type, act;
+    int64_t out, inp, cols;
+    const int8_t *W; int64_t ldw;
+    const float *w_scale;
+    const int8_t *X; int64_t ldx;
+    const float *x_scale;
+    void *Y; int64_t ldy;
+    const void *bias;
+    const void *R; int64_t ldr;
+    void *Z; int64_t ldz;
+    int64_t groups, copies;
+    const int32_t *plan;
+    int64_t w_stride, w_scale_stride, bias_stride;
+} jlust_linear_int8;
+int jlust_hip_linear_int8(const jlust_linear_int8 *op, jlust_stream_t stream);
+int jlust_hip_linear_int8_info(const jlust_linear_int8 *op, jlust_product_info *info);
+
+/*
+ * The experts of every column of an experts x cols matrix L of logits.  Scores are
+ * exp(l) over the column's sum of them, or 1/(1 + exp(-l)); 0 for a logit of -infinity
+ * or NaN, which is never chosen.  An expert's key is its score plus its bias (`bias`:
+ * Float32, Float64 for Float64; null: the logits are the keys).  The experts make
+ * `groups` equal groups in order; of these the `keep` best by their best key (best 1)
+ * or by the sum of their two best scores plus biases (best 2), and of their experts the
+ * `copies` best keys, ties to the lowest index.  ids (copies x cols, from `origin`)
+ * gets them in the order of their keys, weights (bias's type) scale times their
+ * scores, or with renormalize scale times their shares of the chosen scores' sum.
+ * Where no expert is left ids gets origin - 1, weights 0.  Keys are compared in
+ * Float64.  experts <= 4,095, copies <= 64, groups <= 64.
+ */
+enum jlust_score { JLUST_SCORE_SOFTMAX = 0, JLUST_SCORE_SIGMOID = 1 };
+typedef struct jlust_route {
+    int32_t value_type, score, renormalize, origin;
+    int64_t experts, cols, copies, groups, keep, best;
+    const void *L; int64_t ldl;
+    const void *bias;
+    int32_t *ids; int64_t ldi;
+    void *weights; int64_t ldw;
+    double scale;
+} jlust_route;
+int jlust_hip_route(const jlust_route *op, jlust_stream_t stream);
+
+/*
+ * The gradient dL of the logits from that of the weights; ids are what the forward
+ * call chose (an id that names no expert counts for nothing).  The choice itself has
+ * none, and so has the bias.
+ */
+typedef struct jlust_route_grad {
+    int32_t value_type, score, renormalize, origin;
+    int64_t experts, cols, copies;
+    const void *L; int64_t ldl;
+    const int32_t *ids; int64_t ldi;
+    const void *dweights; int64_t lddw;
+    void *dL; int64_t lddl;
+    double scale;
+} jlust_route_grad;
+int jlust_hip_route_grad(const jlust_route_grad *op, jlust_stream_t stream);
+
+/*
+ * The weighted sum of the `copies` columns of X that belong to a column of Y:
+ * Y[:, t] = sum over c < copies of weights[c, t] * X[:, copies*t + c] (.+ R[:, t]).
+ * weights: Float32 (Float64 for Float64).  A column of X whose weight is 0 is not
+ * read.  R may be null or Y.  Its gradients: dX[:, copies*t + c] = weights[c, t] *
+ * dY[:, t] and dweights[c, t] = dot(X[:, copies*t + c], dY[:, t]), each where its
+ * pointer is not null (weights are read for dX alone, X for dweights alone).
+ */
+int jlust_hip_combine(int32_t value_type, int64_t d, int64_t cols, int64_t copies, const void *X, int64_t ldx,
+                      const void *weights, int64_t ldw, const void *R, int64_t ldr, void *Y, int64_t ldy,
+                      jlust_stream_t stream);
+int jlust_hip_combine_grad(int32_t value_type, int64_t d, int64_t cols, int64_t copies, const void *X, int64_t ldx,
+                           const void *weights, int64_t ldw, const void *dY, int64_t lddy, void *dX, int64_t lddx,
+                           void *dweights, int64_t lddw, jlust_stream_t stream);
+
+/*
+ * Dropout: Y = X .* mask ./ (1 - p) (.+ R).  Element (i, j) is kept where field i % 8
+ * (the low half of word 0, its high half, the low half of word 1, ...) of
+ * Philox4x32-10 at the counter {i / 8, j, offset's low word, its high word} under the
+ * key {seed's low word, its high word} is at least p * 2^16, rounded to a whole
+ * number; 1/(1 - p) goes by that number.  A dropped element is 0 whatever X holds.  The
+ * same call on dY is the backward pass.  state (or null): two 64-bit numbers in device
+ * memory, seed and offset, read when the call runs, in a replayed graph each time.  Y
+ * may be X or R.
+ */
+int jlust_hip_dropout(int32_t value_type, int64_t d, int64_t cols, const void *X, int64_t ldx, const void *R, int64_t ldr,
+                      void *Y, int64_t ldy, double p, uint64_t seed, uint64_t offset, const int64_t *state,
+                      jlust_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,9 +18,10 @@ from .errors import (DeviceMismatch, HIPError, IncompatibleExtents, IndexOriginM
 from .formats import (CompressedLevel, DenseLevel, Formats, PeriodicLevel, ShiftedDiagLevel,
                       SingletonLevel, TensorFormat, dim2lvl, lvl2dim)
 from .ops import (AbstractKernelHandle, AbstractUSTBackend, BBMSpMVOp, BlockSpMMOp, BlockSpMVOp,
-                  GroupedLinearGradOp, GroupedLinearOp, HIPBackend, LayerNormGradOp, LayerNormOp,
-                  LinearGradOp, LinearOp, Op, OpType, SDDMMOp, SpMMOp, SpMVOp, default_backend, execute,
-                  matmul, mul_, prepare, supports_backend, update_values_)
+                  CombineGradOp, CombineOp, DropoutOp, GroupedLinearGradOp, GroupedLinearOp, HIPBackend,
+                  LayerNormGradOp, LayerNormOp, LinearGradOp, LinearOp, Op, OpType, QuantizeOp, RouteGradOp,
+                  RouteOp, SDDMMOp, SpMMOp, SpMVOp, default_backend, execute, matmul, mul_, prepare,
+                  supports_backend, update_values_)
 from .block_sparse import (BlockSparseMatrix, BlockStructureError, batch_mul, batch_mul_,
                            update_block_values_)
 from .block_banded import BlockBandedMatrix

@@ -178,6 +178,15 @@ SIGNATURES = {
     "jlust_hip_layer_norm": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _P, _D, _P, _I64, _P, _I64, _P]),
     "jlust_hip_layer_norm_grad": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P, _P,
                                          _P]),
+    "jlust_hip_quantize_columns": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _I64, _P, _P]),
+    "jlust_hip_linear_int8": (_INT, [_P, _P]),
+    "jlust_hip_linear_int8_info": (_INT, [_P, ctypes.POINTER(_I64)]),
+    "jlust_hip_route": (_INT, [_P, _P]),
+    "jlust_hip_route_grad": (_INT, [_P, _P]),
+    "jlust_hip_combine": (_INT, [_I32, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P]),
+    "jlust_hip_combine_grad": (_INT, [_I32, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P]),
+    "jlust_hip_dropout": (_INT, [_I32, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _D, ctypes.c_uint64, ctypes.c_uint64,
+                                 _P, _P]),
 }
 
 STATUS = {

@@ -182,6 +182,10 @@ int preload_linear();
 int preload_linear_half();
 int preload_linear_wide();
 int preload_layer_norm();
+int preload_linear_int8();
+int preload_route();
+int preload_combine();
+int preload_dropout();
 
 #define JLUST_PRELOAD_KERNEL(KERNEL)                                                        \
     do {                                                                                    \

@@ -10,7 +10,7 @@
 // mean costs no digits); the backward kernel also keeps its share of dweight and
 // dbias in registers over all the columns it takes, so X and dY are read once for
 // all three results.  Columns too long for that are read again from L2.
-#include "tile_product.hpp"
+#include "column_chunks.hpp"
 
 namespace jlust {
 namespace {
@@ -21,101 +21,6 @@ template <typename A>
 __device__ __forceinline__ A inv_sqrt(A v)
 {
     return A(1) / sqrt(v);
-}
-
-// The sums of K values over the LANES lanes of a column, in every one of them.
-template <int LANES, int K, typename A>
-__device__ __forceinline__ void column_sum(A (&v)[K], A *lds)
-{
-#pragma unroll
-    for (int d = (LANES < 64 ? LANES : 64) / 2; d; d >>= 1)
-#pragma unroll
-        for (int q = 0; q < K; ++q) v[q] += __shfl_xor(v[q], d, 64);
-    if constexpr (LANES > 64) {
-        constexpr int W = LANES / 64;
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int q = 0; q < K; ++q) lds[wave * K + q] = v[q];
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < K; ++q) {
-            A s = A(0);
-#pragma unroll
-            for (int w = 0; w < W; ++w) s += lds[w * K + q];
-            v[q] = s;
-        }
-    }
-}
-
-// A chunk as it lies in memory, and its values.  Past the column's end: zeros, or
-// where `over` what follows, the next column, which is not summed.  (Half's 8 values
-// read one by one hold the wave up, 60,000 columns of 333: 28.1 and 26.8 us, backward
-// 45.9 and 40.3; Float32's 4 do not, 9,001 of 2,049: 27.1 and 27.8, 57.5 and 59.8.)
-template <typename T>
-__device__ __forceinline__ uint32x4 read_raw(const T *p, int64_t left, bool over = false)
-{
-    constexpr int CH = 16 / sizeof(T);
-    const uint32x4 zero = {0, 0, 0, 0};
-    return left >= CH || (over && left > 0) ? load_chunk(p) : left > 0 ? load_chunk_part(p, left) : zero;
-}
-
-template <typename T, typename A>
-__device__ __forceinline__ void values(uint32x4 v, A (&f)[16 / sizeof(T)])
-{
-    constexpr int CH = 16 / sizeof(T);
-    T e[CH];
-    __builtin_memcpy(e, &v, 16);
-#pragma unroll
-    for (int j = 0; j < CH; ++j) f[j] = A(e[j]);
-}
-
-// Its values again: without this the compiler keeps those of an earlier pass, two
-// or four times the registers of the packed chunk.
-template <typename T, typename A>
-__device__ __forceinline__ void values_again(uint32x4 &v, A (&f)[16 / sizeof(T)])
-{
-    asm("" : "+v"(v));
-    values<T>(v, f);
-}
-
-template <typename T, typename A>
-__device__ __forceinline__ void read_chunk(const T *p, int64_t left, A (&f)[16 / sizeof(T)])
-{
-    values<T>(read_raw(p, left), f);
-}
-
-// 16 bytes past the caches.  Results that the eight L2s of 4 MB do not hold would only
-// push out what is still read (16,384 bfloat16 columns of 4,096: 71.4 us by plain stores
-// and 63.9; backward, 200,003 Float32 columns of 100: 51.6 and 49.2; products' results
-// gain nothing: 8,192 columns 2048 -> 8192, 305 and 307 us).
-constexpr int64_t STREAMED = 32 << 20;         // bytes of a result from which it is stored so
-typedef uint32_t uint32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
-
-template <typename T>
-__device__ __forceinline__ void stream_chunk(T *p, const T *v)
-{
-    uint32x4 u;
-    __builtin_memcpy(&u, v, 16);
-    __builtin_nontemporal_store((uint32x4_any)u, reinterpret_cast<uint32x4_any *>(p));
-}
-
-template <typename T, typename A>
-__device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 / sizeof(T)], bool streamed = false)
-{
-    constexpr int CH = 16 / sizeof(T);
-    T e[CH];
-#pragma unroll
-    for (int j = 0; j < CH; ++j) e[j] = T(f[j]);
-    if (left >= CH) {
-        if (streamed) stream_chunk(p, e);
-        else store_vec<CH>(p, e);
-    } else {
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (j < left) p[j] = e[j];
-    }
 }
 
 // Lane l of a column's LANES holds its chunks l, l + LANES, ..., packed as they are

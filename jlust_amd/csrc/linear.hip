@@ -592,6 +592,52 @@ int linear(const jlust_linear &op, jlust_stream_t stream, jlust_product_info *in
     return launch_tile_product<T>(a, pkc, true, shape, s);
 }
 
+// Products of 8-bit integers, along k on both sides.
+int linear_int8(const jlust_linear_int8 &op, jlust_stream_t stream, jlust_product_info *info = nullptr)
+{
+    const PlanParts pl = plan_parts(op.plan, op.cols, op.groups, op.copies);
+    TileArgs a;
+    a.m = op.out;
+    a.n = op.cols;
+    a.k = op.inp;
+    a.P = op.W;
+    a.ldp = op.ldw;
+    a.gp = op.w_stride;
+    a.ps = op.w_scale;
+    a.gs = op.w_scale_stride;
+    a.Q = op.X;
+    a.ldq = op.ldx;
+    a.qs = op.x_scale;
+    a.qrow = pl.src;
+    a.crow = pl.perm;
+    a.offsets = pl.offsets;
+    a.groups = (int)op.groups;
+    a.C = op.Y;
+    a.ldc = op.ldy;
+    a.bias = op.bias;
+    a.gb = op.bias_stride;
+    a.R = op.R;
+    a.ldr = op.ldr;
+    a.Z = op.Z;
+    a.ldz = op.ldz;
+    a.act = op.act;
+    int shape = 0;
+    size_t bytes = 0;
+    if (int st = plan_tile_product<int8_t>(&a, true, true, &shape, &bytes)) return st;
+    if (info) {
+        *info = info_of(a, shape, false, false, false, bytes);
+        return JLUST_STATUS_SUCCESS;
+    }
+    if (bytes)
+        if (int st = scratch(stream, bytes, &a.part)) return st;
+    hipStream_t s = (hipStream_t)stream;
+    switch (op.value_type) {
+    case JLUST_VALUE_F32: return launch_tile_product8<float>(a, shape, s);
+    case JLUST_VALUE_F16: return launch_tile_product8<_Float16>(a, shape, s);
+    default: return launch_tile_product8<__bf16>(a, shape, s);
+    }
+}
+
 // ------------------------------------------------------------------- gradients
 
 template <typename T>
@@ -841,6 +887,32 @@ int check_linear(const jlust_linear *op)
                                 {"Z", op->Z, op->out, op->cols, op->ldz, false}});
 }
 
+// 128 * 128 of each of inp products add up to less than 2^31.
+constexpr int64_t MAX_INP8 = ((int64_t)1 << 17) - 1;
+
+int check_linear_int8(const jlust_linear_int8 *op)
+{
+    clear_error();
+    if (!op) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_int8: null argument");
+    const char *who = "linear_int8";
+    if (int st = check_common(who, op->value_type, op->act, 1, op->out, op->inp, op->cols, op->groups, op->copies, op->plan))
+        return st;
+    if (op->value_type == JLUST_VALUE_F64)
+        return fail(JLUST_STATUS_UNSUPPORTED_VALUE_TYPE, "%s: results are Float32, Float16 or BFloat16", who);
+    if (op->inp > MAX_INP8)
+        return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: %lld products of a sum may pass 32 bits, at most %lld", who,
+                    (long long)op->inp, (long long)MAX_INP8);
+    const int64_t xcols = op->groups ? op->cols / op->copies : op->cols;
+    if (int st = check_operands(who, {{"w_scale", op->w_scale, op->out, 1, op->out, true},
+                                      {"x_scale", op->x_scale, xcols, 1, xcols, op->out > 0}}))
+        return st;
+    return check_operands(who, {{"W", op->W, op->inp, op->out, op->ldw, true},
+                                {"X", op->X, op->inp, xcols, op->ldx, true},
+                                {"Y", op->Y, op->out, op->cols, op->ldy, true},
+                                {"R", op->R, op->out, op->cols, op->ldr, false},
+                                {"Z", op->Z, op->out, op->cols, op->ldz, false}});
+}
+
 int check_linear_grad(const jlust_linear_grad *op)
 {
     clear_error();
@@ -884,6 +956,23 @@ extern "C" int jlust_hip_linear_grad(const jlust_linear_grad *op, jlust_stream_t
         });
     }
     return by_type(op->value_type, [&](auto t) { return linear_grad<decltype(t)>(*op, stream); });
+}
+
+extern "C" int jlust_hip_linear_int8(const jlust_linear_int8 *op, jlust_stream_t stream)
+{
+    if (int st = check_linear_int8(op)) return st;
+    if (int st = require_device(nullptr)) return st;
+    if (op->out == 0 || op->cols == 0) return JLUST_STATUS_SUCCESS;
+    return linear_int8(*op, stream);
+}
+
+extern "C" int jlust_hip_linear_int8_info(const jlust_linear_int8 *op, jlust_product_info *info)
+{
+    if (int st = check_linear_int8(op)) return st;
+    if (!info) return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear_int8_info: null result");
+    *info = jlust_product_info{};
+    if (op->out == 0 || op->cols == 0) return JLUST_STATUS_SUCCESS;
+    return linear_int8(*op, nullptr, info);
 }
 
 extern "C" int jlust_hip_linear_info(const jlust_linear *op, jlust_product_info *info)

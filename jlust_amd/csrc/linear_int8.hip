@@ -1,0 +1,249 @@
+// linear_int8.hip -- the dense products of 8-bit integers, and the columns' scales and
+// integers that they take.
+#include "column_chunks.hpp"
+#include "tile_kernel.hpp"
+
+namespace jlust {
+
+template int plan_tile_product<int8_t>(TileArgs *, bool, bool, int *, size_t *);
+
+namespace {
+
+template <typename O, int BM, int BN, int WM, int WN>
+int launch_registers(const TileArgs &a, hipStream_t s)
+{
+    hipLaunchKernelGGL((tile_product_kernel<int8_t, true, true, BM, BN, WM, WN, O>), dim3((unsigned)work_groups(a, false)),
+                       dim3(WM * WN * 64), 0, s, a);
+    return check_launch("tile_product_kernel");
+}
+
+template <typename O, int BM, int BN, int WM, int WN, int BK, int NB>
+int launch_copied(const TileArgs &a, hipStream_t s)
+{
+    hipLaunchKernelGGL((tile_copy_kernel<int8_t, true, true, BM, BN, WM, WN, BK, NB, O>), dim3((unsigned)work_groups(a, false)),
+                       dim3(WM * WN * 64), 0, s, a);
+    return check_launch("tile_copy_kernel");
+}
+
+}  // namespace
+
+template <typename O>
+int launch_tile_product8(const TileArgs &args, int shape, hipStream_t s)
+{
+    TileArgs a = args;
+    if (a.split == 1) a.part = nullptr;
+    int st;
+    switch (shape) {
+    case FEW_16:
+        hipLaunchKernelGGL((few_columns_kernel<int8_t, true, 1, O>), dim3((unsigned)work_groups(a, false)), dim3(Few<1>::WAVES * 64), 0,
+                           s, a);
+        st = check_launch("few_columns_kernel");
+        break;
+    case REG_32: st = launch_registers<O, 128, 32, 4, 1>(a, s); break;
+    case COPY_256: st = launch_copied<O, 256, 256, 2, 4, 128, 2>(a, s); break;
+    case COPY_TALL: st = launch_copied<O, 256, 128, 2, 2, 64, 3>(a, s); break;
+    case COPY_128: st = launch_copied<O, 128, 128, 2, 2, 128, 2>(a, s); break;
+    default: st = launch_registers<O, 64, 64, 2, 2>(a, s); break;
+    }
+    if (st || a.split == 1) return st;
+    const int64_t items = a.n * ((a.m + 3) / 4);
+    const bool shares = a.split > 16;
+    const dim3 grid((unsigned)((items + (shares ? 15 : 255)) / (shares ? 16 : 256)));
+    if (shares) hipLaunchKernelGGL((split_reduce_kernel<int8_t, false, 16, O>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((split_reduce_kernel<int8_t, false, 1, O>), grid, dim3(256), 0, s, a);
+    return check_launch("split_reduce_kernel");
+}
+
+template int launch_tile_product8<float>(const TileArgs &, int, hipStream_t);
+template int launch_tile_product8<_Float16>(const TileArgs &, int, hipStream_t);
+template int launch_tile_product8<__bf16>(const TileArgs &, int, hipStream_t);
+
+// ------------------------------------------------------------------ quantising
+
+namespace {
+
+// The largest |x| of a column by its bits, which NaN and infinity end: bits of values
+// without their sign are in the values' order.
+template <int LANES>
+__device__ __forceinline__ uint32_t column_top(uint32_t v, uint32_t *lds)
+{
+#pragma unroll
+    for (int d = (LANES < 64 ? LANES : 64) / 2; d; d >>= 1) {
+        const uint32_t o = __shfl_xor(v, d, 64);
+        v = o > v ? o : v;
+    }
+    if constexpr (LANES > 64) {
+        constexpr int W = LANES / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) v = lds[w] > v ? lds[w] : v;
+    }
+    return v;
+}
+
+struct Scale { float s, inv; bool tiny; };
+
+// 1/s may be infinite below the normal range: there x is divided.
+__device__ __forceinline__ Scale scale_from(uint32_t top)
+{
+    if (top >= 0x7F800000u) return {__builtin_nanf(""), 0.0f, false};
+    const float s = (float)((double)__builtin_bit_cast(float, top) / 127.0);
+    return {s, s > 0 ? 1.0f / s : 0.0f, s < 1.1754944e-38f};
+}
+
+// x / s to the nearest whole number, halves to the even one: the product with 1/s is off
+// by a little, so the nearest is found again from x - q s, which is exact (a multiple of
+// half s's last place, at most about s/2).
+__device__ __forceinline__ int8_t quantized(float x, const Scale &c)
+{
+    if (!(c.s > 0)) return 0;                      // 0 and NaN
+    float q = rintf(c.tiny ? x / c.s : x * c.inv);
+    const float t = 2 * fmaf(-q, c.s, x), a = fabsf(t);
+    if (a > c.s || (a == c.s && ((int)q & 1))) q += copysignf(1.0f, t);
+    q = q > 127.0f ? 127.0f : q < -127.0f ? -127.0f : q;
+    return (int8_t)q;
+}
+
+template <int CH>
+__device__ __forceinline__ void store_bytes(int8_t *p, int64_t left, const int8_t (&q)[CH])
+{
+    if (left >= CH) {
+        store_vec<CH>(p, q);
+    } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+            if (j < left) p[j] = q[j];
+    }
+}
+
+// A column stays in the registers of LANES lanes, VPL chunks each, between its read and
+// its write.
+template <typename T, int LANES, int VPL>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void quantize_kernel(int64_t d, int64_t cols, const T *__restrict__ X,
+                                                                             int64_t ldx, int8_t *__restrict__ Q, int64_t ldq,
+                                                                             float *__restrict__ scales)
+{
+    constexpr int CH = 16 / sizeof(T), NT = LANES > 256 ? LANES : 256, COLS = NT / LANES;
+    __shared__ uint32_t s_top[NT / 64];
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < cols; c0 += (int64_t)gridDim.x * COLS) {
+        const int64_t c = c0 + sub;
+        const bool live = c < cols, over = sizeof(T) == 2 && c + 1 < cols && d >= CH;
+        uint32x4 x[VPL];
+        float f[CH];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const int64_t at = (int64_t)(lane + LANES * i) * CH;
+            x[i] = read_raw(X + c * ldx + at, live ? d - at : 0, over);
+        }
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const int64_t left = live ? d - (int64_t)(lane + LANES * i) * CH : 0;
+            values<T>(x[i], f);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const uint32_t b = __builtin_bit_cast(uint32_t, f[j]) & 0x7FFFFFFFu;
+                if (j < left && b > top) top = b;
+            }
+        }
+        const Scale s = scale_from(column_top<LANES>(top, s_top));
+        if (!live) continue;
+        if (lane == 0) scales[c] = s.s;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const int64_t at = (int64_t)(lane + LANES * i) * CH;
+            if (at >= d) continue;
+            int8_t q[CH];
+            values_again<T>(x[i], f);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) q[j] = quantized(f[j], s);
+            store_bytes(Q + c * ldq + at, d - at, q);
+        }
+    }
+}
+
+// Columns of any length: the second pass reads them again.
+template <typename T>
+__global__ __launch_bounds__(1024) void quantize_long_kernel(int64_t d, int64_t cols, const T *__restrict__ X, int64_t ldx,
+                                                             int8_t *__restrict__ Q, int64_t ldq, float *__restrict__ scales)
+{
+    constexpr int CH = 16 / sizeof(T);
+    __shared__ uint32_t s_top[16];
+    for (int64_t c = blockIdx.x; c < cols; c += gridDim.x) {
+        uint32_t top = 0;
+        float f[CH];
+        for (int64_t at = (int64_t)threadIdx.x * CH; at < d; at += 1024 * CH) {
+            read_chunk(X + c * ldx + at, d - at, f);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const uint32_t b = __builtin_bit_cast(uint32_t, f[j]) & 0x7FFFFFFFu;
+                if (b > top) top = b;
+            }
+        }
+        const Scale s = scale_from(column_top<1024>(top, s_top));
+        if (threadIdx.x == 0) scales[c] = s.s;
+        for (int64_t at = (int64_t)threadIdx.x * CH; at < d; at += 1024 * CH) {
+            int8_t q[CH];
+            read_chunk(X + c * ldx + at, d - at, f);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) q[j] = quantized(f[j], s);
+            store_bytes(Q + c * ldq + at, d - at, q);
+        }
+    }
+}
+
+template <typename T>
+int quantize(int64_t d, int64_t cols, const void *X, int64_t ldx, int8_t *Q, int64_t ldq, float *scales, hipStream_t s)
+{
+    const int64_t chunks = (d * (int64_t)sizeof(T) + 15) / 16;
+    auto launch = [&](auto kernel, int lanes) {
+        const int nt = lanes > 256 ? lanes : 256;
+        hipLaunchKernelGGL(kernel, dim3(column_blocks(cols, nt / lanes)), dim3(nt), 0, s, d, cols, (const T *)X, ldx, Q, ldq, scales);
+    };
+    if (chunks <= 16) launch(quantize_kernel<T, 16, 1>, 16);
+    else if (chunks <= 64) launch(quantize_kernel<T, 64, 1>, 64);
+    else if (chunks <= 128) launch(quantize_kernel<T, 64, 2>, 64);
+    else if (chunks <= 256) launch(quantize_kernel<T, 64, 4>, 64);
+    else if (chunks <= 512) launch(quantize_kernel<T, 256, 2>, 256);
+    else if (chunks <= 1024) launch(quantize_kernel<T, 256, 4>, 256);
+    else if (chunks <= 2048) launch(quantize_kernel<T, 512, 4>, 512);
+    else launch(quantize_long_kernel<T>, 1024);
+    return check_launch("quantize_kernel");
+}
+
+}  // namespace
+}  // namespace jlust
+
+using namespace jlust;
+
+extern "C" int jlust_hip_quantize_columns(int32_t value_type, int64_t d, int64_t cols, const void *X, int64_t ldx, int8_t *Q,
+                                          int64_t ldq, float *scales, jlust_stream_t stream)
+{
+    clear_error();
+    const char *who = "quantize";
+    if (int st = check_extents(who, value_type, d, cols)) return st;
+    if (value_type == JLUST_VALUE_F64)
+        return fail(JLUST_STATUS_UNSUPPORTED_VALUE_TYPE, "%s: columns are Float32, Float16 or BFloat16", who);
+    if (int st = check_matrix(who, "X", X, d, cols, ldx, true)) return st;
+    if (int st = check_matrix(who, "Q", Q, d, cols, ldq, true)) return st;
+    if (bad_ptr(scales, cols)) return fail(JLUST_STATUS_INVALID_ARGUMENT, "%s: scales are null", who);
+    if (int st = require_device(nullptr)) return st;
+    if (cols == 0) return JLUST_STATUS_SUCCESS;
+    hipStream_t s = (hipStream_t)stream;
+    switch (value_type) {
+    case JLUST_VALUE_F32: return quantize<float>(d, cols, X, ldx, Q, ldq, scales, s);
+    case JLUST_VALUE_F16: return quantize<_Float16>(d, cols, X, ldx, Q, ldq, scales, s);
+    default: return quantize<__bf16>(d, cols, X, ldx, Q, ldq, scales, s);
+    }
+}
+
+namespace jlust {
+int preload_linear_int8()
+{
+    JLUST_PRELOAD_KERNEL((quantize_kernel<float, 64, 1>));
+    return JLUST_STATUS_SUCCESS;
+}
+}  // namespace jlust

@@ -10,6 +10,7 @@ namespace jlust {
 
 typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
@@ -124,7 +125,8 @@ struct Stage {
     }
 
     // 16-bit operands: what lane (li, g) feeds to a 16x16x32 step: row
-    // 16*tile + li, k = 32*s + 8*g .. + 7.
+    // 16*tile + li, k = 32*s + 8*g .. + 7.  8-bit ones along k: 16 of k to a 16x16x64
+    // step in the place of 8.
     __device__ __forceinline__ static uint32x4 frag16(const char *lds, int tile, int s)
     {
         const int li = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
@@ -183,6 +185,14 @@ __device__ __forceinline__ floatx16 mma(uint32x4 a, uint32x4 b, floatx16 c, __bf
 __device__ __forceinline__ floatx16 mma(uint32x4 a, uint32x4 b, floatx16 c, _Float16)
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ intx4 mma(uint32x4 a, uint32x4 b, intx4 c, int8_t)
+{
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, a), __builtin_bit_cast(intx4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ intx16 mma(uint32x4 a, uint32x4 b, intx16 c, int8_t)
+{
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(intx4, a), __builtin_bit_cast(intx4, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ floatx4 mma(float a, float b, floatx4 c)
 {
@@ -251,6 +261,19 @@ __device__ __forceinline__ void finish(const TileArgs &a, const T *bias, const T
 #pragma unroll
     for (int e = 0; e < V; ++e) t[e] = T(s[e]);
     store_some<V>((T *)a.C + row * a.ldc + mm, left, t);
+}
+
+// The scales of a group's V rows of P from m on (0 past the edge and in no group), and
+// that of the row of Q that n stands for.
+template <int V>
+__device__ __forceinline__ void load_scales(const TileArgs &a, int group, int64_t m, float *by)
+{
+    load_some<V>(a.ps + group * a.gs + m, group < a.groups && m < a.m ? a.m - m : 0, by);
+}
+
+__device__ __forceinline__ float scale_of(const TileArgs &a, int group, int64_t n)
+{
+    return group < a.groups ? a.qs[a.qrow ? a.qrow[n] : n] : 0.0f;
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -365,12 +388,13 @@ template <typename A, int TM> struct SumRows {
     __device__ __forceinline__ static int at(int r, int c) { return r * CHUNKS * 16 + ((c ^ (r & FLIP)) << 4); }
 };
 
-template <typename T, bool KSUM, int TM, int RUNS, typename Put>
+template <typename T, bool KSUM, int TM, int RUNS, typename O, typename Put>
 __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int piece, int group, int n0, int nend, int64_t m0, Put &&put)
 {
     using A = typename Elem<T>::Acc;
     using SR = SumRows<A, TM>;
-    constexpr int CH = 16 / sizeof(T), ACH = 16 / sizeof(A), LANES = TM / CH, ROWS = 64 / LANES, ITER = (16 + ROWS - 1) / ROWS;
+    constexpr bool SCALED = !std::is_same_v<T, O>;
+    constexpr int CH = SCALED ? 8 : 16 / sizeof(O), ACH = 16 / sizeof(A), LANES = TM / CH, ROWS = 64 / LANES, ITER = (16 + ROWS - 1) / ROWS;
     const int lane = threadIdx.x & 63;
     const int r0 = lane < LANES * ROWS ? lane / LANES : 16;
     char *mine = lds + (threadIdx.x >> 6) * SR::BYTES;
@@ -378,19 +402,26 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int pi
     TileArgs b = a;
     if constexpr (KSUM) b.C = (T *)a.C + group * a.gc;
     if (!a.offsets) b.groups = 1;
-    T bias[CH];
+    O bias[CH];
     load_bias<CH>(b, group, m, bias);
+    float by[SCALED ? CH : 1];
+    if constexpr (SCALED) load_scales<CH>(b, group, m, by);
     const int64_t part_rows = KSUM && a.offsets ? a.n * a.groups : a.n;
     const int64_t part_row = piece * part_rows + (KSUM ? group * a.n : 0);
 #pragma unroll
     for (int run = 0; run < RUNS; ++run) {
         // What the rows need from memory, all of it before the first is used.
         int row[ITER];
-        T res[ITER][CH];
+        O res[ITER][CH];
+        float qs[SCALED ? ITER : 1];
 #pragma unroll
         for (int it = 0; it < ITER; ++it) {
             const int r = r0 + it * ROWS, n = n0 + 16 * run + r;
             row[it] = r < 16 && n < nend && left > 0 ? n : -1;
+        }
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int it = 0; it < ITER; ++it) qs[it] = row[it] >= 0 && !a.part ? scale_of(b, group, row[it]) : 0.0f;
         }
         if (!a.part && a.crow) {
 #pragma unroll
@@ -398,7 +429,7 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int pi
         }
         if (a.R && !a.part) {
 #pragma unroll
-            for (int it = 0; it < ITER; ++it) load_some<CH>((const T *)a.R + row[it] * a.ldr + m, row[it] >= 0 ? left : 0, res[it]);
+            for (int it = 0; it < ITER; ++it) load_some<CH>((const O *)a.R + row[it] * a.ldr + m, row[it] >= 0 ? left : 0, res[it]);
         }
         wave_sync();
         put(run, mine);
@@ -410,8 +441,16 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int pi
             A v[CH];
 #pragma unroll
             for (int e = 0; e < CH; e += ACH) __builtin_memcpy(v + e, mine + SR::at(r, (lane % LANES * CH + e) / ACH), 16);
-            if (a.part) store_some<CH>((A *)a.part + (part_row + row[it]) * a.m + m, left, v);
-            else finish<CH, T, A>(b, bias, res[it], row[it], m, v);
+            if (a.part) {
+                store_some<CH>((A *)a.part + (part_row + row[it]) * a.m + m, left, v);
+            } else if constexpr (SCALED) {
+                float f[CH];
+#pragma unroll
+                for (int e = 0; e < CH; ++e) f[e] = (float)v[e] * (qs[it] * by[e]);
+                finish<CH, O, float>(b, bias, res[it], row[it], m, f);
+            } else {
+                finish<CH, T, A>(b, bias, res[it], row[it], m, v);
+            }
         }
     }
 }
@@ -437,7 +476,7 @@ __device__ __forceinline__ void put_rows(const A4 (&acc)[MT][NTL], int j, char *
 // registers.  One LDS tile of 128 bytes of k per row: while the waves multiply
 // it, their loads of the next one are in flight to registers, and two
 // workgroups a CU fill each other's waits.
-template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN>
+template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, typename O = T>
 __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const TileArgs a)
 {
     using A4 = typename Elem<T>::Acc4;
@@ -487,7 +526,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 if (s && k + BK / 2 >= kend) break;
-                if constexpr (sizeof(T) == 2) {
+                if constexpr (sizeof(T) <= 2) {
                     uint32x4 p[MT], q[NTL];
 #pragma unroll
                     for (int j = 0; j < NTL; ++j) q[j] = SQ::frag16(lq, wn0 / 16 + j, s);
@@ -514,7 +553,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
 
     __syncthreads();
     auto put = [&](int j, char *to) { put_rows<typename Elem<T>::Acc, MT, NTL, TM>(acc, j, to); };
-    finish_tile<T, KSUM, TM, NTL>(a, lds, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
+    finish_tile<T, KSUM, TM, NTL, O>(a, lds, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
 }
 
 // ----------------------------------------------- tiles by copies to LDS
@@ -666,16 +705,16 @@ __device__ __forceinline__ void copies_done()
 // As tile_product_kernel for operands whose chunks lie whole and aligned, NB
 // LDS tiles in turn: while one is multiplied, the copies of the next NB - 1 are
 // under way, and a step has one barrier.
-template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB>
+template <typename T, bool PKC, bool QKC, int BM, int BN, int WM, int WN, int BK, int NB, typename O = T>
 __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 32 ? 3 : 2) void tile_copy_kernel(const TileArgs a)
 {
-    constexpr bool HALF = sizeof(T) == 2;
+    constexpr bool HALF = sizeof(T) <= 2;
     constexpr int STEP = HALF ? 32 : 16;                // rows and columns of a matrix step
     constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, MT = TM / STEP, NTL = TN / STEP;
     constexpr int LM = BM > 64 && BM < 128 ? 128 : BM;  // rows of P in LDS
     constexpr bool KSUM = !PKC && !QKC;
     using A = typename Elem<T>::Acc;
-    using Sum = std::conditional_t<HALF, floatx16, floatx4>;
+    using Sum = std::conditional_t<sizeof(T) == 1, intx16, std::conditional_t<HALF, floatx16, floatx4>>;
     using CP = Copy<T, PKC, LM, NT, BK>;
     using CQ = Copy<T, QKC, BN, NT, BK>;
     // Arrays of their own: the compiler then knows which copies an LDS read waits for.
@@ -717,7 +756,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
             asm("" : "+v"(pa), "+v"(qa));          // its flips are made here, not held in registers over the loop
             if constexpr (HALF) {
 #pragma unroll
-                for (int s = 0; s < BK / 16; ++s) {
+                for (int s = 0; s < BK * (int)sizeof(T) / 32; ++s) {
                     uint32x4 p[MT], q[NTL];
 #pragma unroll
                     for (int j = 0; j < NTL; ++j) q[j] = CQ::frag(from + CP::BYTES, qa, j, s);
@@ -803,7 +842,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    float v[4];
+                    A v[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = acc[i][run / 2][4 * q + e];
                     __builtin_memcpy(to + SumRows<A, TM>::at(lane & 15, 8 * i + 2 * q + (lane >> 5)), v, 16);
@@ -812,7 +851,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
             put_rows<A, MT, NTL, TM>(acc, run, to);
         }
     };
-    finish_tile<T, KSUM, TM, TN / 16>(a, lds0, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
+    finish_tile<T, KSUM, TM, TN / 16, O>(a, lds0, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
 }
 
 // ------------------------------------------------------------ few columns
@@ -831,14 +870,17 @@ template <int TILES> struct Few {
     static constexpr int WAVES = TILES == 1 ? 8 : 16, STEPS = TILES == 1 ? 4 : 2;
 };
 
-template <typename T, bool PKC, int TILES>
+template <typename T, bool PKC, int TILES, typename O = T>
 __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(const TileArgs a)
 {
     using F = Few<TILES>;
-    constexpr int CH = 8, WAVES = F::WAVES, STEPS = F::STEPS, M = 16 * TILES, SPAN = 32 * STEPS;
+    using A = typename Elem<T>::Acc;
+    using A4 = typename Elem<T>::Acc4;
+    constexpr bool SCALED = !std::is_same_v<T, O>;
+    constexpr int CH = 16 / sizeof(T), K = 4 * CH, WAVES = F::WAVES, STEPS = F::STEPS, M = 16 * TILES, SPAN = K * STEPS;
     constexpr int LANES = M / CH, ROWS = 64 / LANES;       // sc: lanes of a row of k, rows of one read
     static_assert(PKC || ROWS * TILES == 32, "TILES reads make a step");
-    __shared__ __align__(16) float s_sum[WAVES][16][M];
+    __shared__ __align__(16) A s_sum[WAVES][16][M];
     __shared__ __align__(16) char s_turn[PKC ? 16 : WAVES * STEPS * 32 * M * 2];
     Work w;
     if (!find_work<false, 16, 64>(a, &w)) return;
@@ -846,11 +888,11 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
     const int64_t m0 = (int64_t)w.tm * M;
     const T *P = (const T *)a.P + w.group * a.gp;
 
-    // kc: 16 bytes of row m0 + li from k = 8 g; sc: 16 bytes of m of every ROWS'th row.
+    // kc: 16 bytes of row m0 + li from k = CH g; sc: 16 bytes of m of every ROWS'th row.
     const T *p;
     int64_t avail = CH;
     if constexpr (PKC) {
-        p = P + (m0 + li < a.m ? m0 + li : a.m - 1) * a.ldp + 8 * g;
+        p = P + (m0 + li < a.m ? m0 + li : a.m - 1) * a.ldp + CH * g;
     } else {
         const int64_t m = m0 + CH * (lane % LANES);
         avail = a.m - m;
@@ -859,13 +901,13 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
     const int64_t over = a.m >= CH ? a.k - 1 : 0;          // as in Stage
     int col = w.n0 + li < w.nend ? w.n0 + li : w.nend - 1;
     if (a.qrow) col = a.qrow[col];
-    const T *q = (const T *)a.Q + (int64_t)col * a.ldq + 8 * g;
+    const T *q = (const T *)a.Q + (int64_t)col * a.ldq + CH * g;
 
     const uint32x4 zero = {0, 0, 0, 0};
     auto read = [&](int k, uint32x4 (&pv)[STEPS][TILES], uint32x4 (&qv)[STEPS]) {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const int at = k + 32 * s, left = w.kend - at - 8 * g;
+            const int at = k + K * s, left = w.kend - at - CH * g;
             qv[s] = left >= CH ? load_chunk(q + at) : left > 0 ? load_chunk_part(q + at, left) : zero;
 #pragma unroll
             for (int u = 0; u < TILES; ++u) {
@@ -879,9 +921,9 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
             }
         }
     };
-    floatx4 acc[TILES];
+    A4 acc[TILES];
 #pragma unroll
-    for (int u = 0; u < TILES; ++u) acc[u] = floatx4{0, 0, 0, 0};
+    for (int u = 0; u < TILES; ++u) acc[u] = A4{0, 0, 0, 0};
     auto multiply = [&](uint32x4 (&pv)[STEPS][TILES], uint32x4 (&qv)[STEPS]) {
         if constexpr (!PKC) {
             char *turn = s_turn + wave * STEPS * 32 * M * 2;
@@ -932,22 +974,29 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
     const int i = threadIdx.x / M, j = threadIdx.x % M, n = w.n0 + i;
     const int64_t m = m0 + j;
     if (i >= 16 || n >= w.nend || m >= a.m) return;
-    float v[1] = {0};
+    A v[1] = {0};
 #pragma unroll
     for (int u = 0; u < WAVES; ++u) v[0] += s_sum[u][i][j];
     TileArgs b = a;
     if (!a.offsets) b.groups = 1;
     const int64_t row = a.crow ? (int64_t)a.crow[n] : n;
-    T bias[1], res[1];
+    O bias[1], res[1];
     load_bias<1>(b, w.group, m, bias);
-    if (a.R) res[0] = ((const T *)a.R)[row * a.ldr + m];
-    finish<1, T, float>(b, bias, res, row, m, v);
+    if (a.R) res[0] = ((const O *)a.R)[row * a.ldr + m];
+    if constexpr (SCALED) {
+        float by[1];
+        load_scales<1>(b, w.group, m, by);
+        float f[1] = {(float)v[0] * (scale_of(b, w.group, n) * by[0])};
+        finish<1, O, float>(b, bias, res, row, m, f);
+    } else {
+        finish<1, T, float>(b, bias, res, row, m, v);
+    }
 }
 
 // Adds the split partial sums and ends as the kernels above would.  256 threads are
 // 256/LANES items of 4 values by LANES shares of the splits, each share added in
 // order and then the shares in theirs.
-template <typename T, bool KSUM, int LANES>
+template <typename T, bool KSUM, int LANES, typename O = T>
 __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
 {
     using A = typename Elem<T>::Acc;
@@ -999,11 +1048,20 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
     } else {
         b.groups = 1;
     }
-    T bias[V], res[V];
+    O bias[V], res[V];
     load_bias<V>(b, group, m, bias);
     const int64_t row = a.crow ? (int64_t)a.crow[n] : n;
-    if (a.R) load_some<V>((const T *)a.R + row * a.ldr + m, a.m - m, res);
-    finish<V, T, A>(b, bias, res, row, m, s);
+    if (a.R) load_some<V>((const O *)a.R + row * a.ldr + m, a.m - m, res);
+    if constexpr (!std::is_same_v<T, O>) {
+        float by[V], f[V];
+        load_scales<V>(b, group, m, by);
+        const float qs = scale_of(b, group, n);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = (float)s[e] * (qs * by[e]);
+        finish<V, O, float>(b, bias, res, row, m, f);
+    } else {
+        finish<V, T, A>(b, bias, res, row, m, s);
+    }
 }
 
 // ------------------------------------------------------------------- host
@@ -1079,7 +1137,23 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
 
     ShapeCost some[4];
     int count = 0;
-    if (sizeof(T) == 2 && !ksum && share <= 16) {
+    if constexpr (sizeof(T) == 1) {
+        // Along k on both sides.  The bytes of a step, and so its time, are 16-bit
+        // values', its k is twice theirs.
+        if (share <= 16 && set(FEW_16, 1)) {
+            some[count++] = {FEW_16, 0.5, 0.035, 4};
+        } else if (share <= 48) {
+            some[count++] = {REG_32, 3.0, 0.25, 5};
+        } else if (fit && (!a->offsets || share >= 1024) && tiles(COPY_256) >= 512 && k > 384) {
+            some[count++] = {COPY_256, 9.0, 0.65, 1};
+        } else {
+            if (fit && k > 384) {
+                some[count++] = {COPY_TALL, 9.0, 0.48, 2};
+                some[count++] = {COPY_128, 8.4, 0.31, 2};
+            }
+            some[count++] = {REG_M64, 4.4, 0.29, 5};
+        }
+    } else if (sizeof(T) == 2 && !ksum && share <= 16) {
         if (!set(FEW_16, 1)) {
             some[count++] = {REG_16, 1.0, 0.5, 6};
         } else if (pkc) {

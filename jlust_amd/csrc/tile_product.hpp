@@ -40,6 +40,11 @@ struct TileArgs {
     // over the k of [offsets[g], offsets[g+1]).
     const int32_t *offsets = nullptr;
     int groups = 0;
+    // Products of 8-bit integers, whose C, bias, R and Z hold another type: what a row
+    // of P and a row of Q are times of.
+    const float *ps = nullptr;          // m values, gs elements between groups
+    int64_t gs = 0;
+    const float *qs = nullptr;          // by the rows of Q
     void *part = nullptr;               // partial sums [split][C's rows][m]
     int split = 1;
     int tiles_m = 0, tiles_n = 0;
@@ -47,9 +52,11 @@ struct TileArgs {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef double doublex4 __attribute__((ext_vector_type(4)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Elem { using Acc = float; using Acc4 = floatx4; };
+template <> struct Elem<int8_t> { using Acc = int; using Acc4 = intx4; };
 template <> struct Elem<double> { using Acc = double; using Acc4 = doublex4; };
 
 // ------------------------------------------------------------ loads, stores
@@ -138,6 +145,9 @@ template <typename T>
 int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes);
 template <typename T>
 int launch_tile_product(const TileArgs &a, bool pkc, bool qkc, int shape, hipStream_t s);
+// The same of 8-bit operands along k, C holding O.
+template <typename O>
+int launch_tile_product8(const TileArgs &a, int shape, hipStream_t s);
 
 // What a shape is: its tile, and whether its operands are copied to LDS.
 struct TileForm { int m, n, copies; };

@@ -15,6 +15,16 @@ one sample, and matrices are column-major as everywhere here.
     execute(LayerNormOp, X, Y, weight=w, bias=b, eps=1e-5, stats=S)
     execute(LayerNormGradOp, X, dY, S, weight=w, dX=.., dweight=.., dbias=..)
 
+    execute(QuantizeOp, X, Xq, xs)
+        Int8 columns with a Float32 scale each: Xq = X ./ xs' to the nearest
+    execute(LinearOp, Wq, Xq, Y, w_scale=ws, x_scale=xs, ...)      # and execute(h, Wq, Xq, Y, ...)
+        the products of Int8 matrices, W*X being (Wq*Xq) .* ws .* xs' with a scale
+        for each row of W (out values, out x groups for a plan's) and each column of
+        X; Wq lies along inp (QuantizeOp of W's transpose makes it).  Y, bias,
+        residual and preact are Float32, Float16 or BFloat16.  No gradient.
+
+experts.py has the operators around a layer's experts and dropout.
+
 Float64, Float32, Float16 and BFloat16, one type for all operands of a call;
 sums and the stats are Float32 (Float64 for Float64).  The results are the
 caller's buffers; execute returns the first of them.  A vector stands for one
@@ -43,6 +53,7 @@ _ACTS = (FN_IDENTITY, FN_RELU, FN_GELU, FN_SILU)
 # in a call of a few microseconds.
 _LINEAR = struct.Struct("@4i19q").pack
 _LINEAR_GRAD = struct.Struct("@4i22q").pack
+_LINEAR_INT8 = struct.Struct("@2i22q").pack
 
 
 # --------------------------------------------------------------------- checks
@@ -112,9 +123,10 @@ def _extents(t, name):
     raise IncompatibleExtents(f"{name}: {t.dim()}-D arrays are not supported")
 
 
-def _weights(t, name, groups, index, T):
+def _weights(t, name, groups, index, T, along_rows=False):
     """(address, layout, leading dimension, group stride, out, inp) of a weight
-    matrix, or of one per group: contiguous along either side."""
+    matrix, or of one per group: contiguous along either side (along_rows: along
+    the first alone)."""
     if t.dtype is not T or t.get_device() != index:
         _same(t, name, index, T)
     shape, strides = t.shape, t.stride()
@@ -125,9 +137,9 @@ def _weights(t, name, groups, index, T):
     if groups and shape[2] != groups:
         raise IncompatibleExtents(f"{name} holds {shape[2]} matrices, expected {groups}")
     s0, s1 = strides[0], strides[1]
-    if (s0 == 1 or out <= 1) and (s1 >= out or inp <= 1) and not (out <= 1 and s1 == 1):
+    if (s0 == 1 or out <= 1) and (s1 >= out or inp <= 1) and (along_rows or not (out <= 1 and s1 == 1)):
         layout, ld = 0, s1 if inp > 1 else max(out, 1)
-    elif (s1 == 1 or inp <= 1) and (s0 >= inp or out <= 1):
+    elif (s1 == 1 or inp <= 1) and (s0 >= inp or out <= 1) and not along_rows:
         layout, ld = 1, s0 if out > 1 else max(inp, 1)
     else:
         raise NonCanonicalStorage(f"{name}: a matrix is column-major or the transpose of one, got strides "
@@ -256,11 +268,15 @@ def _columns(X, Y, h):
     return n, xc
 
 
-def _linear(h, W, X, Y, bias=None, act=None, residual=None, preact=None):
+def _linear(h, W, X, Y, bias=None, act=None, residual=None, preact=None, w_scale=None, x_scale=None):
     w = W if type(W) is torch.Tensor else _raw(W, "W")
     x = X if type(X) is torch.Tensor else _raw(X, "X")
     y = Y if type(Y) is torch.Tensor else _raw(Y, "Y")
     T = w.dtype
+    if T is torch.int8:
+        return _linear_int8(h, w, x, Y, y, bias, act, residual, preact, w_scale, x_scale)
+    if w_scale is not None or x_scale is not None:
+        raise UnsupportedValueType(T, _BE, f"w_scale and x_scale belong to Int8 operands, W is {T}")
     vt, index = _first(w, "W")
     groups, copies, plan = 0, 1, 0
     if h is not None:
@@ -277,6 +293,53 @@ def _linear(h, W, X, Y, bias=None, act=None, residual=None, preact=None):
     _run(_lib.lib().jlust_hip_linear, index, "linear", T,
          _LINEAR(vt, _act(act), layout, 0, out, inp, n, wp, ldw, xp, ldx, yp, ldy, bp, rp, ldr, zp, ldz, groups, copies,
                  plan, ws, bs))
+    return Y
+
+
+def _linear_int8(h, w, x, Y, y, bias, act, residual, preact, w_scale, x_scale):
+    if w_scale is None or x_scale is None:
+        raise TypeError("the product of Int8 matrices needs w_scale and x_scale")
+    index, T = w.get_device(), y.dtype
+    if index < 0:
+        raise DeviceMismatch(f"HIPBackend needs GPU buffers, W is on {w.device}")
+    vt = _TYPES.get(T)
+    if vt is None or vt == 0:
+        raise UnsupportedValueType(T, _BE, f"the product of Int8 matrices is Float32, Float16 or BFloat16, Y is {T}")
+    groups, copies, plan = 0, 1, 0
+    if h is not None:
+        if h.index != index:
+            raise DeviceMismatch(f"the plan is on {h.dev}, W on {w.device}")
+        groups, copies, plan = h.groups, h.copies, h.use()
+    # A matrix that lies along both sides (one row or column) is read along inp.
+    wp, _, ldw, ws, inp, out = _weights(w.transpose(0, 1) if w.dim() > 1 else w, "W' (Int8 matrices lie along inp)", groups, index,
+                                        torch.int8, along_rows=True)
+    n, xc = _columns(x, y, h)
+    xp, ldx = _matrix(x, "X", inp, xc, index, torch.int8)
+    yp, ldy = _matrix(y, "Y", out, n, index, T)
+    sp, ss = _bias(w_scale, "w_scale", out, groups, index, torch.float32)
+    sx = _norm_vector(x_scale, "x_scale", xc, index, torch.float32)
+    bp, bs = _bias(bias, "bias", out, groups, index, T) if bias is not None else (0, 0)
+    rp, ldr = _matrix(residual, "residual", out, n, index, T)
+    zp, ldz = _matrix(preact, "preact", out, n, index, T)
+    _run(_lib.lib().jlust_hip_linear_int8, index, "linear_int8", T,
+         _LINEAR_INT8(vt, _act(act), out, inp, n, wp, ldw, sp, xp, ldx, sx, yp, ldy, bp, rp, ldr, zp, ldz, groups, copies,
+                      plan, ws, ss, bs))
+    return Y
+
+
+def _quantize(X, Y, scales):
+    x = X if type(X) is torch.Tensor else _raw(X, "X")
+    T = x.dtype
+    vt, index = _first(x, "X")
+    if vt == 0:
+        raise UnsupportedValueType(T, _BE, "QuantizeOp takes Float32, Float16 or BFloat16")
+    d, cols = _extents(x, "X")
+    xp, ldx = _matrix(x, "X", d, cols, index, T)
+    yp, ldy = _matrix(Y, "Y", d, cols, index, torch.int8)
+    sp = _norm_vector(scales, "scales", cols, index, torch.float32)
+    if sp == 0 and cols:
+        raise TypeError("QuantizeOp needs scales")
+    _run(_lib.lib().jlust_hip_quantize_columns, index, "quantize", T, vt, d, cols, xp, ldx, yp, ldy, sp)
     return Y
 
 
@@ -379,8 +442,15 @@ def execute(optype, args, backend, kw):
         return _linear(*_plan(args, "GroupedLinearOp"), **kw)
     if tag == "LayerNorm":
         return _layer_norm(*args, **kw)
+    if tag == "Quantize":
+        return _quantize(*args, **kw)
+    if tag in experts.TAGS:
+        return experts.TAGS[tag](*args, **kw)
     if tag == "LinearGrad":
         return _linear_grad(None, *args, **kw)
     if tag == "GroupedLinearGrad":
         return _linear_grad(*_plan(args, "GroupedLinearGradOp"), **kw)
     return _layer_norm_grad(*args, **kw)
+
+
+from . import experts  # noqa: E402  (it takes this module's checks)

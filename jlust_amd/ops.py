@@ -55,8 +55,15 @@ GroupedLinearOp = OpType("GroupedLinear")
 GroupedLinearGradOp = OpType("GroupedLinearGrad")
 LayerNormOp = OpType("LayerNorm")
 LayerNormGradOp = OpType("LayerNormGrad")
+QuantizeOp = OpType("Quantize")
+# What stands around a layer's experts, and dropout (experts.py; not in the reference).
+RouteOp = OpType("Route")
+RouteGradOp = OpType("RouteGrad")
+CombineOp = OpType("Combine")
+CombineGradOp = OpType("CombineGrad")
+DropoutOp = OpType("Dropout")
 _LAYER_TAGS = frozenset(("Linear", "LinearGrad", "GroupedLinear", "GroupedLinearGrad", "LayerNorm",
-                         "LayerNormGrad"))
+                         "LayerNormGrad", "Quantize", "Route", "RouteGrad", "Combine", "CombineGrad", "Dropout"))
 
 
 # ------------------------------------------------------------------ backends
