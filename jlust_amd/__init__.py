@@ -28,6 +28,7 @@ from .block_banded import BlockBandedMatrix
 from .elementwise import (ElementwiseFn, abs_fn, affine_fn, exp_fn, gelu_fn, identity_fn, log_fn,
                           relu_fn, silu_fn, sqrt_fn, square_fn)
 from .layers import GroupPlan
+from . import experts as _experts  # noqa: F401  (its operators, entered with the package)
 from .convert import (convert_format, convert_index_type, convert_value_type, csc_tensor,
                       dcsr_tensor, sparse_to_dense)
 from ._lib import preload

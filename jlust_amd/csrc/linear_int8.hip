@@ -1,6 +1,7 @@
 // linear_int8.hip -- the dense products of 8-bit integers, and the columns' scales and
 // integers that they take.
 #include "column_chunks.hpp"
+#include "lanes.hpp"
 #include "tile_kernel.hpp"
 
 namespace jlust {
@@ -67,11 +68,7 @@ namespace {
 template <int LANES>
 __device__ __forceinline__ uint32_t column_top(uint32_t v, uint32_t *lds)
 {
-#pragma unroll
-    for (int d = (LANES < 64 ? LANES : 64) / 2; d; d >>= 1) {
-        const uint32_t o = __shfl_xor(v, d, 64);
-        v = o > v ? o : v;
-    }
+    v = over_lanes<(LANES < 64 ? LANES : 64)>(v, Larger());
     if constexpr (LANES > 64) {
         constexpr int W = LANES / 64;
         __syncthreads();
@@ -83,27 +80,30 @@ __device__ __forceinline__ uint32_t column_top(uint32_t v, uint32_t *lds)
     return v;
 }
 
-struct Scale { float s, inv; bool tiny; };
+// A column's scale s; x and s are both times `up` where 1/s would pass the type's range.
+// 0 but for s: the column becomes zeros.
+struct Scale { float s, by, inv, up; };
 
-// 1/s may be infinite below the normal range: there x is divided.
 __device__ __forceinline__ Scale scale_from(uint32_t top)
 {
-    if (top >= 0x7F800000u) return {__builtin_nanf(""), 0.0f, false};
+    if (top >= 0x7F800000u) return {__builtin_nanf(""), 0.0f, 0.0f, 0.0f};
     const float s = (float)((double)__builtin_bit_cast(float, top) / 127.0);
-    return {s, s > 0 ? 1.0f / s : 0.0f, s < 1.1754944e-38f};
+    if (s == 0) return {0.0f, 0.0f, 0.0f, 0.0f};
+    const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, by = s * up;
+    return {s, by, 1.0f / by, up};
 }
 
 // x / s to the nearest whole number, halves to the even one: the product with 1/s is off
 // by a little, so the nearest is found again from x - q s, which is exact (a multiple of
-// half s's last place, at most about s/2).
-__device__ __forceinline__ int8_t quantized(float x, const Scale &c)
+// half s's last place, at most about s/2): an odd q is left at s/2, an even one past it.
+__device__ __forceinline__ int quantized(float x, const Scale &c)
 {
-    if (!(c.s > 0)) return 0;                      // 0 and NaN
-    float q = rintf(c.tiny ? x / c.s : x * c.inv);
-    const float t = 2 * fmaf(-q, c.s, x), a = fabsf(t);
-    if (a > c.s || (a == c.s && ((int)q & 1))) q += copysignf(1.0f, t);
-    q = q > 127.0f ? 127.0f : q < -127.0f ? -127.0f : q;
-    return (int8_t)q;
+    x *= c.up;
+    const float q = rintf(x * c.inv), t = 2 * fmaf(-q, c.by, x);
+    const int n = (int)q, bits = __builtin_bit_cast(int, t);
+    const int past = (bits & 0x7FFFFFFF) > __builtin_bit_cast(int, c.by) - (n & 1) ? (bits >> 31) | 1 : 0;
+    const int m = n + past;
+    return m > 127 ? 127 : m < -127 ? -127 : m;
 }
 
 template <int CH>
@@ -157,9 +157,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void quantize_kernel(int
             const int64_t at = (int64_t)(lane + LANES * i) * CH;
             if (at >= d) continue;
             int8_t q[CH];
+            if (s.up == 0) x[i] = uint32x4{0, 0, 0, 0};
             values_again<T>(x[i], f);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) q[j] = quantized(f[j], s);
+            for (int j = 0; j < CH; ++j) q[j] = (int8_t)quantized(f[j], s);
             store_bytes(Q + c * ldq + at, d - at, q);
         }
     }
@@ -187,9 +188,9 @@ __global__ __launch_bounds__(1024) void quantize_long_kernel(int64_t d, int64_t 
         if (threadIdx.x == 0) scales[c] = s.s;
         for (int64_t at = (int64_t)threadIdx.x * CH; at < d; at += 1024 * CH) {
             int8_t q[CH];
-            read_chunk(X + c * ldx + at, d - at, f);
+            values<T>(read_raw(X + c * ldx + at, s.up == 0 ? 0 : d - at), f);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) q[j] = quantized(f[j], s);
+            for (int j = 0; j < CH; ++j) q[j] = (int8_t)quantized(f[j], s);
             store_bytes(Q + c * ldq + at, d - at, q);
         }
     }
@@ -203,10 +204,13 @@ int quantize(int64_t d, int64_t cols, const void *X, int64_t ldx, int8_t *Q, int
         const int nt = lanes > 256 ? lanes : 256;
         hipLaunchKernelGGL(kernel, dim3(column_blocks(cols, nt / lanes)), dim3(nt), 0, s, d, cols, (const T *)X, ldx, Q, ldq, scales);
     };
+    // Few columns wait for one of them: it goes over more lanes.
+    const bool few = cols <= 512;
     if (chunks <= 16) launch(quantize_kernel<T, 16, 1>, 16);
     else if (chunks <= 64) launch(quantize_kernel<T, 64, 1>, 64);
-    else if (chunks <= 128) launch(quantize_kernel<T, 64, 2>, 64);
-    else if (chunks <= 256) launch(quantize_kernel<T, 64, 4>, 64);
+    else if (chunks <= 128 && !few) launch(quantize_kernel<T, 64, 2>, 64);
+    else if (chunks <= 256 && !few) launch(quantize_kernel<T, 64, 4>, 64);
+    else if (chunks <= 256) launch(quantize_kernel<T, 256, 1>, 256);
     else if (chunks <= 512) launch(quantize_kernel<T, 256, 2>, 256);
     else if (chunks <= 1024) launch(quantize_kernel<T, 256, 4>, 256);
     else if (chunks <= 2048) launch(quantize_kernel<T, 512, 4>, 512);

@@ -8,6 +8,7 @@
 // Keys are Float64: which of two experts is chosen goes by the scores and not by
 // their rounding.  Without a bias the logits are the keys, in the same order.
 #include "column_chunks.hpp"
+#include "lanes.hpp"
 #include "wave.hpp"
 
 #include <cmath>
@@ -31,63 +32,6 @@ struct RouteArgs {
     void *weights;
     int64_t ldw;
     double scale;
-};
-
-// v of another lane: of the one whose number differs in bit 0 or 1, of the mirror place
-// among 8 or 16.
-template <int CTRL, typename A>
-__device__ __forceinline__ A from_lane(A v)
-{
-    if constexpr (sizeof(A) == 4) {
-        return __builtin_bit_cast(A, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-    } else {
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const uint32_t lo = __builtin_amdgcn_mov_dpp((int)u, CTRL, 0xf, 0xf, true);
-        const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xf, 0xf, true);
-        return __builtin_bit_cast(A, (uint64_t)hi << 32 | lo);
-    }
-}
-
-// f of v here and in the other row of 16 (ROWS 16) or half (32) of the wave.
-template <int ROWS, typename A, typename F>
-__device__ __forceinline__ A with_other(A v, F &&f)
-{
-    auto swap = [](uint32_t x) {
-        if constexpr (ROWS == 16) return __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        else return __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    };
-    if constexpr (sizeof(A) == 4) {
-        const auto r = swap(__builtin_bit_cast(uint32_t, v));
-        const uint32_t here = r[0], other = r[1];  // bit_cast of a vector's element takes the first
-        return f(__builtin_bit_cast(A, here), __builtin_bit_cast(A, other));
-    } else {
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
-        return f(__builtin_bit_cast(A, (uint64_t)hi[0] << 32 | lo[0]), __builtin_bit_cast(A, (uint64_t)hi[1] << 32 | lo[1]));
-    }
-}
-
-// f over the first `lanes` (a power of two) lanes of every run of as many, in each of
-// them.  Between vector registers: a step by LDS takes some 100 cycles.
-template <int LANES, typename A, typename F>
-__device__ __forceinline__ A over_lanes(A v, F &&f, int lanes = LANES)
-{
-    if (LANES >= 2 && lanes >= 2) v = f(v, from_lane<0xB1>(v));
-    if (LANES >= 4 && lanes >= 4) v = f(v, from_lane<0x4E>(v));
-    if (LANES >= 8 && lanes >= 8) v = f(v, from_lane<0x141>(v));
-    if (LANES >= 16 && lanes >= 16) v = f(v, from_lane<0x140>(v));
-    if (LANES >= 32 && lanes >= 32) v = with_other<16>(v, f);
-    if (LANES >= 64 && lanes >= 64) v = with_other<32>(v, f);
-    return v;
-}
-
-struct Larger {
-    template <typename A>
-    __device__ __forceinline__ A operator()(A a, A b) const { return b > a ? b : a; }
-};
-struct Plus {
-    template <typename A>
-    __device__ __forceinline__ A operator()(A a, A b) const { return a + b; }
 };
 
 template <int LANES, typename A>
@@ -339,12 +283,23 @@ struct RouteGradArgs {
     double scale;
 };
 
+// exp(l - top) of many scores, where 16-bit results take no more than the hardware's.
+template <typename T, typename A>
+__device__ __forceinline__ A score_below(A l, A top)
+{
+    if constexpr (sizeof(T) == 2) return l == top ? A(1) : __expf(l - top);
+    else return exp_below(l, top);
+}
+
 // With t = scale dw and p the weights' shares of the chosen: softmax renormalised
 // p (t - sum p t), sigmoid renormalised the same times 1 - s, sigmoid t s (1 - s) at the
-// chosen and 0 elsewhere; softmax as it is s_e (t_e - sum s t) everywhere.
-template <typename T, int LANES>
+// chosen and 0 elsewhere; softmax as it is s_e (t_e - sum s t) everywhere.  LANES lanes
+// take a column, CPL chunks of 16 bytes each in registers, so logits are read once (CPL
+// 0: any number, read again).
+template <typename T, int LANES, int CPL>
 __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
 {
+    constexpr int CH = 16 / sizeof(T), HELD = CPL ? CPL : 1;
     using A = typename Elem<T>::Acc;
     constexpr int COLS = 256 / LANES, NP = MAX_COPIES / LANES;
     __shared__ int s_expert[COLS][MAX_COPIES];
@@ -355,14 +310,40 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
         const int64_t c = c0 + sub;
         const bool live = c < a.cols;
         const T *L = (const T *)a.L + c * a.ldl;
-        A top = -INFINITY, total = A(0);
-        if (dense) {
+        A top = -INFINITY, total = A(0), s[HELD][CH];
+        if (CPL > 0 && dense) {
+            uint32x4 raw[HELD];
+#pragma unroll
+            for (int i = 0; i < CPL; ++i) {
+                const int at = (lane + LANES * i) * CH;
+                raw[i] = read_raw(L + at, live ? a.experts - at : 0);
+            }
+#pragma unroll
+            for (int i = 0; i < CPL; ++i) {
+                values<T>(raw[i], s[i]);
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const bool some = live && (lane + LANES * i) * CH + j < a.experts && s[i][j] > A(-INFINITY);
+                    s[i][j] = some ? s[i][j] : A(-INFINITY);
+                    top = s[i][j] > top ? s[i][j] : top;
+                }
+            }
+            top = lanes_max<LANES>(top);
+#pragma unroll
+            for (int i = 0; i < CPL; ++i)
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    s[i][j] = s[i][j] > A(-INFINITY) ? score_below<T>(s[i][j], top) : A(0);
+                    total += s[i][j];
+                }
+            total = lanes_sum<LANES>(total);
+        } else if (dense) {
             if (live)
                 for (int e = lane; e < a.experts; e += LANES) top = A(L[e]) > top ? A(L[e]) : top;
             top = lanes_max<LANES>(top);
             if (live)
                 for (int e = lane; e < a.experts; e += LANES)
-                    if (A(L[e]) > A(-INFINITY)) total += exp_below(A(L[e]), top);
+                    if (A(L[e]) > A(-INFINITY)) total += score_below<T>(A(L[e]), top);
             total = lanes_sum<LANES>(total);
         }
         A l[NP], t[NP], p[NP];
@@ -411,16 +392,37 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
             s_part[sub][i] = at[q] >= 0 ? g : A(0);
         }
         wave_sync();
-        if (live)
+        if constexpr (CPL > 0) {
+            const A inv = total > A(0) ? A(1) / total : A(0);
+#pragma unroll
+            for (int i = 0; i < CPL; ++i) {
+                const int at = (lane + LANES * i) * CH;
+                A g[CH];
+#pragma unroll
+                for (int j = 0; j < CH; ++j) g[j] = A(0);
+                for (int k = 0; k < a.copies; ++k) {
+                    const int e = s_expert[sub][k] - at;
+                    const A v = s_part[sub][k];
+#pragma unroll
+                    for (int j = 0; j < CH; ++j) g[j] += e == j ? v : A(0);
+                }
+                if (dense) {
+#pragma unroll
+                    for (int j = 0; j < CH; ++j) g[j] = s[i][j] * inv * (g[j] - dot);
+                }
+                if (live) write_chunk((T *)a.dL + c * a.lddl + at, a.experts - at, g);
+            }
+        } else if (live) {
             for (int e = lane; e < a.experts; e += LANES) {
                 A g = A(0);
                 for (int i = 0; i < a.copies; ++i) g += s_expert[sub][i] == e ? s_part[sub][i] : A(0);
                 if (dense) {
                     const A v = A(L[e]);
-                    g = v > A(-INFINITY) ? exp_below(v, top) / total * (g - dot) : A(0);
+                    g = v > A(-INFINITY) ? score_below<T>(v, top) / total * (g - dot) : A(0);
                 }
                 ((T *)a.dL)[c * a.lddl + e] = T(g);
             }
+        }
         wave_sync();
     }
 }
@@ -567,8 +569,17 @@ extern "C" int jlust_hip_route_grad(const jlust_route_grad *op, jlust_stream_t s
     a.lddl = op->lddl;
     a.scale = op->scale;
     return with_type(op->value_type, [&](auto t) {
-        hipLaunchKernelGGL((route_grad_kernel<decltype(t), 64>), dim3(column_blocks(a.cols, 4)), dim3(256), 0, (hipStream_t)stream, a);
-        return check_launch("route_grad_kernel");
+        using T = decltype(t);
+        const int64_t chunks = (a.experts * (int64_t)sizeof(T) + 15) / 16;
+        auto launch = [&](auto kernel, int lanes) {
+            hipLaunchKernelGGL(kernel, dim3(column_blocks(a.cols, 256 / lanes)), dim3(256), 0, (hipStream_t)stream, a);
+            return check_launch("route_grad_kernel");
+        };
+        if (chunks <= 16) return launch(route_grad_kernel<T, 16, 1>, 16);
+        if (chunks <= 32) return launch(route_grad_kernel<T, 16, 2>, 16);
+        if (chunks <= 64) return launch(route_grad_kernel<T, 16, 4>, 16);
+        if (chunks <= 256) return launch(route_grad_kernel<T, 64, 4>, 64);
+        return launch(route_grad_kernel<T, 64, 0>, 64);
     });
 }
 

@@ -42,7 +42,7 @@ import torch
 from . import _lib
 from .errors import DeviceMismatch, IncompatibleExtents, NonCanonicalStorage, UnsupportedIndexType, UnsupportedValueType
 from .layers import _BE, _extents, _first, _matrix, _norm_vector, _raw, _run
-from .tensor import OneBased
+from .ops import _layer_calls
 
 # jlust_route and jlust_route_grad of include/jlust_hip.h.
 _ROUTE = struct.Struct("@4i13qd").pack
@@ -58,39 +58,42 @@ def _score(score):
     return kind
 
 
-def _sums(vt):
-    return torch.float64 if vt == 0 else torch.float32
+def _tensor(t, name):
+    return t if type(t) is torch.Tensor else _raw(t, name)
 
 
-def _of_column(t, name, cols):
-    """`t`, a vector of one value a column as a matrix of one row."""
-    t = _raw(t, name)
-    if t.dim() == 1 and cols != 1:
+def _by_column(t, name, cols):
+    """`t` with a column for each of `cols`: a vector holds one value each."""
+    if type(t) is not torch.Tensor:
+        t = _raw(t, name)
+    if cols != 1 and len(t.shape) == 1:
         return t.unsqueeze(0)
     return t
 
 
 def _origin(origin):
-    return (OneBased() if origin is None else origin).offset
+    return 1 if origin is None else origin.offset
 
 
 def _logits(L, ids):
-    l = _raw(L, "L")
+    l = L if type(L) is torch.Tensor else _raw(L, "L")
+    T = l.dtype
     vt, index = _first(l, "L")
     experts, cols = _extents(l, "L")
-    lp, ldl = _matrix(l, "L", experts, cols, index, l.dtype)
-    i = _of_column(ids, "ids", cols)
+    lp, ldl = _matrix(l, "L", experts, cols, index, T)
+    i = _by_column(ids, "ids", cols)
     if i.dtype is not torch.int32:
         raise UnsupportedIndexType(i.dtype, _BE)
-    copies, _ = _extents(i, "ids")
+    copies = i.shape[0] if len(i.shape) else 0
     ip, ldi = _matrix(i, "ids", copies, cols, index, torch.int32)
-    return l.dtype, vt, index, experts, cols, copies, lp, ldl, ip, ldi
+    return T, vt, index, experts, cols, copies, lp, ldl, ip, ldi
 
 
 def _route(L, ids, weights, bias=None, score="softmax", groups=1, keep=None, best=2, renormalize=True, scale=1.0, origin=None):
     T, vt, index, experts, cols, copies, lp, ldl, ip, ldi = _logits(L, ids)
-    wp, ldw = _matrix(_of_column(weights, "weights", cols), "weights", copies, cols, index, _sums(vt))
-    bp = _norm_vector(bias, "bias", experts, index, _sums(vt))
+    S = torch.float32 if vt else torch.float64
+    wp, ldw = _matrix(_by_column(weights, "weights", cols), "weights", copies, cols, index, S)
+    bp = 0 if bias is None else _norm_vector(bias, "bias", experts, index, S)
     _run(_lib.lib().jlust_hip_route, index, "route", T,
          _ROUTE(vt, _score(score), bool(renormalize), _origin(origin), experts, cols, copies, groups,
                 groups if keep is None else keep, best, lp, ldl, bp, ip, ldi, wp, ldw, scale))
@@ -99,7 +102,8 @@ def _route(L, ids, weights, bias=None, score="softmax", groups=1, keep=None, bes
 
 def _route_grad(L, ids, dweights, dL, score="softmax", renormalize=True, scale=1.0, origin=None):
     T, vt, index, experts, cols, copies, lp, ldl, ip, ldi = _logits(L, ids)
-    wp, ldw = _matrix(_of_column(dweights, "dweights", cols), "dweights", copies, cols, index, _sums(vt))
+    wp, ldw = _matrix(_by_column(dweights, "dweights", cols), "dweights", copies, cols, index,
+                      torch.float32 if vt else torch.float64)
     dp, ldd = _matrix(dL, "dL", experts, cols, index, T)
     _run(_lib.lib().jlust_hip_route_grad, index, "route_grad", T,
          _ROUTE_GRAD(vt, _score(score), bool(renormalize), _origin(origin), experts, cols, copies, lp, ldl, ip, ldi, wp, ldw,
@@ -107,41 +111,35 @@ def _route_grad(L, ids, dweights, dL, score="softmax", renormalize=True, scale=1
     return dL
 
 
-def _copies(weights, cols):
-    copies, columns = _extents(weights, "weights")
-    if columns != cols:
-        raise IncompatibleExtents(f"weights has {columns} columns, expected {cols}")
-    return copies
-
-
 def _combine(X, weights, Y, residual=None):
-    x, y = _raw(X, "X"), _raw(Y, "Y")
+    x = X if type(X) is torch.Tensor else _raw(X, "X")
+    y = Y if type(Y) is torch.Tensor else _raw(Y, "Y")
     T = x.dtype
     vt, index = _first(x, "X")
     d, cols = _extents(y, "Y")
-    w = _of_column(weights, "weights", cols)
-    copies = _copies(w, cols)
-    wp, ldw = _matrix(w, "weights", copies, cols, index, _sums(vt))
+    w = _by_column(weights, "weights", cols)
+    copies = w.shape[0] if len(w.shape) else 0
+    wp, ldw = _matrix(w, "weights", copies, cols, index, torch.float32 if vt else torch.float64)
     xp, ldx = _matrix(x, "X", d, copies * cols, index, T)
     yp, ldy = _matrix(y, "Y", d, cols, index, T)
-    rp, ldr = _matrix(residual, "residual", d, cols, index, T)
+    rp, ldr = _matrix(residual, "residual", d, cols, index, T) if residual is not None else (0, 0)
     _run(_lib.lib().jlust_hip_combine, index, "combine", T, vt, d, cols, copies, xp, ldx, wp, ldw, rp, ldr, yp, ldy)
     return Y
 
 
 def _combine_grad(X, weights, dY, dX=None, dweights=None):
-    x, dy = _raw(X, "X"), _raw(dY, "dY")
+    x, dy = _tensor(X, "X"), _tensor(dY, "dY")
     T = x.dtype
     vt, index = _first(x, "X")
+    S = torch.float32 if vt else torch.float64
     d, cols = _extents(dy, "dY")
-    w = _of_column(weights, "weights", cols)
-    copies = _copies(w, cols)
-    wp, ldw = _matrix(w, "weights", copies, cols, index, _sums(vt))
+    w = _by_column(weights, "weights", cols)
+    copies = w.shape[0] if len(w.shape) else 0
+    wp, ldw = _matrix(w, "weights", copies, cols, index, S)
     xp, ldx = _matrix(x, "X", d, copies * cols, index, T)
     dyp, lddy = _matrix(dy, "dY", d, cols, index, T)
     dxp, lddx = _matrix(dX, "dX", d, copies * cols, index, T)
-    dwp, lddw = (0, 0) if dweights is None else _matrix(_of_column(dweights, "dweights", cols), "dweights", copies, cols, index,
-                                                       _sums(vt))
+    dwp, lddw = (0, 0) if dweights is None else _matrix(_by_column(dweights, "dweights", cols), "dweights", copies, cols, index, S)
     _run(_lib.lib().jlust_hip_combine_grad, index, "combine_grad", T, vt, d, cols, copies, xp, ldx, wp, ldw, dyp, lddy, dxp, lddx,
          dwp, lddw)
     return dX if dX is not None else dweights
@@ -166,17 +164,18 @@ def _state(t, index):
 def _dropout(X, Y, p=0.5, seed=None, offset=0, residual=None, state=None):
     if (seed is None) == (state is None):
         raise TypeError("DropoutOp takes seed and offset, or state")
-    x = _raw(X, "X")
+    x = X if type(X) is torch.Tensor else _raw(X, "X")
     T = x.dtype
     vt, index = _first(x, "X")
     d, cols = _extents(x, "X")
     xp, ldx = _matrix(x, "X", d, cols, index, T)
     yp, ldy = _matrix(Y, "Y", d, cols, index, T)
-    rp, ldr = _matrix(residual, "residual", d, cols, index, T)
+    rp, ldr = _matrix(residual, "residual", d, cols, index, T) if residual is not None else (0, 0)
     sp = 0 if state is None else _state(state, index)
     _run(_lib.lib().jlust_hip_dropout, index, "dropout", T, vt, d, cols, xp, ldx, rp, ldr, yp, ldy, p, (seed or 0) & _U64,
          offset & _U64, sp)
     return Y
 
 
-TAGS = {"Route": _route, "RouteGrad": _route_grad, "Combine": _combine, "CombineGrad": _combine_grad, "Dropout": _dropout}
+_layer_calls.update({"Route": _route, "RouteGrad": _route_grad, "Combine": _combine, "CombineGrad": _combine_grad,
+                     "Dropout": _dropout})

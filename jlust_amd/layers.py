@@ -33,6 +33,7 @@ column.
 from __future__ import annotations
 
 import struct
+from functools import partial
 
 import torch
 
@@ -40,7 +41,7 @@ from . import _lib
 from .elementwise import FN_GELU, FN_IDENTITY, FN_RELU, FN_SILU, ElementwiseFn
 from .errors import (DeviceMismatch, IncompatibleExtents, NonCanonicalStorage, UnsupportedFormat,
                      UnsupportedIndexType, UnsupportedValueType)
-from .ops import AbstractKernelHandle, HIPBackend
+from .ops import AbstractKernelHandle, HIPBackend, _layer_calls
 from .tensor import OneBased, USTensor
 
 _BE = HIPBackend()
@@ -123,10 +124,9 @@ def _extents(t, name):
     raise IncompatibleExtents(f"{name}: {t.dim()}-D arrays are not supported")
 
 
-def _weights(t, name, groups, index, T, along_rows=False):
+def _weights(t, name, groups, index, T):
     """(address, layout, leading dimension, group stride, out, inp) of a weight
-    matrix, or of one per group: contiguous along either side (along_rows: along
-    the first alone)."""
+    matrix, or of one per group: contiguous along either side."""
     if t.dtype is not T or t.get_device() != index:
         _same(t, name, index, T)
     shape, strides = t.shape, t.stride()
@@ -137,9 +137,9 @@ def _weights(t, name, groups, index, T, along_rows=False):
     if groups and shape[2] != groups:
         raise IncompatibleExtents(f"{name} holds {shape[2]} matrices, expected {groups}")
     s0, s1 = strides[0], strides[1]
-    if (s0 == 1 or out <= 1) and (s1 >= out or inp <= 1) and (along_rows or not (out <= 1 and s1 == 1)):
+    if (s0 == 1 or out <= 1) and (s1 >= out or inp <= 1) and not (out <= 1 and s1 == 1):
         layout, ld = 0, s1 if inp > 1 else max(out, 1)
-    elif (s1 == 1 or inp <= 1) and (s0 >= inp or out <= 1) and not along_rows:
+    elif (s1 == 1 or inp <= 1) and (s0 >= inp or out <= 1):
         layout, ld = 1, s0 if out > 1 else max(inp, 1)
     else:
         raise NonCanonicalStorage(f"{name}: a matrix is column-major or the transpose of one, got strides "
@@ -296,6 +296,19 @@ def _linear(h, W, X, Y, bias=None, act=None, residual=None, preact=None, w_scale
     return Y
 
 
+def _int8_weights(w, groups):
+    """(address, leading dimension, group stride, out, inp) of Int8 weights."""
+    shape, strides = w.shape, w.stride()
+    if len(shape) != (3 if groups else 2):
+        raise IncompatibleExtents(f"W: expected {'out x inp x groups' if groups else 'out x inp'}, got {w.dim()} dimensions")
+    out, inp = shape[0], shape[1]
+    if groups and shape[2] != groups:
+        raise IncompatibleExtents(f"W holds {shape[2]} matrices, expected {groups}")
+    if (strides[1] != 1 and inp > 1) or (strides[0] < inp and out > 1):
+        raise NonCanonicalStorage(f"W: an Int8 matrix lies along inp, the transpose of a column-major one, got strides {strides}")
+    return w.data_ptr(), strides[0] if out > 1 else max(inp, 1), strides[2] if groups else 0, out, inp
+
+
 def _linear_int8(h, w, x, Y, y, bias, act, residual, preact, w_scale, x_scale):
     if w_scale is None or x_scale is None:
         raise TypeError("the product of Int8 matrices needs w_scale and x_scale")
@@ -303,24 +316,22 @@ def _linear_int8(h, w, x, Y, y, bias, act, residual, preact, w_scale, x_scale):
     if index < 0:
         raise DeviceMismatch(f"HIPBackend needs GPU buffers, W is on {w.device}")
     vt = _TYPES.get(T)
-    if vt is None or vt == 0:
+    if not vt:
         raise UnsupportedValueType(T, _BE, f"the product of Int8 matrices is Float32, Float16 or BFloat16, Y is {T}")
     groups, copies, plan = 0, 1, 0
     if h is not None:
         if h.index != index:
             raise DeviceMismatch(f"the plan is on {h.dev}, W on {w.device}")
         groups, copies, plan = h.groups, h.copies, h.use()
-    # A matrix that lies along both sides (one row or column) is read along inp.
-    wp, _, ldw, ws, inp, out = _weights(w.transpose(0, 1) if w.dim() > 1 else w, "W' (Int8 matrices lie along inp)", groups, index,
-                                        torch.int8, along_rows=True)
+    wp, ldw, ws, out, inp = _int8_weights(w, groups)
     n, xc = _columns(x, y, h)
     xp, ldx = _matrix(x, "X", inp, xc, index, torch.int8)
     yp, ldy = _matrix(y, "Y", out, n, index, T)
     sp, ss = _bias(w_scale, "w_scale", out, groups, index, torch.float32)
     sx = _norm_vector(x_scale, "x_scale", xc, index, torch.float32)
     bp, bs = _bias(bias, "bias", out, groups, index, T) if bias is not None else (0, 0)
-    rp, ldr = _matrix(residual, "residual", out, n, index, T)
-    zp, ldz = _matrix(preact, "preact", out, n, index, T)
+    rp, ldr = _matrix(residual, "residual", out, n, index, T) if residual is not None else (0, 0)
+    zp, ldz = _matrix(preact, "preact", out, n, index, T) if preact is not None else (0, 0)
     _run(_lib.lib().jlust_hip_linear_int8, index, "linear_int8", T,
          _LINEAR_INT8(vt, _act(act), out, inp, n, wp, ldw, sp, xp, ldx, sx, yp, ldy, bp, rp, ldr, zp, ldz, groups, copies,
                       plan, ws, ss, bs))
@@ -431,26 +442,13 @@ def _plan(args, what):
     return args
 
 
-def execute(optype, args, backend, kw):
-    """execute(LinearOp, ...) and the others of this module (ops.execute)."""
-    if backend is not None and not isinstance(backend, HIPBackend):
-        raise UnsupportedFormat(optype.tag, backend, "no such backend in jlust_amd")
-    tag = optype.tag
-    if tag == "Linear":
-        return _linear(None, *args, **kw)
-    if tag == "GroupedLinear":
-        return _linear(*_plan(args, "GroupedLinearOp"), **kw)
-    if tag == "LayerNorm":
-        return _layer_norm(*args, **kw)
-    if tag == "Quantize":
-        return _quantize(*args, **kw)
-    if tag in experts.TAGS:
-        return experts.TAGS[tag](*args, **kw)
-    if tag == "LinearGrad":
-        return _linear_grad(None, *args, **kw)
-    if tag == "GroupedLinearGrad":
-        return _linear_grad(*_plan(args, "GroupedLinearGradOp"), **kw)
-    return _layer_norm_grad(*args, **kw)
-
-
-from . import experts  # noqa: E402  (it takes this module's checks)
+# execute(LinearOp, ...) and the others of this module (ops.execute).
+_layer_calls.update({
+    "Linear": partial(_linear, None),
+    "LinearGrad": partial(_linear_grad, None),
+    "GroupedLinear": lambda *args, **kw: _linear(*_plan(args, "GroupedLinearOp"), **kw),
+    "GroupedLinearGrad": lambda *args, **kw: _linear_grad(*_plan(args, "GroupedLinearGradOp"), **kw),
+    "LayerNorm": _layer_norm,
+    "LayerNormGrad": _layer_norm_grad,
+    "Quantize": _quantize,
+})

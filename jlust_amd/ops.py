@@ -64,6 +64,7 @@ CombineGradOp = OpType("CombineGrad")
 DropoutOp = OpType("Dropout")
 _LAYER_TAGS = frozenset(("Linear", "LinearGrad", "GroupedLinear", "GroupedLinearGrad", "LayerNorm",
                          "LayerNormGrad", "Quantize", "Route", "RouteGrad", "Combine", "CombineGrad", "Dropout"))
+_layer_calls = {}                    # their calls by tag, which layers.py and experts.py enter
 
 
 # ------------------------------------------------------------------ backends
@@ -130,9 +131,12 @@ def execute(optype, *args, backend=None, **kw):
             r = hip_backend.spmv_fast(A, x, y, kw.get("alpha", 1.0), kw.get("beta", 0.0))
             if r is not None:
                 return r
-    if type(optype) is OpType and optype.tag in _LAYER_TAGS:
-        from . import layers
-        return layers.execute(optype, args, backend, kw)
+    if type(optype) is OpType:
+        f = _layer_calls.get(optype.tag)
+        if f is not None:
+            if backend is not None and not isinstance(backend, HIPBackend):
+                raise UnsupportedFormat(optype.tag, backend, "no such backend in jlust_amd")
+            return f(*args, **kw)
     if isinstance(optype, AbstractKernelHandle) or (args and isinstance(args[0], AbstractKernelHandle)):
         h, rest = (optype, args) if isinstance(optype, AbstractKernelHandle) else (args[0], args[1:])
         if getattr(h, "takes_raw", False):
