@@ -4,6 +4,8 @@
 #include "lanes.hpp"
 #include "tile_kernel.hpp"
 
+#include <cmath>
+
 namespace jlust {
 
 template int plan_tile_product<int8_t>(TileArgs *, bool, bool, int *, size_t *);
@@ -63,11 +65,31 @@ template int launch_tile_product8<__bf16>(const TileArgs &, int, hipStream_t);
 
 namespace {
 
-// The largest |x| of a column by its bits, which NaN and infinity end: bits of values
-// without their sign are in the values' order.
-template <int LANES>
-__device__ __forceinline__ uint32_t column_top(uint32_t v, uint32_t *lds)
+typedef uint16_t ushortx2 __attribute__((ext_vector_type(2)));
+
+// The largest |x| of a chunk and `top` by their bits, which NaN and infinity end: bits of
+// values without their sign are in the values' order, 16-bit ones two to a register.
+template <typename T>
+__device__ __forceinline__ uint32_t chunk_top(uint32x4 v, uint32_t top)
 {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = v[i];
+        if constexpr (sizeof(T) == 2) {
+            const ushortx2 m = __builtin_elementwise_max(__builtin_bit_cast(ushortx2, u & 0x7FFF7FFFu), __builtin_bit_cast(ushortx2, top));
+            top = __builtin_bit_cast(uint32_t, m);
+        } else {
+            top = (u & 0x7FFFFFFFu) > top ? u & 0x7FFFFFFFu : top;
+        }
+    }
+    return top;
+}
+
+// The value that the largest bits of a column's lanes stand for.
+template <typename T, int LANES>
+__device__ __forceinline__ float column_top(uint32_t v, uint32_t *lds)
+{
+    if constexpr (sizeof(T) == 2) v = (v >> 16) > (v & 0xFFFF) ? v >> 16 : v & 0xFFFF;
     v = over_lanes<(LANES < 64 ? LANES : 64)>(v, Larger());
     if constexpr (LANES > 64) {
         constexpr int W = LANES / 64;
@@ -77,33 +99,57 @@ __device__ __forceinline__ uint32_t column_top(uint32_t v, uint32_t *lds)
 #pragma unroll
         for (int w = 0; w < W; ++w) v = lds[w] > v ? lds[w] : v;
     }
-    return v;
+    if constexpr (sizeof(T) == 2) return (float)__builtin_bit_cast(T, (uint16_t)v);
+    else return __builtin_bit_cast(float, v);
 }
 
-// A column's scale s; x and s are both times `up` where 1/s would pass the type's range.
-// 0 but for s: the column becomes zeros.
+// A column's scale s.  `up`: x and s are both times it, where 1/s would pass the type's
+// range or s is so small that x/s may pass 127; 0: the column becomes zeros.
 struct Scale { float s, by, inv, up; };
 
-__device__ __forceinline__ Scale scale_from(uint32_t top)
+__device__ __forceinline__ Scale scale_from(float top)
 {
-    if (top >= 0x7F800000u) return {__builtin_nanf(""), 0.0f, 0.0f, 0.0f};
-    const float s = (float)((double)__builtin_bit_cast(float, top) / 127.0);
+    if (!(top < INFINITY)) return {__builtin_nanf(""), 0.0f, 0.0f, 0.0f};
+    const float s = (float)((double)top / 127.0);
     if (s == 0) return {0.0f, 0.0f, 0.0f, 0.0f};
     const float up = s < 0x1p-100f ? 0x1p64f : 1.0f, by = s * up;
     return {s, by, 1.0f / by, up};
 }
 
-// x / s to the nearest whole number, halves to the even one: the product with 1/s is off
-// by a little, so the nearest is found again from x - q s, which is exact (a multiple of
-// half s's last place, at most about s/2): an odd q is left at s/2, an even one past it.
-__device__ __forceinline__ int quantized(float x, const Scale &c)
+// CH values of a column over s to the nearest whole numbers, halves to the even one.
+// x inv + 1.5 2^23 has n, about x/s, in its low bits; inv is off by a little, so the
+// nearest is found again from x - n s, which is exact (a multiple of half s's last place,
+// at most about s/2): an odd n is left at s/2, an even one past it.
+template <typename T>
+__device__ __forceinline__ void quantize_chunk(uint32x4 v, const Scale &c, int8_t (&q)[16 / sizeof(T)])
 {
-    x *= c.up;
-    const float q = rintf(x * c.inv), t = 2 * fmaf(-q, c.by, x);
-    const int n = (int)q, bits = __builtin_bit_cast(int, t);
-    const int past = (bits & 0x7FFFFFFF) > __builtin_bit_cast(int, c.by) - (n & 1) ? (bits >> 31) | 1 : 0;
-    const int m = n + past;
-    return m > 127 ? 127 : m < -127 ? -127 : m;
+    constexpr int CH = 16 / sizeof(T);
+    constexpr float MAGIC = 12582912.0f;
+    if (c.up == 0) v = uint32x4{0, 0, 0, 0};
+    float x[CH];
+    values<T>(v, x);
+    if (c.up != 1) {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) x[j] *= c.up;
+    }
+    int n[CH];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+        const float r = fmaf(x[j], c.inv, MAGIC), t = fmaf(MAGIC - r, c.by, x[j]);
+        const int bits = __builtin_bit_cast(int, r);
+        const float most = __builtin_bit_cast(float, __builtin_bit_cast(int, 0.5f * c.by) - (bits & 1));
+        n[j] = bits + (t > most) - (t < -most);
+    }
+    if (c.up != 1) {
+        constexpr int ZERO = 0x4B400000;           // MAGIC's bits
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            const int m = c.up == 0 ? 0 : n[j] - ZERO;
+            n[j] = m > 127 ? 127 : m < -127 ? -127 : m;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) q[j] = (int8_t)n[j];
 }
 
 template <int CH>
@@ -119,7 +165,7 @@ __device__ __forceinline__ void store_bytes(int8_t *p, int64_t left, const int8_
 }
 
 // A column stays in the registers of LANES lanes, VPL chunks each, between its read and
-// its write.
+// its write; a wave reads its next column before it works on the one it has.
 template <typename T, int LANES, int VPL>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void quantize_kernel(int64_t d, int64_t cols, const T *__restrict__ X,
                                                                              int64_t ldx, int8_t *__restrict__ Q, int64_t ldq,
@@ -128,39 +174,46 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void quantize_kernel(int
     constexpr int CH = 16 / sizeof(T), NT = LANES > 256 ? LANES : 256, COLS = NT / LANES;
     __shared__ uint32_t s_top[NT / 64];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
-    for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < cols; c0 += (int64_t)gridDim.x * COLS) {
-        const int64_t c = c0 + sub;
-        const bool live = c < cols, over = sizeof(T) == 2 && c + 1 < cols && d >= CH;
-        uint32x4 x[VPL];
-        float f[CH];
-        uint32_t top = 0;
+    // A chunk over the end of all but the last column is read whole; what follows the
+    // column is taken out again.
+    auto read = [&](int64_t c, uint32x4 (&x)[VPL]) {
+        const bool over = sizeof(T) == 2 && c + 1 < cols && d >= CH;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int64_t at = (int64_t)(lane + LANES * i) * CH;
-            x[i] = read_raw(X + c * ldx + at, live ? d - at : 0, over);
+            x[i] = read_raw(X + c * ldx + at, c < cols ? d - at : 0, over);
         }
+    };
+    uint32x4 next[VPL];
+    read((int64_t)blockIdx.x * COLS + sub, next);
+    for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < cols; c0 += (int64_t)gridDim.x * COLS) {
+        const int64_t c = c0 + sub;
+        uint32x4 x[VPL];
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) x[i] = next[i];
+        if (c0 + (int64_t)gridDim.x * COLS < cols) read(c + (int64_t)gridDim.x * COLS, next);
+        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int64_t left = live ? d - (int64_t)(lane + LANES * i) * CH : 0;
-            values<T>(x[i], f);
+            const int64_t left = d - (int64_t)(lane + LANES * i) * CH;
+            if (sizeof(T) == 2 && left > 0 && left < CH) {
+                T e[CH];
+                __builtin_memcpy(e, &x[i], 16);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const uint32_t b = __builtin_bit_cast(uint32_t, f[j]) & 0x7FFFFFFFu;
-                if (j < left && b > top) top = b;
+                for (int j = 0; j < CH; ++j) e[j] = j < left ? e[j] : T(0);
+                __builtin_memcpy(&x[i], e, 16);
             }
+            top = chunk_top<T>(x[i], top);
         }
-        const Scale s = scale_from(column_top<LANES>(top, s_top));
-        if (!live) continue;
+        const Scale s = scale_from(column_top<T, LANES>(top, s_top));
+        if (c >= cols) continue;
         if (lane == 0) scales[c] = s.s;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int64_t at = (int64_t)(lane + LANES * i) * CH;
             if (at >= d) continue;
             int8_t q[CH];
-            if (s.up == 0) x[i] = uint32x4{0, 0, 0, 0};
-            values_again<T>(x[i], f);
-#pragma unroll
-            for (int j = 0; j < CH; ++j) q[j] = (int8_t)quantized(f[j], s);
+            quantize_chunk<T>(x[i], s, q);
             store_bytes(Q + c * ldq + at, d - at, q);
         }
     }
@@ -175,22 +228,13 @@ __global__ __launch_bounds__(1024) void quantize_long_kernel(int64_t d, int64_t 
     __shared__ uint32_t s_top[16];
     for (int64_t c = blockIdx.x; c < cols; c += gridDim.x) {
         uint32_t top = 0;
-        float f[CH];
-        for (int64_t at = (int64_t)threadIdx.x * CH; at < d; at += 1024 * CH) {
-            read_chunk(X + c * ldx + at, d - at, f);
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const uint32_t b = __builtin_bit_cast(uint32_t, f[j]) & 0x7FFFFFFFu;
-                if (b > top) top = b;
-            }
-        }
-        const Scale s = scale_from(column_top<1024>(top, s_top));
+        for (int64_t at = (int64_t)threadIdx.x * CH; at < d; at += 1024 * CH)
+            top = chunk_top<T>(read_raw(X + c * ldx + at, d - at), top);
+        const Scale s = scale_from(column_top<T, 1024>(top, s_top));
         if (threadIdx.x == 0) scales[c] = s.s;
         for (int64_t at = (int64_t)threadIdx.x * CH; at < d; at += 1024 * CH) {
             int8_t q[CH];
-            values<T>(read_raw(X + c * ldx + at, s.up == 0 ? 0 : d - at), f);
-#pragma unroll
-            for (int j = 0; j < CH; ++j) q[j] = (int8_t)quantized(f[j], s);
+            quantize_chunk<T>(read_raw(X + c * ldx + at, d - at), s, q);
             store_bytes(Q + c * ldq + at, d - at, q);
         }
     }
@@ -202,7 +246,7 @@ int quantize(int64_t d, int64_t cols, const void *X, int64_t ldx, int8_t *Q, int
     const int64_t chunks = (d * (int64_t)sizeof(T) + 15) / 16;
     auto launch = [&](auto kernel, int lanes) {
         const int nt = lanes > 256 ? lanes : 256;
-        hipLaunchKernelGGL(kernel, dim3(column_blocks(cols, nt / lanes)), dim3(nt), 0, s, d, cols, (const T *)X, ldx, Q, ldq, scales);
+        hipLaunchKernelGGL(kernel, dim3(column_blocks(cols, nt / lanes, 1024)), dim3(nt), 0, s, d, cols, (const T *)X, ldx, Q, ldq, scales);
     };
     // Few columns wait for one of them: it goes over more lanes.
     const bool few = cols <= 512;

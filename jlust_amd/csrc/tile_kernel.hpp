@@ -235,19 +235,13 @@ __device__ __forceinline__ void load_bias(const TileArgs &a, int group, int64_t 
     load_some<V>((const T *)a.bias + group * a.gb + m, some ? a.m - m : 0, b);
 }
 
-// V sums of row `row` of C, columns mm ..: the epilogue; res: R's there.
+// V sums of row `row` of C, columns mm ..: the epilogue; res: R's there.  finish_sum: of
+// sums that have their bias.
 template <int V, typename T, typename A>
-__device__ __forceinline__ void finish(const TileArgs &a, const T *bias, const T *res, int64_t row, int64_t mm, A *s)
+__device__ __forceinline__ void finish_sum(const TileArgs &a, const T *res, int64_t row, int64_t mm, A *s)
 {
     const int64_t left = a.m - mm;
-    if (left <= 0) return;
     T t[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) s[e] += A(bias[e]);
-    if (a.c_wide) {
-        store_some<V>((A *)a.C + row * a.ldc + mm, left, s);
-        return;
-    }
     if (a.Z) {
 #pragma unroll
         for (int e = 0; e < V; ++e) t[e] = T(s[e]);
@@ -261,6 +255,20 @@ __device__ __forceinline__ void finish(const TileArgs &a, const T *bias, const T
 #pragma unroll
     for (int e = 0; e < V; ++e) t[e] = T(s[e]);
     store_some<V>((T *)a.C + row * a.ldc + mm, left, t);
+}
+
+template <int V, typename T, typename A>
+__device__ __forceinline__ void finish(const TileArgs &a, const T *bias, const T *res, int64_t row, int64_t mm, A *s)
+{
+    const int64_t left = a.m - mm;
+    if (left <= 0) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] += A(bias[e]);
+    if (a.c_wide) {
+        store_some<V>((A *)a.C + row * a.ldc + mm, left, s);
+        return;
+    }
+    finish_sum<V, T, A>(a, res, row, mm, s);
 }
 
 // The scales of a group's V rows of P from m on (0 past the edge and in no group), and
@@ -388,13 +396,12 @@ template <typename A, int TM> struct SumRows {
     __device__ __forceinline__ static int at(int r, int c) { return r * CHUNKS * 16 + ((c ^ (r & FLIP)) << 4); }
 };
 
-template <typename T, bool KSUM, int TM, int RUNS, typename O, typename Put>
+template <typename T, bool KSUM, int TM, int RUNS, typename Put>
 __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int piece, int group, int n0, int nend, int64_t m0, Put &&put)
 {
     using A = typename Elem<T>::Acc;
     using SR = SumRows<A, TM>;
-    constexpr bool SCALED = !std::is_same_v<T, O>;
-    constexpr int CH = SCALED ? 8 : 16 / sizeof(O), ACH = 16 / sizeof(A), LANES = TM / CH, ROWS = 64 / LANES, ITER = (16 + ROWS - 1) / ROWS;
+    constexpr int CH = 16 / sizeof(T), ACH = 16 / sizeof(A), LANES = TM / CH, ROWS = 64 / LANES, ITER = (16 + ROWS - 1) / ROWS;
     const int lane = threadIdx.x & 63;
     const int r0 = lane < LANES * ROWS ? lane / LANES : 16;
     char *mine = lds + (threadIdx.x >> 6) * SR::BYTES;
@@ -402,26 +409,19 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int pi
     TileArgs b = a;
     if constexpr (KSUM) b.C = (T *)a.C + group * a.gc;
     if (!a.offsets) b.groups = 1;
-    O bias[CH];
+    T bias[CH];
     load_bias<CH>(b, group, m, bias);
-    float by[SCALED ? CH : 1];
-    if constexpr (SCALED) load_scales<CH>(b, group, m, by);
     const int64_t part_rows = KSUM && a.offsets ? a.n * a.groups : a.n;
     const int64_t part_row = piece * part_rows + (KSUM ? group * a.n : 0);
 #pragma unroll
     for (int run = 0; run < RUNS; ++run) {
         // What the rows need from memory, all of it before the first is used.
         int row[ITER];
-        O res[ITER][CH];
-        float qs[SCALED ? ITER : 1];
+        T res[ITER][CH];
 #pragma unroll
         for (int it = 0; it < ITER; ++it) {
             const int r = r0 + it * ROWS, n = n0 + 16 * run + r;
             row[it] = r < 16 && n < nend && left > 0 ? n : -1;
-        }
-        if constexpr (SCALED) {
-#pragma unroll
-            for (int it = 0; it < ITER; ++it) qs[it] = row[it] >= 0 && !a.part ? scale_of(b, group, row[it]) : 0.0f;
         }
         if (!a.part && a.crow) {
 #pragma unroll
@@ -429,7 +429,7 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int pi
         }
         if (a.R && !a.part) {
 #pragma unroll
-            for (int it = 0; it < ITER; ++it) load_some<CH>((const O *)a.R + row[it] * a.ldr + m, row[it] >= 0 ? left : 0, res[it]);
+            for (int it = 0; it < ITER; ++it) load_some<CH>((const T *)a.R + row[it] * a.ldr + m, row[it] >= 0 ? left : 0, res[it]);
         }
         wave_sync();
         put(run, mine);
@@ -441,18 +441,75 @@ __device__ __forceinline__ void finish_tile(const TileArgs &a, char *lds, int pi
             A v[CH];
 #pragma unroll
             for (int e = 0; e < CH; e += ACH) __builtin_memcpy(v + e, mine + SR::at(r, (lane % LANES * CH + e) / ACH), 16);
-            if (a.part) {
-                store_some<CH>((A *)a.part + (part_row + row[it]) * a.m + m, left, v);
-            } else if constexpr (SCALED) {
-                float f[CH];
-#pragma unroll
-                for (int e = 0; e < CH; ++e) f[e] = (float)v[e] * (qs[it] * by[e]);
-                finish<CH, O, float>(b, bias, res[it], row[it], m, f);
-            } else {
-                finish<CH, T, A>(b, bias, res[it], row[it], m, v);
-            }
+            if (a.part) store_some<CH>((A *)a.part + (part_row + row[it]) * a.m + m, left, v);
+            else finish<CH, T, A>(b, bias, res[it], row[it], m, v);
         }
     }
+}
+
+// The same of 8-bit operands' sums, RUN rows of TW along m at a time (put(run, part of
+// m, its place)), a lane ending 8 values.  What the rows need from memory by their
+// numbers is read for all of them before the first.
+template <typename O, int TM, int RUNS, int RUN, int TW, typename Put>
+__device__ __forceinline__ void finish_scaled(const TileArgs &a, char *lds, int piece, int group, int n0, int nend, int64_t m0, Put &&put)
+{
+    using SR = SumRows<int, TW>;
+    constexpr int CH = 8, LANES = TW / CH, ROWS = 64 / LANES, ITER = RUN / ROWS;
+    static_assert(RUN % ROWS == 0 && TM % TW == 0, "whole rows");
+    const int lane = threadIdx.x & 63, r0 = lane / LANES;
+    char *mine = lds + (threadIdx.x >> 6) * SR::BYTES * (RUN / 16);
+    TileArgs b = a;
+    if (!a.offsets) b.groups = 1;
+    int row[RUNS][ITER];
+    float qs[RUNS][ITER], by[TM / TW][CH], bias[TM / TW][CH];
+#pragma unroll
+    for (int run = 0; run < RUNS; ++run)
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            const int n = n0 + RUN * run + r0 + it * ROWS;
+            row[run][it] = n < nend ? n : -1;
+            qs[run][it] = n < nend && !a.part ? scale_of(b, group, n) : 0.0f;
+            if (n < nend && !a.part && a.crow) row[run][it] = a.crow[n];
+        }
+#pragma unroll
+    for (int h = 0; h < TM / TW; ++h) {
+        O v[CH];
+        load_bias<CH>(b, group, m0 + TW * h + lane % LANES * CH, v);
+#pragma unroll
+        for (int e = 0; e < CH; ++e) bias[h][e] = (float)v[e];
+        load_scales<CH>(b, group, m0 + TW * h + lane % LANES * CH, by[h]);
+    }
+#pragma unroll
+    for (int run = 0; run < RUNS; ++run)
+#pragma unroll
+        for (int h = 0; h < TM / TW; ++h) {
+            const int64_t m = m0 + TW * h + lane % LANES * CH, left = a.m - m;
+            O res[ITER][CH];
+            if (a.R && !a.part) {
+#pragma unroll
+                for (int it = 0; it < ITER; ++it)
+                    load_some<CH>((const O *)a.R + row[run][it] * a.ldr + m, row[run][it] >= 0 ? left : 0, res[it]);
+            }
+            wave_sync();
+            put(run, h, mine);
+            wave_sync();
+#pragma unroll
+            for (int it = 0; it < ITER; ++it) {
+                if (row[run][it] < 0 || left <= 0) continue;
+                const int r = r0 + it * ROWS;
+                int v[CH];
+#pragma unroll
+                for (int e = 0; e < CH; e += 4) __builtin_memcpy(v + e, mine + SR::at(r, (lane % LANES * CH + e) / 4), 16);
+                if (a.part) {
+                    store_some<CH>((int *)a.part + ((int64_t)piece * a.n + row[run][it]) * a.m + m, left, v);
+                    continue;
+                }
+                float f[CH];
+#pragma unroll
+                for (int e = 0; e < CH; ++e) f[e] = fmaf((float)v[e], qs[run][it] * by[h][e], bias[h][e]);
+                finish_sum<CH, O, float>(b, res[it], row[run][it], m, f);
+            }
+        }
 }
 
 // A 16-row run of 16 x 16 tiles: lane (li, g) holds rows 4g .. 4g+3 of column li.
@@ -553,7 +610,9 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void tile_product_kernel(const Tile
 
     __syncthreads();
     auto put = [&](int j, char *to) { put_rows<typename Elem<T>::Acc, MT, NTL, TM>(acc, j, to); };
-    finish_tile<T, KSUM, TM, NTL, O>(a, lds, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
+    if constexpr (std::is_same_v<T, O>) finish_tile<T, KSUM, TM, NTL>(a, lds, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
+    else
+        finish_scaled<O, TM, NTL, 16, TM>(a, lds, w.piece, group, n0 + wn0, nend, m0 + wm0, [&](int j, int, char *to) { put(j, to); });
 }
 
 // ----------------------------------------------- tiles by copies to LDS
@@ -718,7 +777,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
     using CP = Copy<T, PKC, LM, NT, BK>;
     using CQ = Copy<T, QKC, BN, NT, BK>;
     // Arrays of their own: the compiler then knows which copies an LDS read waits for.
-    constexpr int TILE = CP::BYTES + CQ::BYTES, SUMS = WM * WN * SumRows<A, TM>::BYTES;
+    constexpr int TILE = CP::BYTES + CQ::BYTES, SUMS = WM * WN * (sizeof(T) == 1 && TM <= 64 ? 2 : 1) * SumRows<A, TM>::BYTES;
     __shared__ __align__(16) char lds0[TILE > SUMS ? TILE : SUMS];
     __shared__ __align__(16) char lds1[TILE];
     __shared__ __align__(16) char lds2[NB > 2 ? TILE : 16];
@@ -833,6 +892,24 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
         }
     }
     __syncthreads();
+    if constexpr (!std::is_same_v<T, O>) {
+        // As below, 32 columns by up to 64 of m a run.
+        constexpr int TW = TM < 64 ? TM : 64;
+        auto put = [&](int run, int h, char *to) {
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int i = 0; i < TW / 32; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    A v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[h * (TW / 32) + i][run][4 * q + e];
+                    __builtin_memcpy(to + SumRows<A, TW>::at(lane & 31, 8 * i + 2 * q + (lane >> 5)), v, 16);
+                }
+        };
+        finish_scaled<O, TM, NTL, 32, TW>(a, lds0, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
+        return;
+    }
     auto put = [&](int run, char *to) {
         const int lane = threadIdx.x & 63;
         if constexpr (HALF) {
@@ -851,7 +928,7 @@ __global__ __launch_bounds__(WM *WN * 64, sizeof(T) == 2 && BM == 128 && BK == 3
             put_rows<A, MT, NTL, TM>(acc, run, to);
         }
     };
-    finish_tile<T, KSUM, TM, TN / 16, O>(a, lds0, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
+    if constexpr (std::is_same_v<T, O>) finish_tile<T, KSUM, TM, TN / 16>(a, lds0, w.piece, group, n0 + wn0, nend, m0 + wm0, put);
 }
 
 // ------------------------------------------------------------ few columns
@@ -1079,12 +1156,12 @@ constexpr TileShape TILE_SHAPES[] = {{128, 128, 256}, {128, 32, 256}, {128, 16, 
                                      {128, 128, 256}, {16, 16, Few<1>::WAVES * 64}, {32, 16, Few<2>::WAVES * 64}};
 
 // What a shape costs: its rate with a CU full of it (Tflop/s a CU), the time of 64 of
-// k where latency bounds it (us), workgroups a CU.  Measured on products of 64 to
+// k where latency bounds it (us), workgroups a CU, the start and end of a round (us).  Measured on products of 64 to
 // 8,192 columns and 512 to 8,192 rows and k; the estimate below picks within 10 %
 // of the best of them but for three (up to 20 %).  Of groups' products it only ranks
 // the shapes (32 groups, 16,384 columns 2816 -> 1024: 138 us estimated, 194 measured;
 // the sums over columns 93 and 181).
-struct ShapeCost { Shape shape; double rate, latency; int held; };
+struct ShapeCost { Shape shape; double rate, latency; int held; double end = 2; };
 
 // Whether every chunk that a copy reads lies whole in the operands, 16 bytes aligned.
 template <typename T>
@@ -1135,23 +1212,18 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
         return work_groups(*a, ksum) < ((int64_t)1 << 32) / t.threads;
     };
 
-    ShapeCost some[4];
+    ShapeCost some[6];
     int count = 0;
     if constexpr (sizeof(T) == 1) {
-        // Along k on both sides.  The bytes of a step, and so its time, are 16-bit
-        // values', its k is twice theirs.
-        if (share <= 16 && set(FEW_16, 1)) {
-            some[count++] = {FEW_16, 0.5, 0.035, 4};
-        } else if (share <= 48) {
-            some[count++] = {REG_32, 3.0, 0.25, 5};
-        } else if (fit && (!a->offsets || share >= 1024) && tiles(COPY_256) >= 512 && k > 384) {
-            some[count++] = {COPY_256, 9.0, 0.65, 1};
-        } else {
-            if (fit && k > 384) {
-                some[count++] = {COPY_TALL, 9.0, 0.48, 2};
-                some[count++] = {COPY_128, 8.4, 0.31, 2};
-            }
-            some[count++] = {REG_M64, 4.4, 0.29, 5};
+        // Along k on both sides.  A step's bytes are 16-bit values', its k is twice
+        // theirs; measured on 1 to 8,192 columns of 64 to 8,192.
+        if (share <= 16 && set(FEW_16, 1)) some[count++] = {FEW_16, 1.0, 0.035, 4, 4};
+        some[count++] = {REG_32, 3.7, 0.22, 5};
+        some[count++] = {REG_M64, 4.4, 0.21, 5};
+        if (fit && share > 48) {
+            some[count++] = {COPY_128, 7.6, 0.36, 2, 3.7};
+            some[count++] = {COPY_TALL, 7.7, 0.5, 2, 6.6};
+            some[count++] = {COPY_256, 8.8, 0.9, 1, 10};
         }
     } else if (sizeof(T) == 2 && !ksum && share <= 16) {
         if (!set(FEW_16, 1)) {
@@ -1209,7 +1281,7 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
             double rounds = (double)groups / slots;
             rounds = rounds <= 1 ? 1 : rounds < 3 ? (double)((groups + slots - 1) / slots) : rounds;
             const double step = held * work > o.latency ? held * work : o.latency;
-            const double us = rounds * ((double)((k + 64 * p - 1) / (64 * p)) * step + 2) + (p > 1 ? 8 + 1e-6 * p * sums : 0);
+            const double us = rounds * ((double)((k + 64 * p - 1) / (64 * p)) * step + o.end) + (p > 1 ? sizeof(T) == 1 ? 4 + 3e-6 * p * sums : 8 + 1e-6 * p * sums : 0);
             if (best_shape < 0 || us < best) {
                 best = us;
                 best_shape = o.shape;
