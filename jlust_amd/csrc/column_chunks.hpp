@@ -44,6 +44,22 @@ __device__ __forceinline__ uint32x4 read_raw(const T *p, int64_t left, bool over
     return left >= CH || (over && left > 0) ? load_chunk(p) : left > 0 ? load_chunk_part(p, left) : zero;
 }
 
+// The chunk at `at` of a column of d values; WHOLE: d is a whole number of chunks, and
+// what lies past it is the first chunk, read and dropped: no branch around a partial
+// chunk's reads comes between a wave's reads (the gradient of 16,384 columns' routing to
+// 160 experts: 9.3 us and 8.0).
+template <bool WHOLE, typename T>
+__device__ __forceinline__ uint32x4 read_at(const T *column, int64_t at, int64_t d, bool over = false)
+{
+    if constexpr (WHOLE) {
+        const bool in = at < d;
+        const uint32x4 v = load_chunk(column + (in ? at : 0)), zero = {0, 0, 0, 0};
+        return in ? v : zero;
+    } else {
+        return read_raw(column + at, d - at, over);
+    }
+}
+
 template <typename T, typename A>
 __device__ __forceinline__ void values(uint32x4 v, A (&f)[16 / sizeof(T)])
 {
@@ -100,6 +116,37 @@ __device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 
             if (j < left) p[j] = e[j];
     }
 }
+
+// As write_chunk of the chunk at `at` of d values.
+template <bool WHOLE, typename T, typename A>
+__device__ __forceinline__ void write_at(T *column, int64_t at, int64_t d, const A (&f)[16 / sizeof(T)], bool streamed = false)
+{
+    constexpr int CH = 16 / sizeof(T);
+    if constexpr (WHOLE) {
+        if (at < d) write_chunk(column + at, CH, f, streamed);
+    } else {
+        write_chunk(column + at, d - at, f, streamed);
+    }
+}
+
+// n / d by a product, for n below 2^31: m = floor(2^(31 + s) / d) + 1 is below 2^32 and
+// within 2^s / 2^(31 + s) of it with s = ceil(log2 d).
+struct Divider {
+    int64_t d;
+    uint32_t m, shift;
+    bool fits;                                     // all n are below 2^31
+    Divider(int64_t d_, int64_t n) : d(d_), m(0), shift(0), fits(n < (int64_t)1 << 31 && d_ < (int64_t)1 << 31)
+    {
+        if (!fits) return;
+        while (((int64_t)1 << shift) < d) ++shift;
+        m = (uint32_t)(((uint64_t)1 << (31 + shift)) / d + 1);
+        shift += 31;
+    }
+    __device__ __forceinline__ int64_t of(int64_t n) const
+    {
+        return fits ? (int64_t)((uint64_t)(uint32_t)n * m >> shift) : n / d;
+    }
+};
 
 // A launch takes fewer than 2^32 threads: at most 2^21 workgroups, which walk over the
 // items in turn.

@@ -10,22 +10,21 @@ namespace jlust {
 namespace {
 
 // A thread makes a chunk of a column of Y.
-template <typename T>
-__global__ __launch_bounds__(256) void combine_kernel(int64_t d, int64_t cols, int copies, const T *__restrict__ X, int64_t ldx,
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void combine_kernel(int64_t d, int64_t cols, Divider chunks, int copies, const T *__restrict__ X, int64_t ldx,
                                                       const typename Elem<T>::Acc *__restrict__ weights, int64_t ldw, const T *R,
                                                       int64_t ldr, T *Y, int64_t ldy, bool streamed)
 {
     using A = typename Elem<T>::Acc;
     constexpr int CH = 16 / sizeof(T), AHEAD = 4;
-    const int64_t chunks = (d + CH - 1) / CH;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks * cols; i += (int64_t)gridDim.x * 256) {
-        const int64_t t = i / chunks, at = (i - t * chunks) * CH, left = d - at;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks.d * cols; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = chunks.of(i), at = (i - t * chunks.d) * CH, left = WHOLE ? CH : d - at;
         const T *x = X + t * copies * ldx + at;
         const A *w = weights + t * ldw;
         A sum[CH], f[CH];
 #pragma unroll
         for (int j = 0; j < CH; ++j) sum[j] = A(0);
-        uint32x4 r = read_raw(R + t * ldr + at, R ? left : 0);
+        const uint32x4 r = read_raw(R + t * ldr + at, R ? left : 0);
         for (int k = 0; k < copies; k += AHEAD) {
             uint32x4 v[AHEAD];
             A by[AHEAD];
@@ -146,9 +145,14 @@ extern "C" int jlust_hip_combine(int32_t value_type, int64_t d, int64_t cols, in
         using T = decltype(z);
         using A = typename Elem<T>::Acc;
         constexpr int64_t CH = 16 / sizeof(T);
-        hipLaunchKernelGGL((combine_kernel<T>), dim3(column_blocks((d + CH - 1) / CH * cols, 256)), dim3(256), 0, (hipStream_t)stream,
-                           d, cols, (int)copies, (const T *)X, ldx, (const A *)weights, ldw, (const T *)R, ldr, (T *)Y, ldy,
-                           d * cols * (int64_t)sizeof(T) > STREAMED);
+        const int64_t chunks = (d + CH - 1) / CH;
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(column_blocks(chunks * cols, 256)), dim3(256), 0, (hipStream_t)stream, d, cols,
+                               Divider(chunks, chunks * cols), (int)copies, (const T *)X, ldx, (const A *)weights, ldw,
+                               (const T *)R, ldr, (T *)Y, ldy, d * cols * (int64_t)sizeof(T) > STREAMED);
+        };
+        if (d % CH == 0) launch(combine_kernel<T, true>);
+        else launch(combine_kernel<T, false>);
         return check_launch("combine_kernel");
     });
 }
@@ -184,7 +188,7 @@ extern "C" int jlust_hip_combine_grad(int32_t value_type, int64_t d, int64_t col
 namespace jlust {
 int preload_combine()
 {
-    JLUST_PRELOAD_KERNEL((combine_kernel<float>));
+    JLUST_PRELOAD_KERNEL((combine_kernel<float, true>));
     return JLUST_STATUS_SUCCESS;
 }
 }  // namespace jlust

@@ -12,6 +12,7 @@
 #include "wave.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace jlust {
 namespace {
@@ -46,13 +47,15 @@ __device__ __forceinline__ A lanes_sum(A v)
     return over_lanes<LANES>(v, Plus());
 }
 
-// The first of a column's lanes where `is` holds, -1 if none.
+// Whether this is the first of a column's lanes where `is` holds; the lanes of the wave
+// before it in its column.
+__device__ __forceinline__ bool first_of(bool is, uint64_t before) { return is && (__ballot(is) & before) == 0; }
+
 template <int LANES>
-__device__ __forceinline__ int first_lane(bool is)
+__device__ __forceinline__ uint64_t lanes_before()
 {
-    uint64_t mask = __ballot(is);
-    if constexpr (LANES < 64) mask = mask >> (threadIdx.x & (64 - LANES)) & ((1ull << LANES) - 1);
-    return __ffsll((unsigned long long)mask) - 1;
+    const int lane = threadIdx.x & 63;
+    return ((1ull << lane) - 1) & ~((1ull << (lane & ~(LANES - 1))) - 1);
 }
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
@@ -85,24 +88,42 @@ __device__ __forceinline__ void chosen_scores(int score, bool relative, const A 
     }
 }
 
-// LANES lanes take a column, `1 << lane_shift` of them a group, PER experts at most
-// each: lane's experts and then the lanes' are in the experts' order, so the first
-// lane with the best key holds the lowest expert that has it.  K: the keys' type,
-// Float64 but for logits that are the keys themselves.  PER 0: any number of them, in
-// LDS, a wave a workgroup.
-template <typename T, typename K, int LANES, int PER>
-__global__ __launch_bounds__(PER ? 256 : 64, PER ? 3 : 1) void route_kernel(const RouteArgs a)
+// How far apart two Float32 keys are in 64 bits for sure, over 1 + the larger: a
+// sigmoid's is off by 4 u (u = 2^-24: its exponential's argument 0.4, the exponential
+// 0.5, the sum 1, the reciprocal 2), a softmax's by 27 u (its argument 1 and its sum's
+// 20 adds and 2 more, the rest 4), the sum with the bias by u times itself.  Twice that,
+// rounded up.
+constexpr float SIGMOID_APART = 16 * 0x1p-24f, SOFTMAX_APART = 64 * 0x1p-24f;
+
+// What a lane's share of a column is: `count` experts from `first` on.
+struct RouteShare { int lane, group, first, count; };
+
+constexpr int MAX_CANDIDATES = MAX_COPIES + 16;
+
+// Writes the experts of a column to chosen[0 .. copies), -1 where none is left, and
+// softmax's largest logit and sum where the call needs them.  LANES lanes take a column,
+// `1 << lane_shift` of them a group, PER experts at most each (0: any number, their keys
+// in LDS): a lane's experts and then the lanes' are in the experts' order, so the first
+// lane with the best key holds the lowest expert that has it.  K: the keys' type.
+// APPROX: Float32 keys of scores that belong to Float64.  What they leave open, which
+// groups are the last kept and the order of the experts, goes by the sigmoids in Float64
+// of those few that are near enough (`exact`: theirs); true where that does not settle it
+// (more than 16 experts as near to the last one chosen, or softmax, whose Float64 sum takes
+// them all).
+template <typename T, typename K, bool APPROX, int LANES, int PER>
+__device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, const T *L, char *lds, int *chosen, double *exact,
+                                       double *top_, double *total_)
 {
     using A = typename Elem<T>::Acc;
-    constexpr int NT = PER ? 256 : 64, COLS = NT / LANES, NP = MAX_COPIES / LANES, HELD = PER ? PER : 1;
+    using S = std::conditional_t<APPROX, float, double>;                // the scores' type
+    constexpr int HELD = PER ? PER : 1;
     constexpr K NONE = -INFINITY;
-    __shared__ int s_chosen[COLS][MAX_COPIES];
-    extern __shared__ double s_keys[];
-    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, of_group = 1 << a.lane_shift;
-    const int group = lane >> a.lane_shift, place = (lane & (of_group - 1)) * a.per;
-    const int first = group * a.size + place;
+    const int of_group = 1 << a.lane_shift;
     const bool softmax = a.score == JLUST_SCORE_SOFTMAX;
+    const float apart = softmax ? SOFTMAX_APART : SIGMOID_APART;
     const A *bias = (const A *)a.bias;
+    const uint64_t before = lanes_before<LANES>();
+    bool unsure = false;
     K held[HELD];
     // f(j, key) of this lane's keys, which it may change.
     auto each = [&](auto &&f) {
@@ -110,7 +131,7 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER ? 3 : 1) void route_kernel(cons
 #pragma unroll
             for (int j = 0; j < PER; ++j) f(j, held[j]);
         } else {
-            K *keys = (K *)s_keys + lane;
+            K *keys = (K *)lds + w.lane;
             for (int j = 0; j < a.per; ++j) {
                 K k = keys[j * 64];
                 f(j, k);
@@ -118,122 +139,268 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER ? 3 : 1) void route_kernel(cons
             }
         }
     };
+    if (PER > 0 && a.whole) {
+        T raw[HELD] = {};
+        if (w.count) load_vec<HELD>(L + w.first, raw);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) held[j] = w.count && A(raw[j]) > A(-INFINITY) ? K(A(raw[j])) : NONE;
+    } else {
+        each([&](int j, K &k) {
+            const K l = j < w.count ? K(A(L[w.first + j])) : NONE;
+            k = l > NONE ? l : NONE;
+        });
+    }
+    // Softmax's sum is needed where scores are compared or left as they are.
+    S top = -INFINITY, total = 1;
+    if (softmax && (bias || !a.renormalize)) {
+        K m = NONE;
+        each([&](int, K &k) { m = k > m ? k : m; });
+        m = lanes_max<LANES>(m);
+        top = S(m);
+        if (bias) {
+            S sum = 0;
+            each([&](int, K &k) { sum += k > NONE ? exp_below(S(k), top) : S(0); });
+            total = lanes_sum<LANES>(sum);
+        } else {
+            A sum = A(0);
+            each([&](int, K &k) { sum += k > NONE ? exp_below(A(k), A(m)) : A(0); });
+            total = S(lanes_sum<LANES>(sum));
+        }
+    }
+    *top_ = (double)top;
+    *total_ = (double)total;
+    auto score_of = [&](S l, S m, S all) {
+        if constexpr (APPROX) {
+            if (softmax) return l == m ? 1 / all : __expf(l - m) / all;
+            return __builtin_amdgcn_rcpf(1 + __expf(-l));
+        } else {
+            return softmax ? exp_below(l, m) / all : 1 / (1 + exp(-l));
+        }
+    };
+    if (bias) {
+        auto keyed = [&](K &k, A b) {
+            const K v = k > NONE ? K(score_of(S(k), top, total) + S(b)) : NONE;
+            k = v > NONE ? v : NONE;
+        };
+        if (PER > 0 && a.whole) {
+            A add[HELD] = {};
+            if (w.count) load_vec<HELD>(bias + w.first, add);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) keyed(held[j], add[j]);
+        } else {
+            each([&](int j, K &k) { keyed(k, j < w.count ? bias[w.first + j] : A(0)); });
+        }
+    }
+    if (a.keep < a.groups) {
+        K v1 = NONE, v2 = NONE;
+        each([&](int, K &k) {
+            v2 = k > v1 ? v1 : k > v2 ? k : v2;
+            v1 = k > v1 ? k : v1;
+        });
+        K rank, least;                             // least: the last key that its rank goes by
+        const int first_in_wave = threadIdx.x & 63 & ~(LANES - 1);
+        const uint64_t column = (LANES < 64 ? (1ull << (LANES & 63)) - 1 : ~0ull) << first_in_wave;
+        // The best of all the lanes' firsts, and of what is left of them and their seconds.
+        auto best_two = [&](auto &x, auto &y) {
+            const auto m = over_lanes<LANES>(x, Larger(), of_group);
+            const uint64_t mine = __ballot(x == m) >> (threadIdx.x & 63 & ~(of_group - 1));
+            const bool holds = (__ffsll((unsigned long long)mine) - 1) == (w.lane & (of_group - 1));
+            y = over_lanes<LANES>(holds ? y : x, Larger(), of_group);
+            x = m;
+        };
+        // The lanes of the first group whose rank is the best.
+        auto wins = [&](auto r, auto m) {
+            const uint64_t mask = __ballot(r == m && m > -INFINITY) & column;
+            return mask != 0 && (__ffsll((unsigned long long)mask) - 1 - first_in_wave) >> a.lane_shift == w.group;
+        };
+        if (a.best == 1) {
+            rank = least = over_lanes<LANES>(v1, Larger(), of_group);
+        } else {
+            best_two(v1, v2);
+            const K m = v1, rest = v2;
+            least = rest > NONE ? rest : m;
+            S x = S(m), y = S(rest);
+            if (!bias) {
+                const S most = softmax ? S(lanes_max<LANES>(m)) : S(0);
+                x = m > NONE ? score_of(x, most, S(1)) : x;
+                y = rest > NONE ? score_of(y, most, S(1)) : y;
+            }
+            const S sum = m > NONE ? x + (rest > NONE ? y : S(0)) : S(-INFINITY);
+            rank = K(sum);
+            if constexpr (sizeof(K) < sizeof(S)) {
+                // Sums are compared in 64 bits: each group's place among them instead.
+                int above = 0;
+                for (int g = 0; g < a.groups; ++g) {
+                    const S o = __shfl(sum, (threadIdx.x & 63 & ~(LANES - 1)) + (g << a.lane_shift), 64);
+                    above += o > sum || (o == sum && g < w.group);
+                }
+                rank = m > NONE ? K(-above) : NONE;
+            }
+        }
+        bool kept = false;
+        K last = NONE, left = rank;
+        for (int r = 0; r < a.keep; ++r) {
+            last = lanes_max<LANES>(left);
+            if (wins(left, last)) {
+                kept = true;
+                left = NONE;
+            }
+        }
+        if constexpr (APPROX) {
+            const K next = lanes_max<LANES>(left);
+            const float near = a.best * apart * (1 + fabsf(last));
+            const bool open = next > NONE && !(last - next > near);
+            if (softmax) {
+                unsure = open;
+            } else if (__ballot(open)) {
+                // Kept for sure: what is past the best one left out.  Of those as near
+                // as that to the last one kept the best in 64 bits fill the places.
+                const bool sure = rank > next + near, maybe = open && !sure && rank > NONE && !(rank < last - near);
+                double d1 = -INFINITY, d2 = -INFINITY;
+                for (int base = 0; base < a.per; base += 32) {
+                    uint32_t some = 0;
+                    each([&](int j, K &k) {
+                        if (j >= base && j < base + 32 && k > NONE && !(k < least - apart * (1 + fabsf(least)))) some |= 1u << (j - base);
+                    });
+                    if (!maybe) some = 0;
+                    while (__ballot(some != 0)) {
+                        if (some) {
+                            const int e = w.first + base + __ffs(some) - 1;
+                            some &= some - 1;
+                            const double v = 1 / (1 + exp(-(double)A(L[e]))) + (double)bias[e];
+                            d2 = v > d1 ? d1 : v > d2 ? v : d2;
+                            d1 = v > d1 ? v : d1;
+                        }
+                    }
+                }
+                best_two(d1, d2);
+                double wide = !maybe ? -INFINITY : a.best == 2 && d2 > -INFINITY ? d1 + d2 : d1;
+                const bool leads = (w.lane & (of_group - 1)) == 0;
+                const int places = a.keep - __popcll(__ballot(sure && leads) & column);
+                if (open) kept = sure;
+                for (int r = 0; r < a.keep; ++r) {
+                    const double m = lanes_max<LANES>(wide);
+                    if (wins(wide, m) && r < places) {
+                        kept = true;
+                        wide = -INFINITY;
+                    }
+                }
+            }
+        }
+        each([&](int, K &k) { k = kept ? k : NONE; });
+    }
+    const int slots = APPROX ? MAX_CANDIDATES : a.copies;
+    for (int i = w.lane; i < slots; i += LANES) chosen[i] = -1;
+    wave_sync();
+    K best = NONE, last = INFINITY;
+    int at = -1, found = 0;
+    bool close = false;                            // keys so near that their order may be another
+    each([&](int j, K &k) {
+        if (k > best) {
+            best = k;
+            at = j;
+        }
+    });
+    for (int r = 0; r < slots + APPROX; ++r) {
+        const K m = lanes_max<LANES>(best);
+        bool more = m > NONE;
+        if constexpr (APPROX) {
+            // Past the last one asked for: those as near to it.
+            const bool near = more && !(last - m > apart * (1 + fabsf(last)));
+            close |= near;
+            if (r < a.copies) last = m;
+            else more = near && !softmax;
+            if (r == slots || (r >= a.copies && __ballot(more) == 0)) {
+                unsure |= more;
+                break;
+            }
+        }
+        found += more;
+        if (first_of(best == m && more, before)) {
+            chosen[r] = w.first + at;
+            const int gone = at;
+            best = NONE;
+            at = -1;
+            each([&](int j, K &k) {
+                k = j == gone ? NONE : k;
+                if (k > best) {
+                    best = k;
+                    at = j;
+                }
+            });
+        }
+    }
+    if constexpr (APPROX) {
+        if (softmax) return unsure || close;
+        // The experts' order in 64 bits: one's place is how many come before it.
+        if (__ballot(close)) {
+            wave_sync();
+#pragma unroll 1
+            for (int i = w.lane; i < found; i += LANES)
+                exact[i] = 1 / (1 + exp(-(double)A(L[chosen[i]]))) + (double)bias[chosen[i]];
+            wave_sync();
+            int *order = (int *)(exact + MAX_CANDIDATES);
+#pragma unroll 1
+            for (int i = w.lane; i < found; i += LANES) {
+                const double key = exact[i];
+                const int e = chosen[i];
+                int ahead = 0;
+                for (int j = 0; j < found; ++j) ahead += exact[j] > key || (exact[j] == key && chosen[j] < e);
+                order[ahead] = e;
+            }
+            wave_sync();
+#pragma unroll 1
+            for (int i = w.lane; i < found; i += LANES) chosen[i] = order[i];
+        }
+    }
+    return unsure;
+}
+
+// BIASED: keys are scores plus biases, Float64; of other logits than Float64 they are
+// made in Float32 first, and again in Float64 for a column that is not settled by those.
+template <typename T, bool BIASED, int LANES, int PER>
+__global__ __launch_bounds__(PER ? 256 : 64, PER ? 4 : 1) void route_kernel(const RouteArgs a)
+{
+    using A = typename Elem<T>::Acc;
+    constexpr int NT = PER ? 256 : 64, COLS = NT / LANES, NP = MAX_COPIES / LANES;
+    __shared__ int s_chosen[COLS][MAX_CANDIDATES];
+    __shared__ double s_exact[BIASED && sizeof(T) < 8 ? COLS : 1][MAX_CANDIDATES * 3 / 2];
+    extern __shared__ double s_keys[];
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, of_group = 1 << a.lane_shift;
+    const int group = lane >> a.lane_shift, place = (lane & (of_group - 1)) * a.per;
+    const bool softmax = a.score == JLUST_SCORE_SOFTMAX;
     for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < a.cols; c0 += (int64_t)gridDim.x * COLS) {
         const int64_t c = c0 + sub;
         const T *L = (const T *)a.L + c * a.ldl;
         int count = a.size - place < a.per ? a.size - place : a.per;
         if (group >= a.groups || c >= a.cols || count < 0) count = 0;
-        double top = -INFINITY, total = 1;
-        if (PER > 0 && a.whole) {
-            T raw[HELD] = {};
-            if (count) load_vec<HELD>(L + first, raw);
-#pragma unroll
-            for (int j = 0; j < PER; ++j) held[j] = count && A(raw[j]) > A(-INFINITY) ? K(A(raw[j])) : NONE;
+        const RouteShare w{lane, group, group * a.size + place, count};
+        double top, total;
+        if constexpr (!BIASED || sizeof(T) == 8) {
+            choose<T, A, false, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], nullptr, &top, &total);
         } else {
-            each([&](int j, K &k) {
-                const K l = j < count ? K(A(L[first + j])) : NONE;
-                k = l > NONE ? l : NONE;
-            });
-        }
-        // Softmax's sum is needed where scores are compared or left as they are.
-        if (softmax && (bias || !a.renormalize)) {
-            K m = NONE;
-            A sum = A(0);
-            each([&](int, K &k) { m = k > m ? k : m; });
-            m = lanes_max<LANES>(m);
-            top = (double)m;
-            if (bias) {
-                double wide = 0;
-                each([&](int, K &k) { wide += k > NONE ? exp_below((double)k, top) : 0; });
-                total = lanes_sum<LANES>(wide);
-            } else {
-                each([&](int, K &k) { sum += k > NONE ? exp_below(A(k), A(m)) : A(0); });
-                total = (double)lanes_sum<LANES>(sum);
-            }
-        }
-        auto score_of = [&](double l, double m, double all) { return softmax ? exp_below(l, m) / all : 1 / (1 + exp(-l)); };
-        if (bias) {
-            auto keyed = [&](K &k, A b) {
-                const K v = k > NONE ? K(score_of((double)k, top, total) + (double)b) : NONE;
-                k = v > NONE ? v : NONE;
-            };
-            if (PER > 0 && a.whole) {
-                A add[HELD] = {};
-                if (count) load_vec<HELD>(bias + first, add);
-#pragma unroll
-                for (int j = 0; j < PER; ++j) keyed(held[j], add[j]);
-            } else {
-                each([&](int j, K &k) { keyed(k, j < count ? bias[first + j] : A(0)); });
-            }
-        }
-        if (a.keep < a.groups) {
-            K v1 = NONE, v2 = NONE;
-            each([&](int, K &k) {
-                v2 = k > v1 ? v1 : k > v2 ? k : v2;
-                v1 = k > v1 ? k : v1;
-            });
-            K rank;
-            if (a.best == 1) {
-                rank = over_lanes<LANES>(v1, Larger(), of_group);
-            } else {
-                // The best of all the lanes' firsts, and of what is left of them and their seconds.
-                const K m = over_lanes<LANES>(v1, Larger(), of_group);
-                const uint64_t mine = __ballot(v1 == m) >> (threadIdx.x & 63 & ~(of_group - 1));
-                const bool holds = (__ffsll((unsigned long long)mine) - 1) == (lane & (of_group - 1));
-                const K rest = over_lanes<LANES>(holds ? v2 : v1, Larger(), of_group);
-                double x = (double)m, y = (double)rest;
-                if (!bias) {
-                    const double most = softmax ? (double)lanes_max<LANES>(m) : 0;
-                    x = m > NONE ? score_of(x, most, 1) : x;
-                    y = rest > NONE ? score_of(y, most, 1) : y;
+            const bool unsure = choose<T, float, true, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], s_exact[sub], &top, &total);
+            uint64_t open = __ballot(unsure && lane == 0);
+            // A wave takes each such column: its registers hold Float64 keys of four lanes.
+            while (open) {
+                const int at = __ffsll((unsigned long long)open) - 1, theirs = (threadIdx.x & ~63) / LANES + at / LANES;
+                open &= open - 1;
+                constexpr int WIDE = LANES == 64 ? PER : PER > 4 ? PER / 4 : 1;
+                RouteArgs b = a;
+                b.lane_shift += LANES == 64 ? 0 : 2;
+                b.per = (a.size + (1 << b.lane_shift) - 1) >> b.lane_shift;
+                b.whole = b.per == WIDE && a.size % b.per == 0;
+                const int mine = threadIdx.x & 63, g = mine >> b.lane_shift, from = (mine & ((1 << b.lane_shift) - 1)) * b.per;
+                int some = a.size - from < b.per ? a.size - from : b.per;
+                if (g >= a.groups || some < 0) some = 0;
+                double m, all;
+                wave_sync();
+                choose<T, double, false, 64, WIDE>(b, RouteShare{mine, g, g * a.size + from, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
+                                                   (char *)s_keys, s_chosen[theirs], nullptr, &m, &all);
+                if (sub == theirs) {
+                    top = m;
+                    total = all;
                 }
-                const double sum = m > NONE ? x + (rest > NONE ? y : 0) : (double)NONE;
-                rank = K(sum);
-                if constexpr (sizeof(K) == 4) {
-                    // Sums are compared in 64 bits: each group's place among them instead.
-                    int above = 0;
-                    for (int g = 0; g < a.groups; ++g) {
-                        const double o = __shfl(sum, (threadIdx.x & 63 & ~(LANES - 1)) + (g << a.lane_shift), 64);
-                        above += o > sum || (o == sum && g < group);
-                    }
-                    rank = m > NONE ? K(-above) : NONE;
-                }
-            }
-            bool kept = false;
-            for (int r = 0; r < a.keep; ++r) {
-                const K m = lanes_max<LANES>(rank);
-                const int winner = first_lane<LANES>(rank == m && m > NONE);
-                if (winner >= 0 && winner >> a.lane_shift == group) {
-                    kept = true;
-                    rank = NONE;
-                }
-            }
-            each([&](int, K &k) { k = kept ? k : NONE; });
-        }
-        K best = NONE;
-        int at = -1;
-        each([&](int j, K &k) {
-            if (k > best) {
-                best = k;
-                at = j;
-            }
-        });
-        for (int r = 0; r < a.copies; ++r) {
-            const K m = lanes_max<LANES>(best);
-            const int winner = first_lane<LANES>(best == m && m > NONE);
-            if (winner < 0 && lane == 0) s_chosen[sub][r] = -1;
-            if (winner == lane) {
-                s_chosen[sub][r] = first + at;
-                const int gone = at;
-                best = NONE;
-                at = -1;
-                each([&](int j, K &k) {
-                    k = j == gone ? NONE : k;
-                    if (k > best) {
-                        best = k;
-                        at = j;
-                    }
-                });
             }
         }
         wave_sync();
@@ -296,7 +463,7 @@ __device__ __forceinline__ A score_below(A l, A top)
 // chosen and 0 elsewhere; softmax as it is s_e (t_e - sum s t) everywhere.  LANES lanes
 // take a column, CPL chunks of 16 bytes each in registers, so logits are read once (CPL
 // 0: any number, read again).
-template <typename T, int LANES, int CPL>
+template <typename T, bool WHOLE, int LANES, int CPL>
 __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
 {
     constexpr int CH = 16 / sizeof(T), HELD = CPL ? CPL : 1;
@@ -314,16 +481,14 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
         if (CPL > 0 && dense) {
             uint32x4 raw[HELD];
 #pragma unroll
-            for (int i = 0; i < CPL; ++i) {
-                const int at = (lane + LANES * i) * CH;
-                raw[i] = read_raw(L + at, live ? a.experts - at : 0);
-            }
+            for (int i = 0; i < CPL; ++i)
+                raw[i] = read_at<WHOLE>((const T *)a.L + (live ? c : a.cols - 1) * a.ldl, (lane + LANES * i) * CH, a.experts);
 #pragma unroll
             for (int i = 0; i < CPL; ++i) {
                 values<T>(raw[i], s[i]);
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
-                    const bool some = live && (lane + LANES * i) * CH + j < a.experts && s[i][j] > A(-INFINITY);
+                    const bool some = (lane + LANES * i) * CH + (WHOLE ? 0 : j) < a.experts && s[i][j] > A(-INFINITY);
                     s[i][j] = some ? s[i][j] : A(-INFINITY);
                     top = s[i][j] > top ? s[i][j] : top;
                 }
@@ -410,7 +575,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
 #pragma unroll
                     for (int j = 0; j < CH; ++j) g[j] = s[i][j] * inv * (g[j] - dot);
                 }
-                if (live) write_chunk((T *)a.dL + c * a.lddl + at, a.experts - at, g);
+                if (live) write_at<WHOLE>((T *)a.dL + c * a.lddl, at, a.experts, g);
             }
         } else if (live) {
             for (int e = lane; e < a.experts; e += LANES) {
@@ -440,34 +605,34 @@ bool route_lanes(int lanes, RouteArgs *a)
     return true;
 }
 
-template <typename T, typename K, int LANES, int PER>
+template <typename T, bool BIASED, int LANES, int PER>
 int launch_route(RouteArgs a, hipStream_t s)
 {
     constexpr int NT = PER ? 256 : 64;
     a.whole = a.per == PER && a.size % (PER ? PER : 1) == 0;
-    hipLaunchKernelGGL((route_kernel<T, K, LANES, PER>), dim3(column_blocks(a.cols, NT / LANES)), dim3(NT),
-                       PER ? 0 : sizeof(K) * 64 * a.per, s, a);
+    hipLaunchKernelGGL((route_kernel<T, BIASED, LANES, PER>), dim3(column_blocks(a.cols, NT / LANES)), dim3(NT),
+                       PER ? 0 : (BIASED ? sizeof(double) : sizeof(typename Elem<T>::Acc)) * 64 * a.per, s, a);
     return check_launch("route_kernel");
 }
 
 // 16 lanes a column where it fits them and the columns fill the CUs (a round of the
 // best key then serves four columns), else a wave.
-template <typename T, typename K>
+template <typename T, bool BIASED>
 int route(RouteArgs a, hipStream_t s)
 {
     if (a.cols > ROUTE_FEW && route_lanes(16, &a) && a.per <= 16) {
-        if (a.per <= 1) return launch_route<T, K, 16, 1>(a, s);
-        if (a.per <= 2) return launch_route<T, K, 16, 2>(a, s);
-        if (a.per <= 4) return launch_route<T, K, 16, 4>(a, s);
-        if (a.per <= 8) return launch_route<T, K, 16, 8>(a, s);
-        return launch_route<T, K, 16, 16>(a, s);
+        if (a.per <= 1) return launch_route<T, BIASED, 16, 1>(a, s);
+        if (a.per <= 2) return launch_route<T, BIASED, 16, 2>(a, s);
+        if (a.per <= 4) return launch_route<T, BIASED, 16, 4>(a, s);
+        if (a.per <= 8) return launch_route<T, BIASED, 16, 8>(a, s);
+        return launch_route<T, BIASED, 16, 16>(a, s);
     }
     route_lanes(64, &a);
-    if (a.per <= 1) return launch_route<T, K, 64, 1>(a, s);
-    if (a.per <= 2) return launch_route<T, K, 64, 2>(a, s);
-    if (a.per <= 4) return launch_route<T, K, 64, 4>(a, s);
-    if (a.per <= 16) return launch_route<T, K, 64, 16>(a, s);
-    return launch_route<T, K, 64, 0>(a, s);
+    if (a.per <= 1) return launch_route<T, BIASED, 64, 1>(a, s);
+    if (a.per <= 2) return launch_route<T, BIASED, 64, 2>(a, s);
+    if (a.per <= 4) return launch_route<T, BIASED, 64, 4>(a, s);
+    if (a.per <= 16) return launch_route<T, BIASED, 64, 16>(a, s);
+    return launch_route<T, BIASED, 64, 0>(a, s);
 }
 
 int check_route(const char *who, int32_t value_type, int32_t score, int64_t experts, int64_t cols, int64_t copies, double scale)
@@ -533,9 +698,7 @@ extern "C" int jlust_hip_route(const jlust_route *op, jlust_stream_t stream)
     a.scale = op->scale;
     return with_type(op->value_type, [&](auto t) {
         using T = decltype(t);
-        if constexpr (sizeof(T) < 8)
-            if (!a.bias) return route<T, float>(a, (hipStream_t)stream);
-        return route<T, double>(a, (hipStream_t)stream);
+        return a.bias ? route<T, true>(a, (hipStream_t)stream) : route<T, false>(a, (hipStream_t)stream);
     });
 }
 
@@ -575,18 +738,22 @@ extern "C" int jlust_hip_route_grad(const jlust_route_grad *op, jlust_stream_t s
             hipLaunchKernelGGL(kernel, dim3(column_blocks(a.cols, 256 / lanes)), dim3(256), 0, (hipStream_t)stream, a);
             return check_launch("route_grad_kernel");
         };
-        if (chunks <= 16) return launch(route_grad_kernel<T, 16, 1>, 16);
-        if (chunks <= 32) return launch(route_grad_kernel<T, 16, 2>, 16);
-        if (chunks <= 64) return launch(route_grad_kernel<T, 16, 4>, 16);
-        if (chunks <= 256) return launch(route_grad_kernel<T, 64, 4>, 64);
-        return launch(route_grad_kernel<T, 64, 0>, 64);
+        auto go = [&](auto whole) {
+            constexpr bool W = decltype(whole)::value;
+            if (chunks <= 16) return launch(route_grad_kernel<T, W, 16, 1>, 16);
+            if (chunks <= 32) return launch(route_grad_kernel<T, W, 16, 2>, 16);
+            if (chunks <= 64) return launch(route_grad_kernel<T, W, 16, 4>, 16);
+            if (chunks <= 256) return launch(route_grad_kernel<T, W, 64, 4>, 64);
+            return launch(route_grad_kernel<T, W, 64, 0>, 64);
+        };
+        return a.experts % (16 / sizeof(T)) == 0 ? go(std::true_type()) : go(std::false_type());
     });
 }
 
 namespace jlust {
 int preload_route()
 {
-    JLUST_PRELOAD_KERNEL((route_kernel<float, double, 64, 4>));
+    JLUST_PRELOAD_KERNEL((route_kernel<float, true, 64, 4>));
     return JLUST_STATUS_SUCCESS;
 }
 }  // namespace jlust

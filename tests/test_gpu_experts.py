@@ -153,6 +153,24 @@ def test_route_neighbours(J, T):
     check_route(J, host, 4, score="sigmoid", bias=bias.cuda(), groups=8, keep=3)
 
 
+@pytest.mark.parametrize("T", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("cols", [70, 4100])
+def test_route_near_keys(J, T, score, cols):
+    """Columns most of whose keys lie as near to each other as Float32 has it, or are
+    equal: more of them than are looked at one by one, in the last places kept, in the
+    last groups kept, and where a column's neighbours have none such."""
+    gen = torch.Generator().manual_seed(11)
+    E_ = 96
+    host = (torch.randn((cols, E_), generator=gen) * 2).to(T)
+    host[::3] = host[::3, :1]
+    host[1::7, 10:60] = host[1::7].amax(1, keepdim=True)
+    host[2::11, 40:] = -INF
+    for bias in (torch.zeros(E_), torch.randperm(E_, generator=gen) * 1e-9, torch.randint(0, 4, (E_,), generator=gen) * 2.0 ** -24):
+        for groups, keep, best, copies in ((1, 1, 1, 6), (8, 3, 2, 9), (8, 3, 1, 36), (4, 1, 2, 24), (1, 1, 1, 64)):
+            check_route(J, host.cuda().t(), copies, score=score, bias=bias.float().cuda(), groups=groups, keep=keep, best=best)
+
+
 GRADS = [(1, 1), (5, 2), (64, 8), (160, 6), (255, 3), (513, 64), (4095, 9)]
 
 
