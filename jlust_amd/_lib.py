@@ -214,15 +214,13 @@ def stream_handle(dev: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
-def raw_stream(index: int) -> int:
-    """The current stream of device `index` as an address."""
-    if _RAW_STREAM is not None:
-        return _RAW_STREAM(index)
+def _public_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
-def current_device() -> int:
-    return _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
+# The current stream of device `index` as an address; the current device's index.
+raw_stream = _RAW_STREAM if _RAW_STREAM is not None else _public_stream
+current_device = _CUR_DEVICE if _CUR_DEVICE is not None else torch.cuda.current_device
 
 
 def on_device(dev: torch.device):

@@ -85,21 +85,6 @@ __device__ __forceinline__ void read_chunk(const T *p, int64_t left, A (&f)[16 /
     values<T>(read_raw(p, left), f);
 }
 
-// 16 bytes past the caches.  Results that the eight L2s of 4 MB do not hold would only
-// push out what is still read (16,384 bfloat16 columns of 4,096: 71.4 us by plain stores
-// and 63.9; backward, 200,003 Float32 columns of 100: 51.6 and 49.2; products' results
-// gain nothing: 8,192 columns 2048 -> 8192, 305 and 307 us).
-constexpr int64_t STREAMED = 32 << 20;         // bytes of a result from which it is stored so
-typedef uint32_t uint32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
-
-template <typename T>
-__device__ __forceinline__ void stream_chunk(T *p, const T *v)
-{
-    uint32x4 u;
-    __builtin_memcpy(&u, v, 16);
-    __builtin_nontemporal_store((uint32x4_any)u, reinterpret_cast<uint32x4_any *>(p));
-}
-
 template <typename T, typename A>
 __device__ __forceinline__ void write_chunk(T *p, int64_t left, const A (&f)[16 / sizeof(T)], bool streamed = false)
 {

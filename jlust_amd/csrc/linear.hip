@@ -621,6 +621,7 @@ int linear_int8(const jlust_linear_int8 &op, jlust_stream_t stream, jlust_produc
     a.Z = op.Z;
     a.ldz = op.ldz;
     a.act = op.act;
+    a.streamed = op.value_type != JLUST_VALUE_F32 && op.out * op.cols * 2 > STREAMED;
     int shape = 0;
     size_t bytes = 0;
     if (int st = plan_tile_product<int8_t>(&a, true, true, &shape, &bytes)) return st;

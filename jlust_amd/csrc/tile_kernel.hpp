@@ -237,7 +237,7 @@ __device__ __forceinline__ void load_bias(const TileArgs &a, int group, int64_t 
 
 // V sums of row `row` of C, columns mm ..: the epilogue; res: R's there.  finish_sum: of
 // sums that have their bias.
-template <int V, typename T, typename A>
+template <int V, bool STREAM, typename T, typename A>
 __device__ __forceinline__ void finish_sum(const TileArgs &a, const T *res, int64_t row, int64_t mm, A *s)
 {
     const int64_t left = a.m - mm;
@@ -254,6 +254,8 @@ __device__ __forceinline__ void finish_sum(const TileArgs &a, const T *res, int6
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) t[e] = T(s[e]);
+    if constexpr (STREAM && V * sizeof(T) == 16)
+        if (a.streamed && left >= V) return stream_chunk((T *)a.C + row * a.ldc + mm, t);
     store_some<V>((T *)a.C + row * a.ldc + mm, left, t);
 }
 
@@ -268,7 +270,7 @@ __device__ __forceinline__ void finish(const TileArgs &a, const T *bias, const T
         store_some<V>((A *)a.C + row * a.ldc + mm, left, s);
         return;
     }
-    finish_sum<V, T, A>(a, res, row, mm, s);
+    finish_sum<V, false, T, A>(a, res, row, mm, s);
 }
 
 // The scales of a group's V rows of P from m on (0 past the edge and in no group), and
@@ -507,7 +509,7 @@ __device__ __forceinline__ void finish_scaled(const TileArgs &a, char *lds, int 
                 float f[CH];
 #pragma unroll
                 for (int e = 0; e < CH; ++e) f[e] = fmaf((float)v[e], qs[run][it] * by[h][e], bias[h][e]);
-                finish_sum<CH, O, float>(b, res[it], row[run][it], m, f);
+                finish_sum<CH, true, O, float>(b, res[it], row[run][it], m, f);
             }
         }
 }

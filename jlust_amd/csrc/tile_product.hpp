@@ -45,6 +45,7 @@ struct TileArgs {
     const float *ps = nullptr;          // m values, gs elements between groups
     int64_t gs = 0;
     const float *qs = nullptr;          // by the rows of Q
+    bool streamed = false;              // whole chunks of 16 bytes of C go past the caches
     void *part = nullptr;               // partial sums [split][C's rows][m]
     int split = 1;
     int tiles_m = 0, tiles_n = 0;
@@ -73,6 +74,22 @@ template <int V, typename T>
 __device__ __forceinline__ void store_vec(T *p, const T *v)
 {
     __builtin_memcpy(p, v, V * sizeof(T));
+}
+
+// 16 bytes past the caches.  Results that the eight L2s of 4 MB do not hold would only
+// push out what is still read (16,384 bfloat16 columns of 4,096: 71.4 us by plain stores
+// and 63.9; backward, 200,003 Float32 columns of 100: 51.6 and 49.2; products' results
+// of 16 bits gain nothing: 8,192 columns 2048 -> 8192, 305 and 307 us; of 8 bits, 220 and
+// 210, 32 experts' 109 and 120).
+constexpr int64_t STREAMED = 32 << 20;         // bytes of a result from which it is stored so
+typedef uint32_t uint32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
+
+template <typename T>
+__device__ __forceinline__ void stream_chunk(T *p, const T *v)
+{
+    uint32x4 u;
+    __builtin_memcpy(&u, v, 16);
+    __builtin_nontemporal_store((uint32x4_any)u, reinterpret_cast<uint32x4_any *>(p));
 }
 
 template <typename T>

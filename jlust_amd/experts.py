@@ -41,7 +41,7 @@ import torch
 
 from . import _lib
 from .errors import DeviceMismatch, IncompatibleExtents, NonCanonicalStorage, UnsupportedIndexType, UnsupportedValueType
-from .layers import _BE, _extents, _first, _matrix, _norm_vector, _raw, _run
+from .layers import _BE, _extents, _first, _matrix, _raw, _run, _vector
 from .ops import _layer_calls
 
 # jlust_route and jlust_route_grad of include/jlust_hip.h.
@@ -71,10 +71,6 @@ def _by_column(t, name, cols):
     return t
 
 
-def _origin(origin):
-    return 1 if origin is None else origin.offset
-
-
 def _logits(L, ids):
     l = L if type(L) is torch.Tensor else _raw(L, "L")
     T = l.dtype
@@ -93,9 +89,9 @@ def _route(L, ids, weights, bias=None, score="softmax", groups=1, keep=None, bes
     T, vt, index, experts, cols, copies, lp, ldl, ip, ldi = _logits(L, ids)
     S = torch.float32 if vt else torch.float64
     wp, ldw = _matrix(_by_column(weights, "weights", cols), "weights", copies, cols, index, S)
-    bp = 0 if bias is None else _norm_vector(bias, "bias", experts, index, S)
+    bp = 0 if bias is None else _vector(bias, "bias", experts, index, S)
     _run(_lib.lib().jlust_hip_route, index, "route", T,
-         _ROUTE(vt, _score(score), bool(renormalize), _origin(origin), experts, cols, copies, groups,
+         _ROUTE(vt, _score(score), bool(renormalize), 1 if origin is None else origin.offset, experts, cols, copies, groups,
                 groups if keep is None else keep, best, lp, ldl, bp, ip, ldi, wp, ldw, scale))
     return ids
 
@@ -106,8 +102,8 @@ def _route_grad(L, ids, dweights, dL, score="softmax", renormalize=True, scale=1
                       torch.float32 if vt else torch.float64)
     dp, ldd = _matrix(dL, "dL", experts, cols, index, T)
     _run(_lib.lib().jlust_hip_route_grad, index, "route_grad", T,
-         _ROUTE_GRAD(vt, _score(score), bool(renormalize), _origin(origin), experts, cols, copies, lp, ldl, ip, ldi, wp, ldw,
-                     dp, ldd, scale))
+         _ROUTE_GRAD(vt, _score(score), bool(renormalize), 1 if origin is None else origin.offset, experts, cols, copies, lp, ldl,
+                     ip, ldi, wp, ldw, dp, ldd, scale))
     return dL
 
 

@@ -56,6 +56,8 @@ _LINEAR = struct.Struct("@4i19q").pack
 _LINEAR_GRAD = struct.Struct("@4i22q").pack
 _LINEAR_INT8 = struct.Struct("@2i22q").pack
 
+_current_device, _raw_stream = _lib.current_device, _lib.raw_stream
+
 
 # --------------------------------------------------------------------- checks
 
@@ -245,8 +247,8 @@ class GroupPlan(AbstractKernelHandle):
 
 def _run(f, index, what, T, *args):
     """f(*args, stream) on the operands' device; returns the stream."""
-    if _lib.current_device() == index:
-        s = _lib.raw_stream(index)
+    if _current_device() == index:
+        s = _raw_stream(index)
         st = f(*args, s)
     else:
         with torch.cuda.device(index):
@@ -296,17 +298,13 @@ def _linear(h, W, X, Y, bias=None, act=None, residual=None, preact=None, w_scale
     return Y
 
 
-def _int8_weights(w, groups):
-    """(address, leading dimension, group stride, out, inp) of Int8 weights."""
-    shape, strides = w.shape, w.stride()
-    if len(shape) != (3 if groups else 2):
-        raise IncompatibleExtents(f"W: expected {'out x inp x groups' if groups else 'out x inp'}, got {w.dim()} dimensions")
-    out, inp = shape[0], shape[1]
-    if groups and shape[2] != groups:
-        raise IncompatibleExtents(f"W holds {shape[2]} matrices, expected {groups}")
-    if (strides[1] != 1 and inp > 1) or (strides[0] < inp and out > 1):
-        raise NonCanonicalStorage(f"W: an Int8 matrix lies along inp, the transpose of a column-major one, got strides {strides}")
-    return w.data_ptr(), strides[0] if out > 1 else max(inp, 1), strides[2] if groups else 0, out, inp
+def _vector(t, name, n, index, T):
+    """The address of a vector of n values."""
+    if type(t) is torch.Tensor and t.dtype is T and t.get_device() == index:
+        shape = t.shape
+        if len(shape) == 1 and shape[0] == n and (n <= 1 or t.stride(0) == 1):
+            return t.data_ptr()
+    return _norm_vector(t, name, n, index, T)              # another kind of operand, or what is wrong with it
 
 
 def _linear_int8(h, w, x, Y, y, bias, act, residual, preact, w_scale, x_scale):
@@ -323,18 +321,29 @@ def _linear_int8(h, w, x, Y, y, bias, act, residual, preact, w_scale, x_scale):
         if h.index != index:
             raise DeviceMismatch(f"the plan is on {h.dev}, W on {w.device}")
         groups, copies, plan = h.groups, h.copies, h.use()
-    wp, ldw, ws, out, inp = _int8_weights(w, groups)
+    shape, strides = w.shape, w.stride()
+    if len(shape) != (3 if groups else 2):
+        raise IncompatibleExtents(f"W: expected {'out x inp x groups' if groups else 'out x inp'}, got {w.dim()} dimensions")
+    out, inp = shape[0], shape[1]
+    if groups and shape[2] != groups:
+        raise IncompatibleExtents(f"W holds {shape[2]} matrices, expected {groups}")
+    if (strides[1] != 1 and inp > 1) or (strides[0] < inp and out > 1):
+        raise NonCanonicalStorage(f"W: an Int8 matrix lies along inp, the transpose of a column-major one, got strides {strides}")
     n, xc = _columns(x, y, h)
     xp, ldx = _matrix(x, "X", inp, xc, index, torch.int8)
     yp, ldy = _matrix(y, "Y", out, n, index, T)
-    sp, ss = _bias(w_scale, "w_scale", out, groups, index, torch.float32)
-    sx = _norm_vector(x_scale, "x_scale", xc, index, torch.float32)
-    bp, bs = _bias(bias, "bias", out, groups, index, T) if bias is not None else (0, 0)
-    rp, ldr = _matrix(residual, "residual", out, n, index, T) if residual is not None else (0, 0)
-    zp, ldz = _matrix(preact, "preact", out, n, index, T) if preact is not None else (0, 0)
+    if groups:
+        sp, ss = _bias(w_scale, "w_scale", out, groups, index, torch.float32)
+        bp, bs = _bias(bias, "bias", out, groups, index, T)
+    else:
+        sp, ss, bs = _vector(w_scale, "w_scale", out, index, torch.float32), 0, 0
+        bp = 0 if bias is None else _vector(bias, "bias", out, index, T)
+    sx = _vector(x_scale, "x_scale", xc, index, torch.float32)
+    rp, ldr = (0, 0) if residual is None else _matrix(residual, "residual", out, n, index, T)
+    zp, ldz = (0, 0) if preact is None else _matrix(preact, "preact", out, n, index, T)
     _run(_lib.lib().jlust_hip_linear_int8, index, "linear_int8", T,
-         _LINEAR_INT8(vt, _act(act), out, inp, n, wp, ldw, sp, xp, ldx, sx, yp, ldy, bp, rp, ldr, zp, ldz, groups, copies,
-                      plan, ws, ss, bs))
+         _LINEAR_INT8(vt, _act(act), out, inp, n, w.data_ptr(), strides[0] if out > 1 else max(inp, 1), sp, xp, ldx, sx, yp, ldy,
+                      bp, rp, ldr, zp, ldz, groups, copies, plan, strides[2] if groups else 0, ss, bs))
     return Y
 
 
@@ -344,13 +353,13 @@ def _quantize(X, Y, scales):
     vt, index = _first(x, "X")
     if vt == 0:
         raise UnsupportedValueType(T, _BE, "QuantizeOp takes Float32, Float16 or BFloat16")
+    if scales is None:
+        raise TypeError("QuantizeOp needs scales")
     d, cols = _extents(x, "X")
     xp, ldx = _matrix(x, "X", d, cols, index, T)
     yp, ldy = _matrix(Y, "Y", d, cols, index, torch.int8)
-    sp = _norm_vector(scales, "scales", cols, index, torch.float32)
-    if sp == 0 and cols:
-        raise TypeError("QuantizeOp needs scales")
-    _run(_lib.lib().jlust_hip_quantize_columns, index, "quantize", T, vt, d, cols, xp, ldx, yp, ldy, sp)
+    _run(_lib.lib().jlust_hip_quantize_columns, index, "quantize", T, vt, d, cols, xp, ldx, yp, ldy,
+         _vector(scales, "scales", cols, index, torch.float32))
     return Y
 
 
