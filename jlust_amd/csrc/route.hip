@@ -359,7 +359,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
 // BIASED: keys are scores plus biases, Float64; of other logits than Float64 they are
 // made in Float32 first, and again in Float64 for a column that is not settled by those.
 template <typename T, bool BIASED, int LANES, int PER>
-__global__ __launch_bounds__(PER ? 256 : 64, PER ? 4 : 1) void route_kernel(const RouteArgs a)
+__global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4) void route_kernel(const RouteArgs a)
 {
     using A = typename Elem<T>::Acc;
     constexpr int NT = PER ? 256 : 64, COLS = NT / LANES, NP = MAX_COPIES / LANES;
@@ -631,6 +631,7 @@ int route(RouteArgs a, hipStream_t s)
     if (a.per <= 1) return launch_route<T, BIASED, 64, 1>(a, s);
     if (a.per <= 2) return launch_route<T, BIASED, 64, 2>(a, s);
     if (a.per <= 4) return launch_route<T, BIASED, 64, 4>(a, s);
+    if (a.per <= 8) return launch_route<T, BIASED, 64, 8>(a, s);
     if (a.per <= 16) return launch_route<T, BIASED, 64, 16>(a, s);
     return launch_route<T, BIASED, 64, 0>(a, s);
 }

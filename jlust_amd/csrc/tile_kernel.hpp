@@ -1219,7 +1219,7 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
     if constexpr (sizeof(T) == 1) {
         // Along k on both sides.  A step's bytes are 16-bit values', its k is twice
         // theirs; measured on 1 to 8,192 columns of 64 to 8,192.
-        if (share <= 16 && set(FEW_16, 1)) some[count++] = {FEW_16, 1.0, 0.035, 4, 4};
+        if (share <= 16 && set(FEW_16, 1)) some[count++] = {FEW_16, 1.0, 0.035, 4, 2.2};
         some[count++] = {REG_32, 3.7, 0.22, 5};
         some[count++] = {REG_M64, 4.4, 0.21, 5};
         if (fit && share > 48) {
@@ -1283,7 +1283,7 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
             double rounds = (double)groups / slots;
             rounds = rounds <= 1 ? 1 : rounds < 3 ? (double)((groups + slots - 1) / slots) : rounds;
             const double step = held * work > o.latency ? held * work : o.latency;
-            const double us = rounds * ((double)((k + 64 * p - 1) / (64 * p)) * step + o.end) + (p > 1 ? sizeof(T) == 1 ? 4 + 3e-6 * p * sums : 8 + 1e-6 * p * sums : 0);
+            const double us = rounds * ((double)((k + 64 * p - 1) / (64 * p)) * step + o.end) + (p > 1 ? sizeof(T) == 1 ? 4.5 + 3e-6 * p * sums : 8 + 1e-6 * p * sums : 0);
             if (best_shape < 0 || us < best) {
                 best = us;
                 best_shape = o.shape;

@@ -193,3 +193,29 @@ def linear8(W, ws, Xq, xs, T, bias, act, R, ids=None, copies=1):
         ey = ey + u * (Y.abs() + L.f64(R).abs())
         Y = Y + L.f64(R)
     return Y, Z, ey, E
+
+
+# Products of 8-bit integers and what is planned for each: the type of Y, out, inp, cols,
+# groups, copies; the sums a workgroup makes (rows, columns), whether its operands are
+# copied to LDS, the pieces of k.
+PLANNED8 = [
+    ("bf16", 1029, 2064, 3, 0, 1, (16, 16, 0, 1)),
+    ("f32", 1029, 2053, 3, 0, 1, (16, 16, 0, 1)),
+    ("f16", 1029, 2064, 10, 3, 2, (16, 16, 0, 1)),
+    ("f32", 53, 208, 40, 3, 2, (64, 64, 0, 1)),
+    ("bf16", 1000, 4112, 130, 0, 1, (64, 64, 0, 4)),
+    ("f32", 1000, 4112, 130, 3, 1, (64, 64, 0, 4)),
+    ("f16", 53, 2064, 20, 0, 1, (64, 64, 0, 16)),
+    ("bf16", 53, 4105, 40, 3, 2, (64, 64, 0, 32)),
+    ("f16", 2053, 2064, 20, 0, 1, (128, 32, 0, 8)),
+    ("f32", 520, 4112, 130, 3, 1, (128, 32, 0, 8)),
+    ("f32", 2053, 1040, 1500, 0, 1, (128, 128, 1, 1)),
+    ("bf16", 136, 208, 14600, 3, 2, (128, 128, 1, 1)),
+    ("f16", 2053, 2064, 1500, 0, 1, (128, 128, 1, 1)),
+    ("bf16", 2499, 400, 4100, 0, 1, (256, 128, 1, 1)),
+    ("f32", 2136, 1040, 2000, 32, 2, (256, 128, 1, 1)),
+    ("f16", 2378, 400, 2000, 32, 2, (256, 128, 1, 1)),
+    ("bf16", 520, 2064, 14600, 0, 1, (256, 256, 1, 1)),
+    ("f32", 520, 2064, 14600, 0, 1, (256, 256, 1, 1)),
+    ("f16", 520, 2064, 14600, 3, 1, (256, 256, 1, 1)),
+]

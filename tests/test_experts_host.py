@@ -90,6 +90,18 @@ def test_int8_sums_that_fit():
     assert _lib.lib().jlust_hip_linear_int8_info(args(n), None) == 1 and _lib.lib().jlust_hip_linear_int8_info(None, info) == 1
 
 
+def test_planned_products():
+    """The kernels that tests/_experts.py says its products reach."""
+    for T, out, inp, cols, groups, copies, plan in E.PLANNED8:
+        info, p = (ctypes.c_int64 * 6)(), 1 << 20
+        args = layers._LINEAR_INT8({"f32": 1, "f16": 2, "bf16": 3}[T], 0, out, inp, cols * copies, p, inp, p, p, inp, p, p, out, 0, 0, 0, 0,
+                                   0, groups, copies, p if groups else 0, inp * out, out, out)
+        assert _lib.lib().jlust_hip_linear_int8_info(args, info) == 0
+        assert tuple(info[:4]) == plan, (out, inp, cols, groups, copies)
+    forms = {c[6][:3] for c in E.PLANNED8}
+    assert forms == {(16, 16, 0), (64, 64, 0), (128, 32, 0), (128, 128, 1), (256, 128, 1), (256, 256, 1)}
+
+
 def test_combine_dropout_and_quantize_refuse():
     lib = _lib.lib()
 

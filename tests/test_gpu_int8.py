@@ -136,15 +136,18 @@ def test_linear_int8(J, T, i, pad, skip):
     check(J, case(i, T, out, inp, cols, k % 3 != 0, k % 2 == 0, pad=pad, skip=skip), T, ACTS[k % 4], keep=k % 5 != 0)
 
 
-# Each with the tile (rows, columns), whether its operands are copied and k's pieces.
-LARGE = [("bf16", 2053, 208, 14600), ("f16", 2104, 400, 14600), ("f32", 2053, 640, 14600), ("bf16", 1000, 2112, 300), ("f32", 264, 1040, 4100),
-         ("f16", 1000, 4112, 300), ("bf16", 520, 400, 9000), ("f32", 1531, 2056, 40), ("bf16", 4104, 1001, 600)]
-
-
-@pytest.mark.parametrize("T,out,inp,cols", LARGE)
-def test_linear_int8_large_tiles(J, T, out, inp, cols):
+@pytest.mark.parametrize("T,out,inp,cols,groups,copies", [c[:6] for c in E.PLANNED8])
+def test_linear_int8_kernels(J, T, out, inp, cols, groups, copies):
+    """Every kernel and pieces of k (tests/_experts.py says which), no edge whole."""
     T = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[T]
-    check(J, case(out, T, out, inp, cols, True, False), T, "silu" if cols % 3 else None)
+    s = case(out + cols, T, out, inp, cols, True, cols % 3 == 0, groups or None, copies)
+    act = ACTS[(out + cols) % 4]
+    if not groups:
+        return check(J, s, T, act)
+    gen = torch.Generator().manual_seed(cols)
+    ids = torch.randint(0, groups + 1, (cols, copies), generator=gen, dtype=torch.int32).cuda()
+    ids = ids.t() if copies > 1 else ids[:, 0].contiguous()
+    check(J, s, T, act, ids, copies, J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups))
 
 
 @pytest.mark.parametrize("cols", [1, 40, 300])
