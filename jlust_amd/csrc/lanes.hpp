@@ -59,6 +59,7 @@ struct Larger {                                    // of numbers, one instructio
     __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_fmaxf(a, b); }
     __device__ __forceinline__ double operator()(double a, double b) const { return __builtin_fmax(a, b); }
     __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return b > a ? b : a; }
+    __device__ __forceinline__ int operator()(int a, int b) const { return b > a ? b : a; }
 };
 struct Plus {
     template <typename A>

@@ -292,42 +292,91 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     const int slots = APPROX ? MAX_CANDIDATES : a.copies;
     for (int i = w.lane; i < slots; i += LANES) chosen[i] = -1;
     wave_sync();
-    K best = NONE, last = INFINITY;
-    int at = -1, found = 0;
+    int found = 0;
     bool close = false;                            // keys so near that their order may be another
-    each([&](int j, K &k) {
-        if (k > best) {
-            best = k;
-            at = j;
-        }
-    });
-    for (int r = 0; r < slots + APPROX; ++r) {
-        const K m = lanes_max<LANES>(best);
-        bool more = m > NONE;
-        if constexpr (APPROX) {
-            // Past the last one asked for: those as near to it.
-            const bool near = more && !(last - m > apart * (1 + fabsf(last)));
-            close |= near;
-            if (r < a.copies) last = m;
-            else more = near && !softmax;
-            if (r == slots || (r >= a.copies && __ballot(more) == 0)) {
-                unsure |= more;
-                break;
-            }
-        }
-        found += more;
-        if (first_of(best == m && more, before)) {
-            chosen[r] = w.first + at;
-            const int gone = at;
-            best = NONE;
-            at = -1;
-            each([&](int j, K &k) {
-                k = j == gone ? NONE : k;
-                if (k > best) {
-                    best = k;
-                    at = j;
+    if constexpr (APPROX) {
+        // Keys by whole numbers in their order, the expert's place in the last bits, where
+        // the larger is the earlier: a round takes a key out and finds the next best in three
+        // steps a key, seven with the places in registers of their own.
+        constexpr int PLACE = PER ? PER - 1 : 127, GONE = INT32_MIN;
+        const float near_by = apart + 4 * (PLACE + 1) * 0x1p-24f;      // and what the bits took from two keys
+        int packed[HELD];
+        auto flip = [](int b) { return b ^ (b >> 31 & INT32_MAX); };
+        auto pass = [&](auto &&f) {
+            if constexpr (PER > 0) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) f(packed[j]);
+            } else {
+                int *keys = (int *)lds + w.lane;
+                for (int j = 0; j < a.per; ++j) {
+                    int k = keys[j * 64];
+                    f(k);
+                    keys[j * 64] = k;
                 }
+            }
+        };
+        each([&](int j, K &k) {
+            const int p = k > NONE ? (flip(__builtin_bit_cast(int, k)) & ~PLACE) | (PLACE - j) : GONE;
+            if constexpr (PER > 0) packed[j] = p;
+            else k = __builtin_bit_cast(float, p);
+        });
+        int best = GONE;
+        pass([&](int &k) { best = k > best ? k : best; });
+        auto value = [&](int m) { return __builtin_bit_cast(float, flip(m & ~PLACE)); };
+        auto near = [&](float last, int m) { return m != GONE && !(last - value(m) > near_by * (1 + fabsf(last))); };
+        auto take = [&](int r, int m) {
+            chosen[r] = w.first + PLACE - (m & PLACE);
+            best = GONE;
+            pass([&](int &k) {
+                k = k == m ? GONE : k;
+                best = k > best ? k : best;
             });
+        };
+        int m = lanes_max<LANES>(best), last = GONE;
+        for (int r = 0; r < a.copies; ++r) {
+            found += m != GONE;
+            if (first_of(best == m && m != GONE, before)) take(r, m);
+            last = m;
+            m = lanes_max<LANES>(best);
+            close |= near(value(last), m);
+        }
+        // Past the last one asked for: those as near to it.
+        if (__ballot(close) && !softmax)
+            for (int r = a.copies;; ++r) {
+                const bool more = near(value(last), m);
+                if (__ballot(more) == 0) break;
+                if (r == slots) {
+                    unsure |= more;
+                    break;
+                }
+                found += more;
+                if (first_of(best == m && more, before)) take(r, m);
+                m = lanes_max<LANES>(best);
+            }
+    } else {
+        K best = NONE;
+        int at = -1;
+        each([&](int j, K &k) {
+            if (k > best) {
+                best = k;
+                at = j;
+            }
+        });
+        for (int r = 0; r < a.copies; ++r) {
+            const K m = lanes_max<LANES>(best);
+            if (first_of(best == m && m > NONE, before)) {
+                chosen[r] = w.first + at;
+                const int gone = at;
+                best = NONE;
+                at = -1;
+                each([&](int j, K &k) {
+                    k = j == gone ? NONE : k;
+                    if (k > best) {
+                        best = k;
+                        at = j;
+                    }
+                });
+            }
         }
     }
     if constexpr (APPROX) {
