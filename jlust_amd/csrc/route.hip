@@ -198,6 +198,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             v1 = k > v1 ? k : v1;
         });
         K rank, least;                             // least: the last key that its rank goes by
+        float undone = 0;                          // what a rank's two keys have of each other's sign
         const int first_in_wave = threadIdx.x & 63 & ~(LANES - 1);
         const uint64_t column = (LANES < 64 ? (1ull << (LANES & 63)) - 1 : ~0ull) << first_in_wave;
         // The best of all the lanes' firsts, and of what is left of them and their seconds.
@@ -227,6 +228,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             }
             const S sum = m > NONE ? x + (rest > NONE ? y : S(0)) : S(-INFINITY);
             rank = K(sum);
+            if constexpr (APPROX) undone = rest > NONE && y < 0 && x > 0 ? -2 * y : 0;
             if constexpr (sizeof(K) < sizeof(S)) {
                 // Sums are compared in 64 bits: each group's place among them instead.
                 int above = 0;
@@ -248,7 +250,9 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
         }
         if constexpr (APPROX) {
             const K next = lanes_max<LANES>(left);
-            const float near = a.best * apart * (1 + fabsf(last));
+            // Keys of two signs make a sum smaller than they are: their error is not.
+            if (__ballot(undone > 0)) undone = lanes_max<LANES>(undone);
+            const float near = a.best * apart * (1 + fabsf(last) + undone);
             const bool open = next > NONE && !(last - next > near);
             if (softmax) {
                 unsure = open;

@@ -1218,7 +1218,8 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
     int count = 0;
     if constexpr (sizeof(T) == 1) {
         // Along k on both sides.  A step's bytes are 16-bit values', its k is twice
-        // theirs; measured on 1 to 8,192 columns of 64 to 8,192.
+        // theirs; measured on 1 to 8,192 columns of 64 to 8,192 (43 products: 2.4 % past the
+        // best on average, at most 37 %, with k = 64 and 13,574 rows of n in 4 groups).
         if (share <= 16 && set(FEW_16, 1)) some[count++] = {FEW_16, 1.0, 0.035, 4, 2.2};
         some[count++] = {REG_32, 3.7, 0.22, 5};
         some[count++] = {REG_M64, 4.4, 0.21, 5};

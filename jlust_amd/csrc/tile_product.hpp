@@ -80,7 +80,7 @@ __device__ __forceinline__ void store_vec(T *p, const T *v)
 // push out what is still read (16,384 bfloat16 columns of 4,096: 71.4 us by plain stores
 // and 63.9; backward, 200,003 Float32 columns of 100: 51.6 and 49.2; products' results
 // of 16 bits gain nothing: 8,192 columns 2048 -> 8192, 305 and 307 us; of 8 bits, 220 and
-// 210, 32 experts' 109 and 120).
+// 210, 32 experts' 120 and 109).
 constexpr int64_t STREAMED = 32 << 20;         // bytes of a result from which it is stored so
 typedef uint32_t uint32x4_any __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
