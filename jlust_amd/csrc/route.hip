@@ -91,9 +91,9 @@ __device__ __forceinline__ void chosen_scores(int score, bool relative, const A 
 // How far apart two Float32 keys are in 64 bits for sure, over 1 + the larger: a
 // sigmoid's is off by 4 u (u = 2^-24: its exponential's argument 0.4, the exponential
 // 0.5, the sum 1, the reciprocal 2), a softmax's by 27 u (its argument 1 and its sum's
-// 20 adds and 2 more, the rest 4), the sum with the bias by u times itself.  Twice that,
-// rounded up.
-constexpr float SIGMOID_APART = 16 * 0x1p-24f, SOFTMAX_APART = 64 * 0x1p-24f;
+// 20 adds and 2 more, the rest 4; a lane of more than 16 experts adds up to 124), the sum
+// with the bias by u times itself.  Twice that, rounded up.
+constexpr float SIGMOID_APART = 16 * 0x1p-24f, SOFTMAX_APART = 64 * 0x1p-24f, SOFTMAX_APART_LONG = 288 * 0x1p-24f;
 
 // What a lane's share of a column is: `count` experts from `first` on.
 struct RouteShare { int lane, group, first, count; };
@@ -120,7 +120,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     constexpr K NONE = -INFINITY;
     const int of_group = 1 << a.lane_shift;
     const bool softmax = a.score == JLUST_SCORE_SOFTMAX;
-    const float apart = softmax ? SOFTMAX_APART : SIGMOID_APART;
+    const float apart = !softmax ? SIGMOID_APART : PER ? SOFTMAX_APART : SOFTMAX_APART_LONG;
     const A *bias = (const A *)a.bias;
     const uint64_t before = lanes_before<LANES>();
     bool unsure = false;

@@ -186,6 +186,19 @@ def test_route_sums_of_two_signs(J, T, score, cols):
         check_route(J, host.cuda().t(), copies, score=score, bias=bias.cuda(), groups=8, keep=keep, best=2)
 
 
+def test_route_long_sums(J):
+    """A softmax whose sum adds 123 terms of 0.9 u to 1 in turn (u = 2^-24, a group of 124
+    experts): the first score is 1 - 110 u, and with its bias behind another group's -80 u."""
+    u = 2.0 ** -24
+    host = torch.full((2, 33, 124), -40.0)
+    host[:, 0, 1:] = float(np.log(0.9 * u))
+    host[:, 0, 0] = 0
+    bias = torch.full((33, 124), -5.0)
+    bias[0, 0], bias[2, 7] = -1, -80 * u
+    ids, _ = check_route(J, host.view(2, -1).cuda().t(), 1, bias=bias.view(-1).cuda(), groups=33, keep=1, best=1)
+    assert (ids == 2 * 124 + 7 + 1).all()
+
+
 GRADS = [(1, 1), (5, 2), (64, 8), (160, 6), (255, 3), (513, 64), (4095, 9)]
 
 
