@@ -61,19 +61,22 @@ __device__ __forceinline__ uint64_t lanes_before()
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 
-// exp(l - top), 1 where both are the same infinity.
+// exp(l - top), 1 where both are the same infinity.  Made in any case, as the scores
+// below are, and dropped where it does not count: a branch a score took three times the
+// instructions of the scores.
 template <typename A>
 __device__ __forceinline__ A exp_below(A l, A top)
 {
-    return l == top ? A(1) : exp_of(l - top);
+    const A v = exp_of(l - top);
+    return l == top ? A(1) : v;
 }
 
 // The chosen experts' scores up to a factor that they share, from their logits: NP
-// each of LANES lanes (-inf: none).  Softmax: exp(l - m) with m the largest.  Sigmoid
+// each of LANES lanes, the first `parts` of which hold some (-inf: none).  Softmax: exp(l - m) with m the largest.  Sigmoid
 // renormalised: times exp(-m) with m the largest, 0 at most, so that scores below the
 // type's range keep their ratios; else as it is.
 template <int LANES, int NP, typename A>
-__device__ __forceinline__ void chosen_scores(int score, bool relative, const A (&l)[NP], A (&p)[NP])
+__device__ __forceinline__ void chosen_scores(int score, bool relative, int parts, const A (&l)[NP], A (&p)[NP])
 {
     A m = -INFINITY;
 #pragma unroll
@@ -82,11 +85,17 @@ __device__ __forceinline__ void chosen_scores(int score, bool relative, const A 
     if (score == JLUST_SCORE_SIGMOID) m = !relative || m > A(0) ? A(0) : m;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
+        p[q] = A(0);
+        if (q >= parts) continue;
         if (!(l[q] > A(-INFINITY))) p[q] = A(0);
         else if (score == JLUST_SCORE_SOFTMAX) p[q] = exp_below(l[q], m);
         else p[q] = l[q] > A(0) ? A(1) / (A(1) + exp_of(-l[q])) : exp_below(l[q], m) / (A(1) + exp_of(l[q]));
     }
 }
+
+// The middle one of three numbers.
+__device__ __forceinline__ float middle(float a, float b, float c) { return __builtin_amdgcn_fmed3f(a, b, c); }
+__device__ __forceinline__ double middle(double a, double b, double c) { return fmax(fmin(a, b), fmin(fmax(a, b), c)); }
 
 // How far apart two Float32 keys are in 64 bits for sure, over 1 + the larger: a
 // sigmoid's is off by 4 u (u = 2^-24: its exponential's argument 0.4, the exponential
@@ -159,43 +168,58 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
         top = S(m);
         if (bias) {
             S sum = 0;
-            each([&](int, K &k) { sum += k > NONE ? exp_below(S(k), top) : S(0); });
+            each([&](int, K &k) {
+                const S v = exp_below(S(k), top);
+                sum += k > NONE ? v : S(0);
+            });
             total = lanes_sum<LANES>(sum);
         } else {
             A sum = A(0);
-            each([&](int, K &k) { sum += k > NONE ? exp_below(A(k), A(m)) : A(0); });
+            each([&](int, K &k) {
+                const A v = exp_below(A(k), A(m));
+                sum += k > NONE ? v : A(0);
+            });
             total = S(lanes_sum<LANES>(sum));
         }
     }
     *top_ = (double)top;
     *total_ = (double)total;
-    auto score_of = [&](S l, S m, S all) {
+    auto part_of = [&](S l, S m, S all) {
         if constexpr (APPROX) {
-            if (softmax) return l == m ? 1 / all : __expf(l - m) / all;
-            return __builtin_amdgcn_rcpf(1 + __expf(-l));
+            const S v = __expf(l - m);
+            return (l == m ? S(1) : v) / all;
         } else {
-            return softmax ? exp_below(l, m) / all : 1 / (1 + exp(-l));
+            return exp_below(l, m) / all;
         }
     };
+    auto sigmoid = [&](S l) {
+        if constexpr (APPROX) return __builtin_amdgcn_rcpf(1 + __expf(-l));
+        else return 1 / (1 + exp(-l));
+    };
     if (bias) {
-        auto keyed = [&](K &k, A b) {
-            const K v = k > NONE ? K(score_of(S(k), top, total) + S(b)) : NONE;
-            k = v > NONE ? v : NONE;
-        };
-        if (PER > 0 && a.whole) {
-            A add[HELD] = {};
-            if (w.count) load_vec<HELD>(bias + w.first, add);
+        auto key_all = [&](auto &&score) {
+            auto keyed = [&](K &k, A b) {
+                K v = K(score(S(k)) + S(b));
+                v = k > NONE ? v : NONE;
+                k = Larger()(v, NONE);             // of NaN, NONE
+            };
+            if (PER > 0 && a.whole) {
+                A add[HELD] = {};
+                if (w.count) load_vec<HELD>(bias + w.first, add);
 #pragma unroll
-            for (int j = 0; j < PER; ++j) keyed(held[j], add[j]);
-        } else {
-            each([&](int j, K &k) { keyed(k, j < w.count ? bias[w.first + j] : A(0)); });
-        }
+                for (int j = 0; j < PER; ++j) keyed(held[j], add[j]);
+            } else {
+                each([&](int j, K &k) { keyed(k, j < w.count ? bias[w.first + j] : A(0)); });
+            }
+        };
+        if (softmax) key_all([&](S l) { return part_of(l, top, total); });
+        else key_all(sigmoid);
     }
     if (a.keep < a.groups) {
         K v1 = NONE, v2 = NONE;
         each([&](int, K &k) {
-            v2 = k > v1 ? v1 : k > v2 ? k : v2;
-            v1 = k > v1 ? k : v1;
+            v2 = middle(v1, v2, k);
+            v1 = Larger()(v1, k);
         });
         K rank, least;                             // least: the last key that its rank goes by
         float undone = 0;                          // what a rank's two keys have of each other's sign
@@ -223,8 +247,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             S x = S(m), y = S(rest);
             if (!bias) {
                 const S most = softmax ? S(lanes_max<LANES>(m)) : S(0);
-                x = m > NONE ? score_of(x, most, S(1)) : x;
-                y = rest > NONE ? score_of(y, most, S(1)) : y;
+                x = m > NONE ? softmax ? part_of(x, most, S(1)) : sigmoid(x) : x;
+                y = rest > NONE ? softmax ? part_of(y, most, S(1)) : sigmoid(y) : y;
             }
             const S sum = m > NONE ? x + (rest > NONE ? y : S(0)) : S(-INFINITY);
             rank = K(sum);
@@ -300,46 +324,45 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     bool close = false;                            // keys so near that their order may be another
     if constexpr (APPROX) {
         // Keys by whole numbers in their order, the expert's place in the last bits, where
-        // the larger is the earlier: a round takes a key out and finds the next best in three
-        // steps a key, seven with the places in registers of their own.
-        constexpr int PLACE = PER ? PER - 1 : 127, GONE = INT32_MIN;
+        // the larger is the earlier: a lane's are all different, and the next one after m is
+        // where m - 1 - k is the least, which for a key already taken wraps around to more
+        // than for any other: a subtraction and half a minimum a key and round.
+        constexpr uint32_t PLACE = PER ? PER - 1 : 127, GONE = 0, LIVE = 0x00800000;       // of -infinity, less
         const float near_by = apart + 4 * (PLACE + 1) * 0x1p-24f;      // and what the bits took from two keys
-        int packed[HELD];
-        auto flip = [](int b) { return b ^ (b >> 31 & INT32_MAX); };
+        uint32_t packed[HELD];
         auto pass = [&](auto &&f) {
             if constexpr (PER > 0) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) f(packed[j]);
             } else {
-                int *keys = (int *)lds + w.lane;
-                for (int j = 0; j < a.per; ++j) {
-                    int k = keys[j * 64];
-                    f(k);
-                    keys[j * 64] = k;
-                }
+                const uint32_t *keys = (const uint32_t *)lds + w.lane;
+                for (int j = 0; j < a.per; ++j) f(keys[j * 64]);
             }
         };
         each([&](int j, K &k) {
-            const int p = k > NONE ? (flip(__builtin_bit_cast(int, k)) & ~PLACE) | (PLACE - j) : GONE;
+            const int bits = __builtin_bit_cast(int, k);
+            const uint32_t p = (uint32_t)((bits ^ (bits >> 31 | INT32_MIN)) & ~PLACE) | (PLACE - j);
             if constexpr (PER > 0) packed[j] = p;
             else k = __builtin_bit_cast(float, p);
         });
-        int best = GONE;
-        pass([&](int &k) { best = k > best ? k : best; });
-        auto value = [&](int m) { return __builtin_bit_cast(float, flip(m & ~PLACE)); };
-        auto near = [&](float last, int m) { return m != GONE && !(last - value(m) > near_by * (1 + fabsf(last))); };
-        auto take = [&](int r, int m) {
-            chosen[r] = w.first + PLACE - (m & PLACE);
-            best = GONE;
-            pass([&](int &k) {
-                k = k == m ? GONE : k;
-                best = k > best ? k : best;
-            });
+        uint32_t best = GONE;
+        pass([&](uint32_t k) { best = k > best ? k : best; });
+        auto value = [&](uint32_t m) {
+            const int bits = (int)(m & ~PLACE);
+            return __builtin_bit_cast(float, bits ^ (~(bits >> 31) | INT32_MIN));
         };
-        int m = lanes_max<LANES>(best), last = GONE;
+        auto near = [&](float last, uint32_t m) { return m >= LIVE && !(last - value(m) > near_by * (1 + fabsf(last))); };
+        auto take = [&](int r, uint32_t m) {
+            chosen[r] = w.first + (int)(PLACE - (m & PLACE));
+            uint32_t least = UINT32_MAX;
+            pass([&](uint32_t k) { least = m - 1 - k < least ? m - 1 - k : least; });
+            best = m - 1 - least;
+            best = best < m ? best : GONE;
+        };
+        uint32_t m = lanes_max<LANES>(best), last = GONE;
         for (int r = 0; r < a.copies; ++r) {
-            found += m != GONE;
-            if (first_of(best == m && m != GONE, before)) take(r, m);
+            found += m >= LIVE;
+            if (first_of(best == m && m >= LIVE, before)) take(r, m);
             last = m;
             m = lanes_max<LANES>(best);
             close |= near(value(last), m);
@@ -422,68 +445,68 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4)
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, of_group = 1 << a.lane_shift;
     const int group = lane >> a.lane_shift, place = (lane & (of_group - 1)) * a.per;
     const bool softmax = a.score == JLUST_SCORE_SOFTMAX;
-    for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < a.cols; c0 += (int64_t)gridDim.x * COLS) {
-        const int64_t c = c0 + sub;
-        const T *L = (const T *)a.L + c * a.ldl;
-        int count = a.size - place < a.per ? a.size - place : a.per;
-        if (group >= a.groups || c >= a.cols || count < 0) count = 0;
-        const RouteShare w{lane, group, group * a.size + place, count};
-        double top, total;
-        if constexpr (!BIASED || sizeof(T) == 8) {
-            choose<T, A, false, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], nullptr, &top, &total);
-        } else {
-            const bool unsure = choose<T, float, true, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], s_exact[sub], &top, &total);
-            uint64_t open = __ballot(unsure && lane == 0);
-            // A wave takes each such column: its registers hold Float64 keys of four lanes.
-            while (open) {
-                const int at = __ffsll((unsigned long long)open) - 1, theirs = (threadIdx.x & ~63) / LANES + at / LANES;
-                open &= open - 1;
-                constexpr int WIDE = LANES == 64 ? PER : PER > 4 ? PER / 4 : 1;
-                RouteArgs b = a;
-                b.lane_shift += LANES == 64 ? 0 : 2;
-                b.per = (a.size + (1 << b.lane_shift) - 1) >> b.lane_shift;
-                b.whole = b.per == WIDE && a.size % b.per == 0;
-                const int mine = threadIdx.x & 63, g = mine >> b.lane_shift, from = (mine & ((1 << b.lane_shift) - 1)) * b.per;
-                int some = a.size - from < b.per ? a.size - from : b.per;
-                if (g >= a.groups || some < 0) some = 0;
-                double m, all;
-                wave_sync();
-                choose<T, double, false, 64, WIDE>(b, RouteShare{mine, g, g * a.size + from, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
-                                                   (char *)s_keys, s_chosen[theirs], nullptr, &m, &all);
-                if (sub == theirs) {
-                    top = m;
-                    total = all;
-                }
+    const int64_t c0 = (int64_t)blockIdx.x * COLS;
+    const int64_t c = c0 + sub;
+    const T *L = (const T *)a.L + c * a.ldl;
+    int count = a.size - place < a.per ? a.size - place : a.per;
+    if (group >= a.groups || c >= a.cols || count < 0) count = 0;
+    const RouteShare w{lane, group, group * a.size + place, count};
+    double top, total;
+    if constexpr (!BIASED || sizeof(T) == 8) {
+        choose<T, A, false, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], nullptr, &top, &total);
+    } else {
+        const bool unsure = choose<T, float, true, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], s_exact[sub], &top, &total);
+        uint64_t open = __ballot(unsure && lane == 0);
+        // A wave takes each such column: its registers hold Float64 keys of four lanes.
+        while (open) {
+            const int at = __ffsll((unsigned long long)open) - 1, theirs = (threadIdx.x & ~63) / LANES + at / LANES;
+            open &= open - 1;
+            constexpr int WIDE = LANES == 64 ? PER : PER > 4 ? PER / 4 : 1;
+            RouteArgs b = a;
+            b.lane_shift += LANES == 64 ? 0 : 2;
+            b.per = (a.size + (1 << b.lane_shift) - 1) >> b.lane_shift;
+            b.whole = b.per == WIDE && a.size % b.per == 0;
+            const int mine = threadIdx.x & 63, g = mine >> b.lane_shift, from = (mine & ((1 << b.lane_shift) - 1)) * b.per;
+            int some = a.size - from < b.per ? a.size - from : b.per;
+            if (g >= a.groups || some < 0) some = 0;
+            double m, all;
+            wave_sync();
+            choose<T, double, false, 64, WIDE>(b, RouteShare{mine, g, g * a.size + from, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
+                                               (char *)s_keys, s_chosen[theirs], nullptr, &m, &all);
+            if (sub == theirs) {
+                top = m;
+                total = all;
             }
         }
-        wave_sync();
-        A l[NP], p[NP];
-        int e[NP];
+    }
+    wave_sync();
+    A l[NP], p[NP];
+    int e[NP];
+    const int parts = (a.copies + LANES - 1) / LANES;
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-            const int i = lane + q * LANES;
-            e[q] = i < a.copies && c < a.cols ? s_chosen[sub][i] : -1;
-            l[q] = e[q] >= 0 ? A(L[e[q]]) : A(-INFINITY);
-        }
-        wave_sync();
-        A sum = A(0);
-        if (softmax && !a.renormalize) {
+    for (int q = 0; q < NP; ++q) {
+        const int i = lane + q * LANES;
+        e[q] = i < a.copies && c < a.cols ? s_chosen[sub][i] : -1;
+        l[q] = e[q] >= 0 ? A(L[e[q]]) : A(-INFINITY);
+    }
+    wave_sync();
+    A sum = A(0);
+    if (softmax && !a.renormalize) {
 #pragma unroll
-            for (int q = 0; q < NP; ++q) p[q] = e[q] >= 0 ? exp_below(l[q], A(top)) / A(total) : A(0);
-        } else {
-            chosen_scores<LANES>(a.score, a.renormalize, l, p);
-        }
+        for (int q = 0; q < NP; ++q) p[q] = e[q] >= 0 ? exp_below(l[q], A(top)) / A(total) : A(0);
+    } else {
+        chosen_scores<LANES>(a.score, a.renormalize, parts, l, p);
+    }
 #pragma unroll
-        for (int q = 0; q < NP; ++q) sum += p[q];
-        sum = a.renormalize ? lanes_sum<LANES>(sum) : A(1);
-        if (c >= a.cols) continue;
+    for (int q = 0; q < NP; ++q) sum += p[q];
+    sum = a.renormalize ? lanes_sum<LANES>(sum) : A(1);
+    if (c >= a.cols) return;
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-            const int i = lane + q * LANES;
-            if (i >= a.copies) continue;
-            a.ids[c * a.ldi + i] = e[q] + a.origin;
-            ((A *)a.weights)[c * a.ldw + i] = e[q] >= 0 ? A(a.scale) * (p[q] / sum) : A(0);
-        }
+    for (int q = 0; q < NP; ++q) {
+        const int i = lane + q * LANES;
+        if (q >= parts || i >= a.copies) continue;
+        a.ids[c * a.ldi + i] = e[q] + a.origin;
+        ((A *)a.weights)[c * a.ldw + i] = e[q] >= 0 ? A(a.scale) * (p[q] / sum) : A(0);
     }
 }
 
@@ -507,8 +530,12 @@ struct RouteGradArgs {
 template <typename T, typename A>
 __device__ __forceinline__ A score_below(A l, A top)
 {
-    if constexpr (sizeof(T) == 2) return l == top ? A(1) : __expf(l - top);
-    else return exp_below(l, top);
+    if constexpr (sizeof(T) == 2) {
+        const A v = __expf(l - top);
+        return l == top ? A(1) : v;
+    } else {
+        return exp_below(l, top);
+    }
 }
 
 // With t = scale dw and p the weights' shares of the chosen: softmax renormalised
@@ -526,122 +553,122 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
     __shared__ A s_part[COLS][MAX_COPIES];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const bool softmax = a.score == JLUST_SCORE_SOFTMAX, dense = softmax && !a.renormalize;
-    for (int64_t c0 = (int64_t)blockIdx.x * COLS; c0 < a.cols; c0 += (int64_t)gridDim.x * COLS) {
-        const int64_t c = c0 + sub;
-        const bool live = c < a.cols;
-        const T *L = (const T *)a.L + c * a.ldl;
-        A top = -INFINITY, total = A(0), s[HELD][CH];
-        if (CPL > 0 && dense) {
-            uint32x4 raw[HELD];
+    const int64_t c0 = (int64_t)blockIdx.x * COLS;
+    const int64_t c = c0 + sub;
+    const bool live = c < a.cols;
+    const T *L = (const T *)a.L + c * a.ldl;
+    A top = -INFINITY, total = A(0), s[HELD][CH];
+    if (CPL > 0 && dense) {
+        uint32x4 raw[HELD];
 #pragma unroll
-            for (int i = 0; i < CPL; ++i)
-                raw[i] = read_at<WHOLE>((const T *)a.L + (live ? c : a.cols - 1) * a.ldl, (lane + LANES * i) * CH, a.experts);
+        for (int i = 0; i < CPL; ++i)
+            raw[i] = read_at<WHOLE>((const T *)a.L + (live ? c : a.cols - 1) * a.ldl, (lane + LANES * i) * CH, a.experts);
 #pragma unroll
-            for (int i = 0; i < CPL; ++i) {
-                values<T>(raw[i], s[i]);
+        for (int i = 0; i < CPL; ++i) {
+            values<T>(raw[i], s[i]);
 #pragma unroll
-                for (int j = 0; j < CH; ++j) {
-                    const bool some = (lane + LANES * i) * CH + (WHOLE ? 0 : j) < a.experts && s[i][j] > A(-INFINITY);
-                    s[i][j] = some ? s[i][j] : A(-INFINITY);
-                    top = s[i][j] > top ? s[i][j] : top;
-                }
-            }
-            top = lanes_max<LANES>(top);
-#pragma unroll
-            for (int i = 0; i < CPL; ++i)
-#pragma unroll
-                for (int j = 0; j < CH; ++j) {
-                    s[i][j] = s[i][j] > A(-INFINITY) ? score_below<T>(s[i][j], top) : A(0);
-                    total += s[i][j];
-                }
-            total = lanes_sum<LANES>(total);
-        } else if (dense) {
-            if (live)
-                for (int e = lane; e < a.experts; e += LANES) top = A(L[e]) > top ? A(L[e]) : top;
-            top = lanes_max<LANES>(top);
-            if (live)
-                for (int e = lane; e < a.experts; e += LANES)
-                    if (A(L[e]) > A(-INFINITY)) total += score_below<T>(A(L[e]), top);
-            total = lanes_sum<LANES>(total);
-        }
-        A l[NP], t[NP], p[NP];
-        int at[NP];
-#pragma unroll
-        for (int q = 0; q < NP; ++q) {
-            const int i = lane + q * LANES;
-            at[q] = -1;
-            l[q] = -INFINITY;
-            t[q] = A(0);
-            if (live && i < a.copies) {
-                const int64_t e = (int64_t)a.ids[c * a.ldi + i] - a.origin;
-                if (e >= 0 && e < a.experts) {
-                    at[q] = (int)e;
-                    l[q] = A(L[e]);
-                    t[q] = A(a.scale) * ((const A *)a.dw)[c * a.lddw + i];
-                }
+            for (int j = 0; j < CH; ++j) {
+                const bool some = (lane + LANES * i) * CH + (WHOLE ? 0 : j) < a.experts && s[i][j] > A(-INFINITY);
+                s[i][j] = some ? s[i][j] : A(-INFINITY);
+                top = s[i][j] > top ? s[i][j] : top;
             }
         }
-        A sum = A(0), dot = A(0);
-        if (dense) {
+        top = lanes_max<LANES>(top);
 #pragma unroll
-            for (int q = 0; q < NP; ++q) p[q] = l[q] > A(-INFINITY) ? exp_below(l[q], top) / total : A(0);
-        } else {
-            chosen_scores<LANES>(a.score, a.renormalize, l, p);
-            if (a.renormalize) {
+        for (int i = 0; i < CPL; ++i)
 #pragma unroll
-                for (int q = 0; q < NP; ++q) sum += p[q];
-                sum = lanes_sum<LANES>(sum);
+            for (int j = 0; j < CH; ++j) {
+                const A v = score_below<T>(s[i][j], top);
+                s[i][j] = s[i][j] > A(-INFINITY) ? v : A(0);
+                total += s[i][j];
+            }
+        total = lanes_sum<LANES>(total);
+    } else if (dense) {
+        if (live)
+            for (int e = lane; e < a.experts; e += LANES) top = A(L[e]) > top ? A(L[e]) : top;
+        top = lanes_max<LANES>(top);
+        if (live)
+            for (int e = lane; e < a.experts; e += LANES)
+                if (A(L[e]) > A(-INFINITY)) total += score_below<T>(A(L[e]), top);
+        total = lanes_sum<LANES>(total);
+    }
+    A l[NP], t[NP], p[NP];
+    int at[NP];
+    const int parts = (a.copies + LANES - 1) / LANES;
 #pragma unroll
-                for (int q = 0; q < NP; ++q) p[q] = p[q] > A(0) ? p[q] / sum : A(0);
+    for (int q = 0; q < NP; ++q) {
+        const int i = lane + q * LANES;
+        at[q] = -1;
+        l[q] = -INFINITY;
+        t[q] = A(0);
+        if (q < parts && live && i < a.copies) {
+            const int64_t e = (int64_t)a.ids[c * a.ldi + i] - a.origin;
+            if (e >= 0 && e < a.experts) {
+                at[q] = (int)e;
+                l[q] = A(L[e]);
+                t[q] = A(a.scale) * ((const A *)a.dw)[c * a.lddw + i];
             }
         }
-        if (softmax || a.renormalize) {
+    }
+    A sum = A(0), dot = A(0);
+    if (dense) {
 #pragma unroll
-            for (int q = 0; q < NP; ++q) dot += p[q] * t[q];
-            dot = lanes_sum<LANES>(dot);
+        for (int q = 0; q < NP; ++q) p[q] = q < parts && l[q] > A(-INFINITY) ? exp_below(l[q], top) / total : A(0);
+    } else {
+        chosen_scores<LANES>(a.score, a.renormalize, parts, l, p);
+        if (a.renormalize) {
+#pragma unroll
+            for (int q = 0; q < NP; ++q) sum += p[q];
+            sum = lanes_sum<LANES>(sum);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) p[q] = q < parts && p[q] > A(0) ? p[q] / sum : A(0);
         }
+    }
+    if (softmax || a.renormalize) {
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-            const int i = lane + q * LANES;
-            if (i >= a.copies) continue;
-            A g = dense ? t[q] : p[q] * (t[q] - dot);
-            if (!softmax) g *= A(1) / (A(1) + exp_of(l[q]));
-            s_expert[sub][i] = at[q];
-            s_part[sub][i] = at[q] >= 0 ? g : A(0);
-        }
-        wave_sync();
-        if constexpr (CPL > 0) {
-            const A inv = total > A(0) ? A(1) / total : A(0);
+        for (int q = 0; q < NP; ++q) dot += p[q] * t[q];
+        dot = lanes_sum<LANES>(dot);
+    }
 #pragma unroll
-            for (int i = 0; i < CPL; ++i) {
-                const int at = (lane + LANES * i) * CH;
-                A g[CH];
+    for (int q = 0; q < NP; ++q) {
+        const int i = lane + q * LANES;
+        if (q >= parts || i >= a.copies) continue;
+        A g = dense ? t[q] : p[q] * (t[q] - dot);
+        if (!softmax) g *= A(1) / (A(1) + exp_of(l[q]));
+        s_expert[sub][i] = at[q];
+        s_part[sub][i] = at[q] >= 0 ? g : A(0);
+    }
+    wave_sync();
+    if constexpr (CPL > 0) {
+        const A inv = total > A(0) ? A(1) / total : A(0);
 #pragma unroll
-                for (int j = 0; j < CH; ++j) g[j] = A(0);
-                for (int k = 0; k < a.copies; ++k) {
-                    const int e = s_expert[sub][k] - at;
-                    const A v = s_part[sub][k];
+        for (int i = 0; i < CPL; ++i) {
+            const int at = (lane + LANES * i) * CH;
+            A g[CH];
 #pragma unroll
-                    for (int j = 0; j < CH; ++j) g[j] += e == j ? v : A(0);
-                }
-                if (dense) {
+            for (int j = 0; j < CH; ++j) g[j] = A(0);
+            for (int k = 0; k < a.copies; ++k) {
+                const int e = s_expert[sub][k] - at;
+                const A v = s_part[sub][k];
 #pragma unroll
-                    for (int j = 0; j < CH; ++j) g[j] = s[i][j] * inv * (g[j] - dot);
-                }
-                if (live) write_at<WHOLE>((T *)a.dL + c * a.lddl, at, a.experts, g);
+                for (int j = 0; j < CH; ++j) g[j] += e == j ? v : A(0);
             }
-        } else if (live) {
-            for (int e = lane; e < a.experts; e += LANES) {
-                A g = A(0);
-                for (int i = 0; i < a.copies; ++i) g += s_expert[sub][i] == e ? s_part[sub][i] : A(0);
-                if (dense) {
-                    const A v = A(L[e]);
-                    g = v > A(-INFINITY) ? score_below<T>(v, top) / total * (g - dot) : A(0);
-                }
-                ((T *)a.dL)[c * a.lddl + e] = T(g);
+            if (dense) {
+#pragma unroll
+                for (int j = 0; j < CH; ++j) g[j] = s[i][j] * inv * (g[j] - dot);
             }
+            if (live) write_at<WHOLE>((T *)a.dL + c * a.lddl, at, a.experts, g);
         }
-        wave_sync();
+    } else if (live) {
+        for (int e = lane; e < a.experts; e += LANES) {
+            A g = A(0);
+            for (int i = 0; i < a.copies; ++i) g += s_expert[sub][i] == e ? s_part[sub][i] : A(0);
+            if (dense) {
+                const A v = A(L[e]);
+                g = v > A(-INFINITY) ? score_below<T>(v, top) / total * (g - dot) : A(0);
+            }
+            ((T *)a.dL)[c * a.lddl + e] = T(g);
+        }
     }
 }
 
@@ -658,14 +685,40 @@ bool route_lanes(int lanes, RouteArgs *a)
     return true;
 }
 
+// launch(a, blocks) for the columns of `a`, `each` a workgroup: a workgroup that walked
+// over several would hold what it asks of its arguments in registers over the walk
+// (16,384 columns of 256 experts in 8 groups: 18.0 us and 13.6), so past the columns of
+// 2^21 workgroups another launch follows.
+template <typename T, typename Args, typename F>
+int by_launches(Args a, int64_t each, F &&launch)
+{
+    using A = typename Elem<T>::Acc;
+    const int64_t most = ((int64_t)1 << 21) * each, cols = a.cols;
+    for (int64_t c = 0; c < cols; c += most) {
+        a.cols = cols - c < most ? cols - c : most;
+        if (int st = launch(a, (unsigned)((a.cols + each - 1) / each))) return st;
+        a.L = (const T *)a.L + most * a.ldl;
+        a.ids += most * a.ldi;
+        if constexpr (std::is_same_v<Args, RouteArgs>) {
+            a.weights = (A *)a.weights + most * a.ldw;
+        } else {
+            a.dw = (const A *)a.dw + most * a.lddw;
+            a.dL = (T *)a.dL + most * a.lddl;
+        }
+    }
+    return JLUST_STATUS_SUCCESS;
+}
+
 template <typename T, bool BIASED, int LANES, int PER>
 int launch_route(RouteArgs a, hipStream_t s)
 {
     constexpr int NT = PER ? 256 : 64;
     a.whole = a.per == PER && a.size % (PER ? PER : 1) == 0;
-    hipLaunchKernelGGL((route_kernel<T, BIASED, LANES, PER>), dim3(column_blocks(a.cols, NT / LANES)), dim3(NT),
-                       PER ? 0 : (BIASED ? sizeof(double) : sizeof(typename Elem<T>::Acc)) * 64 * a.per, s, a);
-    return check_launch("route_kernel");
+    return by_launches<T>(a, NT / LANES, [&](const RouteArgs &some, unsigned blocks) {
+        hipLaunchKernelGGL((route_kernel<T, BIASED, LANES, PER>), dim3(blocks), dim3(NT),
+                           PER ? 0 : (BIASED ? sizeof(double) : sizeof(typename Elem<T>::Acc)) * 64 * a.per, s, some);
+        return check_launch("route_kernel");
+    });
 }
 
 // 16 lanes a column where it fits them and the columns fill the CUs (a round of the
@@ -789,8 +842,10 @@ extern "C" int jlust_hip_route_grad(const jlust_route_grad *op, jlust_stream_t s
         using T = decltype(t);
         const int64_t chunks = (a.experts * (int64_t)sizeof(T) + 15) / 16;
         auto launch = [&](auto kernel, int lanes) {
-            hipLaunchKernelGGL(kernel, dim3(column_blocks(a.cols, 256 / lanes)), dim3(256), 0, (hipStream_t)stream, a);
-            return check_launch("route_grad_kernel");
+            return by_launches<T>(a, 256 / lanes, [&](const RouteGradArgs &some, unsigned blocks) {
+                hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, some);
+                return check_launch("route_grad_kernel");
+            });
         };
         auto go = [&](auto whole) {
             constexpr bool W = decltype(whole)::value;

@@ -199,6 +199,23 @@ def test_route_long_sums(J):
     assert (ids == 2 * 124 + 7 + 1).all()
 
 
+def test_route_past_one_launch(J):
+    """More columns than 2^21 workgroups take: two experts, so that the choice is a comparison
+    and the weight a logistic, and the gradient p (1 - p) (dw) with p the chosen one's share."""
+    cols = (1 << 25) + 37
+    logits = torch.randn((cols, 2), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).t()
+    ids, w = torch.empty(cols, dtype=torch.int32, device="cuda"), torch.empty(cols, device="cuda")
+    J.execute(J.RouteOp, logits, ids, w, renormalize=False)
+    assert torch.equal(ids, (logits[1] > logits[0]).int() + 1)
+    p = torch.sigmoid((logits[0].double() - logits[1]).abs())
+    u = (16 + 4 * 14 + 2) * 2.0 ** -24             # E.weight_bound of logits within 7
+    assert ((w - p).abs() <= u * p).all()
+    dL = torch.empty_like(logits)
+    J.execute(J.RouteGradOp, logits, ids, torch.ones_like(w), dL, renormalize=False)
+    g = torch.where(ids == 1, p * (1 - p), -p * (1 - p))
+    assert ((dL[0] - g).abs() <= 4 * u * p).all() and ((dL[1] + g).abs() <= 4 * u * p).all()     # terms of p and p * p, twice as in test_route_grad
+
+
 GRADS = [(1, 1), (5, 2), (64, 8), (160, 6), (255, 3), (513, 64), (4095, 9)]
 
 
