@@ -104,7 +104,8 @@ __device__ __forceinline__ double middle(double a, double b, double c) { return 
 // with the bias by u times itself.  Twice that, rounded up.
 constexpr float SIGMOID_APART = 16 * 0x1p-24f, SOFTMAX_APART = 64 * 0x1p-24f, SOFTMAX_APART_LONG = 288 * 0x1p-24f;
 
-// What a lane's share of a column is: `count` experts from `first` on.
+// What a lane's share of a column is: `count` experts from `first` on; of none `first` is
+// 0, which may be read: a branch around every read waits for the read before.
 struct RouteShare { int lane, group, first, count; };
 
 constexpr int MAX_CANDIDATES = MAX_COPIES + 16;
@@ -149,14 +150,14 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
         }
     };
     if (PER > 0 && a.whole) {
-        T raw[HELD] = {};
-        if (w.count) load_vec<HELD>(L + w.first, raw);
+        T raw[HELD];
+        load_vec<HELD>(L + w.first, raw);
 #pragma unroll
         for (int j = 0; j < PER; ++j) held[j] = w.count && A(raw[j]) > A(-INFINITY) ? K(A(raw[j])) : NONE;
     } else {
         each([&](int j, K &k) {
-            const K l = j < w.count ? K(A(L[w.first + j])) : NONE;
-            k = l > NONE ? l : NONE;
+            const A l = A(L[w.first + (j < w.count ? j : 0)]);
+            k = j < w.count && l > A(-INFINITY) ? K(l) : NONE;
         });
     }
     // Softmax's sum is needed where scores are compared or left as they are.
@@ -204,12 +205,12 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
                 k = Larger()(v, NONE);             // of NaN, NONE
             };
             if (PER > 0 && a.whole) {
-                A add[HELD] = {};
-                if (w.count) load_vec<HELD>(bias + w.first, add);
+                A add[HELD];
+                load_vec<HELD>(bias + w.first, add);
 #pragma unroll
                 for (int j = 0; j < PER; ++j) keyed(held[j], add[j]);
             } else {
-                each([&](int j, K &k) { keyed(k, j < w.count ? bias[w.first + j] : A(0)); });
+                each([&](int j, K &k) { keyed(k, bias[w.first + (j < w.count ? j : 0)]); });
             }
         };
         if (softmax) key_all([&](S l) { return part_of(l, top, total); });
@@ -221,7 +222,9 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             v2 = middle(v1, v2, k);
             v1 = Larger()(v1, k);
         });
-        K rank, least;                             // least: the last key that its rank goes by
+        using R = std::conditional_t<APPROX, K, S>;    // sums are compared in 64 bits
+        R rank;
+        K least;                                   // the last key that its rank goes by
         float undone = 0;                          // what a rank's two keys have of each other's sign
         const int first_in_wave = threadIdx.x & 63 & ~(LANES - 1);
         const uint64_t column = (LANES < 64 ? (1ull << (LANES & 63)) - 1 : ~0ull) << first_in_wave;
@@ -239,7 +242,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             return mask != 0 && (__ffsll((unsigned long long)mask) - 1 - first_in_wave) >> a.lane_shift == w.group;
         };
         if (a.best == 1) {
-            rank = least = over_lanes<LANES>(v1, Larger(), of_group);
+            least = over_lanes<LANES>(v1, Larger(), of_group);
+            rank = R(least);
         } else {
             best_two(v1, v2);
             const K m = v1, rest = v2;
@@ -251,25 +255,16 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
                 y = rest > NONE ? softmax ? part_of(y, most, S(1)) : sigmoid(y) : y;
             }
             const S sum = m > NONE ? x + (rest > NONE ? y : S(0)) : S(-INFINITY);
-            rank = K(sum);
+            rank = sum;
             if constexpr (APPROX) undone = rest > NONE && y < 0 && x > 0 ? -2 * y : 0;
-            if constexpr (sizeof(K) < sizeof(S)) {
-                // Sums are compared in 64 bits: each group's place among them instead.
-                int above = 0;
-                for (int g = 0; g < a.groups; ++g) {
-                    const S o = __shfl(sum, (threadIdx.x & 63 & ~(LANES - 1)) + (g << a.lane_shift), 64);
-                    above += o > sum || (o == sum && g < w.group);
-                }
-                rank = m > NONE ? K(-above) : NONE;
-            }
         }
         bool kept = false;
-        K last = NONE, left = rank;
+        R last = -INFINITY, left = rank;
         for (int r = 0; r < a.keep; ++r) {
             last = lanes_max<LANES>(left);
             if (wins(left, last)) {
                 kept = true;
-                left = NONE;
+                left = -INFINITY;
             }
         }
         if constexpr (APPROX) {
@@ -447,10 +442,10 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4)
     const bool softmax = a.score == JLUST_SCORE_SOFTMAX;
     const int64_t c0 = (int64_t)blockIdx.x * COLS;
     const int64_t c = c0 + sub;
-    const T *L = (const T *)a.L + c * a.ldl;
+    const T *L = (const T *)a.L + (c < a.cols ? c : a.cols - 1) * a.ldl;
     int count = a.size - place < a.per ? a.size - place : a.per;
     if (group >= a.groups || c >= a.cols || count < 0) count = 0;
-    const RouteShare w{lane, group, group * a.size + place, count};
+    const RouteShare w{lane, group, count ? group * a.size + place : 0, count};
     double top, total;
     if constexpr (!BIASED || sizeof(T) == 8) {
         choose<T, A, false, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], nullptr, &top, &total);
@@ -471,7 +466,7 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4)
             if (g >= a.groups || some < 0) some = 0;
             double m, all;
             wave_sync();
-            choose<T, double, false, 64, WIDE>(b, RouteShare{mine, g, g * a.size + from, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
+            choose<T, double, false, 64, WIDE>(b, RouteShare{mine, g, some ? g * a.size + from : 0, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
                                                (char *)s_keys, s_chosen[theirs], nullptr, &m, &all);
             if (sub == theirs) {
                 top = m;
