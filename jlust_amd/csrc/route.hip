@@ -115,17 +115,19 @@ constexpr int MAX_CANDIDATES = MAX_COPIES + 16;
 // `1 << lane_shift` of them a group, PER experts at most each (0: any number, their keys
 // in LDS): a lane's experts and then the lanes' are in the experts' order, so the first
 // lane with the best key holds the lowest expert that has it.  K: the keys' type.
-// APPROX: Float32 keys of scores that belong to Float64.  What they leave open, which
-// groups are the last kept and the order of the experts, goes by the sigmoids in Float64
+// APPROX: Float32 keys, with a bias of scores that belong to Float64, without one the
+// logits, whose last bits the rounds do without.  What they leave open, which groups are
+// the last kept and the order of the experts, goes by the sigmoids (or logits) in Float64
 // of those few that are near enough (`exact`: theirs); true where that does not settle it
-// (more than 16 experts as near to the last one chosen, or softmax, whose Float64 sum takes
-// them all).
-template <typename T, typename K, bool APPROX, int LANES, int PER>
+// (more than 16 experts as near to the last one chosen, or softmax with a bias, whose
+// Float64 sum takes them all).
+template <typename T, typename K, bool APPROX, bool BIASED, int LANES, int PER>
 __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, const T *L, char *lds, int *chosen, double *exact,
                                        double *top_, double *total_)
 {
     using A = typename Elem<T>::Acc;
-    using S = std::conditional_t<APPROX, float, double>;                // the scores' type
+    constexpr bool ROUGH = APPROX && BIASED;
+    using S = std::conditional_t<ROUGH, float, double>;                 // the scores' type
     constexpr int HELD = PER ? PER : 1;
     constexpr K NONE = -INFINITY;
     const int of_group = 1 << a.lane_shift;
@@ -162,12 +164,12 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     }
     // Softmax's sum is needed where scores are compared or left as they are.
     S top = -INFINITY, total = 1;
-    if (softmax && (bias || !a.renormalize)) {
+    if (softmax && (BIASED || !a.renormalize)) {
         K m = NONE;
         each([&](int, K &k) { m = k > m ? k : m; });
         m = lanes_max<LANES>(m);
         top = S(m);
-        if (bias) {
+        if (BIASED) {
             S sum = 0;
             each([&](int, K &k) {
                 const S v = exp_below(S(k), top);
@@ -186,7 +188,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     *top_ = (double)top;
     *total_ = (double)total;
     auto part_of = [&](S l, S m, S all) {
-        if constexpr (APPROX) {
+        if constexpr (ROUGH) {
             const S v = __expf(l - m);
             return (l == m ? S(1) : v) / all;
         } else {
@@ -194,10 +196,10 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
         }
     };
     auto sigmoid = [&](S l) {
-        if constexpr (APPROX) return __builtin_amdgcn_rcpf(1 + __expf(-l));
+        if constexpr (ROUGH) return __builtin_amdgcn_rcpf(1 + __expf(-l));
         else return 1 / (1 + exp(-l));
     };
-    if (bias) {
+    if constexpr (BIASED) {
         auto key_all = [&](auto &&score) {
             auto keyed = [&](K &k, A b) {
                 K v = K(score(S(k)) + S(b));
@@ -222,7 +224,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             v2 = middle(v1, v2, k);
             v1 = Larger()(v1, k);
         });
-        using R = std::conditional_t<APPROX, K, S>;    // sums are compared in 64 bits
+        using R = std::conditional_t<ROUGH, K, S>;    // sums are compared in 64 bits
         R rank;
         K least;                                   // the last key that its rank goes by
         float undone = 0;                          // what a rank's two keys have of each other's sign
@@ -249,14 +251,14 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             const K m = v1, rest = v2;
             least = rest > NONE ? rest : m;
             S x = S(m), y = S(rest);
-            if (!bias) {
+            if (!BIASED) {
                 const S most = softmax ? S(lanes_max<LANES>(m)) : S(0);
                 x = m > NONE ? softmax ? part_of(x, most, S(1)) : sigmoid(x) : x;
                 y = rest > NONE ? softmax ? part_of(y, most, S(1)) : sigmoid(y) : y;
             }
             const S sum = m > NONE ? x + (rest > NONE ? y : S(0)) : S(-INFINITY);
             rank = sum;
-            if constexpr (APPROX) undone = rest > NONE && y < 0 && x > 0 ? -2 * y : 0;
+            if constexpr (ROUGH) undone = rest > NONE && y < 0 && x > 0 ? -2 * y : 0;
         }
         bool kept = false;
         R last = -INFINITY, left = rank;
@@ -267,7 +269,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
                 left = -INFINITY;
             }
         }
-        if constexpr (APPROX) {
+        if constexpr (ROUGH) {
             const K next = lanes_max<LANES>(left);
             // Keys of two signs make a sum smaller than they are: their error is not.
             if (__ballot(undone > 0)) undone = lanes_max<LANES>(undone);
@@ -317,12 +319,16 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     wave_sync();
     int found = 0;
     bool close = false;                            // keys so near that their order may be another
-    if constexpr (APPROX) {
+    if constexpr (sizeof(K) == 4) {
         // Keys by whole numbers in their order, the expert's place in the last bits, where
         // the larger is the earlier: a lane's are all different, and the next one after m is
         // where m - 1 - k is the least, which for a key already taken wraps around to more
-        // than for any other: a subtraction and half a minimum a key and round.
-        constexpr uint32_t PLACE = PER ? PER - 1 : 127, GONE = 0, LIVE = 0x00800000;       // of -infinity, less
+        // than for any other: a subtraction and half a minimum a key and round.  16-bit
+        // logits leave the last 13 bits free, which hold the expert's number: equal ones are
+        // in order over all lanes.
+        constexpr bool FREE = !APPROX;
+        constexpr uint32_t PLACE = FREE ? 4095 : PER ? PER - 1 : 127, GONE = 0, LIVE = 0x00800000;        // of -infinity, less
+        static_assert(MAX_EXPERTS <= 4095, "a number in 12 bits");
         const float near_by = apart + 4 * (PLACE + 1) * 0x1p-24f;      // and what the bits took from two keys
         uint32_t packed[HELD];
         auto pass = [&](auto &&f) {
@@ -335,8 +341,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             }
         };
         each([&](int j, K &k) {
-            const int bits = __builtin_bit_cast(int, k);
-            const uint32_t p = (uint32_t)((bits ^ (bits >> 31 | INT32_MIN)) & ~PLACE) | (PLACE - j);
+            const int bits = __builtin_bit_cast(int, ROUGH ? k : k + K(0));        // -0 is 0, as near as it gets
+            const uint32_t p = (uint32_t)((bits ^ (bits >> 31 | INT32_MIN)) & ~PLACE) + (PLACE - j - (FREE ? w.first : 0));
             if constexpr (PER > 0) packed[j] = p;
             else k = __builtin_bit_cast(float, p);
         });
@@ -346,9 +352,16 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             const int bits = (int)(m & ~PLACE);
             return __builtin_bit_cast(float, bits ^ (~(bits >> 31) | INT32_MIN));
         };
-        auto near = [&](float last, uint32_t m) { return m >= LIVE && !(last - value(m) > near_by * (1 + fabsf(last))); };
+        auto near = [&](uint32_t last, uint32_t m) {
+            if constexpr (ROUGH) {
+                const float v = value(last);
+                return m >= LIVE && !(v - value(m) > near_by * (1 + fabsf(v)));
+            } else {
+                return APPROX && m >= LIVE && (m | PLACE) == (last | PLACE);
+            }
+        };
         auto take = [&](int r, uint32_t m) {
-            chosen[r] = w.first + (int)(PLACE - (m & PLACE));
+            chosen[r] = (FREE ? 0 : w.first) + (int)(PLACE - (m & PLACE));
             uint32_t least = UINT32_MAX;
             pass([&](uint32_t k) { least = m - 1 - k < least ? m - 1 - k : least; });
             best = m - 1 - least;
@@ -360,12 +373,12 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             if (first_of(best == m && m >= LIVE, before)) take(r, m);
             last = m;
             m = lanes_max<LANES>(best);
-            close |= near(value(last), m);
+            close |= near(last, m);
         }
         // Past the last one asked for: those as near to it.
-        if (__ballot(close) && !softmax)
+        if (APPROX && __ballot(close) && !(ROUGH && softmax))
             for (int r = a.copies;; ++r) {
-                const bool more = near(value(last), m);
+                const bool more = near(last, m);
                 if (__ballot(more) == 0) break;
                 if (r == slots) {
                     unsure |= more;
@@ -402,13 +415,13 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
         }
     }
     if constexpr (APPROX) {
-        if (softmax) return unsure || close;
+        if (ROUGH && softmax) return unsure || close;
         // The experts' order in 64 bits: one's place is how many come before it.
         if (__ballot(close)) {
             wave_sync();
 #pragma unroll 1
             for (int i = w.lane; i < found; i += LANES)
-                exact[i] = 1 / (1 + exp(-(double)A(L[chosen[i]]))) + (double)bias[chosen[i]];
+                exact[i] = ROUGH ? 1 / (1 + exp(-(double)A(L[chosen[i]]))) + (double)bias[chosen[i]] : (double)A(L[chosen[i]]);
             wave_sync();
             int *order = (int *)(exact + MAX_CANDIDATES);
 #pragma unroll 1
@@ -427,15 +440,17 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     return unsure;
 }
 
-// BIASED: keys are scores plus biases, Float64; of other logits than Float64 they are
-// made in Float32 first, and again in Float64 for a column that is not settled by those.
+// BIASED: keys are scores plus biases, Float64, else the logits.  But for 16-bit and
+// Float64 logits they are made in Float32 first, and again in Float64 for a column that is
+// not settled by those.
 template <typename T, bool BIASED, int LANES, int PER>
 __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4) void route_kernel(const RouteArgs a)
 {
     using A = typename Elem<T>::Acc;
     constexpr int NT = PER ? 256 : 64, COLS = NT / LANES, NP = MAX_COPIES / LANES;
     __shared__ int s_chosen[COLS][MAX_CANDIDATES];
-    __shared__ double s_exact[BIASED && sizeof(T) < 8 ? COLS : 1][MAX_CANDIDATES * 3 / 2];
+    constexpr bool APPROX = BIASED ? sizeof(T) < 8 : sizeof(T) == 4;
+    __shared__ double s_exact[APPROX ? COLS : 1][MAX_CANDIDATES * 3 / 2];
     extern __shared__ double s_keys[];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, of_group = 1 << a.lane_shift;
     const int group = lane >> a.lane_shift, place = (lane & (of_group - 1)) * a.per;
@@ -447,10 +462,10 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4)
     if (group >= a.groups || c >= a.cols || count < 0) count = 0;
     const RouteShare w{lane, group, count ? group * a.size + place : 0, count};
     double top, total;
-    if constexpr (!BIASED || sizeof(T) == 8) {
-        choose<T, A, false, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], nullptr, &top, &total);
+    if constexpr (!APPROX) {
+        choose<T, A, false, BIASED, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], nullptr, &top, &total);
     } else {
-        const bool unsure = choose<T, float, true, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], s_exact[sub], &top, &total);
+        const bool unsure = choose<T, float, true, BIASED, LANES, PER>(a, w, L, (char *)s_keys, s_chosen[sub], s_exact[sub], &top, &total);
         uint64_t open = __ballot(unsure && lane == 0);
         // A wave takes each such column: its registers hold Float64 keys of four lanes.
         while (open) {
@@ -466,7 +481,7 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4)
             if (g >= a.groups || some < 0) some = 0;
             double m, all;
             wave_sync();
-            choose<T, double, false, 64, WIDE>(b, RouteShare{mine, g, some ? g * a.size + from : 0, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
+            choose<T, double, false, BIASED, 64, WIDE>(b, RouteShare{mine, g, some ? g * a.size + from : 0, some}, (const T *)a.L + (c0 + theirs) * a.ldl,
                                                (char *)s_keys, s_chosen[theirs], nullptr, &m, &all);
             if (sub == theirs) {
                 top = m;
@@ -711,7 +726,7 @@ int launch_route(RouteArgs a, hipStream_t s)
     a.whole = a.per == PER && a.size % (PER ? PER : 1) == 0;
     return by_launches<T>(a, NT / LANES, [&](const RouteArgs &some, unsigned blocks) {
         hipLaunchKernelGGL((route_kernel<T, BIASED, LANES, PER>), dim3(blocks), dim3(NT),
-                           PER ? 0 : (BIASED ? sizeof(double) : sizeof(typename Elem<T>::Acc)) * 64 * a.per, s, some);
+                           PER ? 0 : (BIASED || sizeof(T) >= 4 ? sizeof(double) : sizeof(float)) * 64 * a.per, s, some);
         return check_launch("route_kernel");
     });
 }

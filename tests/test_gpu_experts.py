@@ -199,6 +199,23 @@ def test_route_long_sums(J):
     assert (ids == 2 * 124 + 7 + 1).all()
 
 
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("cols", [50, 4100])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_near_logits(J, T, cols, score):
+    """Without a bias: logits whose last bits alone differ, equal ones, more of them than
+    are looked at one by one, zeros of both signs."""
+    gen = torch.Generator().manual_seed(13)
+    host = (torch.randn((cols, 120), generator=gen) * 2).to(T)
+    bits = {2: torch.int16, 4: torch.int32, 8: torch.int64}[host.element_size()]
+    some = host[::2].view(bits)
+    some[:, 30:50] = some[:, :1] + torch.randint(-9, 9, (some.shape[0], 20), generator=gen).to(bits)
+    host[4::5, 60:110] = host[4::5].amax(1, keepdim=True)
+    host[3::7] = (torch.randint(-1, 2, (len(host[3::7]), 120), generator=gen) * 0.0).to(T)
+    for groups, keep, best, copies in ((1, 1, 1, 6), (8, 3, 2, 9), (8, 3, 1, 36), (1, 1, 1, 64)):
+        check_route(J, host.cuda().t(), copies, score=score, groups=groups, keep=keep, best=best, renormalize=groups > 1)
+
+
 def test_route_past_one_launch(J):
     """More columns than 2^21 workgroups take: two experts, so that the choice is a comparison
     and the weight a logistic, and the gradient p (1 - p) (dw) with p the chosen one's share."""
