@@ -345,6 +345,91 @@ bool worth_packing(int64_t m, int64_t n, int64_t k, int64_t values, bool sides)
     return 2e-6 * m * n * k * gain > 3 + values * (sizeof(T) * 0.65e-6);
 }
 
+// Of 8-bit integers: where the estimate of the product from copies, and 6 us of two more
+// launches and the values read and written, is a fifth below that through registers (8,191
+// columns 2047 -> 8191: 436 us and 171, 2,965 columns 4152 -> 2560: 82 and 64; the one
+// measured that lost: 49,968 columns of 9 groups 712 -> 390, 59 and 70).
+bool worth_packing8(const TileArgs &a, bool bad_w, int64_t ldw, int64_t gp, bool bad_x, int64_t ldx, int64_t values)
+{
+    TileArgs as_is = a, packed = a;
+    if (bad_w) {
+        packed.P = nullptr;
+        packed.ldp = ldw;
+        packed.gp = gp;
+        packed.p_pad = true;
+    }
+    if (bad_x) {
+        packed.Q = nullptr;
+        packed.ldq = ldx;
+        packed.q_pad = true;
+    }
+    int shape = 0;
+    size_t bytes = 0;
+    double lies = 0, copied = 0;
+    if (plan_tile_product<int8_t>(&as_is, true, true, &shape, &bytes, &lies) ||
+        plan_tile_product<int8_t>(&packed, true, true, &shape, &bytes, &copied))
+        return false;
+    return lies > 1.2 * (copied + 6 + values * 0.43e-6);
+}
+
+// What a product packs first: W's rows and X's that do not lie well, into `bytes` of
+// scratch.
+struct Packing {
+    int64_t matrices, w_rows, w_len, w_values, x_rows, x_values;
+    size_t bytes;
+};
+
+template <typename T, typename Op>
+Packing plan_packing(const Op &op, bool pkc, TileArgs *a)
+{
+    const int64_t batch = op.groups ? op.groups : 1, w_rows = pkc ? op.out : op.inp, w_len = pkc ? op.inp : op.out;
+    const int64_t x_rows = op.cols / (op.groups ? op.copies : 1), ldw = padded<T>(w_len), ldx = padded<T>(op.inp);
+    const bool bad_w = !lies_well<T>(op.W, w_len, op.ldw, op.groups ? op.w_stride : 0), bad_x = !lies_well<T>(op.X, op.inp, op.ldx, 0);
+    const int64_t matrices = packed_matrices(op.groups, op.w_stride);
+    const int64_t w_values = bad_w ? matrices * w_rows * ldw : 0, x_values = bad_x ? x_rows * ldx : 0;
+    Packing pk{matrices, w_rows, w_len, w_values, x_rows, x_values, 0};
+    bool worth = op.cols > 48 * batch && w_values + x_values > 0;
+    if constexpr (sizeof(T) == 1) worth = worth && worth_packing8(*a, bad_w, ldw, matrices > 1 ? w_rows * ldw : 0, bad_x, ldx, w_values + x_values);
+    else worth = worth && worth_packing<T>(op.out, op.cols, op.inp, w_values + x_values, bad_w && !pkc);
+    if (worth) {
+        if (bad_w) {
+            a->P = nullptr;
+            a->ldp = ldw;
+            a->gp = matrices > 1 ? w_rows * ldw : 0;
+            a->p_pad = true;
+        }
+        if (bad_x) {
+            a->Q = nullptr;
+            a->ldq = ldx;
+            a->q_pad = true;
+        }
+        pk.bytes = align256(sizeof(T) * w_values) + align256(sizeof(T) * x_values);
+    }
+    return pk;
+}
+
+// Packs them, and takes `bytes` of scratch for that and the partial sums.
+template <typename T, typename Op>
+int pack_operands(const Op &op, const Packing &pk, size_t bytes, TileArgs *a, jlust_stream_t stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    void *ws = nullptr;
+    if (int st = scratch(stream, bytes, &ws)) return st;
+    char *at = (char *)ws;
+    if (a->p_pad) {
+        if (int st = pack_rows<T>(pk.w_rows, pk.w_len, op.W, op.ldw, pk.matrices, op.w_stride, nullptr, nullptr, at, a->ldp, s)) return st;
+        a->P = at;
+        at += align256(sizeof(T) * pk.w_values);
+    }
+    if (a->q_pad) {
+        if (int st = pack_rows<T>(pk.x_rows, op.inp, op.X, op.ldx, 1, 0, nullptr, nullptr, at, a->ldq, s)) return st;
+        a->Q = at;
+        at += align256(sizeof(T) * pk.x_values);
+    }
+    a->part = at;
+    return JLUST_STATUS_SUCCESS;
+}
+
 // dbias of a group: the sums of its runs, in order; 32 m by LANES runs at a time (8
 // where groups have few: 13 us by 32 and 5 by 8 for 32 groups of 8 runs).
 template <typename T, int LANES>
@@ -545,50 +630,17 @@ int linear(const jlust_linear &op, jlust_stream_t stream, jlust_product_info *in
     a.ldz = op.ldz;
     a.act = op.act;
     const bool pkc = op.w_layout == 1;
-    const int64_t batch = op.groups ? op.groups : 1, w_rows = pkc ? op.out : op.inp, w_len = pkc ? op.inp : op.out;
-    const int64_t x_rows = op.cols / (op.groups ? op.copies : 1), ldw = padded<T>(w_len), ldx = padded<T>(op.inp);
-    const bool bad_w = !lies_well<T>(op.W, w_len, op.ldw, op.groups ? op.w_stride : 0), bad_x = !lies_well<T>(op.X, op.inp, op.ldx, 0);
-    const int64_t matrices = packed_matrices(op.groups, op.w_stride);
-    const int64_t w_values = bad_w ? matrices * w_rows * ldw : 0, x_values = bad_x ? x_rows * ldx : 0;
-    size_t pack = 0;
-    if (op.cols > 48 * batch && worth_packing<T>(op.out, op.cols, op.inp, w_values + x_values, bad_w && !pkc)) {
-        if (bad_w) {
-            a.P = nullptr;
-            a.ldp = ldw;
-            a.gp = matrices > 1 ? w_rows * ldw : 0;
-            a.p_pad = true;
-        }
-        if (bad_x) {
-            a.Q = nullptr;
-            a.ldq = ldx;
-            a.q_pad = true;
-        }
-        pack = align256(sizeof(T) * w_values) + align256(sizeof(T) * x_values);
-    }
+    const Packing pk = plan_packing<T>(op, pkc, &a);
     int shape = 0;
     size_t bytes = 0;
     if (int st = plan_tile_product<T>(&a, pkc, true, &shape, &bytes)) return st;
     if (info) {
-        *info = info_of(a, shape, a.p_pad, a.q_pad, false, pack + bytes);
+        *info = info_of(a, shape, a.p_pad, a.q_pad, false, pk.bytes + bytes);
         return JLUST_STATUS_SUCCESS;
     }
     hipStream_t s = (hipStream_t)stream;
-    if (pack + bytes) {
-        void *ws = nullptr;
-        if (int st = scratch(stream, pack + bytes, &ws)) return st;
-        char *at = (char *)ws;
-        if (a.p_pad) {
-            if (int st = pack_rows<T>(w_rows, w_len, op.W, op.ldw, matrices, op.w_stride, nullptr, nullptr, at, ldw, s)) return st;
-            a.P = at;
-            at += align256(sizeof(T) * w_values);
-        }
-        if (a.q_pad) {
-            if (int st = pack_rows<T>(x_rows, op.inp, op.X, op.ldx, 1, 0, nullptr, nullptr, at, ldx, s)) return st;
-            a.Q = at;
-            at += align256(sizeof(T) * x_values);
-        }
-        a.part = at;
-    }
+    if (pk.bytes + bytes)
+        if (int st = pack_operands<T>(op, pk, pk.bytes + bytes, &a, stream)) return st;
     return launch_tile_product<T>(a, pkc, true, shape, s);
 }
 
@@ -621,16 +673,19 @@ int linear_int8(const jlust_linear_int8 &op, jlust_stream_t stream, jlust_produc
     a.Z = op.Z;
     a.ldz = op.ldz;
     a.act = op.act;
-    a.streamed = op.value_type != JLUST_VALUE_F32 && op.out * op.cols * 2 > STREAMED;
+    // Lines written in part past the caches are slow: 8,192 columns 2048 -> 8196 232 us, 181
+    // by plain stores.
+    a.streamed = op.value_type != JLUST_VALUE_F32 && op.out * op.cols * 2 > STREAMED && (((uintptr_t)op.Y | (uintptr_t)(op.ldy * 2)) & 127) == 0;
+    const Packing pk = plan_packing<int8_t>(op, true, &a);
     int shape = 0;
     size_t bytes = 0;
     if (int st = plan_tile_product<int8_t>(&a, true, true, &shape, &bytes)) return st;
     if (info) {
-        *info = info_of(a, shape, false, false, false, bytes);
+        *info = info_of(a, shape, a.p_pad, a.q_pad, false, pk.bytes + bytes);
         return JLUST_STATUS_SUCCESS;
     }
-    if (bytes)
-        if (int st = scratch(stream, bytes, &a.part)) return st;
+    if (pk.bytes + bytes)
+        if (int st = pack_operands<int8_t>(op, pk, pk.bytes + bytes, &a, stream)) return st;
     hipStream_t s = (hipStream_t)stream;
     switch (op.value_type) {
     case JLUST_VALUE_F32: return launch_tile_product8<float>(a, shape, s);

@@ -3,9 +3,9 @@
 
 namespace jlust {
 
-template int plan_tile_product<_Float16>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<_Float16>(TileArgs *, bool, bool, int *, size_t *, double *);
 template int launch_tile_product<_Float16>(const TileArgs &, bool, bool, int, hipStream_t);
-template int plan_tile_product<__bf16>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<__bf16>(TileArgs *, bool, bool, int *, size_t *, double *);
 template int launch_tile_product<__bf16>(const TileArgs &, bool, bool, int, hipStream_t);
 
 TileForm tile_form(int shape)

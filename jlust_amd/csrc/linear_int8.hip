@@ -8,7 +8,7 @@
 
 namespace jlust {
 
-template int plan_tile_product<int8_t>(TileArgs *, bool, bool, int *, size_t *);
+template int plan_tile_product<int8_t>(TileArgs *, bool, bool, int *, size_t *, double *);
 
 namespace {
 

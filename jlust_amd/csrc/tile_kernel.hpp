@@ -1184,7 +1184,7 @@ inline int64_t work_groups(const TileArgs &a, bool ksum)
 }
 
 template <typename T>
-int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes)
+int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes, double *estimate)
 {
     const bool ksum = !pkc && !qkc, grouped = a->offsets && !ksum;
     const int64_t batch = ksum && a->offsets ? a->groups : 1;
@@ -1220,9 +1220,10 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
         // Along k on both sides.  A step's bytes are 16-bit values', its k is twice
         // theirs; measured on 1 to 8,192 columns of 64 to 8,192 (43 products: 2.4 % past the
         // best on average, at most 37 %, with k = 64 and 13,574 rows of n in 4 groups).
+        // Rows off 16 bytes through registers: two thirds of the rate.
         if (share <= 16 && set(FEW_16, 1)) some[count++] = {FEW_16, 1.0, 0.035, 4, 2.2};
-        some[count++] = {REG_32, 3.7, 0.22, 5};
-        some[count++] = {REG_M64, 4.4, 0.21, 5};
+        some[count++] = {REG_32, fit ? 3.7 : 2.6, 0.22, 5};
+        some[count++] = {REG_M64, fit ? 4.4 : 2.9, 0.21, 5};
         if (fit && share > 48) {
             some[count++] = {COPY_128, 7.6, 0.36, 2, 3.7};
             some[count++] = {COPY_TALL, 7.7, 0.5, 2, 6.6};
@@ -1296,6 +1297,7 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
         return fail(JLUST_STATUS_INVALID_ARGUMENT, "linear: %lld x %lld sums (%lld groups) are more tiles than one launch takes",
                     (long long)a->m, (long long)a->n, (long long)a->groups);
     set(best_shape, split);
+    if (estimate) *estimate = best;
     *part_bytes = split > 1 ? (size_t)split * sums * sizeof(typename Elem<T>::Acc) : 0;
     return JLUST_STATUS_SUCCESS;
 }

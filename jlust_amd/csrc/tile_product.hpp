@@ -159,7 +159,7 @@ __device__ __forceinline__ bool find_run(const int32_t *__restrict__ offsets, in
 // partial sums are to be at a->part when it is launched.  INVALID_ARGUMENT where one
 // launch does not take all the tiles.
 template <typename T>
-int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes);
+int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_bytes, double *estimate = nullptr);
 template <typename T>
 int launch_tile_product(const TileArgs &a, bool pkc, bool qkc, int shape, hipStream_t s);
 // The same of 8-bit operands along k, C holding O.

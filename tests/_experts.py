@@ -219,3 +219,14 @@ PLANNED8 = [
     ("f32", 520, 2064, 14600, 0, 1, (256, 256, 1, 1)),
     ("f16", 520, 2064, 14600, 3, 1, (256, 256, 1, 1)),
 ]
+
+# Products of 8-bit integers that pack operands first: type, out, inp, cols, groups, copies,
+# how far W and X lie off 16 bytes, whether the groups share W; the tile, what is packed (1:
+# W, 2: X).
+PACKED8 = [
+    ("bf16", 2053, 1033, 2500, 0, 1, 0, 0, False, (128, 128, 3)),
+    ("f32", 2053, 1040, 2500, 0, 1, 1, 0, False, (128, 128, 1)),
+    ("f16", 2053, 1040, 2500, 0, 1, 0, 5, False, (128, 128, 2)),
+    ("bf16", 1029, 1033, 3000, 3, 2, 0, 0, False, (128, 128, 3)),
+    ("f16", 1029, 1033, 3000, 3, 2, 7, 0, True, (128, 128, 3)),
+]

@@ -102,6 +102,19 @@ def test_planned_products():
     assert forms == {(16, 16, 0), (64, 64, 0), (128, 32, 0), (128, 128, 1), (256, 128, 1), (256, 256, 1)}
 
 
+def test_packed_products():
+    """What tests/_experts.py says is packed, and the scratch it takes."""
+    for T, out, inp, cols, groups, copies, woff, xoff, shared, plan in E.PACKED8:
+        info, p = (ctypes.c_int64 * 6)(), 1 << 20
+        args = layers._LINEAR_INT8({"f32": 1, "f16": 2, "bf16": 3}[T], 0, out, inp, cols * copies, p + woff, inp, p, p + xoff, inp, p, p,
+                                   out, 0, 0, 0, 0, 0, groups, copies, p if groups else 0, 0 if shared else inp * out, out, out)
+        assert _lib.lib().jlust_hip_linear_int8_info(args, info) == 0
+        assert (info[0], info[1], info[4]) == plan and info[2] == 1, (out, inp, cols, tuple(info))
+        ld = (inp + 15) // 16 * 16
+        most = (plan[2] & 1) * ld * out * (1 if shared else max(groups, 1)) + (plan[2] >> 1) * ld * cols
+        assert most <= info[5] < most + 512
+
+
 def test_combine_dropout_and_quantize_refuse():
     lib = _lib.lib()
 

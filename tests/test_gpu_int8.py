@@ -150,6 +150,54 @@ def test_linear_int8_kernels(J, T, out, inp, cols, groups, copies):
     check(J, s, T, act, ids, copies, J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups))
 
 
+@pytest.mark.parametrize("T,out,inp,cols,groups,copies,woff,xoff,shared", [c[:9] for c in E.PACKED8])
+def test_linear_int8_packed(J, T, out, inp, cols, groups, copies, woff, xoff, shared):
+    """Operands that lie badly for copies are packed first (tests/_experts.py says which);
+    the same once more, into the scratch that holds the last ones."""
+    T = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[T]
+    s = case(out + cols, T, out, inp, cols, True, woff > 0, 1 if shared else groups or None, copies)
+    for k, off in (("W", woff), ("Xq", xoff)):
+        if off:
+            v = s[k]
+            buf = torch.zeros(v.numel() + 16, dtype=torch.int8, device="cuda")
+            s[k] = torch.as_strided(buf, v.shape, v.stride(), off)
+            s[k].copy_(v)
+    if shared:
+        s["W"] = s["W"].expand(-1, -1, groups)
+        s["ws"], s["b"] = s["ws"].expand(-1, groups).t().contiguous().t(), s["b"].expand(-1, groups).t().contiguous().t()
+    ids = h = None
+    if groups:
+        ids = torch.randint(0, groups + 1, (cols, copies), generator=torch.Generator().manual_seed(cols), dtype=torch.int32).cuda().t()
+        h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
+    check(J, s, T, "silu", ids, copies, h)
+    s["Xq"].neg_()
+    check(J, s, T, None, ids, copies, h, keep=False)
+
+
+def test_packed_int8_in_a_graph(J):
+    """A product that packs its operands, captured after a call of its size and replayed."""
+    s = case(1, torch.bfloat16, 2053, 1033, 2500, True, False)
+    kw = dict(w_scale=s["ws"], x_scale=s["xs"], bias=s["b"], act=J.gelu_fn)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        J.execute(J.LinearOp, s["W"], s["Xq"], s["Y"], **kw)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            J.execute(J.LinearOp, s["W"], s["Xq"], s["Y"], **kw)
+    torch.cuda.synchronize()
+    for r in range(3):
+        s["Xq"].copy_(s["Xq"].roll(1, 0))
+        s["Y"].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = s["Y"].clone()
+        J.execute(J.LinearOp, s["W"], s["Xq"], s["Y"], **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(got, s["Y"]), r
+
+
 @pytest.mark.parametrize("cols", [1, 40, 300])
 def test_sums_at_the_end_of_32_bits(J, cols):
     """131,071 products of -128 and -128 are 2^31 - 2^14."""
