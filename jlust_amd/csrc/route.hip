@@ -552,7 +552,9 @@ __device__ __forceinline__ A score_below(A l, A top)
 // p (t - sum p t), sigmoid renormalised the same times 1 - s, sigmoid t s (1 - s) at the
 // chosen and 0 elsewhere; softmax as it is s_e (t_e - sum s t) everywhere.  LANES lanes
 // take a column, CPL chunks of 16 bytes each in registers, so logits are read once (CPL
-// 0: any number, read again).
+// 0: any number, read again).  What goes to the chosen passes through a row of LDS; asking
+// of every element which of the chosen it is took 23.1 us for 13,433 Float32 columns of
+// 298 with 14 chosen, 12.5 so (160 bfloat16 experts, 6 chosen: 7.9 and 6.7).
 template <typename T, bool WHOLE, int LANES, int CPL>
 __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
 {
@@ -561,6 +563,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
     constexpr int COLS = 256 / LANES, NP = MAX_COPIES / LANES;
     __shared__ int s_expert[COLS][MAX_COPIES];
     __shared__ A s_part[COLS][MAX_COPIES];
+    __shared__ __align__(16) A s_row[CPL ? COLS : 1][CPL ? LANES * CPL * CH : 1];      // the parts at their experts
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const bool softmax = a.score == JLUST_SCORE_SOFTMAX, dense = softmax && !a.renormalize;
     const int64_t c0 = (int64_t)blockIdx.x * COLS;
@@ -648,21 +651,28 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
         s_expert[sub][i] = at[q];
         s_part[sub][i] = at[q] >= 0 ? g : A(0);
     }
+    if constexpr (CPL > 0) {
+        A none[CH] = {};
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) __builtin_memcpy(&s_row[sub][(lane + LANES * i) * CH], none, sizeof(none));
+    }
     wave_sync();
     if constexpr (CPL > 0) {
+        // An expert that is named twice gets both parts, the same sum from either.
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+            if (q >= parts || at[q] < 0) continue;
+            A g = A(0);
+            for (int k = 0; k < a.copies; ++k) g += s_expert[sub][k] == at[q] ? s_part[sub][k] : A(0);
+            s_row[sub][at[q]] = g;
+        }
+        wave_sync();
         const A inv = total > A(0) ? A(1) / total : A(0);
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
             const int at = (lane + LANES * i) * CH;
             A g[CH];
-#pragma unroll
-            for (int j = 0; j < CH; ++j) g[j] = A(0);
-            for (int k = 0; k < a.copies; ++k) {
-                const int e = s_expert[sub][k] - at;
-                const A v = s_part[sub][k];
-#pragma unroll
-                for (int j = 0; j < CH; ++j) g[j] += e == j ? v : A(0);
-            }
+            __builtin_memcpy(g, &s_row[sub][at], sizeof(g));
             if (dense) {
 #pragma unroll
                 for (int j = 0; j < CH; ++j) g[j] = s[i][j] * inv * (g[j] - dot);
