@@ -32,7 +32,8 @@
  *    queued and HIP graphs that captured a call stay valid.  Capturing a call
  *    in a graph: make one call of the same size on the capturing stream first
  *    (no allocation may happen inside a capture); prepared plans own their
- *    buffers and need no such warm-up.
+ *    buffers and need no such warm-up.  Graphs captured on one stream share its
+ *    buffer: replay them in turn, or capture each on a stream of its own.
  *  - Return value: a jlust_status code.  A message for the last failure on the
  *    calling thread is available from jlust_hip_last_error().
  *  - There is no CPU fallback: with no usable GPU every compute entry point

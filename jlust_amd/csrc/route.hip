@@ -440,9 +440,9 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
     return unsure;
 }
 
-// BIASED: keys are scores plus biases, Float64, else the logits.  But for 16-bit and
-// Float64 logits they are made in Float32 first, and again in Float64 for a column that is
-// not settled by those.
+// BIASED: keys are scores plus biases, Float64, else the logits.  But for Float64 logits,
+// and 16-bit ones without a bias, they are Float32 first, and Float64 for a column that
+// those do not settle.
 template <typename T, bool BIASED, int LANES, int PER>
 __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4) void route_kernel(const RouteArgs a)
 {

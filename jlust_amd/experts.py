@@ -8,8 +8,9 @@ reference): a column is a token, a node of a graph or a sample, as in layers.py.
         softmax or the sigmoid of the logits, an expert's key its score plus its
         bias (without one, its logit); the experts make `groups` equal groups, of
         which the `keep` best are looked at, ranked by their best key (best=1) or by
-        the sum of their two best scores plus biases (best=2).  Equal keys go to the
-        lower expert.  A weight is scale times the score, or with renormalize times
+        the sum of their two best scores plus biases (best=2; of one alone where no
+        second is left).  Equal keys go to the lower expert, equal groups to the first.
+        At most 4,095 experts, 64 groups and 64 experts a column.  A weight is scale times the score, or with renormalize times
         its share of the chosen scores' sum.  An expert whose logit (or bias) is -Inf
         or NaN is never chosen; where none is left the id is origin - 1, which names
         no group to prepare(GroupedLinearOp, ids), and the weight 0.

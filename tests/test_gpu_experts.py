@@ -496,6 +496,40 @@ def make_block(J, T, *shape):
     return s
 
 
+def test_offsets_past_32_bits(J):
+    """Columns 2^20 values apart, the last of them past 2^32: the same as side by side."""
+    T, far, n = torch.bfloat16, 1 << 20, 4100
+    gen = torch.Generator().manual_seed(2)
+
+    def apart(t, fill=0):
+        buf = torch.empty(far * (t.shape[1] - 1) + t.shape[0], dtype=t.dtype, device="cuda")
+        v = torch.as_strided(buf, t.shape, (1, far))
+        v.copy_(t) if fill is not None else None
+        return v
+
+    X, w = L.colmajor(40, n, T, gen), torch.rand((n // 2, 2), generator=gen).cuda().t()
+    logits = L.colmajor(16, n, T, gen)
+    far_x, far_l = apart(X), apart(logits)
+
+    def calls(x, l, like):
+        ids, lw = like(torch.empty((n, 3), dtype=torch.int32, device="cuda").t()), like(torch.empty((n, 3), device="cuda").t())
+        y, s, dx = like(torch.empty_like(X)), like(torch.empty((n // 2, 40), dtype=T, device="cuda").t()), like(torch.empty_like(X))
+        q, qs, dl = like(torch.empty((n, 40), dtype=torch.int8, device="cuda").t()), torch.empty(n, device="cuda"), like(torch.empty_like(logits))
+        dw = torch.empty((n // 2, 2), device="cuda").t()
+        J.execute(J.RouteOp, l, ids, lw)
+        J.execute(J.RouteGradOp, l, ids, lw, dl)
+        J.execute(J.CombineOp, x, w, s)
+        J.execute(J.CombineGradOp, x, w, s, dX=dx, dweights=dw)
+        J.execute(J.DropoutOp, x, y, p=0.25, seed=5, offset=6)
+        J.execute(J.QuantizeOp, x, q, qs)
+        Y = like(torch.empty((n, 40), dtype=T, device="cuda").t())
+        J.execute(J.LinearOp, q[:, :40].t().contiguous(), q, Y, w_scale=qs[:40], x_scale=qs)
+        return ids, lw, dl, s, dx, dw, y, q, qs, Y
+
+    for near, away in zip(calls(X, logits, lambda t: t), calls(far_x, far_l, lambda t: apart(t, None))):
+        assert torch.equal(near, away)
+
+
 def test_layer_of_experts(J):
     """Route, experts, sum, dropout and residual, and back, in Float64 against autograd
     of the formulas (both off by some 1e-13 of values near 1: 1e-10 is far from both)."""
