@@ -18,7 +18,7 @@ namespace jlust {
 namespace {
 
 constexpr int64_t MAX_EXPERTS = 4095, MAX_COPIES = 64, MAX_ROUTE_GROUPS = 64;
-constexpr int64_t ROUTE_FEW = 4096;            // columns, up to which a wave takes one
+constexpr int64_t ROUTE_FEW = 2560;            // columns, up to which a wave takes one
 
 struct RouteArgs {
     int64_t cols;
@@ -742,7 +742,9 @@ int launch_route(RouteArgs a, hipStream_t s)
 }
 
 // 16 lanes a column where it fits them and the columns fill the CUs (a round of the
-// best key then serves four columns), else a wave.
+// best key then serves four columns), else a wave (us by a wave and by 16 lanes, sigmoids
+// with a bias: 256 experts in 8 groups 7.0 and 7.6 for 2,048 columns, 9.2 and 7.8 for 4,096,
+// 23.1 and 12.4 for 16,384; 64 experts 5.1 and 5.4, 5.7 and 5.2, 12.8 and 6.4).
 template <typename T, bool BIASED>
 int route(RouteArgs a, hipStream_t s)
 {
