@@ -178,9 +178,14 @@ extern "C" int jlust_hip_combine_grad(int32_t value_type, int64_t d, int64_t col
         using T = decltype(z);
         const int64_t chunks = (d * (int64_t)sizeof(T) + 15) / 16;
         auto go = [&](auto f) { return f(d, cols, (int)copies, X, ldx, weights, ldw, dY, lddy, dX, lddx, dweights, lddw, s); };
+        // Few lanes for short columns, a workgroup's for long ones and where columns are few
+        // (us by 16, 32, 64 and 256 lanes: 100,000 columns of 16 chunks, two copies, 21, 24, 38,
+        // 120; 100,000 of 25 chunks 42, 33, 39, 126; 40,000 of 64 chunks, four copies, 73, 69, 66,
+        // 112; 20,000 of 128 chunks 33, 33, 32, 35; 64 of them, eight copies, 16, 10, 6.7, 5.5;
+        // 8,000 of 512 chunks 267, 251, 241, 211; 64 of them 55, 30, 17, 7.6).
         if (chunks <= 16) return go(launch_grad<T, 16>);
         if (chunks <= 32) return go(launch_grad<T, 32>);
-        if (chunks <= 512) return go(launch_grad<T, 64>);
+        if (chunks <= 64 || (chunks < 192 && cols > 1024)) return go(launch_grad<T, 64>);
         return go(launch_grad<T, 256>);
     });
 }
