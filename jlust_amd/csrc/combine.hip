@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(int64_t d, int64_t co
             A by[COPIES], dot[COPIES];
 #pragma unroll
             for (int q = 0; q < COPIES; ++q) {
-                by[q] = live && k + q < copies ? weights[t * ldw + k + q] : A(0);
+                by[q] = dX && live && k + q < copies ? weights[t * ldw + k + q] : A(0);     // a call without dX has none
                 dot[q] = A(0);
             }
             for (int64_t at = (int64_t)lane * CH; live && at < d; at += LANES * CH) {

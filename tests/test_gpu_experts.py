@@ -330,6 +330,26 @@ def test_combine(J, T, d, cols, copies, pad):
 
 
 @pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("d,cols,copies", [(100, 33, 1), (100, 130, 2), (250, 40, 5), (700, 9, 8), (2047, 65, 3), (2047, 1100, 1), (8, 1, 64)])
+def test_combine_grad_reads_what_it_needs(J, T, d, cols, copies):
+    """By the C entry: dweights without weights and dX without X, null and with no leading
+    dimension, are those of the call that has both (every number of lanes a column)."""
+    from jlust_amd import _lib
+    gen = torch.Generator().manual_seed(d)
+    X, dY = L.colmajor(d, cols * copies, T, gen), L.colmajor(d, cols, T, gen)
+    w = torch.randn((cols, copies), generator=gen).to(sums(T)).cuda().t()
+    dX, dw = torch.full_like(X, NAN), torch.full_like(w, NAN)
+    J.execute(J.CombineGradOp, X, w, dY, dX=dX, dweights=dw)
+    one, two = torch.full_like(X, NAN), torch.full_like(w, NAN)
+    vt, s = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}[T], torch.cuda.current_stream().cuda_stream
+    f = _lib.lib().jlust_hip_combine_grad
+    assert f(vt, d, cols, copies, X.data_ptr(), d, 0, 0, dY.data_ptr(), d, 0, 0, two.data_ptr(), copies, s) == 0
+    assert f(vt, d, cols, copies, 0, 0, w.data_ptr(), copies, dY.data_ptr(), d, one.data_ptr(), d, 0, 0, s) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(one, dX) and torch.equal(two, dw)
+
+
+@pytest.mark.parametrize("T", L.TYPES)
 def test_combine_skips_weights_of_zero(J, T):
     """A column whose weight is 0 may hold anything; a NaN weight shows."""
     gen = torch.Generator().manual_seed(0)
