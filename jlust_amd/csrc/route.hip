@@ -11,6 +11,7 @@
 #include "lanes.hpp"
 #include "wave.hpp"
 
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -238,9 +239,9 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
             y = over_lanes<LANES>(holds ? y : x, Larger(), of_group);
             x = m;
         };
-        // The lanes of the first group whose rank is the best.
-        auto wins = [&](auto r, auto m) {
-            const uint64_t mask = __ballot(r == m && m > -INFINITY) & column;
+        // The lanes of the first group that is `in` and whose rank is the best.
+        auto wins = [&](bool in, auto r, auto m) {
+            const uint64_t mask = __ballot(in && r == m) & column;
             return mask != 0 && (__ffsll((unsigned long long)mask) - 1 - first_in_wave) >> a.lane_shift == w.group;
         };
         if (a.best == 1) {
@@ -256,21 +257,24 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
                 x = m > NONE ? softmax ? part_of(x, most, S(1)) : sigmoid(x) : x;
                 y = rest > NONE ? softmax ? part_of(y, most, S(1)) : sigmoid(y) : y;
             }
-            const S sum = m > NONE ? x + (rest > NONE ? y : S(0)) : S(-INFINITY);
-            rank = sum;
+            const S sum = x + (rest > NONE ? y : S(0));
+            // A Float32 sum of a group with a candidate may be less than the type holds; as
+            // its lowest value it is near all others past that, for 64 bits to settle.
+            rank = !(m > NONE) ? S(-INFINITY) : ROUGH ? Larger()(sum, S(-FLT_MAX)) : sum;
             if constexpr (ROUGH) undone = rest > NONE && y < 0 && x > 0 ? -2 * y : 0;
         }
-        bool kept = false;
-        R last = -INFINITY, left = rank;
+        // Which groups have a candidate goes by their keys: a Float64 sum may be -infinity.
+        bool kept = false, waits = least > NONE;
+        R last = -INFINITY;
         for (int r = 0; r < a.keep; ++r) {
-            last = lanes_max<LANES>(left);
-            if (wins(left, last)) {
+            last = lanes_max<LANES>(waits ? rank : R(-INFINITY));
+            if (wins(waits, rank, last)) {
                 kept = true;
-                left = -INFINITY;
+                waits = false;
             }
         }
         if constexpr (ROUGH) {
-            const K next = lanes_max<LANES>(left);
+            const K next = lanes_max<LANES>(waits ? rank : NONE);
             // Keys of two signs make a sum smaller than they are: their error is not.
             if (__ballot(undone > 0)) undone = lanes_max<LANES>(undone);
             const float near = a.best * apart * (1 + fabsf(last) + undone);
@@ -305,7 +309,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const RouteShare &w, 
                 if (open) kept = sure;
                 for (int r = 0; r < a.keep; ++r) {
                     const double m = lanes_max<LANES>(wide);
-                    if (wins(wide, m) && r < places) {
+                    if (wins(wide > -INFINITY, wide, m) && r < places) {
                         kept = true;
                         wide = -INFINITY;
                     }

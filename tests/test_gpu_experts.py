@@ -216,6 +216,36 @@ def test_route_near_logits(J, T, cols, score):
         check_route(J, host.cuda().t(), copies, score=score, groups=groups, keep=keep, best=best, renormalize=groups > 1)
 
 
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_far_biases(J, T, score):
+    """Biases at the ends of their type, as masks have them: a group whose two best keys
+    add up to less than the type holds is as good as any that is left, and of several such
+    the order is that of the sums in 64 bits (Float64's own are equal where they pass it).
+    The same columns 200 times over are routed by another number of lanes."""
+    gen = torch.Generator().manual_seed(14)
+    low = torch.finfo(sums(T)).min
+    host = torch.randn((13, 16), generator=gen).to(T)
+    logits, many = host.cuda().t(), host.repeat(200, 1).cuda().t()
+    part = torch.tensor([0.59, 0.88, 1.0, 0.51], dtype=torch.float64).repeat_interleave(4)
+    edge = torch.tensor([[0.5, 0.5], [0.25, 0.75], [0.5 + 2e-7, 0.5], [0.5, 0.5 - 2e-7]], dtype=torch.float64).repeat(1, 2).reshape(-1)
+    masks = {"groups": torch.tensor([0.0] * 4 + [1.0] * 12), "all": torch.ones(16), "parts": part, "large": -part, "edge": edge,
+             "one": torch.tensor([0.0, 1.0, 1.0, 1.0] * 4), "signs": torch.tensor([1.0, -1.0, 1.0, 0.0] * 4)}
+    for m in masks.values():
+        for alone in (False, True):                # a group of one key before one of two
+            bias = (m.double() * low).to(sums(T))
+            if alone:
+                bias[1:4] = -INF
+            for groups, keep, best, copies in ((4, 2, 2, 5), (4, 3, 2, 9), (4, 3, 1, 9), (8, 5, 2, 7), (16, 9, 2, 6), (2, 1, 2, 8)):
+                kw = dict(score=score, bias=bias.cuda(), groups=groups, keep=keep, best=best)
+                ids, w = check_route(J, logits, copies, **kw)
+                ids2, w2 = ints(copies, 2600)[1], torch.empty((2600, copies), dtype=sums(T), device="cuda").t()
+                J.execute(J.RouteOp, many, ids2, w2, **kw)
+                assert torch.equal(ids2, ids.repeat(1, 200)), (groups, keep, best)
+                lim = 2 * E.weight_bound(logits, L.sums_u(T), score).cuda() * w.double() + 2 * L.TINY[sums(T)]
+                assert ((w2.double() - w.repeat(1, 200)).abs() <= lim.repeat(1, 200)).all()
+
+
 def test_route_past_one_launch(J):
     """More columns than 2^21 workgroups take: two experts, so that the choice is a comparison
     and the weight a logistic, and the gradient p (1 - p) (dw) with p the chosen one's share."""
