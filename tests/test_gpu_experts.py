@@ -285,6 +285,24 @@ def test_route_grad(J, T, score, renormalize, experts, copies):
     L.close(dL, ref, bound, "dL")
 
 
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("score,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("experts,copies", [(96, 17), (96, 40), (64, 64)])
+def test_route_grad_of_many_copies(J, T, score, renormalize, experts, copies):
+    """More of a column's experts than it has lanes; the last workgroup's columns not all there."""
+    cols, gen = 45, torch.Generator().manual_seed(copies)
+    logits = L.colmajor(experts, cols, T, gen, 2.0, pad=1)
+    logits[5:50, 1] = -INF
+    logits[:, 2] = -INF
+    ids, w = ints(copies, cols)[1], torch.empty((cols, copies), dtype=sums(T), device="cuda").t()
+    J.execute(J.RouteOp, logits, ids, w, score=score, renormalize=renormalize, scale=1.5)
+    dw = torch.randn((cols, copies), generator=gen).to(sums(T)).cuda().t()
+    dL = L.colmajor(experts, cols, T, gen).fill_(NAN)
+    J.execute(J.RouteGradOp, logits, ids, dw, dL, score=score, renormalize=renormalize, scale=1.5)
+    ref, size = E.route_grad(logits, ids, dw, score, renormalize, 1.5)
+    L.close(dL, ref, 2 * E.weight_bound(logits, L.sums_u(T), score)[None, :] * size, "dL")
+
+
 @pytest.mark.parametrize("score,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
 def test_route_grad_against_differences(J, score, renormalize):
     """sum(dw .* w) by central differences with the chosen experts kept: step 1e-5,
