@@ -259,6 +259,37 @@ def test_scales_that_are_not_numbers(J):
     assert torch.equal(torch.isnan(s["Y"]), mask) and torch.equal(s["Y"][~mask], good[~mask])
 
 
+@pytest.mark.parametrize("T,out,inp,cols,groups,copies", [c[:6] for c in E.PLANNED8])
+def test_scales_far_from_one(J, T, out, inp, cols, groups, copies):
+    """Scales over all of Float32, negative ones too, by every kernel: a result is right where it is within
+    its type's range, though the product of its scales may not be; a sum of 0 gives the bias."""
+    T = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[T]
+    s = case(out + cols, T, out, inp, cols, True, False, groups or None, copies)
+    gen = torch.Generator().manual_seed(inp)
+
+    def far(n):
+        x = torch.exp2(torch.rand(n, generator=gen, dtype=torch.float64) * 276 - 149) * torch.where(torch.rand(n, generator=gen) < 0.5, -1.0, 1.0)
+        return x.float()
+
+    s["ws"].copy_(far(s["ws"].shape))
+    s["xs"].copy_(far(s["xs"].shape))
+    s["W"][3], s["Xq"][:, cols // 2] = 0, 0
+    ids = h = None
+    if groups:
+        ids = torch.randint(0, groups + 1, (cols, copies), generator=gen, dtype=torch.int32).cuda()
+        ids = ids.t() if copies > 1 else ids[:, 0].contiguous()
+        h = J.prepare(J.HIPBackend(), J.GroupedLinearOp, ids, n_groups=groups)
+    J.execute(J.LinearOp if h is None else h, s["W"], s["Xq"], s["Y"], w_scale=s["ws"], x_scale=s["xs"], bias=s["b"])
+    ref, _, bound, _ = E.linear8(s["W"], s["ws"], s["Xq"], s["xs"], T, s["b"], None, None, ids, copies)
+    got, most = L.f64(s["Y"]), torch.finfo(T).max
+    lim = bound + L.U[T] * ref.abs() + 2.0 ** -149
+    past, within = ref.abs() - lim > most, ref.abs() + lim <= most
+    assert past.any() and within.any()
+    assert torch.equal(got[past], torch.sign(ref[past]) * float("inf"))
+    zero = torch.zeros_like(ref)
+    L.close(torch.where(within, got, zero).to(T), torch.where(within, ref, zero), torch.where(within, bound, zero), "Y")
+
+
 def test_in_place_residual_and_empty(J):
     s = case(3, torch.bfloat16, 70, 96, 20, True, True)
     kw = dict(w_scale=s["ws"], x_scale=s["xs"], bias=s["b"])
