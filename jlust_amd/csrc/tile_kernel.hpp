@@ -286,18 +286,18 @@ __device__ __forceinline__ float scale_of(const TileArgs &a, int group, int64_t 
     return group < a.groups ? a.qs[a.qrow ? a.qrow[n] : n] : 0.0f;
 }
 
-// Whether a row's scale may take a sum past Float32's range by itself (or is NaN).
-__device__ __forceinline__ bool far_scale(float qs) { return !(fabsf(qs) <= 1); }
-
 // V sums times both scales, one after the other, so that no step leaves Float32's range
 // where the result does not (the scales' product may): below the normal range a whole
-// number times a scale is exact, and a scale of Q that is FAR comes last.
-template <bool FAR, int V>
+// number times a scale is exact, and of qs = lo hi a part past 1 comes last.  (8,192
+// bfloat16 columns 2048 -> 8192 with gelu 183.2 us by the scales' product and 184.8 so; rows
+// with such a qs by a loop of their own cost Float32 results 10 % for want of registers.)
+template <int V>
 __device__ __forceinline__ void scale_sums(const int *sum, float qs, const float *by, const float *bias, float *f)
 {
-    const bool last = FAR && far_scale(qs);
+    const bool small = fabsf(qs) <= 1;
+    const float lo = small ? qs : 1.0f, hi = small ? 1.0f : qs;
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = fmaf((float)sum[e] * (last ? by[e] : qs), last ? qs : by[e], bias[e]);
+    for (int e = 0; e < V; ++e) f[e] = fmaf((float)sum[e] * lo * by[e], hi, bias[e]);
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -477,7 +477,6 @@ __device__ __forceinline__ void finish_scaled(const TileArgs &a, char *lds, int 
     TileArgs b = a;
     if (!a.offsets) b.groups = 1;
     int row[RUNS][ITER];
-    bool far = false;
     float qs[RUNS][ITER], by[TM / TW][CH], bias[TM / TW][CH];
 #pragma unroll
     for (int run = 0; run < RUNS; ++run)
@@ -487,7 +486,6 @@ __device__ __forceinline__ void finish_scaled(const TileArgs &a, char *lds, int 
             row[run][it] = n < nend ? n : -1;
             qs[run][it] = n < nend && !a.part ? scale_of(b, group, n) : 0.0f;
             if (n < nend && !a.part && a.crow) row[run][it] = a.crow[n];
-            far |= far_scale(qs[run][it]);
         }
 #pragma unroll
     for (int h = 0; h < TM / TW; ++h) {
@@ -497,43 +495,36 @@ __device__ __forceinline__ void finish_scaled(const TileArgs &a, char *lds, int 
         for (int e = 0; e < CH; ++e) bias[h][e] = (float)v[e];
         load_scales<CH>(b, group, m0 + TW * h + lane % LANES * CH, by[h]);
     }
-    // Far scales are rare, and a choice between two orders at every row holds the others up:
-    // 8,192 columns 2048 -> 8192 184 us with the product of the scales first, 187 so, 185 by
-    // a loop of their own.
-    auto end = [&](auto some_far) {
 #pragma unroll
-        for (int run = 0; run < RUNS; ++run)
+    for (int run = 0; run < RUNS; ++run)
 #pragma unroll
-            for (int h = 0; h < TM / TW; ++h) {
-                const int64_t m = m0 + TW * h + lane % LANES * CH, left = a.m - m;
-                O res[ITER][CH];
-                if (a.R && !a.part) {
+        for (int h = 0; h < TM / TW; ++h) {
+            const int64_t m = m0 + TW * h + lane % LANES * CH, left = a.m - m;
+            O res[ITER][CH];
+            if (a.R && !a.part) {
 #pragma unroll
-                    for (int it = 0; it < ITER; ++it)
-                        load_some<CH>((const O *)a.R + row[run][it] * a.ldr + m, row[run][it] >= 0 ? left : 0, res[it]);
-                }
-                wave_sync();
-                put(run, h, mine);
-                wave_sync();
-#pragma unroll
-                for (int it = 0; it < ITER; ++it) {
-                    if (row[run][it] < 0 || left <= 0) continue;
-                    const int r = r0 + it * ROWS;
-                    int v[CH];
-#pragma unroll
-                    for (int e = 0; e < CH; e += 4) __builtin_memcpy(v + e, mine + SR::at(r, (lane % LANES * CH + e) / 4), 16);
-                    if (a.part) {
-                        store_some<CH>((int *)a.part + ((int64_t)piece * a.n + row[run][it]) * a.m + m, left, v);
-                        continue;
-                    }
-                    float f[CH];
-                    scale_sums<decltype(some_far)::value, CH>(v, qs[run][it], by[h], bias[h], f);
-                    finish_sum<CH, true, O, float>(b, res[it], row[run][it], m, f);
-                }
+                for (int it = 0; it < ITER; ++it)
+                    load_some<CH>((const O *)a.R + row[run][it] * a.ldr + m, row[run][it] >= 0 ? left : 0, res[it]);
             }
-    };
-    if (__ballot(far)) end(std::true_type());
-    else end(std::false_type());
+            wave_sync();
+            put(run, h, mine);
+            wave_sync();
+#pragma unroll
+            for (int it = 0; it < ITER; ++it) {
+                if (row[run][it] < 0 || left <= 0) continue;
+                const int r = r0 + it * ROWS;
+                int v[CH];
+#pragma unroll
+                for (int e = 0; e < CH; e += 4) __builtin_memcpy(v + e, mine + SR::at(r, (lane % LANES * CH + e) / 4), 16);
+                if (a.part) {
+                    store_some<CH>((int *)a.part + ((int64_t)piece * a.n + row[run][it]) * a.m + m, left, v);
+                    continue;
+                }
+                float f[CH];
+                scale_sums<CH>(v, qs[run][it], by[h], bias[h], f);
+                finish_sum<CH, true, O, float>(b, res[it], row[run][it], m, f);
+            }
+        }
 }
 
 // A 16-row run of 16 x 16 tiles: lane (li, g) holds rows 4g .. 4g+3 of column li.
@@ -1087,7 +1078,7 @@ __global__ __launch_bounds__(Few<TILES>::WAVES * 64) void few_columns_kernel(con
     if constexpr (SCALED) {
         float by[1], f[1], added[1] = {(float)bias[0]};
         load_scales<1>(b, w.group, m, by);
-        scale_sums<true, 1>(v, scale_of(b, w.group, n), by, added, f);
+        scale_sums<1>(v, scale_of(b, w.group, n), by, added, f);
         finish_sum<1, false, O, float>(b, res, row, m, f);
     } else {
         finish<1, T, float>(b, bias, res, row, m, v);
@@ -1158,7 +1149,7 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const TileArgs a)
         load_scales<V>(b, group, m, by);
 #pragma unroll
         for (int e = 0; e < V; ++e) added[e] = (float)bias[e];
-        scale_sums<true, V>(s, scale_of(b, group, n), by, added, f);
+        scale_sums<V>(s, scale_of(b, group, n), by, added, f);
         finish_sum<V, false, O, float>(b, res, row, m, f);
     } else {
         finish<V, T, A>(b, bias, res, row, m, s);
