@@ -520,7 +520,7 @@ __global__ __launch_bounds__(PER ? 256 : 64, PER == 0 ? 1 : LANES == 64 ? 3 : 4)
         const int i = lane + q * LANES;
         if (q >= parts || i >= a.copies) continue;
         a.ids[c * a.ldi + i] = e[q] + a.origin;
-        ((A *)a.weights)[c * a.ldw + i] = e[q] >= 0 ? A(a.scale) * (p[q] / sum) : A(0);
+        ((A *)a.weights)[c * a.ldw + i] = e[q] >= 0 ? A(a.scale * (double)(p[q] / sum)) : A(0);
     }
 }
 
@@ -623,7 +623,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
             if (e >= 0 && e < a.experts) {
                 at[q] = (int)e;
                 l[q] = A(L[e]);
-                t[q] = A(a.scale) * ((const A *)a.dw)[c * a.lddw + i];
+                t[q] = A(a.scale * (double)((const A *)a.dw)[c * a.lddw + i]);
             }
         }
     }

@@ -303,6 +303,35 @@ def test_route_grad_of_many_copies(J, T, score, renormalize, experts, copies):
     L.close(dL, ref, 2 * E.weight_bound(logits, L.sums_u(T), score)[None, :] * size, "dL")
 
 
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("score,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("scale", [1e45, 1e-55])
+def test_route_scales_past_float32(J, T, score, renormalize, scale):
+    """A scale that Float32 does not hold, and weights and gradients that it does: far scores
+    times a large one, large gradients times a small one; a share of 0 is 0 by any."""
+    host = torch.tensor([[0.0, -30.0, -45.0, -55.0], [1.0, 0.5, -0.5, -200.0]])
+    host = (host - 20 if score == "sigmoid" else host).to(T)
+    logits = host.cuda().t()
+    ids, w = ints(4, 2)[1], torch.empty((2, 4), dtype=sums(T), device="cuda").t()
+    kw = dict(score=score, renormalize=renormalize, scale=scale)
+    J.execute(J.RouteOp, logits, ids, w, **kw)
+    ref_ids, ref = E.route(logits, 4, **kw)
+    assert torch.equal(ids.cpu(), ref_ids)
+    most, u = torch.finfo(sums(T)).max, L.sums_u(T)
+    lim = E.weight_bound(logits, u, score)[None, :] * ref.abs() + L.TINY[sums(T)] * max(1.0, scale)      # a share is off by as much itself
+    past = ref - lim > most
+    got = L.f64(w)
+    assert torch.equal(torch.isinf(got), past) and ((got - ref).abs() <= lim)[~past].all()
+    dw = torch.full((2, 4), 1e30 if scale < 1 else 1e-30, dtype=sums(T), device="cuda").t()
+    dw[1] *= -0.5
+    dL = torch.full((2, 4), NAN, dtype=T, device="cuda").t()
+    J.execute(J.RouteGradOp, logits, ids, dw, dL, **kw)
+    ref, size = E.route_grad(logits, ids, dw, score, renormalize, scale)
+    bound = 2 * E.weight_bound(logits, u, score)[None, :] * size
+    if T != torch.float16 or scale < 1:            # Float16 does not hold the large ones
+        L.close(dL, ref, bound, "dL")
+
+
 @pytest.mark.parametrize("score,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
 def test_route_grad_against_differences(J, score, renormalize):
     """sum(dw .* w) by central differences with the chosen experts kept: step 1e-5,
