@@ -622,7 +622,8 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteGradArgs a)
             const int64_t e = (int64_t)a.ids[c * a.ldi + i] - a.origin;
             if (e >= 0 && e < a.experts) {
                 at[q] = (int)e;
-                l[q] = A(L[e]);
+                const A v = A(L[e]);
+                l[q] = v > A(-INFINITY) ? v : A(-INFINITY);        // of NaN too the score is 0
                 t[q] = A(a.scale * (double)((const A *)a.dw)[c * a.lddw + i]);
             }
         }

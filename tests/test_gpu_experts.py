@@ -332,6 +332,27 @@ def test_route_scales_past_float32(J, T, score, renormalize, scale):
         L.close(dL, ref, bound, "dL")
 
 
+@pytest.mark.parametrize("T", L.TYPES)
+@pytest.mark.parametrize("score,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+def test_route_grad_of_logits_that_are_no_numbers(J, T, score, renormalize):
+    """An id whose logit is NaN has the score 0, as one of -infinity has: both have the same
+    gradients."""
+    gen = torch.Generator().manual_seed(6)
+    a = L.colmajor(10, 5, T, gen)
+    b = a.clone()
+    a[3], b[3] = NAN, -INF
+    ids = torch.tensor([[4, 1, 9]] * 5, dtype=torch.int32, device="cuda").t()
+    dw = torch.randn((5, 3), generator=gen).to(sums(T)).cuda().t()
+    got = []
+    for l in (a, b):
+        dL = torch.full((5, 10), NAN, dtype=T, device="cuda").t()
+        J.execute(J.RouteGradOp, l, ids, dw, dL, score=score, renormalize=renormalize)
+        got.append(dL)
+    assert torch.equal(got[0], got[1])
+    ref, size = E.route_grad(b, ids, dw, score, renormalize)
+    L.close(got[0], ref, 2 * E.weight_bound(b, L.sums_u(T), score)[None, :] * size, "dL")
+
+
 @pytest.mark.parametrize("score,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
 def test_route_grad_against_differences(J, score, renormalize):
     """sum(dw .* w) by central differences with the chosen experts kept: step 1e-5,
