@@ -1231,8 +1231,8 @@ int plan_tile_product(TileArgs *a, bool pkc, bool qkc, int *shape, size_t *part_
     int count = 0;
     if constexpr (sizeof(T) == 1) {
         // Along k on both sides.  A step's bytes are 16-bit values', its k is twice
-        // theirs; measured on 1 to 8,192 columns of 64 to 8,192 (43 products: 2.4 % past the
-        // best on average, at most 37 %, with k = 64 and 13,574 rows of n in 4 groups).
+        // theirs; measured on 1 to 8,192 columns of 64 to 8,192 (48 products: 5 % past the
+        // best on average, at most 35 %, with k = 64 and 13,574 rows of n in 4 groups).
         // Rows off 16 bytes through registers: two thirds of the rate.
         if (share <= 16 && set(FEW_16, 1)) some[count++] = {FEW_16, 1.0, 0.035, 4, 2.2};
         some[count++] = {REG_32, fit ? 3.7 : 2.6, 0.22, 5};
